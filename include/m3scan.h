@@ -25,6 +25,7 @@
  *   redpanda/engine/mamba.py:82-89, 450-452 RMSNorm + in_proj + silu, small batch -> m3_rows_linear
  *   redpanda/engine/mamba.py:454, 463       x_proj + dt_proj product, small batch -> m3_xdt_proj
  *   redpanda/engine/mamba.py:497, 591-595   out_proj + residual add, small batch -> m3_rows_linear
+ *   redpanda/engine/mamba.py:82-89          RMSNorm, forward and backward -> m3_norm_fwd / m3_norm_bwd
  *
  * Shapes (B batch, L length, D = d_inner, N = d_state, n_rot rotational lanes,
  * N - n_rot tracking lanes):
@@ -440,6 +441,165 @@ M3_API int m3_scan_bwd_noalloc(const m3_scan_desc* desc,
                 const void* dy, int32_t dtype_dy, const float* ckpt,
                 void* d_delta, void* d_u, void* d_Bc, void* d_Cc,
                 float* d_A_real_p, float* d_A_imag_p, float* d_track_p, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Sequence-model operators beside the trapezoidal scan: layer and RMS norms
+ * with their backward pass, the short causal convolution and the selective
+ * scan (prompts, training, single tokens), and drawing a token from logits.
+ * Row-strided inputs: row r starts at base + r * ld elements; a (B, L, .)
+ * tensor has the rows b * L + t.  Arithmetic, states and sums are fp32 (64-bit
+ * where stated); outputs are rounded once to their element type.  All results
+ * are independent of scheduling (no floating-point atomics). */
+
+typedef struct m3_norm_desc {
+  int64_t rows;       /* >= 1 */
+  int32_t d;          /* 1..32768 */
+  int32_t dtype_x;    /* element type of x and dx */
+  int32_t dtype_y;    /* element type of y and g */
+  int32_t rms;        /* non-zero: RMS norm (no mean, no bias) */
+  float eps;          /* >= 0 */
+} m3_norm_desc;
+
+/* y = (x - mean) * rstd * w + b over rows of d elements, rstd =
+ * 1 / sqrt(mean((x - mean)^2) + eps); mean is 0 for the RMS norm (the RMSNorm
+ * of mamba.py:82-89; the layer norms of search_mamba.py's heads).
+ *   x (rows, ld_x); w (d,) float32; b (d,) float32 or NULL; y (rows, d)
+ *   mean, rstd (rows,) float32 for the backward, or NULL.  y may be x when
+ *   ld_x == d and both have one element type. */
+M3_API int m3_norm_fwd(const m3_norm_desc* desc, const void* x, int64_t ld_x, const float* w,
+            const float* b, void* y, float* mean, float* rstd, void* stream);
+
+/* Workspace bytes of m3_norm_bwd on the current device. */
+M3_API size_t m3_norm_bwd_workspace_bytes(const m3_norm_desc* desc);
+
+/* Backward of m3_norm_fwd: g (rows, d) the gradient of y; dx (rows, d); dw and
+ * db (d,) float32 (db NULL when there is no bias); mean is not read for the RMS
+ * norm.  The weight gradients are summed over the rows in a fixed order. */
+M3_API int m3_norm_bwd(const m3_norm_desc* desc, const void* x, int64_t ld_x, const float* w,
+            const float* mean, const float* rstd, const void* g, void* dx, float* dw, float* db,
+            void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct m3_conv_desc {
+  int32_t batch;      /* B >= 1 */
+  int32_t seqlen;     /* L >= 1; 1 for the step */
+  int32_t d_inner;    /* D >= 1 */
+  int32_t width;      /* K taps, 1..8 */
+  int32_t dtype;      /* element type of x, y, the state and their gradients */
+  int32_t silu;       /* non-zero: y = silu(p), else y = p */
+} m3_conv_desc;
+
+/* Causal convolution over time, one filter per channel:
+ *   p[b,t,d] = bias[d] + sum_k w[d,k] x[b, t-K+1+k, d]
+ *   x (B*L, ld_x); w (D, K) float32; b (D,) float32 or NULL; y (B, L, D)
+ *   state      (B, K-1, D) or NULL (zeros): the input rows before x, oldest first
+ *   lengths    (B,) int32 or NULL (all L), clamped to [0, L]: steps at or past a
+ *              row's length are not read, and y is zero there
+ *   state_out  (B, K-1, D) or NULL: the last K-1 rows of [state; x[:length]];
+ *              must not be state, nor y x. */
+M3_API int m3_causal_conv_fwd(const m3_conv_desc* desc, const void* x, int64_t ld_x,
+            const float* w, const float* b, const void* state, const int32_t* lengths, void* y,
+            void* state_out, void* stream);
+
+/* Workspace bytes of m3_causal_conv_bwd on the current device. */
+M3_API size_t m3_causal_conv_bwd_workspace_bytes(const m3_conv_desc* desc);
+
+/* Backward: g (B, L, D) the gradient of y; dx (B, L, D), zero at steps past a
+ * length; dw (D, K), db (D,) float32 (db may be NULL without a bias).  The state
+ * gets no gradient.  dx must be neither x nor g. */
+M3_API int m3_causal_conv_bwd(const m3_conv_desc* desc, const void* x, int64_t ld_x,
+            const float* w, const float* b, const void* state, const int32_t* lengths,
+            const void* g, void* dx, float* dw, float* db, void* workspace,
+            size_t workspace_bytes, void* stream);
+
+/* One token per row (seqlen 1): y (B, D) from [state; x], x (B, ld_x); the
+ * state (B, K-1, D) moves up by one row in place. */
+M3_API int m3_causal_conv_step(const m3_conv_desc* desc, void* state, const void* x, int64_t ld_x,
+            const float* w, const float* b, void* y, void* stream);
+
+typedef struct m3_sel_desc {
+  int32_t batch;      /* B >= 1 */
+  int32_t seqlen;     /* L >= 1; 1 for the step */
+  int32_t d_inner;    /* D >= 1 */
+  int32_t d_state;    /* N, 1..128 */
+  int32_t dtype;      /* element type of u, dt, z, B, C, y and their gradients */
+  int32_t softplus;   /* non-zero: step size softplus(dt + dt_bias), else dt + dt_bias */
+} m3_sel_desc;
+
+typedef struct m3_sel_args {
+  const void* u;  int64_t ld_u;     /* (B*L, ld_u), D columns */
+  const void* dt; int64_t ld_dt;    /* (B*L, ld_dt), D columns */
+  const void* z;  int64_t ld_z;     /* (B*L, ld_z), D columns, or NULL: no gate */
+  const void* B;  int64_t ld_b;     /* (B*L, ld_b), N columns */
+  const void* C;  int64_t ld_c;     /* (B*L, ld_c), N columns */
+  const float* A;                   /* (D, N) */
+  const float* d_skip;              /* (D,) or NULL */
+  const float* dt_bias;             /* (D,) or NULL */
+  const float* state;               /* (B, D, N) the state before the first step, or NULL: zero */
+  const int32_t* lengths;           /* (B,) or NULL: all L; clamped to [0, L] */
+} m3_sel_args;
+
+/* Selective scan, per row b, channel d and state n:
+ *   de_t = softplus(dt_t + dt_bias),   h_t = exp(de_t A) h_{t-1} + de_t u_t B_t
+ *   y_t  = (sum_n C_t h_t + d_skip u_t) * silu(z_t)
+ *   y       (B, L, D); zero at steps at or past a row's length, whose inputs are
+ *           not read
+ *   h_last  (B, D, N) float32 or NULL: the state at each row's length (not state)
+ *   ckpt    m3_selective_ckpt_floats() floats for the backward, 16-byte aligned,
+ *           or NULL
+ *   workspace >= m3_selective_fwd_workspace_bytes() bytes (0 for large batches;
+ *           few rows are split along time), 16-byte aligned */
+M3_API size_t m3_selective_ckpt_floats(const m3_sel_desc* desc);
+M3_API size_t m3_selective_fwd_workspace_bytes(const m3_sel_desc* desc);
+M3_API int m3_selective_fwd(const m3_sel_desc* desc, const m3_sel_args* args, void* y,
+            float* h_last, float* ckpt, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct m3_sel_grads {
+  void* d_u; void* d_dt; void* d_z;          /* (B, L, D); d_z unused without z */
+  void* d_B; void* d_C;                      /* (B, L, N), aligned to 4 elements */
+  float* d_A;                                /* (D, N) */
+  float* d_skip; float* d_dt_bias;           /* (D,) or NULL */
+} m3_sel_grads;
+
+/* Backward of m3_selective_fwd: g (B, L, D) the gradient of y, ckpt the
+ * forward's.  The states get no gradient. */
+M3_API size_t m3_selective_bwd_workspace_bytes(const m3_sel_desc* desc);
+M3_API int m3_selective_bwd(const m3_sel_desc* desc, const m3_sel_args* args, const void* g,
+            const float* ckpt, const m3_sel_grads* grads, void* workspace,
+            size_t workspace_bytes, void* stream);
+
+/* One token per row (seqlen 1), in place on h (B, D, N) float32; y (B, D).
+ * args->state and args->lengths must be NULL; at most 524280 rows. */
+M3_API int m3_selective_step(const m3_sel_desc* desc, const m3_sel_args* args, float* h, void* y,
+            void* stream);
+
+typedef struct m3_sample_desc {
+  int32_t rows;         /* >= 1 */
+  int32_t vocab;        /* V, 1..262144 */
+  int32_t dtype;        /* element type of logits */
+  float temperature;    /* settings of every row, where no array is given */
+  int32_t top_k;
+  float top_p;
+  float min_p;
+} m3_sample_desc;
+
+/* Draws one token per row.  With w_i = exp((x_i - max) / temperature) over the
+ * candidates (x_i neither -infinity nor NaN; where the maximum is +infinity its
+ * holders weigh 1 and the others 0), ordered by x descending, then index:
+ *   top_k   keeps the first k (<= 0: all)
+ *   top_p   of those, the shortest prefix with at least top_p of their weight,
+ *           one token at least (>= 1: all)
+ *   min_p   of those, the tokens with w_i >= min(min_p, 1)
+ * and the token is the smallest index whose cumulative weight over the kept
+ * tokens, in index order, exceeds uniform * their total (the last kept one when
+ * none does).  temperature <= 0 or NaN takes the first token of the order; a row
+ * without candidates gives -1.  Weights are summed as 64-bit integers of the
+ * double-precision exponentials.
+ *   logits (rows, ld); uniform (rows,) in [0, 1); temperature, top_p, min_p
+ *   (rows,) float32 and top_k (rows,) int32 arrays override the descriptor's
+ *   values where not NULL; out (rows,) int64. */
+M3_API int m3_sample(const m3_sample_desc* desc, const void* logits, int64_t ld,
+            const float* uniform, const float* temperature, const int32_t* top_k,
+            const float* top_p, const float* min_p, int64_t* out, void* stream);
 
 /* Reads (and clears when clear != 0) the device-side error word of the
  * current device; *code receives 0 or an M3_ERR_* value. */

@@ -1,0 +1,91 @@
+"""Host-side helpers of the operator modules: device, stream and row layout.
+
+A call of a small operator costs more on the host than on the GPU, so these do
+the least that is right: no device switch when the tensors are on the current
+device, no copy or cast of what already has the kernels' layout and type.
+"""
+
+import contextlib
+
+import torch
+
+from ._lib import M3_BF16, M3_F32
+
+_CODES = {torch.float32: M3_F32, torch.bfloat16: M3_BF16}
+_HERE = contextlib.nullcontext()
+
+
+def code(dtype):
+    """The library's code of an element type."""
+    c = _CODES.get(dtype)
+    if c is None:
+        raise TypeError(f"unsupported dtype {dtype}: float32 or bfloat16")
+    return c
+
+
+def device_index(*ts):
+    """Index of the CUDA device that every tensor (None: skipped) is on."""
+    dev = -1
+    for t in ts:
+        if t is None:
+            continue
+        i = t.get_device()
+        if i < 0:
+            raise RuntimeError("m3 ops run on CUDA tensors only (no CPU fallback)")
+        if dev < 0:
+            dev = i
+        elif i != dev:
+            raise RuntimeError("m3 ops need every tensor on one device")
+    return dev
+
+
+def on_device(index):
+    """Context in which device ``index`` is the current one."""
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def raw_stream(index):
+    """The device's current stream as the integer the C ABI takes."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def f32(t):
+    """A parameter as contiguous float32 (itself when it is)."""
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().to(torch.float32).contiguous()
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def needs_grad(*ts):
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def seq_rows(t):
+    """A (B, L, n) tensor whose rows (b, t) have one stride, and that stride."""
+    B, L, n = t.shape
+    if t.is_contiguous():
+        return t, n
+    s0, s1, s2 = t.stride()
+    if s2 == 1 and (L == 1 or B == 1 or s0 == L * s1):
+        ld = s1 if L > 1 else s0 if B > 1 else n
+        if ld >= n:
+            return t, ld
+    return t.contiguous(), n
+
+
+def rows(t):
+    """The same for (rows, n)."""
+    r, n = t.shape
+    if t.is_contiguous():
+        return t, n
+    if t.stride(1) == 1 and (r == 1 or t.stride(0) >= n):
+        return t, (t.stride(0) if r > 1 else n)
+    return t.contiguous(), n

@@ -35,8 +35,49 @@ class StepDesc(ctypes.Structure):
                 ("dtype_du", _I), ("dtype_bc", _I)]
 
 
+class NormDesc(ctypes.Structure):
+    """``m3_norm_desc``."""
+    _fields_ = [("rows", ctypes.c_int64), ("d", _I), ("dtype_x", _I), ("dtype_y", _I),
+                ("rms", _I), ("eps", ctypes.c_float)]
+
+
+class ConvDesc(ctypes.Structure):
+    """``m3_conv_desc``."""
+    _fields_ = [("batch", _I), ("seqlen", _I), ("d_inner", _I), ("width", _I), ("dtype", _I),
+                ("silu", _I)]
+
+
+class SelDesc(ctypes.Structure):
+    """``m3_sel_desc``."""
+    _fields_ = [("batch", _I), ("seqlen", _I), ("d_inner", _I), ("d_state", _I), ("dtype", _I),
+                ("softplus", _I)]
+
+
+class SelArgs(ctypes.Structure):
+    """``m3_sel_args``."""
+    _fields_ = [(n + s, t) for n in ("u", "dt", "z", "B", "C")
+                for s, t in (("", _P), ("_ld", ctypes.c_int64))] + [
+        (n, _P) for n in ("A", "d_skip", "dt_bias", "state", "lengths")]
+
+
+class SelGrads(ctypes.Structure):
+    """``m3_sel_grads``."""
+    _fields_ = [(n, _P) for n in ("d_u", "d_dt", "d_z", "d_B", "d_C", "d_A", "d_skip",
+                                  "d_dt_bias")]
+
+
+class SampleDesc(ctypes.Structure):
+    """``m3_sample_desc``."""
+    _fields_ = [("rows", _I), ("vocab", _I), ("dtype", _I), ("temperature", ctypes.c_float),
+                ("top_k", _I), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float)]
+
+
 _D = ctypes.POINTER(ScanDesc)
 _S = ctypes.POINTER(StepDesc)
+_N = ctypes.POINTER(NormDesc)
+_C = ctypes.POINTER(ConvDesc)
+_E = ctypes.POINTER(SelDesc)
+_A = ctypes.POINTER(SelArgs)
 
 SIGNATURES = {
     "m3_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -87,6 +128,23 @@ SIGNATURES = {
                                                 ctypes.c_int64, _I, _I, _P, _P, ctypes.c_float,
                                                 _P, _P, _P, _P, _P, ctypes.c_int64, _P, _P, _I,
                                                 _P]),
+    "m3_norm_fwd": (ctypes.c_int, [_N, _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P]),
+    "m3_norm_bwd_workspace_bytes": (_Z, [_N]),
+    "m3_norm_bwd": (ctypes.c_int, [_N, _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _Z,
+                                   _P]),
+    "m3_causal_conv_fwd": (ctypes.c_int, [_C, _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P, _P]),
+    "m3_causal_conv_bwd_workspace_bytes": (_Z, [_C]),
+    "m3_causal_conv_bwd": (ctypes.c_int, [_C, _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P, _P,
+                                          _P, _P, _Z, _P]),
+    "m3_causal_conv_step": (ctypes.c_int, [_C, _P, _P, ctypes.c_int64, _P, _P, _P, _P]),
+    "m3_selective_ckpt_floats": (_Z, [_E]),
+    "m3_selective_fwd_workspace_bytes": (_Z, [_E]),
+    "m3_selective_fwd": (ctypes.c_int, [_E, _A, _P, _P, _P, _P, _Z, _P]),
+    "m3_selective_bwd_workspace_bytes": (_Z, [_E]),
+    "m3_selective_bwd": (ctypes.c_int, [_E, _A, _P, _P, ctypes.POINTER(SelGrads), _P, _Z, _P]),
+    "m3_selective_step": (ctypes.c_int, [_E, _A, _P, _P, _P]),
+    "m3_sample": (ctypes.c_int, [ctypes.POINTER(SampleDesc), _P, ctypes.c_int64, _P, _P, _P, _P,
+                                 _P, _P, _P]),
 }
 
 _lock = threading.Lock()

@@ -5,6 +5,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include "m3_api_util.h"
 #include "m3_common.cuh"
 #include "m3_internal.h"
 #include "m3_tiles.h"
@@ -42,32 +43,6 @@ bool select_tile(int n_rot, int n_track, Tile* out) {
 namespace {
 
 constexpr int kMaxState = 128;
-
-int device_sms() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return -1; }
-  int sms = 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return -1;
-  }
-  return sms;
-}
-
-int check_device() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return M3_ERR_NO_DEVICE; }
-  int major = 0;
-  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return M3_ERR_NO_DEVICE;
-  }
-  return major == 10 ? M3_OK : M3_ERR_NO_DEVICE;
-}
-
-bool dtype_ok(int dt) { return dt == M3_F32 || dt == M3_BF16; }
-int dsize(int dt) { return dt == M3_BF16 ? 2 : 4; }
-bool aligned(const void* p, int a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 int check_scan_desc(const m3_scan_desc* d, Tile* tile) {
   if (!d) return M3_ERR_NULL;
@@ -107,8 +82,6 @@ struct BwdLayout {
   int G, Bg;
   size_t off_a, off_bc, off_du, total;
 };
-
-size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 bool bwd_layout(const m3_scan_desc* d, const Tile& t, BwdLayout* lay) {
   if (t.NDB == 0) return false;

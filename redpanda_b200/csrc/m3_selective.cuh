@@ -1,0 +1,220 @@
+// Device code shared by the selective scan's forward, backward and step.
+//
+// Per row b, channel d, state n:
+//   de_t = softplus(dt_t + dt_bias)   (or dt_t + dt_bias)
+//   h_t  = exp(de_t A) h_{t-1} + de_t u_t B_t
+//   y_t  = (sum_n C_t h_t + D u_t) silu(z_t)
+//
+// Layout: a lane group of LN threads owns two adjacent channels; thread q of the
+// group holds states 4q .. 4q+3 of both.  Steps are staged kSelSteps at a time
+// through shared memory; a step past the row's length is staged with de = 0,
+// which leaves the state as it is (exp(0) = 1, nothing added), so no branch on
+// the length is left in the recurrence.  State products are packed pairs of
+// states (fma.rn.f32x2).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "m3_math.cuh"
+#include "m3_ops.h"
+#include "m3_prologue.cuh"
+#include "m3_vec.cuh"
+
+namespace m3 {
+
+constexpr int kS = kSelSteps;
+
+template <int LN> struct Sel {
+  static constexpr int NT = LN >= 16 ? 256 : 128;   // threads per CTA
+  static constexpr int DT = NT / LN * 2;            // channels per CTA
+  static constexpr int NP = 4 * LN;                 // states kept per channel
+  static constexpr int EPT = kS * DT / NT;          // staged elements per thread and tensor
+  static constexpr int QPT = (kS * LN + NT - 1) / NT;   // staged state quads per thread (B or C)
+};
+
+__device__ __forceinline__ int sel_length(const int* lengths, int b, int L) {
+  if (lengths == nullptr) return L;
+  const int n = lengths[b];
+  return n < 0 ? 0 : n > L ? L : n;
+}
+
+// Step size of one element (bias added, softplus or not).
+__device__ __forceinline__ float step_size(float x, int softplus) {
+  return softplus ? softplus20(x) : x;
+}
+
+// Sum over the LN lanes of a group of NV values per lane, transposed: in each
+// round a lane keeps the half of the values that its lane bit names and adds
+// the partner's copy, so with NV = LN lane q ends with total q in v[0], and
+// with NV = c LN it holds totals q c .. q c + c - 1 in v[0 .. c-1].  NV < LN
+// finishes with plain butterflies (several lanes hold the same total).  Fixed
+// order.
+template <int NV, int LN, int M = LN / 2>
+__device__ __forceinline__ void lane_sum(float* v, int q) {
+  if constexpr (M >= 1) {
+    if constexpr (NV >= 2) {
+      const bool up = (q & M) != 0;
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) {
+        const float keep = up ? v[NV / 2 + i] : v[i];
+        const float send = up ? v[i] : v[NV / 2 + i];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, M);
+      }
+      lane_sum<NV / 2, LN, M / 2>(v, q);
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], M);
+      lane_sum<1, LN, M / 2>(v, q);
+    }
+  }
+}
+
+__device__ __forceinline__ float2 ex2_pair(float2 x) {
+  return make_float2(ex2_approx(x.x), ex2_approx(x.y));
+}
+
+// A2 = A log2(e) of the thread's states of channels c, c+1 (zero past D or N,
+// where the state stays zero).
+__device__ __forceinline__ void load_a2(float2 (&a2)[2][2], const float* A, int c, int n0, int D,
+                                        int N) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = (c + k < D && n0 + j < N) ? A[(size_t)(c + k) * N + n0 + j] * kLog2e : 0.f;
+    a2[k][0] = make_float2(v[0], v[1]);
+    a2[k][1] = make_float2(v[2], v[3]);
+  }
+}
+
+// The thread's states of channels c, c+1 from / to a (B, D, N) tensor.
+__device__ __forceinline__ void load_state(float2 (&h)[2][2], const float* src, size_t b, int c,
+                                           int n0, int D, int N) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = (src != nullptr && c + k < D && n0 + j < N)
+                 ? src[(b * D + c + k) * N + n0 + j] : 0.f;
+    h[k][0] = make_float2(v[0], v[1]);
+    h[k][1] = make_float2(v[2], v[3]);
+  }
+}
+__device__ __forceinline__ void store_state(const float2 (&h)[2][2], float* dst, size_t b, int c,
+                                            int n0, int D, int N) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float v[4] = {h[k][0].x, h[k][0].y, h[k][1].x, h[k][1].y};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + k < D && n0 + j < N) dst[(b * D + c + k) * N + n0 + j] = v[j];
+  }
+}
+// The same for the padded (rows, D, NP) buffers (16-byte aligned quads).
+__device__ __forceinline__ void load_quads(float2 (&h)[2][2], const float* src, size_t row, int c,
+                                           int q, int D, int NP) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c + k < D) v = *reinterpret_cast<const float4*>(src + (row * D + c + k) * NP + 4 * q);
+    h[k][0] = make_float2(v.x, v.y);
+    h[k][1] = make_float2(v.z, v.w);
+  }
+}
+__device__ __forceinline__ void store_quads(const float2 (&h)[2][2], float* dst, size_t row, int c,
+                                            int q, int D, int NP) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (c + k < D)
+      *reinterpret_cast<float4*>(dst + (row * D + c + k) * NP + 4 * q) =
+          make_float4(h[k][0].x, h[k][0].y, h[k][1].x, h[k][1].y);
+}
+
+// ------------------------------------------------------------- staged rows
+// Element e of a thread in a (kS, DT) tile: VW consecutive channels at a time.
+template <typename T, int LN> struct TileMap {
+  using G = Sel<LN>;
+  static constexpr int VMAX = 16 / (int)sizeof(T);
+  static constexpr int VW = G::EPT < VMAX ? G::EPT : VMAX;   // channels per load
+  static constexpr int NVEC = G::EPT / VW;
+  static constexpr int PER_ROW = G::DT / VW;
+  static __device__ __forceinline__ int row(int i) {
+    return ((int)threadIdx.x + i * G::NT) / PER_ROW;
+  }
+  static __device__ __forceinline__ int col(int i) {
+    return ((int)threadIdx.x + i * G::NT) % PER_ROW * VW;
+  }
+};
+
+// Loads the thread's elements of rows [t0, t0 + kS) of a (L, ld) tensor whose
+// first row is base; rows at or past n and channels past D read as zero.
+template <typename T, int LN>
+__device__ __forceinline__ void load_tile(Pack<T, TileMap<T, LN>::VW> (&out)[TileMap<T, LN>::NVEC],
+                                          const T* base, long long ld, int t0, int n, int c0,
+                                          int D, bool vec) {
+  using M = TileMap<T, LN>;
+#pragma unroll
+  for (int i = 0; i < M::NVEC; ++i) {
+    const int t = t0 + M::row(i), c = c0 + M::col(i);
+    out[i] = zero_pack<T, M::VW>();
+    if (t < n && c < D) {
+      const T* p = base + (size_t)t * ld + c;
+      if (vec) out[i] = ld_pack<T, M::VW>(p);   // D is a multiple of VW
+      else
+#pragma unroll
+        for (int j = 0; j < M::VW; ++j)
+          if (c + j < D) out[i].v[j] = p[j];
+    }
+  }
+}
+template <typename T, int LN>
+__device__ __forceinline__ void store_tile(const Pack<T, TileMap<T, LN>::VW>& v, int i, T* base,
+                                           long long ld, int t0, int L, int c0, int D, bool vec) {
+  using M = TileMap<T, LN>;
+  const int t = t0 + M::row(i), c = c0 + M::col(i);
+  if (t < L && c < D) {
+    T* p = base + (size_t)t * ld + c;
+    if (vec) st_pack<T, M::VW>(p, v);
+    else
+#pragma unroll
+      for (int j = 0; j < M::VW; ++j)
+        if (c + j < D) p[j] = v.v[j];
+  }
+}
+
+// Loads the thread's state quads of rows [t0, t0 + kS) of B or C.
+template <typename T, int LN>
+__device__ __forceinline__ void load_quad_rows(Pack<T, 4> (&out)[Sel<LN>::QPT], const T* base,
+                                               long long ld, int t0, int n, int N, bool vec) {
+  using G = Sel<LN>;
+#pragma unroll
+  for (int i = 0; i < G::QPT; ++i) {
+    const int e = (int)threadIdx.x + i * G::NT;
+    const int t = t0 + e / LN, k = e % LN * 4;
+    out[i] = zero_pack<T, 4>();
+    if (e < kS * LN && t < n && k < N) {
+      const T* p = base + (size_t)t * ld + k;
+      if (vec) out[i] = ld_pack<T, 4>(p);       // N is a multiple of 4
+      else
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (k + j < N) out[i].v[j] = p[j];
+    }
+  }
+}
+template <typename T, int LN>
+__device__ __forceinline__ void put_quad_rows(const Pack<T, 4> (&v)[Sel<LN>::QPT], float* s) {
+  using G = Sel<LN>;
+#pragma unroll
+  for (int i = 0; i < G::QPT; ++i) {
+    const int e = (int)threadIdx.x + i * G::NT;
+    if (e < kS * LN)
+      *reinterpret_cast<float4*>(s + e / LN * G::NP + e % LN * 4) =
+          make_float4(v[i].get(0), v[i].get(1), v[i].get(2), v[i].get(3));
+  }
+}
+
+}  // namespace m3
