@@ -64,8 +64,10 @@ bool sel_layout(const m3_sel_desc* d, SelLayout* l) {
   l->tiles = (d->d_inner + sel_tile(ln) - 1) / sel_tile(ln);
   l->splits = sel_splits(d->batch, d->seqlen, d->d_inner, d->d_state, sms);
   l->cps = (l->nch + l->splits - 1) / l->splits;
-  // backward: CTAs walk rows of the batch, about four CTAs per SM in all
-  long long bg = 4LL * sms / ((long long)l->tiles * l->splits);
+  // backward: CTAs walk rows of the batch, one wave of them
+  const int per = sel_bwd_resident(d->d_state, d->dtype);
+  if (per <= 0) return false;
+  long long bg = (long long)per * sms / ((long long)l->tiles * l->splits);
   if (bg > d->batch) bg = d->batch;
   if (bg < 1) bg = 1;
   l->bgroups = (int)bg;

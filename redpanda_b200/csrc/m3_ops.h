@@ -112,6 +112,7 @@ struct SelParams {
   int vec_d, vec_n;                                      // vector rows allowed
 };
 int sel_splits(int B, int L, int D, int N, int sms);
+int sel_bwd_resident(int N, int dtype);                // CTAs of the backward per SM, 0: error
 cudaError_t launch_sel_fwd(const SelParams& p, cudaStream_t s);
 
 struct SelBwdParams {

@@ -40,9 +40,47 @@ __device__ __forceinline__ int sel_length(const int* lengths, int b, int L) {
   return n < 0 ? 0 : n > L ? L : n;
 }
 
-// Step size of one element (bias added, softplus or not).
+// softplus(x) = max(x, 0) + log(1 + t), t = e^-|x|, without the library's
+// log1p and exp (about 50 instructions per element, more than a short state's
+// recurrence costs): t on the MUFU unit, its argument's rounding added back to
+// first order (hi + lo is |x| log2 e to twice the precision); and
+// log(1 + t) = 2 artanh(s), s = t / (2 + t) <= 1/3, by its series
+// s + s^3/3 + ... + s^13/13 (what is left out is below 2e-8 of it).  Relative
+// error a few 1e-7 over the whole range, past torch's threshold of 20 too,
+// where log(1 + t) is below half an ulp of x.
+constexpr float kLog2eLo = 0x1.4ae0cp-26f;      // log2(e) - kLog2e
+
+__device__ __forceinline__ float exp_neg(float ax) {   // e^-ax, ax >= 0
+  const float hi = -ax * kLog2e;
+  const float lo = fmaf(-ax, kLog2eLo, fmaf(-ax, kLog2e, -hi));
+  const float t = ex2_approx(hi);
+  return ax >= 126.f ? 0.f : fmaf(t * 0x1.62e43p-1f, lo, t);   // NaN passes
+}
+__device__ __forceinline__ float log1p_of(float t) {   // t in [0, 1]
+  const float s = __fdividef(t, 2.f + t), q = s * s;
+  float p = 1.f / 13.f;
+  p = fmaf(p, q, 1.f / 11.f);
+  p = fmaf(p, q, 1.f / 9.f);
+  p = fmaf(p, q, 1.f / 7.f);
+  p = fmaf(p, q, 1.f / 5.f);
+  p = fmaf(p, q, 1.f / 3.f);
+  p = fmaf(p, q, 1.f);
+  return 2.f * s * p;
+}
+// Step size of one element (bias added, softplus or not); `slope` gets its
+// derivative.
 __device__ __forceinline__ float step_size(float x, int softplus) {
-  return softplus ? softplus20(x) : x;
+  if (!softplus) return x;
+  return fmaxf(x, 0.f) + log1p_of(exp_neg(fabsf(x)));
+}
+__device__ __forceinline__ float step_size(float x, int softplus, float* slope) {
+  if (!softplus) {
+    *slope = 1.f;
+    return x;
+  }
+  const float t = exp_neg(fabsf(x)), r = __fdividef(1.f, 1.f + t);
+  *slope = x > 0.f ? r : t * r;
+  return fmaxf(x, 0.f) + log1p_of(t);
 }
 
 // Sum over the LN lanes of a group of NV values per lane, transposed: in each
@@ -149,24 +187,46 @@ template <typename T, int LN> struct TileMap {
   }
 };
 
-// Loads the thread's elements of rows [t0, t0 + kS) of a (L, ld) tensor whose
-// first row is base; rows at or past n and channels past D read as zero.
+// A thread's own copy of what it will stage, filled ahead of use: 4, 8 or 16
+// bytes at a time by cp.async, so that loads are in flight over a whole group of
+// steps without holding registers.  Only the thread that copied reads it back
+// (after copies_wait), so no barrier is needed.
+__device__ __forceinline__ void copies_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool in) {
+  const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES),
+               "r"(in ? BYTES : 0) : "memory");   // not in range: zeros
+}
+
+// The thread's elements of rows [t0, t0 + kS) of a (L, ld) tensor whose first row
+// is base into its slots (slot[i] of thread x at slots[i * NT + x]); rows at or
+// past n and channels past D become zero.
 template <typename T, int LN>
-__device__ __forceinline__ void load_tile(Pack<T, TileMap<T, LN>::VW> (&out)[TileMap<T, LN>::NVEC],
-                                          const T* base, long long ld, int t0, int n, int c0,
-                                          int D, bool vec) {
+__device__ __forceinline__ void fetch_tile(Pack<T, TileMap<T, LN>::VW>* slots, const T* base,
+                                           long long ld, int t0, int n, int c0, int D, bool vec) {
   using M = TileMap<T, LN>;
+  constexpr int BYTES = M::VW * (int)sizeof(T);
 #pragma unroll
   for (int i = 0; i < M::NVEC; ++i) {
     const int t = t0 + M::row(i), c = c0 + M::col(i);
-    out[i] = zero_pack<T, M::VW>();
-    if (t < n && c < D) {
-      const T* p = base + (size_t)t * ld + c;
-      if (vec) out[i] = ld_pack<T, M::VW>(p);   // D is a multiple of VW
-      else
+    const bool in = t < n && c < D;
+    const T* p = base + (in ? (size_t)t * ld + c : 0);
+    Pack<T, M::VW>* dst = slots + i * Sel<LN>::NT + threadIdx.x;
+    if (BYTES >= 4 && vec) {   // D is a multiple of VW
+      copy_async<(BYTES >= 4 ? BYTES : 4)>(dst, p, in);
+    } else {
+      Pack<T, M::VW> v = zero_pack<T, M::VW>();
+      if (in)
 #pragma unroll
         for (int j = 0; j < M::VW; ++j)
-          if (c + j < D) out[i].v[j] = p[j];
+          if (c + j < D) v.load_one(j, p);
+      *dst = v;
     }
   }
 }
@@ -181,39 +241,32 @@ __device__ __forceinline__ void store_tile(const Pack<T, TileMap<T, LN>::VW>& v,
     else
 #pragma unroll
       for (int j = 0; j < M::VW; ++j)
-        if (c + j < D) p[j] = v.v[j];
+        if (c + j < D) v.store_one(j, p);
   }
 }
 
-// Loads the thread's state quads of rows [t0, t0 + kS) of B or C.
+// The thread's state quads of rows [t0, t0 + kS) of B or C into its slots.
 template <typename T, int LN>
-__device__ __forceinline__ void load_quad_rows(Pack<T, 4> (&out)[Sel<LN>::QPT], const T* base,
-                                               long long ld, int t0, int n, int N, bool vec) {
+__device__ __forceinline__ void fetch_quads(Pack<T, 4>* slots, const T* base, long long ld, int t0,
+                                            int n, int N, bool vec) {
   using G = Sel<LN>;
 #pragma unroll
   for (int i = 0; i < G::QPT; ++i) {
     const int e = (int)threadIdx.x + i * G::NT;
     const int t = t0 + e / LN, k = e % LN * 4;
-    out[i] = zero_pack<T, 4>();
-    if (e < kS * LN && t < n && k < N) {
-      const T* p = base + (size_t)t * ld + k;
-      if (vec) out[i] = ld_pack<T, 4>(p);       // N is a multiple of 4
-      else
+    const bool in = e < kS * LN && t < n && k < N;
+    const T* p = base + (in ? (size_t)t * ld + k : 0);
+    Pack<T, 4>* dst = slots + i * G::NT + threadIdx.x;
+    if (vec) {                 // N is a multiple of 4
+      copy_async<4 * (int)sizeof(T)>(dst, p, in);
+    } else {
+      Pack<T, 4> v = zero_pack<T, 4>();
+      if (in)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (k + j < N) out[i].v[j] = p[j];
+          if (k + j < N) v.load_one(j, p);
+      *dst = v;
     }
-  }
-}
-template <typename T, int LN>
-__device__ __forceinline__ void put_quad_rows(const Pack<T, 4> (&v)[Sel<LN>::QPT], float* s) {
-  using G = Sel<LN>;
-#pragma unroll
-  for (int i = 0; i < G::QPT; ++i) {
-    const int e = (int)threadIdx.x + i * G::NT;
-    if (e < kS * LN)
-      *reinterpret_cast<float4*>(s + e / LN * G::NP + e % LN * 4) =
-          make_float4(v[i].get(0), v[i].get(1), v[i].get(2), v[i].get(3));
   }
 }
 

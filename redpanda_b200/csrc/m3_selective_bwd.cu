@@ -5,7 +5,7 @@
 //   dC_t  = sum_d gy h_t              dB_t = sum_d dh_t de u
 //   s1    = sum_n dh_t B_t            w = dh_t exp(de A) h_{t-1}
 //   du    = D gy + de s1              d de = u s1 + sum_n w A
-//   dA    = sum_{b,t} w de            ddt = d de sigmoid(dt + bias) = d de (1 - e^-de)
+//   dA    = sum_{b,t} w de            ddt = d de sigmoid(dt + bias)
 //   dz    = dy (C.h + D u) silu'(z)   dD = sum gy u,  dbias = sum ddt
 //
 // The forward leaves the state before every chunk of kSelSteps steps.  A CTA
@@ -34,59 +34,183 @@ constexpr int kSub = 4;                      // steps per recomputed group
 constexpr int kNSub = kSelSteps / kSub;
 constexpr float kLn2 = 0x1.62e43p-1f;
 
-template <int LN> struct BwdSmem {
-  using G = Sel<LN>;
-  static constexpr int NW = G::NT / 32;
-  float B[kS * G::NP], C[kS * G::NP];
-  float4 D[kS][G::DT];                       // (de, de u, gy, -)
-  float4 H[kNSub][2][G::NT];                 // states at each group's start
-  float R[kS][3][G::DT];                     // s1, s2 (in units of 1/log2 e), C.h
-  float BC[2][kSub][NW][2 * G::NP];          // warps' sums of dB, dC
+// Sums over the warp's 32 / LN lane groups (dB, dC) without selects: the halves
+// of a transposed reduction are chosen by the order in which a lane holds its
+// states.  Lanes with bit 4 set hold their two pairs swapped, lanes with bit 3
+// set the members of each pair (as far as there are groups to add), so that a
+// lane always keeps its first and sends its second half.  B and C are staged in
+// every order that occurs.
+template <int LN> struct Order {
+  static constexpr int GROUPS = 32 / LN;
+  static constexpr int COPIES = GROUPS >= 4 ? 4 : GROUPS;   // of B and C
+  static __device__ __forceinline__ int pair(int lane) { return GROUPS >= 2 ? lane >> 4 & 1 : 0; }
+  static __device__ __forceinline__ int elem(int lane) { return GROUPS >= 4 ? lane >> 3 & 1 : 0; }
 };
 
-// Sum over a warp's 32 / LN lane groups of 8 values per lane, transposed:
-// lane l ends with 8 LN / 32 totals (at least one), the first of index
-// first_bc(l).
-template <int NV, int LN, int M = 16>
-__device__ __forceinline__ void group_sum(float* v, int lane) {
-  if constexpr (M >= LN) {
-    if constexpr (NV >= 2) {
-      const bool up = (lane & M) != 0;
+template <typename T, int LN> struct BwdSmem {
+  using G = Sel<LN>;
+  using M = TileMap<T, LN>;
+  using Tile = Pack<T, M::VW>[M::NVEC * G::NT];
+  using Quads = Pack<T, 4>[G::QPT * G::NT];
+  static constexpr int NW = G::NT / 32, CP = Order<LN>::COPIES;
+  alignas(16) float B[CP][kS * G::NP], C[CP][kS * G::NP];
+  alignas(16) float2 D[kS][G::DT];           // (de, de u)
+  alignas(16) float Y[kS][G::DT];            // gy
+  alignas(16) float P[kS][G::DT];            // the step size's slope
+  alignas(16) float4 H[kNSub][2][G::NT];     // states at each group's start
+  alignas(16) float R[kS][3][G::DT];         // s1, s2 (in units of 1/log2 e), C.h
+  alignas(16) float BC[2][kSub][NW][2 * G::NP];   // warps' sums of dB, dC
+  alignas(16) Tile u[2], z[2], g[2], dt;
+  alignas(16) Quads b, c;
+};
+
+// A quad in a lane's order, and back.
+__device__ __forceinline__ float4 reorder(float4 v, int pair, int elem) {
+  if (pair) v = make_float4(v.z, v.w, v.x, v.y);
+  if (elem) v = make_float4(v.y, v.x, v.w, v.z);
+  return v;
+}
+__device__ __forceinline__ void set_pairs(float2 (&h)[2], float4 v) {
+  h[0] = make_float2(v.x, v.y);
+  h[1] = make_float2(v.z, v.w);
+}
+__device__ __forceinline__ float4 quad_of(const float2 (&h)[2]) {
+  return make_float4(h[0].x, h[0].y, h[1].x, h[1].y);
+}
+// The quad 4q .. 4q+3 of channel c in a (D, N) or (rows, D, N) tensor, element
+// loads (zero past D or N).
+__device__ __forceinline__ float4 load_quad_any(const float* src, size_t row, int c, int n0, int D,
+                                                int N) {
+  float v[4];
 #pragma unroll
-      for (int i = 0; i < NV / 2; ++i) {
-        const float keep = up ? v[NV / 2 + i] : v[i];
-        const float send = up ? v[i] : v[NV / 2 + i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, M);
+  for (int j = 0; j < 4; ++j)
+    v[j] = (src != nullptr && c < D && n0 + j < N) ? src[(row * D + c) * N + n0 + j] : 0.f;
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ float4 load_quad_pad(const float* src, size_t row, int c, int q, int D,
+                                                int NP) {
+  return c < D ? *reinterpret_cast<const float4*>(src + (row * D + c) * NP + 4 * q)
+               : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+__device__ __forceinline__ float2 shfl_pair(float2 v, int m) {
+  return make_float2(__shfl_xor_sync(0xffffffffu, v.x, m), __shfl_xor_sync(0xffffffffu, v.y, m));
+}
+
+// The chunk's staged values from the thread's slots (t0: first step).
+template <typename T, int LN, bool SUM>
+__device__ __forceinline__ void bwd_stage(BwdSmem<T, LN>& sm, const SelParams& p, int buf, int t0,
+                                          int n, bool gate,
+                                          const float (&bias)[TileMap<T, LN>::VW]) {
+  using G = Sel<LN>;
+  using M = TileMap<T, LN>;
+#pragma unroll
+  for (int i = 0; i < M::NVEC; ++i) {
+    const int r = M::row(i), cc = M::col(i), x = i * G::NT + threadIdx.x;
+    const bool live = t0 + r < n;
+    const Pack<T, M::VW> cd = sm.dt[x], cg = sm.g[buf][x];
+    Pack<T, M::VW> cu, cz;
+    if (!SUM) cu = sm.u[buf][x];
+    if (gate) cz = sm.z[buf][x];
+#pragma unroll
+    for (int j = 0; j < M::VW; ++j) {
+      float slope = 0.f;
+      const float de = live ? step_size(cd.get(j) + bias[j], p.softplus, &slope) : 0.f;
+      float gy = cg.get(j);
+      if (gate) gy *= silu_f(cz.get(j));
+      const float du = SUM ? 0.f : de * cu.get(j);
+      sm.D[r][cc + j] = make_float2(de, du);
+      sm.Y[r][cc + j] = gy;
+      if (!SUM) sm.P[r][cc + j] = slope;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < G::QPT; ++i) {
+    const int e = (int)threadIdx.x + i * G::NT;
+    if (e < kS * LN) {
+      const Pack<T, 4> vc = sm.c[e];
+      const float4 c4 = make_float4(vc.get(0), vc.get(1), vc.get(2), vc.get(3));
+      float4 b4 = c4;
+      if (!SUM) {
+        const Pack<T, 4> vb = sm.b[e];
+        b4 = make_float4(vb.get(0), vb.get(1), vb.get(2), vb.get(3));
       }
-      group_sum<NV / 2, LN, M / 2>(v, lane);
-    } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], M);
-      group_sum<1, LN, M / 2>(v, lane);
+#pragma unroll
+      for (int k = 0; k < (SUM ? 1 : Order<LN>::COPIES); ++k) {
+        const int pair = Order<LN>::COPIES >= 4 ? k >> 1 : k;
+        const int elem = Order<LN>::COPIES >= 4 ? k & 1 : 0;
+        *reinterpret_cast<float4*>(sm.C[k] + 4 * e) = reorder(c4, pair, elem);
+        if (!SUM) *reinterpret_cast<float4*>(sm.B[k] + 4 * e) = reorder(b4, pair, elem);
+      }
     }
   }
 }
 
-// SUM: only the gradient that a run hands to the run before it, and the sum of
-// its step sizes.
+// A row's tensors.
+template <typename T> struct RowPtrs {
+  const T *u, *dt, *z, *g, *B, *C;
+  __device__ __forceinline__ RowPtrs(const SelBwdParams& bp, size_t rows) {
+    const SelParams& p = bp.f;
+    u = static_cast<const T*>(p.u) + rows * p.ld_u;
+    dt = static_cast<const T*>(p.dt) + rows * p.ld_dt;
+    z = p.z ? static_cast<const T*>(p.z) + rows * p.ld_z : nullptr;
+    g = static_cast<const T*>(bp.g) + rows * p.D;
+    B = static_cast<const T*>(p.Bm) + rows * p.ld_b;
+    C = static_cast<const T*>(p.Cm) + rows * p.ld_c;
+  }
+};
+
 template <typename T, int LN, bool SUM>
-__global__ void __launch_bounds__(Sel<LN>::NT) sel_bwd_kernel(const SelBwdParams bp) {
+__device__ __forceinline__ void bwd_fetch(BwdSmem<T, LN>& sm, const SelBwdParams& bp,
+                                          const RowPtrs<T>& r, int buf, int t0, int n, int c0) {
+  const SelParams& p = bp.f;
+  fetch_tile<T, LN>(sm.dt, r.dt, p.ld_dt, t0, n, c0, p.D, p.vec_d);
+  fetch_tile<T, LN>(sm.g[buf], r.g, p.D, t0, n, c0, p.D, bp.vec_g);
+  if (r.z) fetch_tile<T, LN>(sm.z[buf], r.z, p.ld_z, t0, n, c0, p.D, p.vec_d);
+  fetch_quads<T, LN>(sm.c, r.C, p.ld_c, t0, n, p.N, p.vec_n);
+  if (!SUM) {
+    fetch_tile<T, LN>(sm.u[buf], r.u, p.ld_u, t0, n, c0, p.D, p.vec_d);
+    fetch_quads<T, LN>(sm.b, r.B, p.ld_b, t0, n, p.N, p.vec_n);
+  }
+  copies_commit();
+}
+
+// Registers per thread: three CTAs per SM pay for N in 17..32 (1081 us against
+// 1214 us with the two that 255 registers allow, 256 rows x 64 steps x 1536
+// channels, N = 32, bf16), not for N <= 16 (306 us against 329 us, 2 x 4001 x
+// 1536, N = 16, fp32).
+template <int LN> constexpr int bwd_min_ctas() { return LN == 8 ? 3 : 1; }
+
+template <typename T, int LN>
+__global__ void __launch_bounds__(Sel<LN>::NT, bwd_min_ctas<LN>())
+sel_bwd_kernel(const SelBwdParams bp) {
   using G = Sel<LN>;
   using M = TileMap<T, LN>;
-  using Sm = BwdSmem<LN>;
+  using Sm = BwdSmem<T, LN>;
+  using O = Order<LN>;
   const SelParams& p = bp.f;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   Sm& sm = *reinterpret_cast<Sm*>(raw_smem);
   const int q = threadIdx.x % LN, grp = threadIdx.x / LN;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c0 = blockIdx.x * G::DT, c = c0 + 2 * grp, n0 = 4 * q;
-  const int split = SUM ? blockIdx.y % (p.splits - 1) + 1 : blockIdx.y % p.splits;
-  const int bg = SUM ? blockIdx.y / (p.splits - 1) : blockIdx.y / p.splits;
+  const int c0 = blockIdx.x * G::DT, n0 = 4 * q;
+  const int split = blockIdx.y % p.splits, bg = blockIdx.y / p.splits;
   const int ch0 = split * p.cps, ch1 = min(ch0 + p.cps, p.nch);
+  // the lane's order of its states, and of its channels (the upper half of a
+  // group's lanes takes the second channel first)
+  const int pr = O::pair(lane), el = O::elem(lane), up = (q & (LN / 2)) != 0;
+  const int cc2[2] = {2 * grp + up, 2 * grp + 1 - up};
+  const float* sB = sm.B[O::COPIES >= 4 ? 2 * pr + el : pr];
+  const float* sC = sm.C[O::COPIES >= 4 ? 2 * pr + el : pr];
 
   float2 a2[2][2], dA[2][2];
-  load_a2(a2, p.A, c, n0, p.D, p.N);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) dA[k][0] = dA[k][1] = make_float2(0.f, 0.f);
+  for (int k = 0; k < 2; ++k) {
+    const float4 v = load_quad_any(p.A, 0, c0 + cc2[k], n0, p.D, p.N);
+    set_pairs(a2[k], reorder(make_float4(v.x * kLog2e, v.y * kLog2e, v.z * kLog2e, v.w * kLog2e),
+                             pr, el));
+    dA[k][0] = dA[k][1] = make_float2(0.f, 0.f);
+  }
   // a thread's staged elements share their columns
   float bias[M::VW], dsk[M::VW], dD[M::VW], dbias[M::VW];
 #pragma unroll
@@ -100,196 +224,196 @@ __global__ void __launch_bounds__(Sel<LN>::NT) sel_bwd_kernel(const SelBwdParams
   for (size_t b = bg; b < (size_t)p.B; b += bp.bgroups) {
     const int n = sel_length(p.lengths, (int)b, p.L);
     const size_t rows = b * p.L;
-    const T* u = static_cast<const T*>(p.u) + rows * p.ld_u;
-    const T* dt = static_cast<const T*>(p.dt) + rows * p.ld_dt;
-    const T* z = p.z ? static_cast<const T*>(p.z) + rows * p.ld_z : nullptr;
-    const T* g = static_cast<const T*>(bp.g) + rows * p.D;
-    const T* Bm = static_cast<const T*>(p.Bm) + rows * p.ld_b;
-    const T* Cm = static_cast<const T*>(p.Cm) + rows * p.ld_c;
+    const RowPtrs<T> rp(bp, rows);
+    const bool gate = rp.z != nullptr;
     T* du = static_cast<T*>(bp.du) + rows * p.D;
     T* ddt = static_cast<T*>(bp.ddt) + rows * p.D;
-    T* dz = p.z ? static_cast<T*>(bp.dz) + rows * p.D : nullptr;
+    T* dz = gate ? static_cast<T*>(bp.dz) + rows * p.D : nullptr;
+    const bool vec = p.vec_d && bp.vec_g;
 
+    // chunks past the row's length: no gradient
+    int ch = ch1 - 1;
+    for (; ch >= ch0 && ch * kS >= n; --ch)
+#pragma unroll
+      for (int i = 0; i < M::NVEC; ++i) {
+        const auto zero = zero_pack<T, M::VW>();
+        store_tile<T, LN>(zero, i, du, p.D, ch * kS, p.L, c0, p.D, vec);
+        store_tile<T, LN>(zero, i, ddt, p.D, ch * kS, p.L, c0, p.D, vec);
+        if (dz) store_tile<T, LN>(zero, i, dz, p.D, ch * kS, p.L, c0, p.D, vec);
+      }
+    if (ch < ch0) continue;
+    bwd_fetch<T, LN, false>(sm, bp, rp, ch & 1, ch * kS, n, c0);
     float2 dh[2][2];
-    if (!SUM && bp.qin != nullptr && split + 1 < p.splits)
-      load_quads(dh, bp.qin, (size_t)split * p.B + b, c, q, p.D, G::NP);
-    else
 #pragma unroll
-      for (int k = 0; k < 2; ++k) dh[k][0] = dh[k][1] = make_float2(0.f, 0.f);
-    float dsum[2] = {0.f, 0.f};
+    for (int k = 0; k < 2; ++k) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (bp.qin != nullptr && split + 1 < p.splits)
+        v = load_quad_pad(bp.qin, (size_t)split * p.B + b, c0 + cc2[k], q, p.D, G::NP);
+      set_pairs(dh[k], reorder(v, pr, el));
+    }
 
-    for (int ch = ch1 - 1; ch >= ch0; --ch) {
-      const int t0 = ch * kS;
-      if (t0 >= n) {   // past the row's length: no gradient
-        if (!SUM)
-#pragma unroll
-          for (int i = 0; i < M::NVEC; ++i) {
-            const auto zero = zero_pack<T, M::VW>();
-            store_tile<T, LN>(zero, i, du, p.D, t0, p.L, c0, p.D, p.vec_d && bp.vec_g);
-            store_tile<T, LN>(zero, i, ddt, p.D, t0, p.L, c0, p.D, p.vec_d && bp.vec_g);
-            if (dz) store_tile<T, LN>(zero, i, dz, p.D, t0, p.L, c0, p.D, p.vec_d && bp.vec_g);
-          }
-        continue;
-      }
-      Pack<T, M::VW> ru[M::NVEC], rg[M::NVEC], rz[M::NVEC];
-      {
-        Pack<T, M::VW> rd[M::NVEC];
-        Pack<T, 4> nb[G::QPT], nc[G::QPT];
-        load_tile<T, LN>(rd, dt, p.ld_dt, t0, n, c0, p.D, p.vec_d);
-        load_tile<T, LN>(rg, g, p.D, t0, n, c0, p.D, bp.vec_g);
-        if (z) load_tile<T, LN>(rz, z, p.ld_z, t0, n, c0, p.D, p.vec_d);
-        load_quad_rows<T, LN>(nc, Cm, p.ld_c, t0, n, p.N, p.vec_n);
-        if (!SUM) {
-          load_tile<T, LN>(ru, u, p.ld_u, t0, n, c0, p.D, p.vec_d);
-          load_quad_rows<T, LN>(nb, Bm, p.ld_b, t0, n, p.N, p.vec_n);
-        }
-#pragma unroll
-        for (int i = 0; i < M::NVEC; ++i) {
-          const int r = M::row(i), cc = M::col(i);
-          const bool live = t0 + r < n;
-#pragma unroll
-          for (int j = 0; j < M::VW; ++j) {
-            const float de = live ? step_size(rd[i].get(j) + bias[j], p.softplus) : 0.f;
-            float gy = rg[i].get(j);
-            if (z) gy *= silu_f(rz[i].get(j));
-            sm.D[r][cc + j] = make_float4(de, SUM ? 0.f : de * ru[i].get(j), gy, 0.f);
-          }
-        }
-        put_quad_rows<T, LN>(nc, sm.C);
-        if (!SUM) put_quad_rows<T, LN>(nb, sm.B);
-      }
-      __syncthreads();
-      if (SUM) {
-#pragma unroll 4
-        for (int t = kS - 1; t >= 0; --t) {
-          const float4 cc = *reinterpret_cast<const float4*>(sm.C + t * G::NP + n0);
-          const float2 c2[2] = {make_float2(cc.x, cc.y), make_float2(cc.z, cc.w)};
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float4 dd = sm.D[t][2 * grp + k];
-            dsum[k] += dd.x;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              dh[k][j] = __fmul2_rn(ex2_pair(__fmul2_rn(f2(dd.x), a2[k][j])),
-                                    __ffma2_rn(f2(dd.z), c2[j], dh[k][j]));
-          }
-        }
-        __syncthreads();
-        continue;
-      }
-      // states at every group's start
+    for (; ch >= ch0; --ch) {
+      const int t0 = ch * kS, buf = ch & 1;
+      // the state before the chunk
       float2 h[2][2];
-      if (ch > 0) load_quads(h, p.ckpt, b * (p.nch - 1) + ch - 1, c, q, p.D, G::NP);
-      else load_state(h, p.h0, b, c, n0, p.D, p.N);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        set_pairs(h[k], ch > 0 ? load_quad_pad(p.ckpt, b * (p.nch - 1) + ch - 1, c0 + cc2[k], q,
+                                               p.D, G::NP)
+                               : load_quad_any(p.h0, b, c0 + cc2[k], n0, p.D, p.N));
+      copies_wait();
+      bwd_stage<T, LN, false>(sm, p, buf, t0, n, gate, bias);
+      __syncthreads();
+      if (ch > ch0) bwd_fetch<T, LN, false>(sm, bp, rp, buf ^ 1, t0 - kS, n, c0);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) set_pairs(h[k], reorder(quad_of(h[k]), pr, el));
+      // states at every group's start
 #pragma unroll 1
       for (int sub = 0; sub < kNSub; ++sub) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          sm.H[sub][k][threadIdx.x] = make_float4(h[k][0].x, h[k][0].y, h[k][1].x, h[k][1].y);
+        for (int k = 0; k < 2; ++k) sm.H[sub][k][threadIdx.x] = quad_of(h[k]);
         if (sub == kNSub - 1) break;
 #pragma unroll
         for (int s = 0; s < kSub; ++s) {
           const int t = sub * kSub + s;
-          const float4 bb = *reinterpret_cast<const float4*>(sm.B + t * G::NP + n0);
-          const float2 b2[2] = {make_float2(bb.x, bb.y), make_float2(bb.z, bb.w)};
+          float2 b2[2];
+          set_pairs(b2, *reinterpret_cast<const float4*>(sB + t * G::NP + n0));
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float2 dd = *reinterpret_cast<const float2*>(&sm.D[t][2 * grp + k]);
+            const float2 dd = sm.D[t][cc2[k]];
+            const float2 de = f2(dd.x), deu = f2(dd.y);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-              h[k][j] = __ffma2_rn(ex2_pair(__fmul2_rn(f2(dd.x), a2[k][j])), h[k][j],
-                                   __fmul2_rn(f2(dd.y), b2[j]));
+              h[k][j] = __ffma2_rn(ex2_pair(__fmul2_rn(de, a2[k][j])), h[k][j],
+                                   __fmul2_rn(deu, b2[j]));
           }
         }
       }
 #pragma unroll 1
       for (int sub = kNSub - 1; sub >= 0; --sub) {
         float2 ga[kSub][2][2], gh[kSub][2][2];   // gate, gate * state before
-        float ys[2 * kSub], ss[4 * kSub];
+        float sy[kSub], s1[kSub], s2[kSub];      // of the lane's first channel
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float4 v = sm.H[sub][k][threadIdx.x];
-          h[k][0] = make_float2(v.x, v.y);
-          h[k][1] = make_float2(v.z, v.w);
-        }
+        for (int k = 0; k < 2; ++k) set_pairs(h[k], sm.H[sub][k][threadIdx.x]);
 #pragma unroll
         for (int s = 0; s < kSub; ++s) {
           const int t = sub * kSub + s;
-          const float4 bb = *reinterpret_cast<const float4*>(sm.B + t * G::NP + n0);
-          const float4 cc = *reinterpret_cast<const float4*>(sm.C + t * G::NP + n0);
-          const float2 b2[2] = {make_float2(bb.x, bb.y), make_float2(bb.z, bb.w)};
-          const float2 c2[2] = {make_float2(cc.x, cc.y), make_float2(cc.z, cc.w)};
+          float2 b2[2], c2[2];
+          set_pairs(b2, *reinterpret_cast<const float4*>(sB + t * G::NP + n0));
+          set_pairs(c2, *reinterpret_cast<const float4*>(sC + t * G::NP + n0));
+          float ys[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float2 dd = *reinterpret_cast<const float2*>(&sm.D[t][2 * grp + k]);
+            const float2 dd = sm.D[t][cc2[k]];
+            const float2 de = f2(dd.x), deu = f2(dd.y);
             float2 y2;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              ga[s][k][j] = ex2_pair(__fmul2_rn(f2(dd.x), a2[k][j]));
+              ga[s][k][j] = ex2_pair(__fmul2_rn(de, a2[k][j]));
               gh[s][k][j] = __fmul2_rn(ga[s][k][j], h[k][j]);
-              h[k][j] = __ffma2_rn(f2(dd.y), b2[j], gh[s][k][j]);
+              h[k][j] = __ffma2_rn(deu, b2[j], gh[s][k][j]);
               y2 = j ? __ffma2_rn(h[k][j], c2[j], y2) : __fmul2_rn(h[k][j], c2[j]);
             }
-            ys[2 * s + k] = y2.x + y2.y;
+            ys[k] = y2.x + y2.y;
           }
+          // the lane keeps its first channel, its partner the other one
+          sy[s] = ys[0] + __shfl_xor_sync(0xffffffffu, ys[1], LN / 2);
         }
 #pragma unroll
         for (int s = kSub - 1; s >= 0; --s) {
           const int t = sub * kSub + s;
-          const float4 bb = *reinterpret_cast<const float4*>(sm.B + t * G::NP + n0);
-          const float4 cc = *reinterpret_cast<const float4*>(sm.C + t * G::NP + n0);
-          const float2 b2[2] = {make_float2(bb.x, bb.y), make_float2(bb.z, bb.w)};
-          const float2 c2[2] = {make_float2(cc.x, cc.y), make_float2(cc.z, cc.w)};
+          float2 b2[2], c2[2];
+          set_pairs(b2, *reinterpret_cast<const float4*>(sB + t * G::NP + n0));
+          set_pairs(c2, *reinterpret_cast<const float4*>(sC + t * G::NP + n0));
           float2 vb[2], vc[2];
+          float x1[2], x2[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float4 dd = sm.D[t][2 * grp + k];
-            const float2 de = f2(dd.x), deu = f2(dd.y), gy = f2(dd.z);
-            float2 x1, x2;
+            const float2 dd = sm.D[t][cc2[k]];
+            const float2 de = f2(dd.x), deu = f2(dd.y);
+            const float2 gy = f2(sm.Y[t][cc2[k]]);
+            float2 y1, y2;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const float2 ht = __ffma2_rn(deu, b2[j], gh[s][k][j]);
               dh[k][j] = __ffma2_rn(gy, c2[j], dh[k][j]);
               vc[j] = k ? __ffma2_rn(gy, ht, vc[j]) : __fmul2_rn(gy, ht);
               vb[j] = k ? __ffma2_rn(deu, dh[k][j], vb[j]) : __fmul2_rn(deu, dh[k][j]);
-              x1 = j ? __ffma2_rn(dh[k][j], b2[j], x1) : __fmul2_rn(dh[k][j], b2[j]);
+              y1 = j ? __ffma2_rn(dh[k][j], b2[j], y1) : __fmul2_rn(dh[k][j], b2[j]);
               const float2 w = __fmul2_rn(dh[k][j], gh[s][k][j]);
-              x2 = j ? __ffma2_rn(w, a2[k][j], x2) : __fmul2_rn(w, a2[k][j]);
+              y2 = j ? __ffma2_rn(w, a2[k][j], y2) : __fmul2_rn(w, a2[k][j]);
               dA[k][j] = __ffma2_rn(w, de, dA[k][j]);
               dh[k][j] = __fmul2_rn(dh[k][j], ga[s][k][j]);
             }
-            ss[4 * s + 2 * k] = x1.x + x1.y;
-            ss[4 * s + 2 * k + 1] = x2.x + x2.y;
+            x1[k] = y1.x + y1.y;
+            x2[k] = y2.x + y2.y;
           }
-          float v[8] = {vb[0].x, vb[0].y, vb[1].x, vb[1].y, vc[0].x, vc[0].y, vc[1].x, vc[1].y};
-          group_sum<8, LN>(v, lane);
-          constexpr int KEEP = LN >= 32 ? 8 : LN == 16 ? 4 : LN == 8 ? 2 : 1;
-          const int v0 = LN == 2 ? lane / 4 : lane / LN * KEEP;
+          s1[s] = x1[0] + __shfl_xor_sync(0xffffffffu, x1[1], LN / 2);
+          s2[s] = x2[0] + __shfl_xor_sync(0xffffffffu, x2[1], LN / 2);
+          // sums over the warp's lane groups
           float* bc = sm.BC[sub & 1][s][warp];
-          if (LN != 2 || (lane & 2) == 0)
+          if constexpr (O::GROUPS == 1) {
 #pragma unroll
-            for (int i = 0; i < KEEP; ++i)
-              bc[(v0 + i) / 4 * G::NP + n0 + (v0 + i) % 4] = v[i];
-        }
-        // channel sums over the lane group: total (step, channel, s1 | s2)
-        lane_sum<4 * kSub, LN>(ss, q);
-        constexpr int K1 = 4 * kSub >= LN ? 4 * kSub / LN : 1;
-        constexpr int P1 = 4 * kSub >= LN ? 1 : LN / (4 * kSub);
-        if (q % P1 == 0)
-#pragma unroll
-          for (int i = 0; i < K1; ++i) {
-            const int x = q / P1 * K1 + i;
-            sm.R[sub * kSub + x / 4][x & 1][2 * grp + (x >> 1 & 1)] = ss[i];
+            for (int j = 0; j < 2; ++j) {
+              *reinterpret_cast<float2*>(bc + n0 + 2 * j) = vb[j];
+              *reinterpret_cast<float2*>(bc + G::NP + n0 + 2 * j) = vc[j];
+            }
+          } else {
+            float2 pb = __fadd2_rn(vb[0], shfl_pair(vb[1], 16));
+            float2 pc = __fadd2_rn(vc[0], shfl_pair(vc[1], 16));
+            if constexpr (O::GROUPS == 2) {
+              *reinterpret_cast<float2*>(bc + n0 + 2 * pr) = pb;
+              *reinterpret_cast<float2*>(bc + G::NP + n0 + 2 * pr) = pc;
+            } else {
+              float eb = pb.x + __shfl_xor_sync(0xffffffffu, pb.y, 8);
+              float ec = pc.x + __shfl_xor_sync(0xffffffffu, pc.y, 8);
+              const int at = n0 + 2 * pr + el;
+              if constexpr (O::GROUPS == 4) {
+                bc[at] = eb;
+                bc[G::NP + at] = ec;
+              } else {   // dB to the lanes without bit 2, dC to the others
+                const bool hi = (lane & 4) != 0;
+                float v = (hi ? ec : eb) + __shfl_xor_sync(0xffffffffu, hi ? eb : ec, 4);
+                if constexpr (O::GROUPS == 16) v += __shfl_xor_sync(0xffffffffu, v, 2);
+                if (O::GROUPS < 16 || (lane & 2) == 0) bc[(hi ? G::NP : 0) + at] = v;
+              }
+            }
           }
-        if (z) {
-          lane_sum<2 * kSub, LN>(ys, q);
-          constexpr int K2 = 2 * kSub >= LN ? 2 * kSub / LN : 1;
-          constexpr int P2 = 2 * kSub >= LN ? 1 : LN / (2 * kSub);
-          if (q % P2 == 0)
+        }
+        // channel sums over the group's remaining lanes: halves of the steps
+        constexpr int M1 = LN / 4, M2 = LN / 8;
+        if constexpr (M1 >= 1) {
+          const bool hi = (q & M1) != 0;
 #pragma unroll
-            for (int i = 0; i < K2; ++i) {
-              const int x = q / P2 * K2 + i;
-              sm.R[sub * kSub + x / 2][2][2 * grp + (x & 1)] = ys[i];
+          for (int s = 0; s < 2; ++s) {
+            s1[s] = (hi ? s1[s + 2] : s1[s]) + __shfl_xor_sync(0xffffffffu, hi ? s1[s] : s1[s + 2], M1);
+            s2[s] = (hi ? s2[s + 2] : s2[s]) + __shfl_xor_sync(0xffffffffu, hi ? s2[s] : s2[s + 2], M1);
+            sy[s] = (hi ? sy[s + 2] : sy[s]) + __shfl_xor_sync(0xffffffffu, hi ? sy[s] : sy[s + 2], M1);
+          }
+        }
+        if constexpr (M2 >= 1) {
+          const bool hi = (q & M2) != 0;
+          s1[0] = (hi ? s1[1] : s1[0]) + __shfl_xor_sync(0xffffffffu, hi ? s1[0] : s1[1], M2);
+          s2[0] = (hi ? s2[1] : s2[0]) + __shfl_xor_sync(0xffffffffu, hi ? s2[0] : s2[1], M2);
+          sy[0] = (hi ? sy[1] : sy[0]) + __shfl_xor_sync(0xffffffffu, hi ? sy[0] : sy[1], M2);
+#pragma unroll
+          for (int m = M2 / 2; m >= 1; m >>= 1) {
+            s1[0] += __shfl_xor_sync(0xffffffffu, s1[0], m);
+            s2[0] += __shfl_xor_sync(0xffffffffu, s2[0], m);
+            sy[0] += __shfl_xor_sync(0xffffffffu, sy[0], m);
+          }
+        }
+        {
+          constexpr int KEEP = M2 >= 1 ? 1 : M1 >= 1 ? 2 : 4;   // steps per lane
+          const int s0 = M2 >= 1 ? (q & M1 ? 2 : 0) + (q & M2 ? 1 : 0)
+                                 : M1 >= 1 ? (q & M1 ? 2 : 0) : 0;
+          if (M2 <= 1 || (q & (M2 - 1)) == 0)
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i) {
+              float (*o)[G::DT] = sm.R[sub * kSub + s0 + i];
+              o[0][cc2[0]] = s1[i];
+              o[1][cc2[0]] = s2[i];
+              o[2][cc2[0]] = sy[i];
             }
         }
         __syncthreads();
@@ -305,47 +429,45 @@ __global__ void __launch_bounds__(Sel<LN>::NT) sel_bwd_kernel(const SelBwdParams
       // the last group's barrier is behind every write of sm.R
 #pragma unroll
       for (int i = 0; i < M::NVEC; ++i) {
-        const int r = M::row(i), cc = M::col(i);
-        Pack<T, M::VW> odu, oddt, odz;
+        const int r = M::row(i), cc = M::col(i), x = i * G::NT + threadIdx.x;
+        const Pack<T, M::VW> cu = sm.u[buf][x], cg = sm.g[buf][x];
+        Pack<T, M::VW> cz, odu, oddt, odz;
+        if (gate) cz = sm.z[buf][x];
 #pragma unroll
         for (int j = 0; j < M::VW; ++j) {
-          const float4 dd = sm.D[r][cc + j];
-          const float s1 = sm.R[r][0][cc + j], s2 = sm.R[r][1][cc + j] * kLn2;
-          const float uu = ru[i].get(j);
-          odu.put(j, fmaf(dsk[j], dd.z, dd.x * s1));
-          float d = fmaf(uu, s1, s2);
-          if (p.softplus) d *= -expm1f(-dd.x);
+          const float gy = sm.Y[r][cc + j];
+          const float v1 = sm.R[r][0][cc + j], v2 = sm.R[r][1][cc + j] * kLn2;
+          const float uu = cu.get(j);
+          odu.put(j, fmaf(dsk[j], gy, sm.D[r][cc + j].x * v1));
+          const float d = fmaf(uu, v1, v2) * sm.P[r][cc + j];
           oddt.put(j, d);
-          dD[j] = fmaf(dd.z, uu, dD[j]);
+          dD[j] = fmaf(gy, uu, dD[j]);
           dbias[j] += d;
-          if (z) {
-            const float zz = rz[i].get(j), yp = fmaf(dsk[j], uu, sm.R[r][2][cc + j]);
-            odz.put(j, rg[i].get(j) * yp * dsilu_f(zz, sigmoid_f(zz)));
+          if (gate) {
+            const float zz = cz.get(j), yp = fmaf(dsk[j], uu, sm.R[r][2][cc + j]);
+            odz.put(j, cg.get(j) * yp * dsilu_f(zz, sigmoid_f(zz)));
           }
         }
-        const bool vec = p.vec_d && bp.vec_g;
         store_tile<T, LN>(odu, i, du, p.D, t0, p.L, c0, p.D, vec);
         store_tile<T, LN>(oddt, i, ddt, p.D, t0, p.L, c0, p.D, vec);
         if (dz) store_tile<T, LN>(odz, i, dz, p.D, t0, p.L, c0, p.D, vec);
       }
       __syncthreads();   // sm.D and sm.R are written again
     }
-    if (SUM) {
-      const size_t row = (size_t)split * p.B + b;
-      store_quads(dh, bp.qsum, row, c, q, p.D, G::NP);
-      if (q < 2 && c + q < p.D) p.dsum[row * p.D + c + q] = dsum[q];
-    }
   }
-  if (SUM) return;
   // partials over this CTA's rows: dA, then dD and dbias of each channel
   constexpr int PW = G::NP + 2;
   float* part = bp.part_a + (size_t)blockIdx.y * p.D * PW;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    if (c + k < p.D) {
-      float* o = part + (size_t)(c + k) * PW + n0;
-      *reinterpret_cast<float2*>(o) = dA[k][0];
-      *reinterpret_cast<float2*>(o + 2) = dA[k][1];
+    if (c0 + cc2[k] < p.D) {
+      float* o = part + (size_t)(c0 + cc2[k]) * PW + n0;
+      // the inverse order: members first, then pairs
+      float4 v = quad_of(dA[k]);
+      if (el) v = make_float4(v.y, v.x, v.w, v.z);
+      if (pr) v = make_float4(v.z, v.w, v.x, v.y);
+      *reinterpret_cast<float2*>(o) = make_float2(v.x, v.y);
+      *reinterpret_cast<float2*>(o + 2) = make_float2(v.z, v.w);
     }
   // threads with the same columns add in order
   constexpr int RPT = G::NT / M::PER_ROW;
@@ -364,6 +486,65 @@ __global__ void __launch_bounds__(Sel<LN>::NT) sel_bwd_kernel(const SelBwdParams
     for (int i = 0; i < RPT; ++i) v += red[(i * 2 + which) * G::DT + x];
     if (c0 + x < p.D) part[(size_t)(c0 + x) * PW + G::NP + which] = v;
   }
+}
+
+// What a run hands to the run before it (the gradient of the state it starts
+// from, as if nothing came after it), and the sum of its step sizes.
+template <typename T, int LN>
+__global__ void __launch_bounds__(Sel<LN>::NT) sel_bwd_sum_kernel(const SelBwdParams bp) {
+  using G = Sel<LN>;
+  using M = TileMap<T, LN>;
+  using Sm = BwdSmem<T, LN>;
+  const SelParams& p = bp.f;
+  extern __shared__ __align__(16) unsigned char raw_smem[];
+  Sm& sm = *reinterpret_cast<Sm*>(raw_smem);
+  const int q = threadIdx.x % LN, grp = threadIdx.x / LN;
+  const int tiles = (p.D + G::DT - 1) / G::DT;
+  const int c0 = blockIdx.x % tiles * G::DT, c = c0 + 2 * grp, n0 = 4 * q;
+  const size_t b = blockIdx.x / tiles;
+  const int split = blockIdx.y + 1;
+  const int ch0 = split * p.cps, ch1 = min(ch0 + p.cps, p.nch);
+  const int n = sel_length(p.lengths, (int)b, p.L);
+  const RowPtrs<T> rp(bp, b * p.L);
+  const bool gate = rp.z != nullptr;
+  int ch = min(ch1, (n + kS - 1) / kS) - 1;
+  if (ch >= ch0) bwd_fetch<T, LN, true>(sm, bp, rp, ch & 1, ch * kS, n, c0);
+  float2 a2[2][2], dh[2][2];
+  load_a2(a2, p.A, c, n0, p.D, p.N);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) dh[k][0] = dh[k][1] = make_float2(0.f, 0.f);
+  float bias[M::VW], dsum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < M::VW; ++j) {
+    const int cc = c0 + M::col(0) + j;
+    bias[j] = (p.dt_bias && cc < p.D) ? p.dt_bias[cc] : 0.f;
+  }
+  for (; ch >= ch0; --ch) {
+    const int t0 = ch * kS;
+    copies_wait();
+    bwd_stage<T, LN, true>(sm, p, ch & 1, t0, n, gate, bias);
+    __syncthreads();
+    if (ch > ch0) bwd_fetch<T, LN, true>(sm, bp, rp, (ch & 1) ^ 1, t0 - kS, n, c0);
+#pragma unroll 4
+    for (int t = kS - 1; t >= 0; --t) {
+      float2 c2[2];
+      set_pairs(c2, *reinterpret_cast<const float4*>(sm.C[0] + t * G::NP + n0));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 de = f2(sm.D[t][2 * grp + k].x);
+        const float2 gy = f2(sm.Y[t][2 * grp + k]);
+        dsum[k] += de.x;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          dh[k][j] = __fmul2_rn(ex2_pair(__fmul2_rn(de, a2[k][j])),
+                                __ffma2_rn(gy, c2[j], dh[k][j]));
+      }
+    }
+    __syncthreads();
+  }
+  const size_t row = (size_t)split * p.B + b;
+  store_quads(dh, bp.qsum, row, c, q, p.D, G::NP);
+  if (q < 2 && c + q < p.D) p.dsum[row * p.D + c + q] = q ? dsum[1] : dsum[0];
 }
 
 // The state's gradient at every run's end, joined from the back.
@@ -440,15 +621,15 @@ template <typename T, int LN>
 cudaError_t bwd_typed(const SelBwdParams& p, cudaStream_t s) {
   using G = Sel<LN>;
   const unsigned tiles = (unsigned)((p.f.D + G::DT - 1) / G::DT);
-  constexpr int smem = (int)sizeof(BwdSmem<LN>);
-  auto* main = sel_bwd_kernel<T, LN, false>;
+  constexpr int smem = (int)sizeof(BwdSmem<T, LN>);
+  auto* main = sel_bwd_kernel<T, LN>;
   cudaError_t e = cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   if (p.f.splits > 1) {
-    auto* sum = sel_bwd_kernel<T, LN, true>;
+    auto* sum = sel_bwd_sum_kernel<T, LN>;
     e = cudaFuncSetAttribute(sum, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    sum<<<dim3(tiles, (p.f.splits - 1) * p.bgroups), G::NT, smem, s>>>(p);
+    sum<<<dim3(tiles * p.f.B, p.f.splits - 1), G::NT, smem, s>>>(p);
     const long long total = (long long)p.f.B * p.f.D * G::NP;
     sel_join_bwd_kernel<<<(unsigned)((total + 127) / 128), 128, 0, s>>>(p, G::NP);
   }
@@ -471,7 +652,36 @@ cudaError_t bwd_lanes(const SelBwdParams& p, cudaStream_t s) {
   }
 }
 
+template <typename T, int LN>
+int resident() {
+  constexpr int smem = (int)sizeof(BwdSmem<T, LN>);
+  auto* kern = sel_bwd_kernel<T, LN>;
+  int n = 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+          cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, Sel<LN>::NT, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
+template <typename T>
+int resident_lanes(int N) {
+  switch (sel_lanes(N)) {
+    case 2: return resident<T, 2>();
+    case 4: return resident<T, 4>();
+    case 8: return resident<T, 8>();
+    case 16: return resident<T, 16>();
+    default: return resident<T, 32>();
+  }
+}
+
 }  // namespace
+
+int sel_bwd_resident(int N, int dtype) {
+  return dtype == M3_BF16 ? resident_lanes<__nv_bfloat16>(N) : resident_lanes<float>(N);
+}
 
 cudaError_t launch_sel_bwd(const SelBwdParams& p, cudaStream_t s) {
   return p.f.dtype == M3_BF16 ? bwd_lanes<__nv_bfloat16>(p, s) : bwd_lanes<float>(p, s);

@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(128) sel_step_kernel(const SelStepParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (n0 + j < p.N) {
-            bv.v[j] = pb[j];
-            cv.v[j] = pc[j];
+            bv.load_one(j, pb);
+            cv.load_one(j, pc);
           }
       }
     }

@@ -18,12 +18,64 @@ template <> struct Elem<__nv_bfloat16> {
 };
 
 // V consecutive elements held as loaded (V * sizeof(T) = 2, 4, 8, 16 or 32
-// bytes; the address must be aligned to min(that, 16)).
-template <typename T, int V>
-struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Pack {
-  T v[V];
-  __device__ __forceinline__ float get(int i) const { return Elem<T>::get(v[i]); }
-  __device__ __forceinline__ void put(int i, float x) { v[i] = Elem<T>::put(x); }
+// bytes; the address must be aligned to min(that, 16)).  bf16 pairs stay in
+// 32-bit words until they are read: an array of 16-bit values would be taken
+// apart where it is loaded, and a load made ahead of its use would be waited for
+// there (the selective scan's bf16 forward ran at half the speed that way).
+// Elements are put in ascending order.
+template <typename T, int V> struct Pack;
+
+template <int V>
+struct alignas(V * 4 < 16 ? V * 4 : 16) Pack<float, V> {
+  float v[V];
+  __device__ __forceinline__ float get(int i) const { return v[i]; }
+  __device__ __forceinline__ void put(int i, float x) { v[i] = x; }
+  __device__ __forceinline__ void load_one(int i, const float* p) { v[i] = p[i]; }
+  __device__ __forceinline__ void store_one(int i, float* p) const { p[i] = v[i]; }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.f;
+  }
+};
+
+template <int V>
+struct alignas(V * 2 < 16 ? V * 2 : 16) Pack<__nv_bfloat16, V> {
+  unsigned w[V / 2];
+  __device__ __forceinline__ float get(int i) const {
+    return __uint_as_float((i & 1) ? (w[i / 2] & 0xffff0000u) : (w[i / 2] << 16));
+  }
+  __device__ __forceinline__ void put(int i, float x) {
+    const unsigned b = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+    w[i / 2] = (i & 1) ? (w[i / 2] | b << 16) : b;
+  }
+  __device__ __forceinline__ void load_one(int i, const __nv_bfloat16* p) {
+    const unsigned b = reinterpret_cast<const unsigned short*>(p)[i];
+    w[i / 2] = (i & 1) ? ((w[i / 2] & 0xffffu) | b << 16) : ((w[i / 2] & 0xffff0000u) | b);
+  }
+  __device__ __forceinline__ void store_one(int i, __nv_bfloat16* p) const {
+    reinterpret_cast<unsigned short*>(p)[i] =
+        (unsigned short)((i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) w[i] = 0u;
+  }
+};
+
+template <>
+struct Pack<__nv_bfloat16, 1> {
+  unsigned short w;
+  __device__ __forceinline__ float get(int) const { return __uint_as_float((unsigned)w << 16); }
+  __device__ __forceinline__ void put(int, float x) {
+    w = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+  }
+  __device__ __forceinline__ void load_one(int, const __nv_bfloat16* p) {
+    w = *reinterpret_cast<const unsigned short*>(p);
+  }
+  __device__ __forceinline__ void store_one(int, __nv_bfloat16* p) const {
+    *reinterpret_cast<unsigned short*>(p) = w;
+  }
+  __device__ __forceinline__ void zero() { w = 0; }
 };
 
 template <typename T, int V>
@@ -39,8 +91,7 @@ __device__ __forceinline__ void st_pack(T* p, const Pack<T, V>& x) {
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> zero_pack() {
   Pack<T, V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = Elem<T>::put(0.f);
+  r.zero();
   return r;
 }
 
