@@ -382,8 +382,8 @@ int m3_sample(const m3_sample_desc* desc, const void* logits, int64_t ld, const 
   p.min_p0 = desc->min_p;
   p.out = reinterpret_cast<long long*>(out);
   p.rows = desc->rows; p.V = desc->vocab; p.dtype = desc->dtype;
-  p.shift = 62;   // the weights of a row add up to at most 2^62
-  while ((1 << (62 - p.shift)) < desc->vocab) --p.shift;
+  p.shift = 50;   // the weights of a row add up to at most 2^62
+  while (p.shift > 62 - 31 && (1LL << (62 - p.shift)) < desc->vocab) --p.shift;
   p.sms = device_sms();
   return status(launch_sample(p, static_cast<cudaStream_t>(stream)));
 }

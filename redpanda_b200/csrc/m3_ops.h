@@ -154,6 +154,7 @@ struct SampleParams {
   int rows, V, dtype;
   int shift;                                             // weights in units of 2^-shift
   int sms;
+  int vec;                                               // 16-byte loads, set by the launcher
 };
 cudaError_t launch_sample(const SampleParams& p, cudaStream_t s);
 

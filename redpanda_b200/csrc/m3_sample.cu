@@ -15,12 +15,19 @@
 // 2^63).  Integer addition is associative, so shared-memory atomics and any
 // thread order give the same sums, and results do not depend on scheduling.
 //
-// One CTA per row.  A prefix of the order (top-k: count k; top-p: weight) ends
-// in a bin of a 2048-bin histogram over (max - x) / T, 64 bins per unit: one
-// pass over the row.  Only that bin's few members are looked at again, by
-// 8-bit digits of the ordered key, down to one value and the number of its ties
-// to keep.  The row stays in shared memory when it fits (read once from HBM);
-// longer rows are read again from L2.
+// One CTA per row, which stays in shared memory when it fits (read once from
+// HBM; longer rows are read again from L2).  The bound is the double-precision
+// exponential of every token whose weight counts, so as few as possible are
+// evaluated:
+//  - temperature 0 and k = 1 need the maximum only;
+//  - up to kList tokens in play (few candidates, or a top-k whose histogram of
+//    2048 bins over (max - x) / T, 64 per unit, ends early): they are gathered,
+//    one per thread, ranked by comparing all pairs, and everything else happens
+//    among them;
+//  - otherwise a top-k or top-p prefix ends in one bin of that histogram (of
+//    counts, or of weights); the bin's members are gathered and ranked.  A bin
+//    with more than kList members (ties) is cut down by 8-bit digits of the
+//    ordered key.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -37,6 +44,7 @@ typedef unsigned long long u64;
 constexpr int kBins = 2048;
 constexpr float kBinsPerUnit = 64.f;
 constexpr int kCacheMax = 32768;   // floats of a row kept in shared memory
+constexpr int kList = 256;         // tokens ranked by comparing all pairs
 
 // A key whose unsigned order is x descending.
 __device__ __forceinline__ unsigned desc_key(float x) {
@@ -45,16 +53,32 @@ __device__ __forceinline__ unsigned desc_key(float x) {
 }
 
 struct Shared {
-  u64 mass[kBins];
-  unsigned count[kBins];
+  unsigned count[kBins];           // counts, or the low words of the weights
+  unsigned high[kBins];            // the high words
   u64 wsum[33];
+  double pow2[32];                 // 2^(j/32)
+  u64 lw[kList], sw[kList];
+  float lx[kList];
+  int li[kList];
+  int ln;
   u64 found_base;
-  u64 found_mass;
   int found;
   float fmax;
   int imax;
   unsigned n;
+  float wm[32];
+  int wi[32];
 };
+
+// Adds to a 64-bit counter kept as two words.
+__device__ __forceinline__ void add64(Shared& sh, int i, u64 w) {
+  const unsigned lo = (unsigned)w, old = atomicAdd(&sh.count[i], lo);
+  const unsigned hi = (unsigned)(w >> 32) + (old + lo < old ? 1u : 0u);
+  if (hi) atomicAdd(&sh.high[i], hi);
+}
+__device__ __forceinline__ u64 get_bin(const Shared& sh, bool mass, int i) {
+  return mass ? ((u64)sh.high[i] << 32 | sh.count[i]) : (u64)sh.count[i];
+}
 
 // Exclusive prefix of v over the CTA's threads; *total gets the sum.
 template <int NT>
@@ -86,12 +110,12 @@ __device__ void find_bin(Shared& sh, bool mass, int nbins, u64 thr) {
   const int i0 = threadIdx.x * per;
   u64 s = 0;
   if (i0 < nbins)
-    for (int i = 0; i < per; ++i) s += mass ? sh.mass[i0 + i] : (u64)sh.count[i0 + i];
+    for (int i = 0; i < per; ++i) s += get_bin(sh, mass, i0 + i);
   u64 total;
   u64 base = block_prefix<NT>(s, sh.wsum, &total);
   if (i0 < nbins && base < thr && base + s >= thr) {
     for (int i = 0; i < per; ++i) {
-      const u64 v = mass ? sh.mass[i0 + i] : (u64)sh.count[i0 + i];
+      const u64 v = get_bin(sh, mass, i0 + i);
       if (base + v >= thr) {
         sh.found = i0 + i;
         sh.found_base = base;
@@ -113,12 +137,15 @@ struct Cut {
   }
 };
 
-template <typename T, int NT, bool CACHE>
+// The row: cached floats, or the logits themselves (NaN as -infinity).
+template <typename T, bool CACHE>
 struct RowReader {
   const T* g;
   const float* s;
   __device__ __forceinline__ float at(int i) const {
-    return CACHE ? s[i] : Elem<T>::get(g[i]);
+    if (CACHE) return s[i];
+    const float v = Elem<T>::get(g[i]);
+    return v > -CUDART_INF_F ? v : -CUDART_INF_F;
   }
 };
 
@@ -126,23 +153,48 @@ template <typename T, int NT, bool CACHE>
 __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
-  float* cache = reinterpret_cast<float*>(raw + sizeof(Shared));
+  float* cache = reinterpret_cast<float*>(raw + (sizeof(Shared) + 15) / 16 * 16);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t row = blockIdx.x;
   const int V = p.V;
   const T* g = static_cast<const T*>(p.logits) + row * p.ld;
-  const RowReader<T, NT, CACHE> x{g, cache};
+  const RowReader<T, CACHE> x{g, cache};
 
   // ---- maximum (lowest index first) and candidates
   float m = -CUDART_INF_F;
   int im = 0x7fffffff;
   unsigned cand = 0;
-  for (int i = tid; i < V; i += NT) {
-    float v = Elem<T>::get(g[i]);
-    if (!(v > -CUDART_INF_F)) v = -CUDART_INF_F;   // NaN as -infinity
-    else ++cand;
-    if (CACHE) cache[i] = v;
+  auto look = [&](int i, float v) -> float {
+    if (v > -CUDART_INF_F) ++cand;
+    else v = -CUDART_INF_F;   // NaN too
     if (v > m) { m = v; im = i; }
+    return v;
+  };
+  constexpr int VW = 16 / (int)sizeof(T);
+  const int head = p.vec ? V / VW * VW : 0;
+  constexpr int UNR = 4;      // loads in flight per thread
+  for (int i0 = tid * VW; i0 < head; i0 += NT * VW * UNR) {
+    Pack<T, VW> v[UNR];
+#pragma unroll
+    for (int k = 0; k < UNR; ++k)
+      if (i0 + k * NT * VW < head) v[k] = ld_pack<T, VW>(g + i0 + k * NT * VW);
+#pragma unroll
+    for (int k = 0; k < UNR; ++k) {
+      const int i = i0 + k * NT * VW;
+      if (i < head) {
+#pragma unroll
+        for (int j = 0; j < VW; j += 4) {
+          const float4 f = make_float4(look(i + j, v[k].get(j)), look(i + j + 1, v[k].get(j + 1)),
+                                       look(i + j + 2, v[k].get(j + 2)),
+                                       look(i + j + 3, v[k].get(j + 3)));
+          if (CACHE) *reinterpret_cast<float4*>(cache + i + j) = f;
+        }
+      }
+    }
+  }
+  for (int i = head + tid; i < V; i += NT) {
+    const float v = look(i, Elem<T>::get(g[i]));
+    if (CACHE) cache[i] = v;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -151,144 +203,266 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     if (om > m || (om == m && oi < im)) { m = om; im = oi; }
     cand += __shfl_xor_sync(0xffffffffu, cand, o);
   }
-  if (tid == 0) { sh.n = 0; sh.fmax = -CUDART_INF_F; sh.imax = 0x7fffffff; }
-  __shared__ float wm[32];
-  __shared__ int wi[32];
-  if (lane == 0) { wm[warp] = m; wi[warp] = im; }
+  if (tid == 0) { sh.n = 0; sh.ln = 0; }
+  if (tid < 32) sh.pow2[tid] = exp2((double)tid / 32);
+  if (lane == 0) { sh.wm[warp] = m; sh.wi[warp] = im; }
   __syncthreads();
   if (lane == 0) atomicAdd(&sh.n, cand);
-  if (tid == 0)
-    for (int w = 0; w < NT / 32; ++w)
-      if (wm[w] > sh.fmax || (wm[w] == sh.fmax && wi[w] < sh.imax)) {
-        sh.fmax = wm[w];
-        sh.imax = wi[w];
-      }
+  float top = sh.wm[0];
+  int itop = sh.wi[0];
+#pragma unroll
+  for (int w = 1; w < NT / 32; ++w)
+    if (sh.wm[w] > top || (sh.wm[w] == top && sh.wi[w] < itop)) {
+      top = sh.wm[w];
+      itop = sh.wi[w];
+    }
   __syncthreads();
-  const float top = sh.fmax;
   const int ncand = (int)sh.n;
   const float temp = p.temperature ? p.temperature[row] : p.temperature0;
-  if (ncand == 0 || !(temp > 0.f)) {
-    if (tid == 0) p.out[row] = ncand == 0 ? -1 : sh.imax;
+  const int k = p.top_k ? p.top_k[row] : p.top_k0;
+  if (ncand == 0 || !(temp > 0.f) || k == 1) {
+    if (tid == 0) p.out[row] = ncand == 0 ? -1 : itop;
     return;
   }
-  const int k = p.top_k ? p.top_k[row] : p.top_k0;
   const float tp = p.top_p ? p.top_p[row] : p.top_p0;
   const double mp = fmin((double)(p.min_p ? p.min_p[row] : p.min_p0), 1.0);
-  const double dtop = (double)top, dtemp = (double)temp, unit = exp2((double)p.shift);
+  const double dtop = (double)top, unit = exp2((double)p.shift);
+  const double scale = CUDART_L2E / (double)temp;   // to powers of 2
   const float inv_t = 1.f / temp;
 
+  // 2^y for y <= 0 by the table of 2^(j/32) and the exponential series of the
+  // rest, |r| <= ln 2 / 64 (P. T. P. Tang, "Table-driven implementation of the
+  // exponential function", ACM TOMS 15, 1989): 14 double-precision operations.
   auto weight = [&](float v) -> double {
-    return v == top ? 1.0 : exp(((double)v - dtop) / dtemp);
+    if (v == top) return 1.0;
+    const double y = ((double)v - dtop) * scale;
+    if (!(y > -1000.0)) return 0.0;
+    constexpr double kShifter = 6755399441055744.0;   // 1.5 * 2^52
+    const double t = fma(y, 32.0, kShifter);
+    const int k32 = __double2loint(t);
+    const double r = fma(t - kShifter, -1.0 / 32, y) * CUDART_LN2;
+    double e = 1.0 / 720;
+    e = fma(e, r, 1.0 / 120);
+    e = fma(e, r, 1.0 / 24);
+    e = fma(e, r, 1.0 / 6);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0) * sh.pow2[k32 & 31];
+    return __hiloint2double(__double2hiint(e) + ((k32 >> 5) << 20), __double2loint(e));
   };
-  auto units = [&](float v) -> u64 { return __double2ull_rn(weight(v) * unit); };
+  // shift <= 50: the integer stands in the low bits of the shifted sum
+  auto in_units = [&](double w) -> u64 {
+    return (u64)__double_as_longlong(fma(w, unit, 4503599627370496.0)) & 0xfffffffffffffull;
+  };
+  auto units = [&](float v) -> u64 { return in_units(weight(v)); };
   // a bin of the order: monotone in v, equal values share it
   auto bin_of = [&](float v) -> int {
     const float d = (top - v) * inv_t * kBinsPerUnit;
     return v == top ? 0 : d < (float)(kBins - 1) ? (int)d : kBins - 1;
   };
 
+  // every token, four at a time from the cache
+  auto for_each = [&](auto&& f) {
+    if (CACHE) {
+      for (int i = 4 * tid; i < V; i += 4 * NT) {
+        const float4 v = *reinterpret_cast<const float4*>(cache + i);
+        f(i, v.x);
+        if (i + 1 < V) f(i + 1, v.y);
+        if (i + 2 < V) f(i + 2, v.z);
+        if (i + 3 < V) f(i + 3, v.w);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = tid; i < V; i += NT) f(i, x.at(i));
+    }
+  };
+  auto clear = [&](int n, bool mass) {
+    __syncthreads();
+    for (int i = tid; i < n; i += NT) {
+      sh.count[i] = 0;
+      if (mass) sh.high[i] = 0;
+    }
+    __syncthreads();
+  };
+  // The number of the target: the smallest cumulative weight to reach.
+  auto target = [&](u64 total) -> u64 {
+    const double at = (double)p.u[row] * (double)total;
+    const u64 thr = at > 0.0 ? (at < (double)total ? (u64)at + 1 : total) : 1;
+    return thr > total ? total : thr;
+  };
+
+  // ---- few tokens in play: among those that f names (at most kList)
+  auto finish = [&](auto&& f) {
+    for_each([&](int i, float v) {
+      if (v > -CUDART_INF_F && f(v)) {
+        const int at = atomicAdd(&sh.ln, 1);
+        if (at < kList) { sh.lx[at] = v; sh.li[at] = i; }
+      }
+    });
+    __syncthreads();
+    const int n = sh.ln;
+    float mx = 0.f;
+    int mi = 0, rank = 0;
+    double w = 0.0;
+    if (tid < n) {
+      mx = sh.lx[tid];
+      mi = sh.li[tid];
+      for (int j = 0; j < n; ++j)
+        rank += sh.lx[j] > mx || (sh.lx[j] == mx && sh.li[j] < mi);
+      w = weight(mx);
+      sh.sw[rank] = (k <= 0 || rank < k) ? in_units(w) : 0;
+    }
+    __syncthreads();
+    // thread r looks at the token of rank r: is it in the top-p prefix?
+    u64 total;
+    const u64 own = tid < n ? sh.sw[tid] : 0;
+    const u64 before = block_prefix<NT>(own, sh.wsum, &total);
+    if (tid < n && !(tid == 0 || tp >= 1.f || (double)before < (double)tp * (double)total))
+      sh.sw[tid] = 0;
+    __syncthreads();
+    u64 mine = 0;
+    if (tid < n) {
+      mine = w >= mp ? sh.sw[rank] : 0;
+      sh.lw[tid] = mine;
+    }
+    block_prefix<NT>(mine, sh.wsum, &total);   // its barriers show lw too
+    const u64 thr = target(total);
+    if (mine) {
+      u64 cum = 0;
+      for (int j = 0; j < n; ++j) cum += sh.li[j] <= mi ? sh.lw[j] : 0;
+      if (cum >= thr && cum - mine < thr) p.out[row] = mi;
+    }
+  };
+  if (ncand <= kList) {
+    finish([](float) { return true; });
+    return;
+  }
+
   Cut cut;
   // The cut of the shortest prefix (of what `cut` keeps) whose measure reaches
-  // thr: counts, or weights.  The histogram of level 0 is in sh.
-  auto select = [&](bool mass, u64 thr) {
-    find_bin<NT>(sh, mass, kBins, thr);
-    const int bin = sh.found;
-    u64 base = sh.found_base;
+  // thr: counts, or weights.  It ends in bin `bin`, with `base` before the bin.
+  auto select = [&](bool mass, u64 thr, int bin, u64 base) {
+    if (tid == 0) sh.ln = 0;
+    __syncthreads();
+    for_each([&](int i, float v) {
+      if (v > -CUDART_INF_F && bin_of(v) == bin && cut.has(desc_key(v), i)) {
+        const int at = atomicAdd(&sh.ln, 1);
+        if (at < kList) { sh.lx[at] = v; sh.li[at] = i; }
+      }
+    });
+    __syncthreads();
+    const int n = sh.ln;
+    Cut c;
+    if (n <= kList) {   // rank the bin's members
+      if (tid < n) sh.lw[tid] = mass ? units(sh.lx[tid]) : 1;
+      __syncthreads();
+      if (tid < n) {
+        const float mx = sh.lx[tid];
+        const int mi = sh.li[tid];
+        u64 upto = base;   // this member included
+        for (int j = 0; j < n; ++j)
+          upto += (sh.lx[j] > mx || (sh.lx[j] == mx && sh.li[j] <= mi)) ? sh.lw[j] : 0;
+        if (upto >= thr && upto - sh.lw[tid] < thr) sh.found = tid;
+      }
+      __syncthreads();
+      const int at = min(sh.found, kList - 1);
+      c.key = desc_key(sh.lx[at]);
+      c.last = sh.li[at];
+      __syncthreads();
+      cut = c;
+      return;
+    }
     unsigned prefix = 0;
     for (int level = 3; level >= 0; --level) {
       const int sft = level * 8;
-      __syncthreads();
-      for (int i = tid; i < 256; i += NT) { sh.count[i] = 0; sh.mass[i] = 0; }
-      __syncthreads();
+      clear(256, true);
       for (int i = tid; i < V; i += NT) {
         const float v = x.at(i);
         if (!(v > -CUDART_INF_F) || bin_of(v) != bin) continue;
         const unsigned key = desc_key(v);
         if (!cut.has(key, i) || (level < 3 && (key >> (sft + 8)) != (prefix >> (sft + 8))))
           continue;
-        atomicAdd(&sh.count[key >> sft & 255], 1u);
-        if (mass) atomicAdd(&sh.mass[key >> sft & 255], units(v));
+        if (mass) add64(sh, key >> sft & 255, units(v));
+        else atomicAdd(&sh.count[key >> sft & 255], 1u);
       }
       __syncthreads();
       find_bin<NT>(sh, mass, 256, thr - base);
       prefix |= (unsigned)sh.found << sft;
       base += sh.found_base;
     }
-    // one value is left: the number of its ties to keep
-    const unsigned ties = sh.count[prefix & 255];
+    // one value is left: how many of its ties to keep
+    c.key = prefix;
     u64 need = thr - base;
     if (mass) {
-      const u64 each = sh.mass[prefix & 255] / ties;
+      const unsigned b = prefix & 0x80000000u ? prefix : ~prefix & 0x7fffffffu;
+      const u64 each = units(__uint_as_float(b));
       need = (need + each - 1) / each;
     }
-    Cut c;
-    c.key = prefix;
-    if (need < ties) {   // the need-th tie by index
-      // warps own runs of indices
-      const int seg = (V + NT / 32 - 1) / (NT / 32), s0 = warp * seg, s1 = min(s0 + seg, V);
-      unsigned mine = 0;
+    // the need-th tie by index: warps own runs of indices
+    const int seg = (V + NT / 32 - 1) / (NT / 32), s0 = warp * seg, s1 = min(s0 + seg, V);
+    auto tie = [&](int i) {
+      return i < s1 && x.at(i) > -CUDART_INF_F && desc_key(x.at(i)) == prefix &&
+             cut.has(prefix, i);
+    };
+    unsigned mine = 0;
+    for (int i = s0 + lane; i - lane < s1; i += 32)
+      mine += __popc(__ballot_sync(0xffffffffu, tie(i)));
+    __syncthreads();
+    if (lane == 0) sh.wsum[warp] = mine;
+    if (tid == 0) sh.found = cut.key == prefix ? cut.last : 0x7fffffff;   // all of them
+    __syncthreads();
+    u64 before = 0;
+    for (int w = 0; w < warp; ++w) before += sh.wsum[w];
+    if (before < need && before + mine >= need) {
+      u64 left = need - before;
       for (int i = s0 + lane; i - lane < s1; i += 32) {
-        const bool t = i < s1 && x.at(i) > -CUDART_INF_F && desc_key(x.at(i)) == prefix &&
-                       cut.has(prefix, i);
-        mine += __popc(__ballot_sync(0xffffffffu, t));
-      }
-      __syncthreads();
-      if (lane == 0) sh.wsum[warp] = mine;
-      __syncthreads();
-      u64 before = 0;
-      for (int w = 0; w < warp; ++w) before += sh.wsum[w];
-      if (before < need && before + mine >= need) {
-        u64 left = need - before;
-        for (int i = s0 + lane; i - lane < s1; i += 32) {
-          const bool t = i < s1 && x.at(i) > -CUDART_INF_F && desc_key(x.at(i)) == prefix &&
-                         cut.has(prefix, i);
-          const unsigned bits = __ballot_sync(0xffffffffu, t);
-          const unsigned cnt = __popc(bits);
-          if (cnt >= left) {
-            if (t && __popc(bits & ((2u << lane) - 1)) == left) sh.found = i;
-            break;
-          }
-          left -= cnt;
+        const bool t = tie(i);
+        const unsigned bits = __ballot_sync(0xffffffffu, t);
+        const unsigned cnt = __popc(bits);
+        if (cnt >= left) {
+          if (t && __popc(bits & ((2u << lane) - 1)) == left) sh.found = i;
+          break;
         }
+        left -= cnt;
       }
-      __syncthreads();
-      c.last = sh.found;
-    } else if (cut.key == prefix) {
-      c.last = cut.last;
     }
+    __syncthreads();
+    c.last = sh.found;
     __syncthreads();
     cut = c;
   };
-  auto clear = [&]() {
-    __syncthreads();
-    for (int i = tid; i < kBins; i += NT) { sh.count[i] = 0; sh.mass[i] = 0; }
-    __syncthreads();
-  };
 
   if (k > 0 && k < ncand) {
-    clear();
-    for (int i = tid; i < V; i += NT) {
-      const float v = x.at(i);
+    clear(kBins, false);
+    for_each([&](int i, float v) {
       if (v > -CUDART_INF_F) atomicAdd(&sh.count[bin_of(v)], 1u);
-    }
+    });
     __syncthreads();
-    select(false, (u64)k);
+    find_bin<NT>(sh, false, kBins, (u64)k);
+    const int bin = sh.found;
+    const u64 base = sh.found_base;
+    if (base + sh.count[bin] <= kList) {   // the prefix's bins hold few tokens
+      finish([&](float v) { return bin_of(v) <= bin; });
+      return;
+    }
+    select(false, (u64)k, bin, base);
   }
   if (tp < 1.f) {
-    clear();
+    clear(kBins, true);
     u64 mine = 0;
-    for (int i = tid; i < V; i += NT) {
-      const float v = x.at(i);
+    for_each([&](int i, float v) {
       if (v > -CUDART_INF_F && cut.has(desc_key(v), i)) {
         const u64 w = units(v);
         mine += w;
-        atomicAdd(&sh.mass[bin_of(v)], w);
+        if (w) add64(sh, bin_of(v), w);
       }
-    }
+    });
     u64 total;
     block_prefix<NT>(mine, sh.wsum, &total);
     const double want = ceil((double)tp * (double)total);
-    select(true, want >= 1.0 ? (u64)want : 1ull);   // NaN and p <= 0: the first token
+    const u64 thr = want >= 1.0 ? (u64)want : 1ull;   // NaN and p <= 0: the first token
+    find_bin<NT>(sh, true, kBins, thr);
+    select(true, thr, sh.found, sh.found_base);
   }
 
   // ---- draw: warps own runs of indices
@@ -298,7 +472,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     const float v = x.at(i);
     if (!(v > -CUDART_INF_F) || !cut.has(desc_key(v), i)) return 0;
     const double w = weight(v);
-    return w >= mp ? __double2ull_rn(w * unit) : 0;
+    return w >= mp ? in_units(w) : 0;
   };
   u64 mine = 0;
   for (int i = s0 + lane; i - lane < s1; i += 32) mine += kept(i);
@@ -312,9 +486,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     if (w < warp) before += sh.wsum[w];
     total += sh.wsum[w];
   }
-  const double at = (double)p.u[row] * (double)total;
-  u64 thr = at > 0.0 ? (at < (double)total ? (u64)at + 1 : total) : 1;
-  if (thr > total) thr = total;
+  const u64 thr = target(total);
   if (before < thr && before + mine >= thr) {
     u64 run = before;
     for (int i = s0 + lane; i - lane < s1; i += 32) {
@@ -337,7 +509,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
 template <typename T, int NT, bool CACHE>
 cudaError_t sample_typed(const SampleParams& p, cudaStream_t s) {
   auto* kern = sample_kernel<T, NT, CACHE>;
-  const int smem = (int)sizeof(Shared) + (CACHE ? p.V * 4 : 0);
+  const int smem = ((int)sizeof(Shared) + 15) / 16 * 16 + (CACHE ? (p.V + 3) / 4 * 16 : 0);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   kern<<<p.rows, NT, smem, s>>>(p);
@@ -353,7 +525,9 @@ cudaError_t sample_rows(const SampleParams& p, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_sample(const SampleParams& p, cudaStream_t s) {
+cudaError_t launch_sample(const SampleParams& p0, cudaStream_t s) {
+  SampleParams p = p0;
+  p.vec = aligned(p.logits, 16) && p.ld % (16 / dsize(p.dtype)) == 0;
   return p.dtype == M3_BF16 ? sample_rows<__nv_bfloat16>(p, s) : sample_rows<float>(p, s);
 }
 
