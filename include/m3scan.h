@@ -463,7 +463,8 @@ typedef struct m3_norm_desc {
 /* y = (x - mean) * rstd * w + b over rows of d elements, rstd =
  * 1 / sqrt(mean((x - mean)^2) + eps); mean is 0 for the RMS norm (the RMSNorm
  * of mamba.py:82-89; the layer norms of search_mamba.py's heads).
- *   x (rows, ld_x); w (d,) float32; b (d,) float32 or NULL; y (rows, d)
+ *   x (rows, ld_x); w (d,) float32; b (d,) float32 or NULL (NULL for the RMS norm);
+ *   y (rows, d)
  *   mean, rstd (rows,) float32 for the backward, or NULL.  y may be x when
  *   ld_x == d and both have one element type. */
 M3_API int m3_norm_fwd(const m3_norm_desc* desc, const void* x, int64_t ld_x, const float* w,

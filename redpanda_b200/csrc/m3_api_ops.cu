@@ -126,6 +126,7 @@ int m3_norm_fwd(const m3_norm_desc* desc, const void* x, int64_t ld_x, const flo
   if (rc != M3_OK) return rc;
   if (ld_x < desc->d) return M3_ERR_SHAPE;
   if (!x || !w || !y) return M3_ERR_NULL;
+  if (desc->rms && b) return M3_ERR_UNSUPPORTED;   // it has no bias
   if (!aligned(x, dsize(desc->dtype_x)) || !aligned(y, dsize(desc->dtype_y)) ||
       !aligned(w, 4) || !aligned(b, 4) || !aligned(mean, 4) || !aligned(rstd, 4))
     return M3_ERR_ALIGN;
@@ -153,6 +154,7 @@ int m3_norm_bwd(const m3_norm_desc* desc, const void* x, int64_t ld_x, const flo
   if (rc != M3_OK) return rc;
   if (ld_x < desc->d) return M3_ERR_SHAPE;
   if (!x || !w || !rstd || (!desc->rms && !mean) || !g || !dx || !dw) return M3_ERR_NULL;
+  if (desc->rms && db) return M3_ERR_UNSUPPORTED;   // it has no bias
   if (!aligned(x, dsize(desc->dtype_x)) || !aligned(dx, dsize(desc->dtype_x)) ||
       !aligned(g, dsize(desc->dtype_y)) || !aligned(w, 4) || !aligned(mean, 4) ||
       !aligned(rstd, 4) || !aligned(dw, 4) || !aligned(db, 4) || !aligned(workspace, 4))
@@ -165,7 +167,7 @@ int m3_norm_bwd(const m3_norm_desc* desc, const void* x, int64_t ld_x, const flo
   p.dw = dw; p.db = db; p.part = static_cast<float*>(workspace);
   p.rows = desc->rows; p.d = desc->d;
   p.dtype_x = desc->dtype_x; p.dtype_y = desc->dtype_y; p.rms = desc->rms != 0;
-  p.ctas = norm_bwd_ctas(desc->rows, desc->d, device_sms());
+  p.sms = device_sms();
   return status(launch_norm_bwd(p, static_cast<cudaStream_t>(stream)));
 }
 

@@ -4,31 +4,65 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "m3scan.h"
 
 namespace m3 {
 
+// SM count and compute capability of a device do not change: asked for once
+// (a query per call is a good part of a small call's time on the host).
+constexpr int kMaxDevices = 64;
+struct DeviceInfo {
+  std::atomic<int> sms{0}, major{0};   // 0: not asked yet
+};
+inline DeviceInfo* device_info() {
+  static DeviceInfo info[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+  if (dev < 0 || dev >= kMaxDevices) return nullptr;
+  DeviceInfo* d = &info[dev];
+  if (d->sms.load(std::memory_order_acquire) == 0) {
+    int sms = 0, major = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    d->major.store(major, std::memory_order_relaxed);
+    d->sms.store(sms, std::memory_order_release);
+  }
+  return d;
+}
+
 // SM count of the current device, -1 when there is none
 inline int device_sms() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return -1; }
-  int sms = 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return -1;
-  }
-  return sms;
+  const DeviceInfo* d = device_info();
+  return d ? d->sms.load(std::memory_order_relaxed) : -1;
 }
 
 inline int check_device() {
+  const DeviceInfo* d = device_info();
+  return d && d->major.load(std::memory_order_relaxed) == 10 ? M3_OK : M3_ERR_NO_DEVICE;
+}
+
+// Lets a kernel use `smem` bytes of dynamic shared memory, once per device and
+// kernel.
+struct OncePerDevice {
+  std::atomic<int> value[kMaxDevices] = {};
+};
+template <auto* kern>
+cudaError_t allow_smem(int smem) {
+  static OncePerDevice done;
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return M3_ERR_NO_DEVICE; }
-  int major = 0;
-  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return M3_ERR_NO_DEVICE;
-  }
-  return major == 10 ? M3_OK : M3_ERR_NO_DEVICE;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < kMaxDevices && done.value[dev].load(std::memory_order_acquire) >= smem)
+    return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && dev < kMaxDevices)
+    done.value[dev].store(smem, std::memory_order_release);
+  return e;
 }
 
 inline bool dtype_ok(int dt) { return dt == M3_F32 || dt == M3_BF16; }

@@ -22,13 +22,39 @@
 #include <stdint.h>
 
 #include "m3_api_util.h"
+#include "m3_math.cuh"
 #include "m3_ops.h"
 #include "m3_vec.cuh"
 
 namespace m3 {
 namespace {
 
-constexpr int kAhead = 4;      // rows in flight per thread
+#ifndef M3_T3
+#define M3_T3 8
+#endif
+constexpr int kAhead = 4;      // rows in flight per thread (backward: of x and dy, twice)
+constexpr int kAheadFwd = M3_T3;
+
+// V fp32 values as packed pairs (V = 1: the second half idles).
+template <int V> struct Vals {
+  static constexpr int H = (V + 1) / 2;
+  float2 v[H];
+  __device__ __forceinline__ float get(int j) const { return j & 1 ? v[j / 2].y : v[j / 2].x; }
+  __device__ __forceinline__ void set(float a) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) v[i] = f2(a);
+  }
+  template <typename T>
+  __device__ __forceinline__ void from(const Pack<T, V>& p) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) v[i] = make_float2(p.get(2 * i), V > 1 ? p.get(2 * i + 1) : 0.f);
+  }
+  // this += a * b
+  __device__ __forceinline__ void fma(const Vals& a, const Vals& b) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) v[i] = __ffma2_rn(a.v[i], b.v[i], v[i]);
+  }
+};
 
 __device__ __forceinline__ int row_length(const int* lengths, int b, int L) {
   if (lengths == nullptr) return L;
@@ -49,13 +75,20 @@ struct Rows {
 };
 
 template <int V, int K>
-__device__ __forceinline__ void load_filter(float (&w)[K][V], float (&b)[V], const float* pw,
-                                            const float* pb, int c, int D) {
+__device__ __forceinline__ void load_filter(Vals<V> (&w)[K], Vals<V>& b, const float* pw,
+                                            const float* pb, int c) {
+  float t[K + 1][2 * Vals<V>::H] = {};
 #pragma unroll
   for (int j = 0; j < V; ++j) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) w[k][j] = pw[(size_t)(c + j) * K + k];
-    b[j] = pb != nullptr ? pb[c + j] : 0.f;
+    for (int k = 0; k < K; ++k) t[k][j] = pw[(size_t)(c + j) * K + k];
+    t[K][j] = pb != nullptr ? pb[c + j] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < Vals<V>::H; ++i) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k].v[i] = make_float2(t[k][2 * i], t[k][2 * i + 1]);
+    b.v[i] = make_float2(t[K][2 * i], t[K][2 * i + 1]);
   }
 }
 
@@ -80,36 +113,30 @@ __global__ void __launch_bounds__(128) conv_fwd_kernel(const ConvParams p) {
   T* y = static_cast<T*>(p.y) + (size_t)b * p.L * p.D + c;
   int t = t0;
   if (t < te) {
-    float w[K][V], bias[V], win[K][V];
-    load_filter<V, K>(w, bias, p.w, p.b, c, p.D);
+    Vals<V> w[K], bias, win[K];
+    load_filter<V, K>(w, bias, p.w, p.b, c);
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) {
-      const Pack<T, V> r = in.at(t0 - (K - 1) + k);
-#pragma unroll
-      for (int j = 0; j < V; ++j) win[k + 1][j] = r.get(j);
-    }
+    for (int k = 0; k < K - 1; ++k) win[k + 1].from(in.at(t0 - (K - 1) + k));
     auto one = [&](const Pack<T, V>& r, int tt) {
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k) win[k] = win[k + 1];
+      win[K - 1].from(r);
+      Vals<V> a = bias;
+#pragma unroll
+      for (int k = 0; k < K; ++k) a.fma(w[k], win[k]);
       Pack<T, V> o;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-#pragma unroll
-        for (int k = 0; k < K - 1; ++k) win[k][j] = win[k + 1][j];
-        win[K - 1][j] = r.get(j);
-        float a = bias[j];
-#pragma unroll
-        for (int k = 0; k < K; ++k) a = fmaf(w[k][j], win[k][j], a);
-        o.put(j, p.silu ? silu_f(a) : a);
-      }
+      for (int j = 0; j < V; ++j) o.put(j, p.silu ? silu_f(a.get(j)) : a.get(j));
       st_pack<T, V>(y + (size_t)tt * p.D, o);
     };
-    for (; t + kAhead <= te; t += kAhead) {
-      Pack<T, V> r[kAhead];
+    for (; t + kAheadFwd <= te; t += kAheadFwd) {
+      Pack<T, V> r[kAheadFwd];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) r[i] = in.at(t + i);
+      for (int i = 0; i < kAheadFwd; ++i) r[i] = ld_pack<T, V>(in.x + (size_t)(t + i) * in.ld);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) one(r[i], t + i);
+      for (int i = 0; i < kAheadFwd; ++i) one(r[i], t + i);
     }
-    for (; t < te; ++t) one(in.at(t), t);
+    for (; t < te; ++t) one(ld_pack<T, V>(in.x + (size_t)t * in.ld), t);
   }
   for (; t < t1; ++t) st_pack<T, V>(y + (size_t)t * p.D, zero_pack<T, V>());
 }
@@ -117,23 +144,20 @@ __global__ void __launch_bounds__(128) conv_fwd_kernel(const ConvParams p) {
 constexpr int kWorkers = 8;    // workers (warps) per CTA of the backward
 
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(32 * kWorkers) conv_bwd_kernel(const ConvBwdParams p) {
+__global__ void __launch_bounds__(32 * kWorkers, K <= 4 ? 2 : 1) conv_bwd_kernel(const ConvBwdParams p) {
   __shared__ float comb[K + 1][32 * V];
   const int lane = threadIdx.x & 31, wk = threadIdx.x >> 5;
   const int c = (blockIdx.x * 32 + lane) * V;
   const bool live = c < p.D;
   const int runs = (p.L + p.tt - 1) / p.tt;
   const long long tasks = (long long)runs * p.B;
-  float dw[K][V], db[V];
+  Vals<V> dw[K], db;
+  db.set(0.f);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    db[j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) dw[k][j] = 0.f;
-  }
+  for (int k = 0; k < K; ++k) dw[k].set(0.f);
   if (live) {
-    float w[K][V], bias[V];
-    load_filter<V, K>(w, bias, p.w, p.b, c, p.D);
+    Vals<V> w[K], bias;
+    load_filter<V, K>(w, bias, p.w, p.b, c);
     for (long long q = (long long)blockIdx.y * kWorkers + wk; q < tasks;
          q += (long long)gridDim.y * kWorkers) {
       const int run = (int)(q % runs), b = (int)(q / runs);
@@ -147,77 +171,80 @@ __global__ void __launch_bounds__(32 * kWorkers) conv_bwd_kernel(const ConvBwdPa
       const int t0 = run * p.tt, t1 = min(t0 + p.tt, p.L), te = min(t1, n);
       // steps [t0, tg) are read: K-1 past the run, for its last dx rows
       const int tg = te > t0 ? min(te + K - 1, n) : t0;
-      float win[K][V], gw[K][V];
+      Pack<T, V> rx[kAhead], rg[kAhead];
+      auto fetch = [&](int t) {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+        for (int i = 0; i < kAhead; ++i)
+          if (t + i < tg) {
+            rx[i] = ld_pack<T, V>(in.x + (size_t)(t + i) * in.ld);
+            rg[i] = ld_pack<T, V>(g + (size_t)(t + i) * p.D);
+          }
+      };
+      fetch(t0);
+      Vals<V> win[K], gw[K];
 #pragma unroll
-        for (int j = 0; j < V; ++j) gw[k][j] = 0.f;
+      for (int k = 0; k < K; ++k) gw[k].set(0.f);
       if (te > t0) {
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) {
-          const Pack<T, V> r = in.at(t0 - (K - 1) + k);
-#pragma unroll
-          for (int j = 0; j < V; ++j) win[k + 1][j] = r.get(j);
-        }
+        for (int k = 0; k < K - 1; ++k) win[k + 1].from(in.at(t0 - (K - 1) + k));
       }
       // after step t the window of g holds g[t-K+1 .. t]: dx[t-K+1] is complete
       auto emit = [&](int s) {
+        Vals<V> a;
+        a.set(0.f);
+#pragma unroll
+        for (int k = 0; k < K; ++k) a.fma(w[k], gw[K - 1 - k]);
         Pack<T, V> o;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float a = 0.f;
-#pragma unroll
-          for (int k = 0; k < K; ++k) a = fmaf(w[k][j], gw[K - 1 - k][j], a);
-          o.put(j, a);
-        }
+        for (int j = 0; j < V; ++j) o.put(j, a.get(j));
         st_pack<T, V>(dx + (size_t)s * p.D, o);
       };
-      auto one = [&](const Pack<T, V>& rx, const Pack<T, V>& rg, int t) {
-        const float own = t < te ? 1.f : 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-#pragma unroll
-          for (int k = 0; k < K - 1; ++k) {
-            win[k][j] = win[k + 1][j];
-            gw[k][j] = gw[k + 1][j];
-          }
-          win[K - 1][j] = rx.get(j);
-          float gt = rg.get(j);
-          if (p.silu) {
-            float a = bias[j];
-#pragma unroll
-            for (int k = 0; k < K; ++k) a = fmaf(w[k][j], win[k][j], a);
-            gt *= dsilu_f(a, sigmoid_f(a));
-          }
-          gw[K - 1][j] = gt;
-          // halo steps belong to the next run
-          const float gm = own != 0.f ? gt : 0.f;
-          db[j] += gm;
-#pragma unroll
-          for (int k = 0; k < K; ++k) dw[k][j] = fmaf(gm, win[k][j], dw[k][j]);
-        }
-        if (t - (K - 1) >= t0) emit(t - (K - 1));
-      };
-      int t = t0;
-      for (; t + kAhead <= tg; t += kAhead) {
-        Pack<T, V> rx[kAhead], rg[kAhead];
+      for (int tb = t0; tb < tg; tb += kAhead) {
+        Pack<T, V> cx[kAhead], cg[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          rx[i] = in.at(t + i);
-          rg[i] = ld_pack<T, V>(g + (size_t)(t + i) * p.D);
+          cx[i] = rx[i];
+          cg[i] = rg[i];
         }
+        fetch(tb + kAhead);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) one(rx[i], rg[i], t + i);
+        for (int i = 0; i < kAhead; ++i) {
+          const int t = tb + i;
+          if (t < tg) {
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k) {
+              win[k] = win[k + 1];
+              gw[k] = gw[k + 1];
+            }
+            win[K - 1].from(cx[i]);
+            Vals<V> gt;
+            gt.from(cg[i]);
+            if (p.silu) {
+              Vals<V> a = bias;
+#pragma unroll
+              for (int k = 0; k < K; ++k) a.fma(w[k], win[k]);
+#pragma unroll
+              for (int h = 0; h < Vals<V>::H; ++h) {
+                gt.v[h].x *= dsilu_f(a.v[h].x, sigmoid_f(a.v[h].x));
+                if (V > 1) gt.v[h].y *= dsilu_f(a.v[h].y, sigmoid_f(a.v[h].y));
+              }
+            }
+            gw[K - 1] = gt;
+            if (t < te) {   // halo steps belong to the next run
+#pragma unroll
+              for (int h = 0; h < Vals<V>::H; ++h) db.v[h] = __fadd2_rn(db.v[h], gt.v[h]);
+#pragma unroll
+              for (int k = 0; k < K; ++k) dw[k].fma(gt, win[k]);
+            }
+            if (t - (K - 1) >= t0) emit(t - (K - 1));
+          }
+        }
       }
-      for (; t < tg; ++t) one(in.at(t), ld_pack<T, V>(g + (size_t)t * p.D), t);
       // the sequence's end: g past it is zero
-      for (; t - (K - 1) < te; ++t) {
+      for (int t = tg; t - (K - 1) < te; ++t) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-#pragma unroll
-          for (int k = 0; k < K - 1; ++k) gw[k][j] = gw[k + 1][j];
-          gw[K - 1][j] = 0.f;
-        }
+        for (int k = 0; k < K - 1; ++k) gw[k] = gw[k + 1];
+        gw[K - 1].set(0.f);
         if (t - (K - 1) >= t0) emit(t - (K - 1));
       }
       for (int s = max(te, t0); s < t1; ++s)
@@ -231,10 +258,10 @@ __global__ void __launch_bounds__(32 * kWorkers) conv_bwd_kernel(const ConvBwdPa
 #pragma unroll
         for (int i = 0; i < K; ++i) {
           float* a = &comb[i][j * 32 + lane];
-          *a = k ? *a + dw[i][j] : dw[i][j];
+          *a = k ? *a + dw[i].get(j) : dw[i].get(j);
         }
         float* a = &comb[K][j * 32 + lane];
-        *a = k ? *a + db[j] : db[j];
+        *a = k ? *a + db.get(j) : db.get(j);
       }
     __syncthreads();
   }
@@ -282,16 +309,17 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const ConvStepParams p) 
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) r[k] = ld_pack<T, V>(st + (size_t)k * p.D);
   r[K - 1] = ld_pack<T, V>(static_cast<const T*>(p.x) + b * p.ld_x + c);
-  float w[K][V], bias[V];
-  load_filter<V, K>(w, bias, p.w, p.b, c, p.D);
+  Vals<V> w[K], a;
+  load_filter<V, K>(w, a, p.w, p.b, c);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    Vals<V> x;
+    x.from(r[k]);
+    a.fma(w[k], x);
+  }
   Pack<T, V> o;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    float a = bias[j];
-#pragma unroll
-    for (int k = 0; k < K; ++k) a = fmaf(w[k][j], r[k].get(j), a);
-    o.put(j, p.silu ? silu_f(a) : a);
-  }
+  for (int j = 0; j < V; ++j) o.put(j, p.silu ? silu_f(a.get(j)) : a.get(j));
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) st_pack<T, V>(st + (size_t)k * p.D, r[k + 1]);
   st_pack<T, V>(static_cast<T*>(p.y) + b * p.D + c, o);
@@ -372,12 +400,12 @@ cudaError_t launch_conv_fwd(const ConvParams& p0, cudaStream_t s) {
 
 void conv_bwd_plan(int B, int L, int D, int sms, int* workers, int* tt) {
   // channel groups of 32 lanes of 4 channels (or of 1: more groups, the same
-  // partials per channel); about 4 CTAs per SM
+  // partials per channel); one wave of two CTAs per SM
   const long long groups = (D + 127) / 128;
   int t = 32;
-  while (t > 8 && groups * B * ((L + t - 1) / t) < (long long)sms * 4 * kWorkers) t /= 2;
+  while (t > 8 && groups * B * ((L + t - 1) / t) < (long long)sms * 2 * kWorkers) t /= 2;
   const long long tasks = (long long)B * ((L + t - 1) / t);
-  long long w = ((long long)sms * 4 + groups - 1) / groups;
+  long long w = (long long)sms * 2 / groups;
   const long long most = (tasks + kWorkers - 1) / kWorkers;
   if (w > most) w = most;
   if (w < 1) w = 1;

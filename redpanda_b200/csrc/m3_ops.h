@@ -20,7 +20,6 @@ struct NormParams {
   int dtype_x, dtype_y, rms;
   float eps;
   int sms;
-  int vec;                            // set by the launcher
 };
 cudaError_t launch_norm_fwd(const NormParams& p, cudaStream_t s);
 
@@ -31,13 +30,12 @@ struct NormBwdParams {
   const void* g;                      // (rows, d) of dtype_y
   void* dx;                           // (rows, d) of dtype_x
   float* dw; float* db;               // (d,), db may be nullptr
-  float* part;                        // (ctas, 2, d)
+  float* part;                        // (norm_bwd_ctas, 2, d)
   long long rows; int d;
   int dtype_x, dtype_y, rms;
-  int ctas;
-  int vec;
+  int sms;
 };
-int norm_bwd_ctas(long long rows, int d, int sms);
+int norm_bwd_ctas(long long rows, int d, int sms);   // partials
 cudaError_t launch_norm_bwd(const NormBwdParams& p, cudaStream_t s);
 
 constexpr int kMaxConvWidth = 8;

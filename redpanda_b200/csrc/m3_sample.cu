@@ -508,9 +508,9 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
 
 template <typename T, int NT, bool CACHE>
 cudaError_t sample_typed(const SampleParams& p, cudaStream_t s) {
-  auto* kern = sample_kernel<T, NT, CACHE>;
+  constexpr auto* kern = sample_kernel<T, NT, CACHE>;
   const int smem = ((int)sizeof(Shared) + 15) / 16 * 16 + (CACHE ? (p.V + 3) / 4 * 16 : 0);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = allow_smem<kern>(smem);
   if (e != cudaSuccess) return e;
   kern<<<p.rows, NT, smem, s>>>(p);
   return cudaGetLastError();

@@ -622,12 +622,12 @@ cudaError_t bwd_typed(const SelBwdParams& p, cudaStream_t s) {
   using G = Sel<LN>;
   const unsigned tiles = (unsigned)((p.f.D + G::DT - 1) / G::DT);
   constexpr int smem = (int)sizeof(BwdSmem<T, LN>);
-  auto* main = sel_bwd_kernel<T, LN>;
-  cudaError_t e = cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  constexpr auto* main = sel_bwd_kernel<T, LN>;
+  cudaError_t e = allow_smem<main>(smem);
   if (e != cudaSuccess) return e;
   if (p.f.splits > 1) {
-    auto* sum = sel_bwd_sum_kernel<T, LN>;
-    e = cudaFuncSetAttribute(sum, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    constexpr auto* sum = sel_bwd_sum_kernel<T, LN>;
+    e = allow_smem<sum>(smem);
     if (e != cudaSuccess) return e;
     sum<<<dim3(tiles * p.f.B, p.f.splits - 1), G::NT, smem, s>>>(p);
     const long long total = (long long)p.f.B * p.f.D * G::NP;
@@ -654,15 +654,18 @@ cudaError_t bwd_lanes(const SelBwdParams& p, cudaStream_t s) {
 
 template <typename T, int LN>
 int resident() {
+  static OncePerDevice known;
   constexpr int smem = (int)sizeof(BwdSmem<T, LN>);
-  auto* kern = sel_bwd_kernel<T, LN>;
-  int n = 0;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-          cudaSuccess ||
+  constexpr auto* kern = sel_bwd_kernel<T, LN>;
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) { cudaGetLastError(); return 0; }
+  if ((n = known.value[dev].load(std::memory_order_acquire)) > 0) return n;
+  if (allow_smem<kern>(smem) != cudaSuccess ||
       cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, Sel<LN>::NT, smem) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
+  known.value[dev].store(n, std::memory_order_release);
   return n;
 }
 

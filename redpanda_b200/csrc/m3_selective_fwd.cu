@@ -215,8 +215,8 @@ template <typename T, int LN, bool SUM>
 cudaError_t fwd_launch(const SelParams& p, int runs, cudaStream_t s) {
   using G = Sel<LN>;
   constexpr int smem = (int)sizeof(FwdSmem<T, LN, SUM>);
-  auto* kern = sel_fwd_kernel<T, LN, SUM>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  constexpr auto* kern = sel_fwd_kernel<T, LN, SUM>;
+  const cudaError_t e = allow_smem<kern>(smem);
   if (e != cudaSuccess) return e;
   const unsigned tiles = (unsigned)((p.D + G::DT - 1) / G::DT);
   kern<<<dim3(tiles * p.B, runs), G::NT, smem, s>>>(p);

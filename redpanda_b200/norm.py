@@ -24,7 +24,8 @@ MAX_D = 32768           # longest row of the kernels
 def _forward(x2, ld, w, b, eps, rms, out_dtype, stats):
     rows, d = x2.shape
     dev = x2.get_device()
-    y = torch.empty((rows, d), device=x2.device, dtype=out_dtype)
+    y = (torch.empty_like(x2) if out_dtype is x2.dtype and ld == d
+         else torch.empty((rows, d), device=x2.device, dtype=out_dtype))
     # one buffer: rstd, then (layer norm) the means
     st = torch.empty((1 if rms else 2, rows), device=x2.device) if stats else None
     if rows:
@@ -60,7 +61,7 @@ class _NormFn(torch.autograd.Function):
         dev = x2.get_device()
         if g.dtype is not out_dtype or not g.is_contiguous():
             g = g.to(out_dtype).contiguous()
-        dx = torch.empty((rows, d), device=x2.device, dtype=x2.dtype)
+        dx = torch.empty_like(x2, memory_format=torch.contiguous_format)
         dwb = torch.empty((1 if bt is None else 2, d), device=x2.device)
         dw, db = (dwb[0], None) if bt is None else dwb.unbind(0)
         if rows:

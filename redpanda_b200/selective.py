@@ -89,7 +89,7 @@ def _check_conv(name, x, weight, bias, state, lengths):
 def _conv_fwd(x, ld, w, b, state, lengths, silu, want_state):
     B, L, D = x.shape
     K = w.shape[1]
-    y = torch.empty((B, L, D), device=x.device, dtype=x.dtype)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     out = torch.empty((B, K - 1, D), device=x.device, dtype=x.dtype) if want_state else None
     if B == 0 or L == 0:
         if out is not None:
@@ -130,9 +130,9 @@ class _ConvFn(torch.autograd.Function):
         K = w.shape[1]
         if g.dtype is not x.dtype or not g.is_contiguous():
             g = g.to(x.dtype).contiguous()
-        dx = torch.empty((B, L, D), device=x.device, dtype=x.dtype)
-        dw = torch.empty((D, K), device=x.device)
-        db = None if b is None else torch.empty(D, device=x.device)
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+        dw = torch.empty_like(w)
+        db = None if b is None else torch.empty_like(b)
         if B == 0 or L == 0:
             dw.zero_()
             if db is not None:
@@ -193,7 +193,7 @@ def m3_causal_conv_step_(state, x_t, weight, bias=None, silu=True):
                          "place) and of x_t's element type")
     code = H.code(x_t.dtype)
     dev = H.device_index(x_t, state, weight, bias)
-    y = torch.empty((B, D), device=x_t.device, dtype=x_t.dtype)
+    y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
     if B == 0:
         return y
     x2, ld = H.rows(x_t)
@@ -228,7 +228,7 @@ def _scan_fwd(prepared, A, Dskip, dt_bias, state, lengths, softplus, want_state,
     dev = u.get_device()
     B, L, D = u.shape
     N = A.shape[1]
-    y = torch.empty((B, L, D), device=u.device, dtype=u.dtype)
+    y = torch.empty_like(u, memory_format=torch.contiguous_format)
     h = torch.empty((B, D, N), device=u.device) if want_state else None
     if B == 0 or L == 0:
         if h is not None:
@@ -284,13 +284,15 @@ class _SelectiveScanFn(torch.autograd.Function):
         dev, ty = u.device, u.dtype
         if g.dtype is not ty or not g.is_contiguous():
             g = g.to(ty).contiguous()
-        du, ddt = torch.empty((2, B, L, D), device=dev, dtype=ty).unbind(0)
-        dz = None if z is None else torch.empty((B, L, D), device=dev, dtype=ty)
-        dB = torch.empty((B, L, N), device=dev, dtype=ty)
-        dC = torch.empty((B, L, N), device=dev, dtype=ty)
-        dA = torch.empty((D, N), device=dev)
-        dD = None if Dskip is None else torch.empty(D, device=dev)
-        dbias = None if dt_bias is None else torch.empty(D, device=dev)
+        fresh = torch.contiguous_format
+        du = torch.empty_like(u, memory_format=fresh)
+        ddt = torch.empty_like(u, memory_format=fresh)
+        dz = None if z is None else torch.empty_like(u, memory_format=fresh)
+        dB = torch.empty_like(Bm, memory_format=fresh)
+        dC = torch.empty_like(Cm, memory_format=fresh)
+        dA = torch.empty_like(A)
+        dD = None if Dskip is None else torch.empty_like(Dskip)
+        dbias = None if dt_bias is None else torch.empty_like(dt_bias)
         if B == 0 or L == 0:
             for t in (dA, dD, dbias):
                 if t is not None:
@@ -376,7 +378,7 @@ def m3_selective_step_(h, u_t, dt_t, A, B_t, C_t, D=None, z=None, dt_bias=None, 
     prepared = _prepare(H.rows, u_t, dt_t, z, B_t, C_t)
     dev = H.device_index(h, u_t, dt_t, A, B_t, C_t, D, z, dt_bias)
     ty = prepared[0][0].dtype
-    y = torch.empty((B, d), device=h.device, dtype=ty)
+    y = torch.empty_like(prepared[0][0], memory_format=torch.contiguous_format)
     if B == 0:
         return y
     a32, d32, b32 = H.f32(A), H.f32(D), H.f32(dt_bias)
