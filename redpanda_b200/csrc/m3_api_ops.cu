@@ -49,41 +49,58 @@ int check_sel(const m3_sel_desc* d) {
   return M3_OK;
 }
 
+// Few rows are split along time into runs, of four chunks at least.  The
+// summaries of the runs cost about three quarters of another pass, so fewer
+// than three runs do not pay.
+int time_splits(int nch, long long ctas, long long want) {
+  long long s = want / ctas;
+  if (s > nch / 4) s = nch / 4;
+  if (s < 3) return 1;
+  const int cps = (int)((nch + s - 1) / s);
+  return (nch + cps - 1) / cps;
+}
+
 struct SelLayout {
   int splits, cps, nch, np, tiles, bgroups, workers;
-  size_t fwd_hin, fwd_hsum, fwd_dsum, fwd_total;
-  size_t bwd_bc, bwd_a, bwd_qin, bwd_qsum, bwd_dsum, bwd_total;
+  size_t hin, hsum, dsum;              // the time split's buffers (backward: qin, qsum)
+  size_t bc, a;                        // the backward's partials
+  size_t total;
 };
 
-bool sel_layout(const m3_sel_desc* d, SelLayout* l) {
+bool sel_layout(const m3_sel_desc* d, bool backward, SelLayout* l) {
   const int sms = device_sms();
   if (sms <= 0) return false;
+  const int per = backward ? sel_bwd_resident(d->d_state, d->dtype)
+                           : sel_fwd_resident(d->d_state, d->dtype);
+  if (per <= 0) return false;
   const int ln = sel_lanes(d->d_state);
+  const int tile = backward ? sel_tile(ln) : sel_fwd_tile(d->d_state);
+  const long long wave = (long long)per * sms;
   l->np = 4 * ln;
   l->nch = (d->seqlen + kSelSteps - 1) / kSelSteps;
-  l->tiles = (d->d_inner + sel_tile(ln) - 1) / sel_tile(ln);
-  l->splits = sel_splits(d->batch, d->seqlen, d->d_inner, d->d_state, sms);
+  l->tiles = (d->d_inner + tile - 1) / tile;
+  // runs for two waves forward and three backward, whose summaries run on
+  // narrower CTAs than the pass itself (2 x 4001 x 1536 steps, N = 16, fp32:
+  // 544 us against 608 us for one and two waves)
+  l->splits = time_splits(l->nch, (long long)d->batch * l->tiles, (backward ? 3 : 2) * wave);
   l->cps = (l->nch + l->splits - 1) / l->splits;
   // backward: CTAs walk rows of the batch, one wave of them
-  const int per = sel_bwd_resident(d->d_state, d->dtype);
-  if (per <= 0) return false;
-  long long bg = (long long)per * sms / ((long long)l->tiles * l->splits);
+  long long bg = wave / ((long long)l->tiles * l->splits);
   if (bg > d->batch) bg = d->batch;
   if (bg < 1) bg = 1;
   l->bgroups = (int)bg;
   l->workers = l->bgroups * l->splits;
   const size_t run = round256((size_t)l->splits * d->batch * d->d_inner * l->np * 4);
   const size_t sums = round256((size_t)l->splits * d->batch * d->d_inner * 4);
-  l->fwd_hin = 0;
-  l->fwd_hsum = run;
-  l->fwd_dsum = 2 * run;
-  l->fwd_total = l->splits > 1 ? 2 * run + sums : 0;
-  l->bwd_bc = 0;
-  l->bwd_a = round256((size_t)l->tiles * d->batch * d->seqlen * 2 * l->np * 4);
-  l->bwd_qin = l->bwd_a + round256((size_t)l->workers * d->d_inner * (l->np + 2) * 4);
-  l->bwd_qsum = l->bwd_qin + run;
-  l->bwd_dsum = l->bwd_qsum + run;
-  l->bwd_total = l->splits > 1 ? l->bwd_dsum + sums : l->bwd_qin;
+  l->hin = 0;
+  l->hsum = run;
+  l->dsum = 2 * run;
+  l->bc = l->splits > 1 ? 2 * run + sums : 0;
+  l->total = l->bc;
+  if (backward) {
+    l->a = l->bc + round256((size_t)l->tiles * d->batch * d->seqlen * 2 * l->np * 4);
+    l->total = l->a + round256((size_t)l->workers * d->d_inner * (l->np + 2) * 4);
+  }
   return true;
 }
 
@@ -257,8 +274,8 @@ size_t m3_selective_ckpt_floats(const m3_sel_desc* desc) {
 
 size_t m3_selective_fwd_workspace_bytes(const m3_sel_desc* desc) {
   SelLayout l;
-  if (check_sel(desc) != M3_OK || !sel_layout(desc, &l)) return 0;
-  return l.fwd_total;
+  if (check_sel(desc) != M3_OK || !sel_layout(desc, false, &l)) return 0;
+  return l.total;
 }
 
 int m3_selective_fwd(const m3_sel_desc* desc, const m3_sel_args* args, void* y, float* h_last,
@@ -276,24 +293,24 @@ int m3_selective_fwd(const m3_sel_desc* desc, const m3_sel_args* args, void* y, 
   memset(&l, 0, sizeof(l));
   if ((rc = fill_sel(desc, args, l, &p)) != M3_OK) return rc;
   if ((rc = check_device()) != M3_OK) return rc;
-  if (!sel_layout(desc, &l)) return M3_ERR_NO_DEVICE;
-  if (l.fwd_total && (!workspace || workspace_bytes < l.fwd_total)) return M3_ERR_WORKSPACE;
+  if (!sel_layout(desc, false, &l)) return M3_ERR_NO_DEVICE;
+  if (l.total && (!workspace || workspace_bytes < l.total)) return M3_ERR_WORKSPACE;
   fill_sel(desc, args, l, &p);
   p.vec_d = p.vec_d && aligned(y, 16);
   p.y = y; p.h_last = h_last; p.ckpt = l.nch > 1 ? ckpt : nullptr;
   if (l.splits > 1) {
     char* ws = static_cast<char*>(workspace);
-    p.hin = reinterpret_cast<float*>(ws + l.fwd_hin);
-    p.hsum = reinterpret_cast<float*>(ws + l.fwd_hsum);
-    p.dsum = reinterpret_cast<float*>(ws + l.fwd_dsum);
+    p.hin = reinterpret_cast<float*>(ws + l.hin);
+    p.hsum = reinterpret_cast<float*>(ws + l.hsum);
+    p.dsum = reinterpret_cast<float*>(ws + l.dsum);
   }
   return status(launch_sel_fwd(p, static_cast<cudaStream_t>(stream)));
 }
 
 size_t m3_selective_bwd_workspace_bytes(const m3_sel_desc* desc) {
   SelLayout l;
-  if (check_sel(desc) != M3_OK || !sel_layout(desc, &l)) return 0;
-  return l.bwd_total;
+  if (check_sel(desc) != M3_OK || !sel_layout(desc, true, &l)) return 0;
+  return l.total;
 }
 
 int m3_selective_bwd(const m3_sel_desc* desc, const m3_sel_args* args, const void* g,
@@ -317,8 +334,8 @@ int m3_selective_bwd(const m3_sel_desc* desc, const m3_sel_args* args, const voi
   memset(&l, 0, sizeof(l));
   if ((rc = fill_sel(desc, args, l, &p.f)) != M3_OK) return rc;
   if ((rc = check_device()) != M3_OK) return rc;
-  if (!sel_layout(desc, &l)) return M3_ERR_NO_DEVICE;
-  if (!workspace || workspace_bytes < l.bwd_total) return M3_ERR_WORKSPACE;
+  if (!sel_layout(desc, true, &l)) return M3_ERR_NO_DEVICE;
+  if (!workspace || workspace_bytes < l.total) return M3_ERR_WORKSPACE;
   if (l.nch > 1 && !ckpt) return M3_ERR_NULL;
   fill_sel(desc, args, l, &p.f);
   p.f.ckpt = const_cast<float*>(ckpt);
@@ -326,12 +343,12 @@ int m3_selective_bwd(const m3_sel_desc* desc, const m3_sel_args* args, const voi
   p.du = grads->d_u; p.ddt = grads->d_dt; p.dz = grads->d_z; p.dB = grads->d_B;
   p.dC = grads->d_C; p.dA = grads->d_A; p.dD = grads->d_skip; p.dbias = grads->d_dt_bias;
   char* ws = static_cast<char*>(workspace);
-  p.part_bc = reinterpret_cast<float*>(ws + l.bwd_bc);
-  p.part_a = reinterpret_cast<float*>(ws + l.bwd_a);
+  p.part_bc = reinterpret_cast<float*>(ws + l.bc);
+  p.part_a = reinterpret_cast<float*>(ws + l.a);
   if (l.splits > 1) {
-    p.qin = reinterpret_cast<float*>(ws + l.bwd_qin);
-    p.qsum = reinterpret_cast<float*>(ws + l.bwd_qsum);
-    p.f.dsum = reinterpret_cast<float*>(ws + l.bwd_dsum);
+    p.qin = reinterpret_cast<float*>(ws + l.hin);
+    p.qsum = reinterpret_cast<float*>(ws + l.hsum);
+    p.f.dsum = reinterpret_cast<float*>(ws + l.dsum);
   }
   p.workers = l.workers;
   p.bgroups = l.bgroups;

@@ -70,4 +70,19 @@ inline int dsize(int dt) { return dt == M3_BF16 ? 2 : 4; }
 inline bool aligned(const void* p, int a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 inline size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+// CTAs of a kernel that an SM holds, 0 on an error; asked for once per device.
+template <auto* kern>
+int resident_ctas(OncePerDevice& known, int threads, int smem) {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) { cudaGetLastError(); return 0; }
+  if ((n = known.value[dev].load(std::memory_order_acquire)) > 0) return n;
+  if (allow_smem<kern>(smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  known.value[dev].store(n, std::memory_order_release);
+  return n;
+}
+
 }  // namespace m3

@@ -29,11 +29,8 @@
 namespace m3 {
 namespace {
 
-#ifndef M3_T3
-#define M3_T3 8
-#endif
 constexpr int kAhead = 4;      // rows in flight per thread (backward: of x and dy, twice)
-constexpr int kAheadFwd = M3_T3;
+constexpr int kAheadFwd = 8;
 
 // V fp32 values as packed pairs (V = 1: the second half idles).
 template <int V> struct Vals {

@@ -28,9 +28,6 @@
 #include "m3_ops.h"
 #include "m3_vec.cuh"
 
-#ifndef M3_T2
-#define M3_T2 1
-#endif
 namespace m3 {
 namespace {
 
@@ -349,7 +346,7 @@ struct LaunchFwd {
   cudaError_t operator()(int nt) {
     const int rpc = WARP ? MAXT / 32 : 1;
     const long long want = (p.rows + rpc - 1) / rpc;
-    const long long cap = (long long)p.sms * (WARP ? MINB * M3_T2 : norm_per_sm(p.d, nt));
+    const long long cap = (long long)p.sms * (WARP ? MINB : norm_per_sm(p.d, nt));
     const int grid = (int)(want < cap ? want : cap);
     if (p.rms) norm_fwd_kernel<TX, TY, VEC, NV, WARP, MAXT, MINB, true><<<grid, nt, 0, s>>>(p);
     else norm_fwd_kernel<TX, TY, VEC, NV, WARP, MAXT, MINB, false><<<grid, nt, 0, s>>>(p);

@@ -109,8 +109,10 @@ struct SelParams {
   float* hin; float* hsum; float* dsum;
   int vec_d, vec_n;                                      // vector rows allowed
 };
-int sel_splits(int B, int L, int D, int N, int sms);
-int sel_bwd_resident(int N, int dtype);                // CTAs of the backward per SM, 0: error
+// CTAs per SM of the forward and the backward (0: error), channels per forward CTA.
+int sel_fwd_resident(int N, int dtype);
+int sel_bwd_resident(int N, int dtype);
+inline int sel_fwd_tile(int N) { return N <= 8 ? 128 : 64; }
 cudaError_t launch_sel_fwd(const SelParams& p, cudaStream_t s);
 
 struct SelBwdParams {

@@ -6,7 +6,7 @@
 //   y_t  = (sum_n C_t h_t + D u_t) silu(z_t)
 //
 // Layout: a lane group of LN threads owns two adjacent channels; thread q of the
-// group holds states 4q .. 4q+3 of both.  Steps are staged kSelSteps at a time
+// group holds states Sq .. Sq+S-1 of both (S = 8 forward, 4 backward).  Steps are staged kSelSteps at a time
 // through shared memory; a step past the row's length is staged with de = 0,
 // which leaves the state as it is (exp(0) = 1, nothing added), so no branch on
 // the length is left in the recurrence.  State products are packed pairs of
@@ -26,13 +26,24 @@ namespace m3 {
 
 constexpr int kS = kSelSteps;
 
-template <int LN> struct Sel {
-  static constexpr int NT = LN >= 16 ? 256 : 128;   // threads per CTA
+// A kernel's tiling: LN lanes per pair of channels, S states per lane and channel,
+// NT threads per CTA.
+template <int LN_, int S_, int NT_> struct Tiling {
+  static constexpr int LN = LN_, S = S_, NT = NT_;
   static constexpr int DT = NT / LN * 2;            // channels per CTA
-  static constexpr int NP = 4 * LN;                 // states kept per channel
+  static constexpr int NP = S * LN;                 // states kept per channel
   static constexpr int EPT = kS * DT / NT;          // staged elements per thread and tensor
-  static constexpr int QPT = (kS * LN + NT - 1) / NT;   // staged state quads per thread (B or C)
+  static constexpr int QUADS = kS * NP / 4;         // staged state quads of B (or C)
+  static constexpr int QPT = (QUADS + NT - 1) / NT; // per thread
 };
+// Backward: four states per lane (its registers hold gates and products of four
+// steps).
+template <int LN> using Sel = Tiling<LN, 4, (LN >= 16 ? 256 : 128)>;
+// Forward and the summaries: eight.  Every register filled from shared memory
+// costs the SM a cycle of its 128 bytes per clock, however many lanes share
+// the value; a lane with more states uses a step's B and C for two channels and
+// its step size for eight states.
+template <int LN> using SelF = Tiling<LN, 8, (LN >= 2 ? 32 * LN : 64)>;
 
 __device__ __forceinline__ int sel_length(const int* lengths, int b, int L) {
   if (lengths == nullptr) return L;
@@ -112,69 +123,46 @@ __device__ __forceinline__ float2 ex2_pair(float2 x) {
   return make_float2(ex2_approx(x.x), ex2_approx(x.y));
 }
 
-// A2 = A log2(e) of the thread's states of channels c, c+1 (zero past D or N,
-// where the state stays zero).
-__device__ __forceinline__ void load_a2(float2 (&a2)[2][2], const float* A, int c, int n0, int D,
-                                        int N) {
+// A quad 4q .. 4q+3 of channel c in a (rows, D, N) tensor by element loads (zero
+// past D or N), and in a padded (rows, D, NP) buffer.
+__device__ __forceinline__ float4 load_quad_any(const float* src, size_t row, int c, int n0, int D,
+                                                int N) {
+  float v[4];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      v[j] = (c + k < D && n0 + j < N) ? A[(size_t)(c + k) * N + n0 + j] * kLog2e : 0.f;
-    a2[k][0] = make_float2(v[0], v[1]);
-    a2[k][1] = make_float2(v[2], v[3]);
-  }
+  for (int j = 0; j < 4; ++j)
+    v[j] = (src != nullptr && c < D && n0 + j < N) ? src[(row * D + c) * N + n0 + j] : 0.f;
+  return make_float4(v[0], v[1], v[2], v[3]);
 }
-
-// The thread's states of channels c, c+1 from / to a (B, D, N) tensor.
-__device__ __forceinline__ void load_state(float2 (&h)[2][2], const float* src, size_t b, int c,
-                                           int n0, int D, int N) {
+__device__ __forceinline__ void store_quad_any(float4 x, float* dst, size_t row, int c, int n0,
+                                               int D, int N) {
+  const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      v[j] = (src != nullptr && c + k < D && n0 + j < N)
-                 ? src[(b * D + c + k) * N + n0 + j] : 0.f;
-    h[k][0] = make_float2(v[0], v[1]);
-    h[k][1] = make_float2(v[2], v[3]);
-  }
+  for (int j = 0; j < 4; ++j)
+    if (c < D && n0 + j < N) dst[(row * D + c) * N + n0 + j] = v[j];
 }
-__device__ __forceinline__ void store_state(const float2 (&h)[2][2], float* dst, size_t b, int c,
-                                            int n0, int D, int N) {
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const float v[4] = {h[k][0].x, h[k][0].y, h[k][1].x, h[k][1].y};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + k < D && n0 + j < N) dst[(b * D + c + k) * N + n0 + j] = v[j];
-  }
+__device__ __forceinline__ float4 load_quad_pad(const float* src, size_t row, int c, int n0, int D,
+                                                int NP) {
+  return c < D ? *reinterpret_cast<const float4*>(src + (row * D + c) * NP + n0)
+               : make_float4(0.f, 0.f, 0.f, 0.f);
 }
-// The same for the padded (rows, D, NP) buffers (16-byte aligned quads).
-__device__ __forceinline__ void load_quads(float2 (&h)[2][2], const float* src, size_t row, int c,
-                                           int q, int D, int NP) {
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c + k < D) v = *reinterpret_cast<const float4*>(src + (row * D + c + k) * NP + 4 * q);
-    h[k][0] = make_float2(v.x, v.y);
-    h[k][1] = make_float2(v.z, v.w);
-  }
+__device__ __forceinline__ void store_quad_pad(float4 v, float* dst, size_t row, int c, int n0,
+                                               int D, int NP) {
+  if (c < D) *reinterpret_cast<float4*>(dst + (row * D + c) * NP + n0) = v;
 }
-__device__ __forceinline__ void store_quads(const float2 (&h)[2][2], float* dst, size_t row, int c,
-                                            int q, int D, int NP) {
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (c + k < D)
-      *reinterpret_cast<float4*>(dst + (row * D + c + k) * NP + 4 * q) =
-          make_float4(h[k][0].x, h[k][0].y, h[k][1].x, h[k][1].y);
+__device__ __forceinline__ void set_pairs(float2* h, float4 v) {
+  h[0] = make_float2(v.x, v.y);
+  h[1] = make_float2(v.z, v.w);
+}
+__device__ __forceinline__ float4 quad_of(const float2* h) {
+  return make_float4(h[0].x, h[0].y, h[1].x, h[1].y);
+}
+__device__ __forceinline__ float4 scaled(float4 v, float a) {
+  return make_float4(v.x * a, v.y * a, v.z * a, v.w * a);
 }
 
 // ------------------------------------------------------------- staged rows
 // Element e of a thread in a (kS, DT) tile: VW consecutive channels at a time.
-template <typename T, int LN> struct TileMap {
-  using G = Sel<LN>;
+template <typename T, typename G> struct TileMap {
   static constexpr int VMAX = 16 / (int)sizeof(T);
   static constexpr int VW = G::EPT < VMAX ? G::EPT : VMAX;   // channels per load
   static constexpr int NVEC = G::EPT / VW;
@@ -186,6 +174,15 @@ template <typename T, int LN> struct TileMap {
     return ((int)threadIdx.x + i * G::NT) % PER_ROW * VW;
   }
 };
+
+// Where the pair of channels (2 p, 2 p + 1) of a staged row stands, in pairs of 16
+// bytes: a thread stages VW neighbouring channels, so without a permutation the
+// threads of a warp would meet in VW / 4 of the banks.
+template <typename M>
+__device__ __forceinline__ int pair_at(int p) {
+  constexpr int UPT = M::VW >= 2 ? M::VW / 2 : 1;
+  return p ^ ((p >> 3) & (UPT - 1));
+}
 
 // A thread's own copy of what it will stage, filled ahead of use: 4, 8 or 16
 // bytes at a time by cp.async, so that loads are in flight over a whole group of
@@ -207,17 +204,17 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src, bool in) 
 // The thread's elements of rows [t0, t0 + kS) of a (L, ld) tensor whose first row
 // is base into its slots (slot[i] of thread x at slots[i * NT + x]); rows at or
 // past n and channels past D become zero.
-template <typename T, int LN>
-__device__ __forceinline__ void fetch_tile(Pack<T, TileMap<T, LN>::VW>* slots, const T* base,
+template <typename T, typename G>
+__device__ __forceinline__ void fetch_tile(Pack<T, TileMap<T, G>::VW>* slots, const T* base,
                                            long long ld, int t0, int n, int c0, int D, bool vec) {
-  using M = TileMap<T, LN>;
+  using M = TileMap<T, G>;
   constexpr int BYTES = M::VW * (int)sizeof(T);
 #pragma unroll
   for (int i = 0; i < M::NVEC; ++i) {
     const int t = t0 + M::row(i), c = c0 + M::col(i);
     const bool in = t < n && c < D;
     const T* p = base + (in ? (size_t)t * ld + c : 0);
-    Pack<T, M::VW>* dst = slots + i * Sel<LN>::NT + threadIdx.x;
+    Pack<T, M::VW>* dst = slots + i * G::NT + threadIdx.x;
     if (BYTES >= 4 && vec) {   // D is a multiple of VW
       copy_async<(BYTES >= 4 ? BYTES : 4)>(dst, p, in);
     } else {
@@ -230,10 +227,10 @@ __device__ __forceinline__ void fetch_tile(Pack<T, TileMap<T, LN>::VW>* slots, c
     }
   }
 }
-template <typename T, int LN>
-__device__ __forceinline__ void store_tile(const Pack<T, TileMap<T, LN>::VW>& v, int i, T* base,
+template <typename T, typename G>
+__device__ __forceinline__ void store_tile(const Pack<T, TileMap<T, G>::VW>& v, int i, T* base,
                                            long long ld, int t0, int L, int c0, int D, bool vec) {
-  using M = TileMap<T, LN>;
+  using M = TileMap<T, G>;
   const int t = t0 + M::row(i), c = c0 + M::col(i);
   if (t < L && c < D) {
     T* p = base + (size_t)t * ld + c;
@@ -246,15 +243,14 @@ __device__ __forceinline__ void store_tile(const Pack<T, TileMap<T, LN>::VW>& v,
 }
 
 // The thread's state quads of rows [t0, t0 + kS) of B or C into its slots.
-template <typename T, int LN>
+template <typename T, typename G>
 __device__ __forceinline__ void fetch_quads(Pack<T, 4>* slots, const T* base, long long ld, int t0,
                                             int n, int N, bool vec) {
-  using G = Sel<LN>;
 #pragma unroll
   for (int i = 0; i < G::QPT; ++i) {
     const int e = (int)threadIdx.x + i * G::NT;
-    const int t = t0 + e / LN, k = e % LN * 4;
-    const bool in = e < kS * LN && t < n && k < N;
+    const int t = t0 + e / (G::NP / 4), k = e % (G::NP / 4) * 4;
+    const bool in = e < G::QUADS && t < n && k < N;
     const T* p = base + (in ? (size_t)t * ld + k : 0);
     Pack<T, 4>* dst = slots + i * G::NT + threadIdx.x;
     if (vec) {                 // N is a multiple of 4

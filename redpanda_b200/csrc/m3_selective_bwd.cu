@@ -49,20 +49,28 @@ template <int LN> struct Order {
 
 template <typename T, int LN> struct BwdSmem {
   using G = Sel<LN>;
-  using M = TileMap<T, LN>;
+  using M = TileMap<T, Sel<LN>>;
   using Tile = Pack<T, M::VW>[M::NVEC * G::NT];
   using Quads = Pack<T, 4>[G::QPT * G::NT];
   static constexpr int NW = G::NT / 32, CP = Order<LN>::COPIES;
   alignas(16) float B[CP][kS * G::NP], C[CP][kS * G::NP];
-  alignas(16) float2 D[kS][G::DT];           // (de, de u)
+  alignas(16) float2 D[kS][G::DT];           // (de, de u), at chan_at(channel)
   alignas(16) float Y[kS][G::DT];            // gy
-  alignas(16) float P[kS][G::DT];            // the step size's slope
+  alignas(16) float P[G::EPT][G::NT];        // a thread's own: the step sizes' slopes
   alignas(16) float4 H[kNSub][2][G::NT];     // states at each group's start
-  alignas(16) float R[kS][3][G::DT];         // s1, s2 (in units of 1/log2 e), C.h
+  // s1, s2 (in units of 1/log2 e), C.h; the padding spreads a warp's steps over
+  // the banks
+  alignas(16) float R[kS][3][G::DT + 8];
   alignas(16) float BC[2][kSub][NW][2 * G::NP];   // warps' sums of dB, dC
   alignas(16) Tile u[2], z[2], g[2], dt;
   alignas(16) Quads b, c;
 };
+
+// Where a channel of a staged row stands (pairs as pair_at places them).
+template <typename M>
+__device__ __forceinline__ int chan_at(int c) {
+  return 2 * pair_at<M>(c / 2) + (c & 1);
+}
 
 // A quad in a lane's order, and back.
 __device__ __forceinline__ float4 reorder(float4 v, int pair, int elem) {
@@ -70,47 +78,23 @@ __device__ __forceinline__ float4 reorder(float4 v, int pair, int elem) {
   if (elem) v = make_float4(v.y, v.x, v.w, v.z);
   return v;
 }
-__device__ __forceinline__ void set_pairs(float2 (&h)[2], float4 v) {
-  h[0] = make_float2(v.x, v.y);
-  h[1] = make_float2(v.z, v.w);
-}
-__device__ __forceinline__ float4 quad_of(const float2 (&h)[2]) {
-  return make_float4(h[0].x, h[0].y, h[1].x, h[1].y);
-}
-// The quad 4q .. 4q+3 of channel c in a (D, N) or (rows, D, N) tensor, element
-// loads (zero past D or N).
-__device__ __forceinline__ float4 load_quad_any(const float* src, size_t row, int c, int n0, int D,
-                                                int N) {
-  float v[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    v[j] = (src != nullptr && c < D && n0 + j < N) ? src[(row * D + c) * N + n0 + j] : 0.f;
-  return make_float4(v[0], v[1], v[2], v[3]);
-}
-__device__ __forceinline__ float4 load_quad_pad(const float* src, size_t row, int c, int q, int D,
-                                                int NP) {
-  return c < D ? *reinterpret_cast<const float4*>(src + (row * D + c) * NP + 4 * q)
-               : make_float4(0.f, 0.f, 0.f, 0.f);
-}
-
 __device__ __forceinline__ float2 shfl_pair(float2 v, int m) {
   return make_float2(__shfl_xor_sync(0xffffffffu, v.x, m), __shfl_xor_sync(0xffffffffu, v.y, m));
 }
 
 // The chunk's staged values from the thread's slots (t0: first step).
-template <typename T, int LN, bool SUM>
+template <typename T, int LN>
 __device__ __forceinline__ void bwd_stage(BwdSmem<T, LN>& sm, const SelParams& p, int buf, int t0,
                                           int n, bool gate,
-                                          const float (&bias)[TileMap<T, LN>::VW]) {
+                                          const float (&bias)[TileMap<T, Sel<LN>>::VW]) {
   using G = Sel<LN>;
-  using M = TileMap<T, LN>;
+  using M = TileMap<T, Sel<LN>>;
 #pragma unroll
   for (int i = 0; i < M::NVEC; ++i) {
     const int r = M::row(i), cc = M::col(i), x = i * G::NT + threadIdx.x;
     const bool live = t0 + r < n;
-    const Pack<T, M::VW> cd = sm.dt[x], cg = sm.g[buf][x];
-    Pack<T, M::VW> cu, cz;
-    if (!SUM) cu = sm.u[buf][x];
+    const Pack<T, M::VW> cd = sm.dt[x], cg = sm.g[buf][x], cu = sm.u[buf][x];
+    Pack<T, M::VW> cz;
     if (gate) cz = sm.z[buf][x];
 #pragma unroll
     for (int j = 0; j < M::VW; ++j) {
@@ -118,29 +102,24 @@ __device__ __forceinline__ void bwd_stage(BwdSmem<T, LN>& sm, const SelParams& p
       const float de = live ? step_size(cd.get(j) + bias[j], p.softplus, &slope) : 0.f;
       float gy = cg.get(j);
       if (gate) gy *= silu_f(cz.get(j));
-      const float du = SUM ? 0.f : de * cu.get(j);
-      sm.D[r][cc + j] = make_float2(de, du);
+      sm.D[r][chan_at<M>(cc + j)] = make_float2(de, de * cu.get(j));
       sm.Y[r][cc + j] = gy;
-      if (!SUM) sm.P[r][cc + j] = slope;
+      sm.P[i * M::VW + j][threadIdx.x] = slope;
     }
   }
 #pragma unroll
   for (int i = 0; i < G::QPT; ++i) {
     const int e = (int)threadIdx.x + i * G::NT;
-    if (e < kS * LN) {
-      const Pack<T, 4> vc = sm.c[e];
+    if (e < G::QUADS) {
+      const Pack<T, 4> vb = sm.b[e], vc = sm.c[e];
+      const float4 b4 = make_float4(vb.get(0), vb.get(1), vb.get(2), vb.get(3));
       const float4 c4 = make_float4(vc.get(0), vc.get(1), vc.get(2), vc.get(3));
-      float4 b4 = c4;
-      if (!SUM) {
-        const Pack<T, 4> vb = sm.b[e];
-        b4 = make_float4(vb.get(0), vb.get(1), vb.get(2), vb.get(3));
-      }
 #pragma unroll
-      for (int k = 0; k < (SUM ? 1 : Order<LN>::COPIES); ++k) {
+      for (int k = 0; k < Order<LN>::COPIES; ++k) {
         const int pair = Order<LN>::COPIES >= 4 ? k >> 1 : k;
         const int elem = Order<LN>::COPIES >= 4 ? k & 1 : 0;
         *reinterpret_cast<float4*>(sm.C[k] + 4 * e) = reorder(c4, pair, elem);
-        if (!SUM) *reinterpret_cast<float4*>(sm.B[k] + 4 * e) = reorder(b4, pair, elem);
+        *reinterpret_cast<float4*>(sm.B[k] + 4 * e) = reorder(b4, pair, elem);
       }
     }
   }
@@ -160,18 +139,17 @@ template <typename T> struct RowPtrs {
   }
 };
 
-template <typename T, int LN, bool SUM>
+template <typename T, int LN>
 __device__ __forceinline__ void bwd_fetch(BwdSmem<T, LN>& sm, const SelBwdParams& bp,
                                           const RowPtrs<T>& r, int buf, int t0, int n, int c0) {
+  using G = Sel<LN>;
   const SelParams& p = bp.f;
-  fetch_tile<T, LN>(sm.dt, r.dt, p.ld_dt, t0, n, c0, p.D, p.vec_d);
-  fetch_tile<T, LN>(sm.g[buf], r.g, p.D, t0, n, c0, p.D, bp.vec_g);
-  if (r.z) fetch_tile<T, LN>(sm.z[buf], r.z, p.ld_z, t0, n, c0, p.D, p.vec_d);
-  fetch_quads<T, LN>(sm.c, r.C, p.ld_c, t0, n, p.N, p.vec_n);
-  if (!SUM) {
-    fetch_tile<T, LN>(sm.u[buf], r.u, p.ld_u, t0, n, c0, p.D, p.vec_d);
-    fetch_quads<T, LN>(sm.b, r.B, p.ld_b, t0, n, p.N, p.vec_n);
-  }
+  fetch_tile<T, G>(sm.dt, r.dt, p.ld_dt, t0, n, c0, p.D, p.vec_d);
+  fetch_tile<T, G>(sm.g[buf], r.g, p.D, t0, n, c0, p.D, bp.vec_g);
+  if (r.z) fetch_tile<T, G>(sm.z[buf], r.z, p.ld_z, t0, n, c0, p.D, p.vec_d);
+  fetch_quads<T, G>(sm.c, r.C, p.ld_c, t0, n, p.N, p.vec_n);
+  fetch_tile<T, G>(sm.u[buf], r.u, p.ld_u, t0, n, c0, p.D, p.vec_d);
+  fetch_quads<T, G>(sm.b, r.B, p.ld_b, t0, n, p.N, p.vec_n);
   copies_commit();
 }
 
@@ -185,7 +163,7 @@ template <typename T, int LN>
 __global__ void __launch_bounds__(Sel<LN>::NT, bwd_min_ctas<LN>())
 sel_bwd_kernel(const SelBwdParams bp) {
   using G = Sel<LN>;
-  using M = TileMap<T, LN>;
+  using M = TileMap<T, Sel<LN>>;
   using Sm = BwdSmem<T, LN>;
   using O = Order<LN>;
   const SelParams& p = bp.f;
@@ -200,6 +178,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
   // group's lanes takes the second channel first)
   const int pr = O::pair(lane), el = O::elem(lane), up = (q & (LN / 2)) != 0;
   const int cc2[2] = {2 * grp + up, 2 * grp + 1 - up};
+  const int ca[2] = {chan_at<M>(cc2[0]), chan_at<M>(cc2[1])};
   const float* sB = sm.B[O::COPIES >= 4 ? 2 * pr + el : pr];
   const float* sC = sm.C[O::COPIES >= 4 ? 2 * pr + el : pr];
 
@@ -207,8 +186,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const float4 v = load_quad_any(p.A, 0, c0 + cc2[k], n0, p.D, p.N);
-    set_pairs(a2[k], reorder(make_float4(v.x * kLog2e, v.y * kLog2e, v.z * kLog2e, v.w * kLog2e),
-                             pr, el));
+    set_pairs(a2[k], reorder(scaled(v, kLog2e), pr, el));
     dA[k][0] = dA[k][1] = make_float2(0.f, 0.f);
   }
   // a thread's staged elements share their columns
@@ -237,18 +215,18 @@ sel_bwd_kernel(const SelBwdParams bp) {
 #pragma unroll
       for (int i = 0; i < M::NVEC; ++i) {
         const auto zero = zero_pack<T, M::VW>();
-        store_tile<T, LN>(zero, i, du, p.D, ch * kS, p.L, c0, p.D, vec);
-        store_tile<T, LN>(zero, i, ddt, p.D, ch * kS, p.L, c0, p.D, vec);
-        if (dz) store_tile<T, LN>(zero, i, dz, p.D, ch * kS, p.L, c0, p.D, vec);
+        store_tile<T, G>(zero, i, du, p.D, ch * kS, p.L, c0, p.D, vec);
+        store_tile<T, G>(zero, i, ddt, p.D, ch * kS, p.L, c0, p.D, vec);
+        if (dz) store_tile<T, G>(zero, i, dz, p.D, ch * kS, p.L, c0, p.D, vec);
       }
     if (ch < ch0) continue;
-    bwd_fetch<T, LN, false>(sm, bp, rp, ch & 1, ch * kS, n, c0);
+    bwd_fetch<T, LN>(sm, bp, rp, ch & 1, ch * kS, n, c0);
     float2 dh[2][2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (bp.qin != nullptr && split + 1 < p.splits)
-        v = load_quad_pad(bp.qin, (size_t)split * p.B + b, c0 + cc2[k], q, p.D, G::NP);
+        v = load_quad_pad(bp.qin, (size_t)split * p.B + b, c0 + cc2[k], n0, p.D, G::NP);
       set_pairs(dh[k], reorder(v, pr, el));
     }
 
@@ -258,13 +236,13 @@ sel_bwd_kernel(const SelBwdParams bp) {
       float2 h[2][2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        set_pairs(h[k], ch > 0 ? load_quad_pad(p.ckpt, b * (p.nch - 1) + ch - 1, c0 + cc2[k], q,
+        set_pairs(h[k], ch > 0 ? load_quad_pad(p.ckpt, b * (p.nch - 1) + ch - 1, c0 + cc2[k], n0,
                                                p.D, G::NP)
                                : load_quad_any(p.h0, b, c0 + cc2[k], n0, p.D, p.N));
       copies_wait();
-      bwd_stage<T, LN, false>(sm, p, buf, t0, n, gate, bias);
+      bwd_stage<T, LN>(sm, p, buf, t0, n, gate, bias);
       __syncthreads();
-      if (ch > ch0) bwd_fetch<T, LN, false>(sm, bp, rp, buf ^ 1, t0 - kS, n, c0);
+      if (ch > ch0) bwd_fetch<T, LN>(sm, bp, rp, buf ^ 1, t0 - kS, n, c0);
 #pragma unroll
       for (int k = 0; k < 2; ++k) set_pairs(h[k], reorder(quad_of(h[k]), pr, el));
       // states at every group's start
@@ -280,7 +258,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
           set_pairs(b2, *reinterpret_cast<const float4*>(sB + t * G::NP + n0));
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float2 dd = sm.D[t][cc2[k]];
+            const float2 dd = sm.D[t][ca[k]];
             const float2 de = f2(dd.x), deu = f2(dd.y);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
@@ -304,7 +282,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
           float ys[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float2 dd = sm.D[t][cc2[k]];
+            const float2 dd = sm.D[t][ca[k]];
             const float2 de = f2(dd.x), deu = f2(dd.y);
             float2 y2;
 #pragma unroll
@@ -329,7 +307,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
           float x1[2], x2[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float2 dd = sm.D[t][cc2[k]];
+            const float2 dd = sm.D[t][ca[k]];
             const float2 de = f2(dd.x), deu = f2(dd.y);
             const float2 gy = f2(sm.Y[t][cc2[k]]);
             float2 y1, y2;
@@ -410,7 +388,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
           if (M2 <= 1 || (q & (M2 - 1)) == 0)
 #pragma unroll
             for (int i = 0; i < KEEP; ++i) {
-              float (*o)[G::DT] = sm.R[sub * kSub + s0 + i];
+              float (*o)[G::DT + 8] = sm.R[sub * kSub + s0 + i];
               o[0][cc2[0]] = s1[i];
               o[1][cc2[0]] = s2[i];
               o[2][cc2[0]] = sy[i];
@@ -438,8 +416,8 @@ sel_bwd_kernel(const SelBwdParams bp) {
           const float gy = sm.Y[r][cc + j];
           const float v1 = sm.R[r][0][cc + j], v2 = sm.R[r][1][cc + j] * kLn2;
           const float uu = cu.get(j);
-          odu.put(j, fmaf(dsk[j], gy, sm.D[r][cc + j].x * v1));
-          const float d = fmaf(uu, v1, v2) * sm.P[r][cc + j];
+          odu.put(j, fmaf(dsk[j], gy, sm.D[r][chan_at<M>(cc + j)].x * v1));
+          const float d = fmaf(uu, v1, v2) * sm.P[i * M::VW + j][threadIdx.x];
           oddt.put(j, d);
           dD[j] = fmaf(gy, uu, dD[j]);
           dbias[j] += d;
@@ -448,9 +426,9 @@ sel_bwd_kernel(const SelBwdParams bp) {
             odz.put(j, cg.get(j) * yp * dsilu_f(zz, sigmoid_f(zz)));
           }
         }
-        store_tile<T, LN>(odu, i, du, p.D, t0, p.L, c0, p.D, vec);
-        store_tile<T, LN>(oddt, i, ddt, p.D, t0, p.L, c0, p.D, vec);
-        if (dz) store_tile<T, LN>(odz, i, dz, p.D, t0, p.L, c0, p.D, vec);
+        store_tile<T, G>(odu, i, du, p.D, t0, p.L, c0, p.D, vec);
+        store_tile<T, G>(oddt, i, ddt, p.D, t0, p.L, c0, p.D, vec);
+        if (dz) store_tile<T, G>(odz, i, dz, p.D, t0, p.L, c0, p.D, vec);
       }
       __syncthreads();   // sm.D and sm.R are written again
     }
@@ -490,29 +468,51 @@ sel_bwd_kernel(const SelBwdParams bp) {
 
 // What a run hands to the run before it (the gradient of the state it starts
 // from, as if nothing came after it), and the sum of its step sizes.
+template <typename T, typename G> struct SumSmem {
+  using M = TileMap<T, G>;
+  using Tile = Pack<T, M::VW>[M::NVEC * G::NT];
+  alignas(16) float4 D[kS][G::DT / 2];       // (de, gy) of two channels, at pair_at(pair)
+  alignas(16) float C[kS * G::NP];
+  alignas(16) Tile z, g, dt;
+  alignas(16) Pack<T, 4> c[G::QPT * G::NT];
+};
 template <typename T, int LN>
-__global__ void __launch_bounds__(Sel<LN>::NT) sel_bwd_sum_kernel(const SelBwdParams bp) {
-  using G = Sel<LN>;
-  using M = TileMap<T, LN>;
-  using Sm = BwdSmem<T, LN>;
+__global__ void __launch_bounds__(SelF<LN>::NT) sel_bwd_sum_kernel(const SelBwdParams bp) {
+  using G = SelF<LN>;
+  using M = TileMap<T, G>;
+  using Sm = SumSmem<T, G>;
+  constexpr int Q = G::S / 4;
   const SelParams& p = bp.f;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   Sm& sm = *reinterpret_cast<Sm*>(raw_smem);
   const int q = threadIdx.x % LN, grp = threadIdx.x / LN;
   const int tiles = (p.D + G::DT - 1) / G::DT;
-  const int c0 = blockIdx.x % tiles * G::DT, c = c0 + 2 * grp, n0 = 4 * q;
+  const int c0 = blockIdx.x % tiles * G::DT, c = c0 + 2 * grp, n0 = G::S * q;
   const size_t b = blockIdx.x / tiles;
   const int split = blockIdx.y + 1;
   const int ch0 = split * p.cps, ch1 = min(ch0 + p.cps, p.nch);
   const int n = sel_length(p.lengths, (int)b, p.L);
   const RowPtrs<T> rp(bp, b * p.L);
   const bool gate = rp.z != nullptr;
+  auto fetch = [&](int t0) {
+    fetch_tile<T, G>(sm.dt, rp.dt, p.ld_dt, t0, n, c0, p.D, p.vec_d);
+    fetch_tile<T, G>(sm.g, rp.g, p.D, t0, n, c0, p.D, bp.vec_g);
+    if (gate) fetch_tile<T, G>(sm.z, rp.z, p.ld_z, t0, n, c0, p.D, p.vec_d);
+    fetch_quads<T, G>(sm.c, rp.C, p.ld_c, t0, n, p.N, p.vec_n);
+    copies_commit();
+  };
   int ch = min(ch1, (n + kS - 1) / kS) - 1;
-  if (ch >= ch0) bwd_fetch<T, LN, true>(sm, bp, rp, ch & 1, ch * kS, n, c0);
-  float2 a2[2][2], dh[2][2];
-  load_a2(a2, p.A, c, n0, p.D, p.N);
+  if (ch >= ch0) fetch(ch * kS);
+  const int at = pair_at<M>(grp);
+  float2 a2[2][2 * Q], dh[2][2 * Q];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) dh[k][0] = dh[k][1] = make_float2(0.f, 0.f);
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      set_pairs(a2[k] + 2 * i,
+                scaled(load_quad_any(p.A, 0, c + k, n0 + 4 * i, p.D, p.N), kLog2e));
+      dh[k][2 * i] = dh[k][2 * i + 1] = make_float2(0.f, 0.f);
+    }
   float bias[M::VW], dsum[2] = {0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < M::VW; ++j) {
@@ -522,29 +522,66 @@ __global__ void __launch_bounds__(Sel<LN>::NT) sel_bwd_sum_kernel(const SelBwdPa
   for (; ch >= ch0; --ch) {
     const int t0 = ch * kS;
     copies_wait();
-    bwd_stage<T, LN, true>(sm, p, ch & 1, t0, n, gate, bias);
+#pragma unroll
+    for (int i = 0; i < M::NVEC; ++i) {
+      const int r = M::row(i), cc = M::col(i), x = i * G::NT + threadIdx.x;
+      const bool live = t0 + r < n;
+      const Pack<T, M::VW> cd = sm.dt[x], cg = sm.g[x];
+      Pack<T, M::VW> cz;
+      if (gate) cz = sm.z[x];
+#pragma unroll
+      for (int j = 0; j < M::VW; j += 2) {
+        const float d0 = live ? step_size(cd.get(j) + bias[j], p.softplus) : 0.f;
+        const float d1 = live ? step_size(cd.get(j + 1) + bias[j + 1], p.softplus) : 0.f;
+        float g0 = cg.get(j), g1 = cg.get(j + 1);
+        if (gate) {
+          g0 *= silu_f(cz.get(j));
+          g1 *= silu_f(cz.get(j + 1));
+        }
+        sm.D[r][pair_at<M>((cc + j) / 2)] = make_float4(d0, g0, d1, g1);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < G::QPT; ++i) {
+      const int e = (int)threadIdx.x + i * G::NT;
+      if (e < G::QUADS) {
+        const Pack<T, 4> v = sm.c[e];
+        *reinterpret_cast<float4*>(sm.C + 4 * e) =
+            make_float4(v.get(0), v.get(1), v.get(2), v.get(3));
+      }
+    }
     __syncthreads();
-    if (ch > ch0) bwd_fetch<T, LN, true>(sm, bp, rp, (ch & 1) ^ 1, t0 - kS, n, c0);
-#pragma unroll 4
+    if (ch > ch0) fetch(t0 - kS);
+#pragma unroll 2
     for (int t = kS - 1; t >= 0; --t) {
-      float2 c2[2];
-      set_pairs(c2, *reinterpret_cast<const float4*>(sm.C[0] + t * G::NP + n0));
+      const float4 dd = sm.D[t][at];
+      dsum[0] += dd.x;
+      dsum[1] += dd.z;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float2 de = f2(sm.D[t][2 * grp + k].x);
-        const float2 gy = f2(sm.Y[t][2 * grp + k]);
-        dsum[k] += de.x;
+      for (int i = 0; i < Q; ++i) {
+        float2 c2[2];
+        set_pairs(c2, *reinterpret_cast<const float4*>(sm.C + t * G::NP + n0 + 4 * i));
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          dh[k][j] = __fmul2_rn(ex2_pair(__fmul2_rn(de, a2[k][j])),
-                                __ffma2_rn(gy, c2[j], dh[k][j]));
+        for (int k = 0; k < 2; ++k) {
+          const float2 de = f2(k ? dd.z : dd.x), gy = f2(k ? dd.w : dd.y);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            dh[k][2 * i + j] =
+                __fmul2_rn(ex2_pair(__fmul2_rn(de, a2[k][2 * i + j])),
+                           __ffma2_rn(gy, c2[j], dh[k][2 * i + j]));
+        }
       }
     }
     __syncthreads();
   }
   const size_t row = (size_t)split * p.B + b;
-  store_quads(dh, bp.qsum, row, c, q, p.D, G::NP);
-  if (q < 2 && c + q < p.D) p.dsum[row * p.D + c + q] = q ? dsum[1] : dsum[0];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+      store_quad_pad(quad_of(dh[k] + 2 * i), bp.qsum, row, c + k, n0 + 4 * i, p.D, G::NP);
+    if (q == 0 && c + k < p.D) p.dsum[row * p.D + c + k] = dsum[k];
+  }
 }
 
 // The state's gradient at every run's end, joined from the back.
@@ -558,10 +595,21 @@ __global__ void __launch_bounds__(128) sel_join_bwd_kernel(const SelBwdParams bp
   const float a2 = n < p.N ? p.A[(size_t)(bd % p.D) * p.N + n] * kLog2e : 0.f;
   const long long sd = (long long)p.B * p.D;
   float v = 0.f;
-#pragma unroll 4
-  for (int s = p.splits - 1; s > 0; --s) {
-    v = fmaf(ex2_approx(p.dsum[s * sd + bd] * a2), v, bp.qsum[s * total + i]);
-    bp.qin[(s - 1) * total + i] = v;
+  constexpr int U = 8;   // runs whose summaries are loaded ahead of the chain
+  for (int s0 = p.splits - 1; s0 > 0; s0 -= U) {
+    float d[U], x[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (s0 - k > 0) {
+        d[k] = p.dsum[(s0 - k) * sd + bd];
+        x[k] = bp.qsum[(s0 - k) * total + i];
+      }
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (s0 - k > 0) {
+        v = fmaf(ex2_approx(d[k] * a2), v, x[k]);
+        bp.qin[(s0 - k - 1) * total + i] = v;
+      }
   }
 }
 
@@ -626,10 +674,13 @@ cudaError_t bwd_typed(const SelBwdParams& p, cudaStream_t s) {
   cudaError_t e = allow_smem<main>(smem);
   if (e != cudaSuccess) return e;
   if (p.f.splits > 1) {
-    constexpr auto* sum = sel_bwd_sum_kernel<T, LN>;
-    e = allow_smem<sum>(smem);
+    using W = SelF<LN / 2>;
+    constexpr int wide = (int)sizeof(SumSmem<T, W>);
+    constexpr auto* sum = sel_bwd_sum_kernel<T, LN / 2>;
+    e = allow_smem<sum>(wide);
     if (e != cudaSuccess) return e;
-    sum<<<dim3(tiles * p.f.B, p.f.splits - 1), G::NT, smem, s>>>(p);
+    const unsigned wtiles = (unsigned)((p.f.D + W::DT - 1) / W::DT);
+    sum<<<dim3(wtiles * p.f.B, p.f.splits - 1), W::NT, wide, s>>>(p);
     const long long total = (long long)p.f.B * p.f.D * G::NP;
     sel_join_bwd_kernel<<<(unsigned)((total + 127) / 128), 128, 0, s>>>(p, G::NP);
   }
@@ -655,18 +706,7 @@ cudaError_t bwd_lanes(const SelBwdParams& p, cudaStream_t s) {
 template <typename T, int LN>
 int resident() {
   static OncePerDevice known;
-  constexpr int smem = (int)sizeof(BwdSmem<T, LN>);
-  constexpr auto* kern = sel_bwd_kernel<T, LN>;
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) { cudaGetLastError(); return 0; }
-  if ((n = known.value[dev].load(std::memory_order_acquire)) > 0) return n;
-  if (allow_smem<kern>(smem) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, Sel<LN>::NT, smem) != cudaSuccess) {
-    cudaGetLastError();
-    return 0;
-  }
-  known.value[dev].store(n, std::memory_order_release);
-  return n;
+  return resident_ctas<sel_bwd_kernel<T, LN>>(known, Sel<LN>::NT, (int)sizeof(BwdSmem<T, LN>));
 }
 
 template <typename T>

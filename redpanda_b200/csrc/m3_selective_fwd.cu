@@ -17,33 +17,33 @@
 namespace m3 {
 namespace {
 
-// What a CTA holds in shared memory.  Two slots per tensor: one in use (u and z
+// What a CTA holds in shared memory.  Two slots for u and z: one in use (they
 // are read again for the output), one being filled.
-template <typename T, int LN, bool SUM> struct FwdSmem {
-  using G = Sel<LN>;
-  using M = TileMap<T, LN>;
+template <typename T, typename G, bool SUM> struct FwdSmem {
+  using M = TileMap<T, G>;
   using Tile = Pack<T, M::VW>[M::NVEC * G::NT];
   using Quads = Pack<T, 4>[G::QPT * G::NT];
-  alignas(16) float2 D[kS][G::DT];           // (de, de u)
+  alignas(16) float4 D[kS][G::DT / 2];       // (de, de u) of two channels, at pair_at(pair);
+                                             // then a step's C.h in the place of de
   alignas(16) float B[kS * G::NP], C[SUM ? 4 : kS * G::NP];
-  alignas(16) float Y[SUM ? 1 : kS][SUM ? 4 : G::DT];
   alignas(16) Tile u[2], z[SUM ? 1 : 2], dt;
   alignas(16) Quads b, c;
 };
 
 // SUM: only the end state and the step-size sum of a run (no y).
 template <typename T, int LN, bool SUM>
-__global__ void __launch_bounds__(Sel<LN>::NT) sel_fwd_kernel(const SelParams p) {
-  using G = Sel<LN>;
-  using M = TileMap<T, LN>;
-  using Sm = FwdSmem<T, LN, SUM>;
-  constexpr int TG = LN / 2;    // steps whose 2-channel totals fill the group's lanes
+__global__ void __launch_bounds__(SelF<LN>::NT) sel_fwd_kernel(const SelParams p) {
+  using G = SelF<LN>;
+  using M = TileMap<T, G>;
+  using Sm = FwdSmem<T, G, SUM>;
+  constexpr int Q = G::S / 4;   // quads per lane and channel
+  static_assert(M::VW % 2 == 0, "channels are staged in pairs");
   extern __shared__ __align__(16) unsigned char raw_smem[];
   Sm& sm = *reinterpret_cast<Sm*>(raw_smem);
   const int q = threadIdx.x % LN, grp = threadIdx.x / LN;
   // channel tiles of one row are neighbours: they read the same rows of B and C
   const int tiles = (p.D + G::DT - 1) / G::DT;
-  const int c0 = blockIdx.x % tiles * G::DT, c = c0 + 2 * grp, n0 = 4 * q;
+  const int c0 = blockIdx.x % tiles * G::DT, c = c0 + 2 * grp, n0 = G::S * q;
   const int split = blockIdx.y;
   const size_t b = blockIdx.x / tiles;
   const int n = sel_length(p.lengths, (int)b, p.L);
@@ -56,27 +56,32 @@ __global__ void __launch_bounds__(Sel<LN>::NT) sel_fwd_kernel(const SelParams p)
   T* y = static_cast<T*>(p.y) + b * p.L * (size_t)p.D;
   auto fetch = [&](int ch) {
     const int t0 = ch * kS;
-    fetch_tile<T, LN>(sm.u[ch & 1], u, p.ld_u, t0, n, c0, p.D, p.vec_d);
-    fetch_tile<T, LN>(sm.dt, dt, p.ld_dt, t0, n, c0, p.D, p.vec_d);
-    fetch_quads<T, LN>(sm.b, Bm, p.ld_b, t0, n, p.N, p.vec_n);
+    fetch_tile<T, G>(sm.u[ch & 1], u, p.ld_u, t0, n, c0, p.D, p.vec_d);
+    fetch_tile<T, G>(sm.dt, dt, p.ld_dt, t0, n, c0, p.D, p.vec_d);
+    fetch_quads<T, G>(sm.b, Bm, p.ld_b, t0, n, p.N, p.vec_n);
     if (!SUM) {
-      if (z) fetch_tile<T, LN>(sm.z[ch & 1], z, p.ld_z, t0, n, c0, p.D, p.vec_d);
-      fetch_quads<T, LN>(sm.c, Cm, p.ld_c, t0, n, p.N, p.vec_n);
+      if (z) fetch_tile<T, G>(sm.z[ch & 1], z, p.ld_z, t0, n, c0, p.D, p.vec_d);
+      fetch_quads<T, G>(sm.c, Cm, p.ld_c, t0, n, p.N, p.vec_n);
     }
     copies_commit();
   };
   if (ch0 * kS < n) fetch(ch0);
 
-  float2 a2[2][2], h[2][2];
-  load_a2(a2, p.A, c, n0, p.D, p.N);
-  if (SUM) {
+  const int at = pair_at<M>(grp);
+  float2 a2[2][2 * Q], h[2][2 * Q];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) h[k][0] = h[k][1] = make_float2(0.f, 0.f);
-  } else if (p.hin != nullptr && split > 0) {
-    load_quads(h, p.hin, (size_t)split * p.B + b, c, q, p.D, G::NP);
-  } else {
-    load_state(h, p.h0, b, c, n0, p.D, p.N);
-  }
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      set_pairs(a2[k] + 2 * i,
+                scaled(load_quad_any(p.A, 0, c + k, n0 + 4 * i, p.D, p.N), kLog2e));
+      set_pairs(h[k] + 2 * i,
+                SUM ? make_float4(0.f, 0.f, 0.f, 0.f)
+                    : p.hin != nullptr && split > 0
+                          ? load_quad_pad(p.hin, (size_t)split * p.B + b, c + k, n0 + 4 * i, p.D,
+                                          G::NP)
+                          : load_quad_any(p.h0, b, c + k, n0 + 4 * i, p.D, p.N));
+    }
   float bias[M::VW], dsk[M::VW];   // a thread's staged elements share their columns
 #pragma unroll
   for (int j = 0; j < M::VW; ++j) {
@@ -91,7 +96,7 @@ __global__ void __launch_bounds__(Sel<LN>::NT) sel_fwd_kernel(const SelParams p)
     if (!SUM && t0 >= n) {   // past the row's length: y is zero, the state stands
 #pragma unroll
       for (int i = 0; i < M::NVEC; ++i)
-        store_tile<T, LN>(zero_pack<T, M::VW>(), i, y, p.D, t0, p.L, c0, p.D, p.vec_d);
+        store_tile<T, G>(zero_pack<T, M::VW>(), i, y, p.D, t0, p.L, c0, p.D, p.vec_d);
       continue;
     }
     copies_wait();
@@ -101,16 +106,16 @@ __global__ void __launch_bounds__(Sel<LN>::NT) sel_fwd_kernel(const SelParams p)
       const bool live = t0 + r < n;
       const Pack<T, M::VW> cd = sm.dt[x], cu = sm.u[ch & 1][x];
 #pragma unroll
-      for (int j = 0; j < M::VW; ++j) {
-        const float de = live ? step_size(cd.get(j) + bias[j], p.softplus) : 0.f;
-        const float du = live ? de * cu.get(j) : 0.f;
-        sm.D[r][cc + j] = make_float2(de, du);
+      for (int j = 0; j < M::VW; j += 2) {
+        const float d0 = live ? step_size(cd.get(j) + bias[j], p.softplus) : 0.f;
+        const float d1 = live ? step_size(cd.get(j + 1) + bias[j + 1], p.softplus) : 0.f;
+        sm.D[r][pair_at<M>((cc + j) / 2)] = make_float4(d0, d0 * cu.get(j), d1, d1 * cu.get(j + 1));
       }
     }
 #pragma unroll
     for (int i = 0; i < G::QPT; ++i) {
       const int e = (int)threadIdx.x + i * G::NT;
-      if (e < kS * LN) {
+      if (e < G::QUADS) {
         const Pack<T, 4> vb = sm.b[e];
         *reinterpret_cast<float4*>(sm.B + 4 * e) =
             make_float4(vb.get(0), vb.get(1), vb.get(2), vb.get(3));
@@ -124,41 +129,60 @@ __global__ void __launch_bounds__(Sel<LN>::NT) sel_fwd_kernel(const SelParams p)
     __syncthreads();
     if (ch + 1 < ch1 && t0 + kS < n) fetch(ch + 1);
     if (!SUM && p.ckpt && ch > 0)
-      store_quads(h, p.ckpt, b * (p.nch - 1) + ch - 1, c, q, p.D, G::NP);
-    // steps of a group: enough for the totals to fill the lanes
-    constexpr int GS = SUM ? 4 : TG;
-#pragma unroll(SUM || TG >= 4 ? 1 : 4 / TG)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+          store_quad_pad(quad_of(h[k] + 2 * i), p.ckpt, b * (p.nch - 1) + ch - 1, c + k,
+                         n0 + 4 * i, p.D, G::NP);
+    // steps of a group: enough for the two channels' totals to fill the lanes
+    constexpr int GS = SUM ? 2 : (LN >= 4 ? LN / 2 : 1);
+#pragma unroll(GS >= 4 ? 1 : 4 / GS)
     for (int g0 = 0; g0 < kS; g0 += GS) {
       float acc[2 * GS];
 #pragma unroll
       for (int s = 0; s < GS; ++s) {
         const int t = g0 + s;
-        const float4 dd = *reinterpret_cast<const float4*>(&sm.D[t][2 * grp]);
-        const float4 bb = *reinterpret_cast<const float4*>(sm.B + t * G::NP + n0);
-        const float2 b2[2] = {make_float2(bb.x, bb.y), make_float2(bb.z, bb.w)};
-        float2 c2[2];
-        if (!SUM) {
-          const float4 cc = *reinterpret_cast<const float4*>(sm.C + t * G::NP + n0);
-          c2[0] = make_float2(cc.x, cc.y);
-          c2[1] = make_float2(cc.z, cc.w);
+        const float4 dd = sm.D[t][at];
+        float2 ys[2];
+        if (SUM) {
+          dsum[0] += dd.x;
+          dsum[1] += dd.z;
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float2 de = f2(k ? dd.z : dd.x), du = f2(k ? dd.w : dd.y);
-          float2 ysum;
+        for (int i = 0; i < Q; ++i) {
+          float2 b2[2], c2[2];
+          set_pairs(b2, *reinterpret_cast<const float4*>(sm.B + t * G::NP + n0 + 4 * i));
+          if (!SUM) set_pairs(c2, *reinterpret_cast<const float4*>(sm.C + t * G::NP + n0 + 4 * i));
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float2 a = ex2_pair(__fmul2_rn(de, a2[k][j]));
-            h[k][j] = __ffma2_rn(a, h[k][j], __fmul2_rn(du, b2[j]));
-            if (!SUM) ysum = j ? __ffma2_rn(h[k][j], c2[j], ysum) : __fmul2_rn(h[k][j], c2[j]);
+          for (int k = 0; k < 2; ++k) {
+            const float2 de = f2(k ? dd.z : dd.x), du = f2(k ? dd.w : dd.y);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int x = 2 * i + j;
+              const float2 a = ex2_pair(__fmul2_rn(de, a2[k][x]));
+              h[k][x] = __ffma2_rn(a, h[k][x], __fmul2_rn(du, b2[j]));
+              if (!SUM)
+                ys[k] = x ? __ffma2_rn(h[k][x], c2[j], ys[k]) : __fmul2_rn(h[k][x], c2[j]);
+            }
           }
-          if (SUM) dsum[k] += k ? dd.z : dd.x;
-          else acc[2 * s + k] = ysum.x + ysum.y;
+        }
+        if (!SUM) {
+          acc[2 * s] = ys[0].x + ys[0].y;
+          acc[2 * s + 1] = ys[1].x + ys[1].y;
         }
       }
       if (!SUM) {
-        lane_sum<2 * GS, LN>(acc, q);   // total q: step q / 2, channel q % 2
-        sm.Y[g0 + (q >> 1)][2 * grp + (q & 1)] = acc[0];
+        // total q: step q / 2, channel q % 2; only this group reads its channels
+        // of sm.D, and its lanes have met in the shuffles
+        lane_sum<2 * GS, LN>(acc, q);
+        __syncwarp();
+        if constexpr (LN == 1) {
+          sm.D[g0][at].x = acc[0];
+          sm.D[g0][at].z = acc[1];
+        } else {
+          reinterpret_cast<float*>(&sm.D[g0 + (q >> 1)][at])[2 * (q & 1)] = acc[0];
+        }
       }
     }
     __syncthreads();
@@ -171,22 +195,32 @@ __global__ void __launch_bounds__(Sel<LN>::NT) sel_fwd_kernel(const SelParams p)
         Pack<T, M::VW> cz, o;
         if (z) cz = sm.z[ch & 1][x];
 #pragma unroll
-        for (int j = 0; j < M::VW; ++j) {
-          float v = fmaf(dsk[j], cu.get(j), sm.Y[r][cc + j]);
-          if (z) v *= silu_f(cz.get(j));
-          o.put(j, live ? v : 0.f);
+        for (int j = 0; j < M::VW; j += 2) {
+          const float4 yy = sm.D[r][pair_at<M>((cc + j) / 2)];
+          float v0 = fmaf(dsk[j], cu.get(j), yy.x), v1 = fmaf(dsk[j + 1], cu.get(j + 1), yy.z);
+          if (z) {
+            v0 *= silu_f(cz.get(j));
+            v1 *= silu_f(cz.get(j + 1));
+          }
+          o.put(j, live ? v0 : 0.f);
+          o.put(j + 1, live ? v1 : 0.f);
         }
-        store_tile<T, LN>(o, i, y, p.D, t0, p.L, c0, p.D, p.vec_d);
+        store_tile<T, G>(o, i, y, p.D, t0, p.L, c0, p.D, p.vec_d);
       }
-      // the next chunk's barrier stands before sm.Y is written again
+      // a thread stages over what it has just read itself
     }
   }
-  if (SUM) {
-    const size_t row = (size_t)split * p.B + b;
-    store_quads(h, p.hsum, row, c, q, p.D, G::NP);
-    if (q < 2 && c + q < p.D) p.dsum[row * p.D + c + q] = q ? dsum[1] : dsum[0];
-  } else if (p.h_last != nullptr && split == p.splits - 1) {
-    store_state(h, p.h_last, b, c, n0, p.D, p.N);
+  const size_t row = SUM ? (size_t)split * p.B + b : b;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      const float4 v = quad_of(h[k] + 2 * i);
+      if (SUM) store_quad_pad(v, p.hsum, row, c + k, n0 + 4 * i, p.D, G::NP);
+      else if (p.h_last != nullptr && split == p.splits - 1)
+        store_quad_any(v, p.h_last, row, c + k, n0 + 4 * i, p.D, p.N);
+    }
+    if (SUM && q == 0 && c + k < p.D) p.dsum[row * p.D + c + k] = dsum[k];
   }
 }
 
@@ -204,17 +238,28 @@ __global__ void __launch_bounds__(128) sel_join_kernel(const SelParams p, int NP
     if (p.h0 != nullptr) h = p.h0[bd * p.N + n];
   }
   const long long sd = (long long)p.B * p.D;
-#pragma unroll 4
-  for (int s = 0; s + 1 < p.splits; ++s) {
-    h = fmaf(ex2_approx(p.dsum[s * sd + bd] * a2), h, p.hsum[s * total + i]);
-    p.hin[(s + 1) * total + i] = h;
+  constexpr int U = 8;   // runs whose summaries are loaded ahead of the chain
+  for (int s0 = 0; s0 + 1 < p.splits; s0 += U) {
+    float d[U], x[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (s0 + k + 1 < p.splits) {
+        d[k] = p.dsum[(s0 + k) * sd + bd];
+        x[k] = p.hsum[(s0 + k) * total + i];
+      }
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (s0 + k + 1 < p.splits) {
+        h = fmaf(ex2_approx(d[k] * a2), h, x[k]);
+        p.hin[(s0 + k + 1) * total + i] = h;
+      }
   }
 }
 
 template <typename T, int LN, bool SUM>
 cudaError_t fwd_launch(const SelParams& p, int runs, cudaStream_t s) {
-  using G = Sel<LN>;
-  constexpr int smem = (int)sizeof(FwdSmem<T, LN, SUM>);
+  using G = SelF<LN>;
+  constexpr int smem = (int)sizeof(FwdSmem<T, G, SUM>);
   constexpr auto* kern = sel_fwd_kernel<T, LN, SUM>;
   const cudaError_t e = allow_smem<kern>(smem);
   if (e != cudaSuccess) return e;
@@ -225,7 +270,7 @@ cudaError_t fwd_launch(const SelParams& p, int runs, cudaStream_t s) {
 
 template <typename T, int LN>
 cudaError_t fwd_typed(const SelParams& p, cudaStream_t s) {
-  using G = Sel<LN>;
+  using G = SelF<LN>;
   if (p.splits > 1) {
     const cudaError_t e = fwd_launch<T, LN, true>(p, p.splits - 1, s);
     if (e != cudaSuccess) return e;
@@ -235,31 +280,39 @@ cudaError_t fwd_typed(const SelParams& p, cudaStream_t s) {
   return fwd_launch<T, LN, false>(p, p.splits, s);
 }
 
+template <typename T, int LN>
+int resident() {
+  static OncePerDevice known;
+  static_assert(SelF<LN>::DT == (LN == 1 ? 128 : 64), "sel_fwd_tile");
+  constexpr int smem = (int)sizeof(FwdSmem<T, SelF<LN>, false>);
+  return resident_ctas<sel_fwd_kernel<T, LN, false>>(known, SelF<LN>::NT, smem);
+}
+template <typename T>
+int resident_lanes(int N) {
+  switch (sel_lanes(N) / 2) {
+    case 1: return resident<T, 1>();
+    case 2: return resident<T, 2>();
+    case 4: return resident<T, 4>();
+    case 8: return resident<T, 8>();
+    default: return resident<T, 16>();
+  }
+}
+
 template <typename T>
 cudaError_t fwd_lanes(const SelParams& p, cudaStream_t s) {
-  switch (sel_lanes(p.N)) {
+  switch (sel_lanes(p.N) / 2) {   // eight states per lane
+    case 1: return fwd_typed<T, 1>(p, s);
     case 2: return fwd_typed<T, 2>(p, s);
     case 4: return fwd_typed<T, 4>(p, s);
     case 8: return fwd_typed<T, 8>(p, s);
-    case 16: return fwd_typed<T, 16>(p, s);
-    default: return fwd_typed<T, 32>(p, s);
+    default: return fwd_typed<T, 16>(p, s);
   }
 }
 
 }  // namespace
 
-// Runs of the time split: enough CTAs for four per SM, when the rows and
-// channel tiles alone give fewer than two.
-int sel_splits(int B, int L, int D, int N, int sms) {
-  const int ln = sel_lanes(N);
-  const long long ctas = (long long)B * ((D + sel_tile(ln) - 1) / sel_tile(ln));
-  const int nch = (L + kSelSteps - 1) / kSelSteps;
-  if (ctas >= 2LL * sms || nch < 4) return 1;
-  long long s = 4LL * sms / ctas;
-  if (s > nch / 2) s = nch / 2;
-  if (s < 2) return 1;
-  const int cps = (int)((nch + s - 1) / s);
-  return (nch + cps - 1) / cps;
+int sel_fwd_resident(int N, int dtype) {
+  return dtype == M3_BF16 ? resident_lanes<__nv_bfloat16>(N) : resident_lanes<float>(N);
 }
 
 cudaError_t launch_sel_fwd(const SelParams& p, cudaStream_t s) {
