@@ -74,12 +74,26 @@ struct Rows {
 template <int V, int K>
 __device__ __forceinline__ void load_filter(Vals<V> (&w)[K], Vals<V>& b, const float* pw,
                                             const float* pb, int c) {
-  float t[K + 1][2 * Vals<V>::H] = {};
+  alignas(16) float t[K + 1][2 * Vals<V>::H] = {};
+  // the taps of V channels are V * K neighbours
+  if constexpr (V == 4) {
+    alignas(16) float f[V * K];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
+    for (int i = 0; i < K; ++i)
+      *reinterpret_cast<float4*>(f + 4 * i) = reinterpret_cast<const float4*>(pw + (size_t)c * K)[i];
 #pragma unroll
-    for (int k = 0; k < K; ++k) t[k][j] = pw[(size_t)(c + j) * K + k];
-    t[K][j] = pb != nullptr ? pb[c + j] : 0.f;
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int k = 0; k < K; ++k) t[k][j] = f[j * K + k];
+    if (pb != nullptr)
+      *reinterpret_cast<float4*>(t[K]) = *reinterpret_cast<const float4*>(pb + c);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) t[k][j] = pw[(size_t)(c + j) * K + k];
+      t[K][j] = pb != nullptr ? pb[c + j] : 0.f;
+    }
   }
 #pragma unroll
   for (int i = 0; i < Vals<V>::H; ++i) {
@@ -293,33 +307,49 @@ __global__ void __launch_bounds__(256) conv_reduce_kernel(const float* part, int
   }
 }
 
-// One token per row: the window is [state, x]; the state moves up by one row.
+// One token per row: the window is [state, x]; the state moves up by one row.  A
+// thread takes its channels of kStepRows rows, all loads ahead of the arithmetic.
+constexpr int kStepRows = 4;
+
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(128) conv_step_kernel(const ConvStepParams p) {
   const int lanes = p.D / V;
   const long long idx = (long long)blockIdx.x * 128 + threadIdx.x;
-  if (idx >= (long long)lanes * p.B) return;
+  const long long blocks = (p.B + kStepRows - 1) / kStepRows;
+  if (idx >= lanes * blocks) return;
   const int c = (int)(idx % lanes) * V;
-  const size_t b = (size_t)(idx / lanes);
-  T* st = static_cast<T*>(p.state) + b * (K - 1) * p.D + c;
-  Pack<T, V> r[K];
+  const size_t b0 = (size_t)(idx / lanes) * kStepRows;
+  const int rows = (int)min((size_t)kStepRows, (size_t)p.B - b0);
+  T* st = static_cast<T*>(p.state) + b0 * (K - 1) * p.D + c;
+  Pack<T, V> r[kStepRows][K];
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) r[k] = ld_pack<T, V>(st + (size_t)k * p.D);
-  r[K - 1] = ld_pack<T, V>(static_cast<const T*>(p.x) + b * p.ld_x + c);
-  Vals<V> w[K], a;
-  load_filter<V, K>(w, a, p.w, p.b, c);
+  for (int i = 0; i < kStepRows; ++i)
+    if (i < rows) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    Vals<V> x;
-    x.from(r[k]);
-    a.fma(w[k], x);
-  }
-  Pack<T, V> o;
+      for (int k = 0; k < K - 1; ++k)
+        r[i][k] = ld_pack<T, V>(st + ((size_t)i * (K - 1) + k) * p.D);
+      r[i][K - 1] = ld_pack<T, V>(static_cast<const T*>(p.x) + (b0 + i) * p.ld_x + c);
+    }
+  Vals<V> w[K], bias;
+  load_filter<V, K>(w, bias, p.w, p.b, c);
 #pragma unroll
-  for (int j = 0; j < V; ++j) o.put(j, p.silu ? silu_f(a.get(j)) : a.get(j));
+  for (int i = 0; i < kStepRows; ++i)
+    if (i < rows) {
+      Vals<V> a = bias;
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) st_pack<T, V>(st + (size_t)k * p.D, r[k + 1]);
-  st_pack<T, V>(static_cast<T*>(p.y) + b * p.D + c, o);
+      for (int k = 0; k < K; ++k) {
+        Vals<V> x;
+        x.from(r[i][k]);
+        a.fma(w[k], x);
+      }
+      Pack<T, V> o;
+#pragma unroll
+      for (int j = 0; j < V; ++j) o.put(j, p.silu ? silu_f(a.get(j)) : a.get(j));
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+        st_pack<T, V>(st + ((size_t)i * (K - 1) + k) * p.D, r[i][k + 1]);
+      st_pack<T, V>(static_cast<T*>(p.y) + (b0 + i) * p.D + c, o);
+    }
 }
 
 // Calls f<T, V, K>() for an element type, vector and width.
@@ -375,7 +405,7 @@ struct StepLaunch {
   cudaStream_t s;
   template <typename T, int V, int K>
   cudaError_t operator()() {
-    const long long n = (long long)(p.D / V) * p.B;
+    const long long n = (long long)(p.D / V) * ((p.B + kStepRows - 1) / kStepRows);
     conv_step_kernel<T, V, K><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
     return cudaGetLastError();
   }
@@ -387,7 +417,8 @@ cudaError_t launch_conv_fwd(const ConvParams& p0, cudaStream_t s) {
   ConvParams p = p0;
   const int a = 4 * dsize(p.dtype);
   const bool vec = p.D % 4 == 0 && p.ld_x % 4 == 0 && aligned(p.x, a) && aligned(p.y, a) &&
-                   aligned(p.state, a) && aligned(p.state_out, a);
+                   aligned(p.state, a) && aligned(p.state_out, a) && aligned(p.w, 16) &&
+                   aligned(p.b, 16);
   // long runs read fewer halo rows, short ones give more threads
   const long long lanes = vec ? p.D / 4 : p.D;
   p.tt = 32;
@@ -413,14 +444,14 @@ void conv_bwd_plan(int B, int L, int D, int sms, int* workers, int* tt) {
 cudaError_t launch_conv_bwd(const ConvBwdParams& p, cudaStream_t s) {
   const int a = 4 * dsize(p.dtype);
   const bool vec = p.D % 4 == 0 && p.ld_x % 4 == 0 && aligned(p.x, a) && aligned(p.g, a) &&
-                   aligned(p.dx, a) && aligned(p.state, a);
+                   aligned(p.dx, a) && aligned(p.state, a) && aligned(p.w, 16) && aligned(p.b, 16);
   return conv_dispatch(p.dtype, vec, p.K, BwdLaunch{p, s});
 }
 
 cudaError_t launch_conv_step(const ConvStepParams& p, cudaStream_t s) {
   const int a = 4 * dsize(p.dtype);
   const bool vec = p.D % 4 == 0 && p.ld_x % 4 == 0 && aligned(p.x, a) && aligned(p.y, a) &&
-                   aligned(p.state, a);
+                   aligned(p.state, a) && aligned(p.w, 16) && aligned(p.b, 16);
   return conv_dispatch(p.dtype, vec, p.K, StepLaunch{p, s});
 }
 

@@ -14,38 +14,28 @@
 namespace m3 {
 namespace {
 
-constexpr int kRows = 8;
+constexpr int kRows = 8, kHalf = 4;
 
-template <typename T, int LN, bool VEC>
-__global__ void __launch_bounds__(128) sel_step_kernel(const SelStepParams p) {
+// FULL: all kRows rows and all states of the lane exist (no predicates; they and
+// the addresses cost more than the recurrence otherwise).
+template <typename T, int LN, bool VEC, bool FULL>
+__device__ __forceinline__ void step_rows(const SelStepParams& p, int q, int d, size_t b0,
+                                          int rows) {
   constexpr int KR = LN <= kRows ? kRows / LN : 1;   // rows per lane
   constexpr int PR = LN <= kRows ? 1 : LN / kRows;   // lanes per row
-  const int q = threadIdx.x % LN, d = (int)(blockIdx.x * (128 / LN) + threadIdx.x / LN);
   const int n0 = 4 * q;
-  const size_t b0 = (size_t)blockIdx.y * kRows;
-  const int rows = (int)min((size_t)kRows, (size_t)p.B - b0);
-  const bool live = d < p.D;
-  const bool has = live && n0 < p.N;
-
+  const bool live = FULL || d < p.D, has = FULL || (live && n0 < p.N);
+  float* const hp = p.h + (b0 * p.D + d) * p.N + n0;
+  const size_t hs = (size_t)p.D * p.N;
   float4 h[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     h[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (has && r < rows) {
-      const float* src = p.h + ((b0 + r) * p.D + d) * p.N + n0;
-      if (VEC) h[r] = *reinterpret_cast<const float4*>(src);
-      else {
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = n0 + j < p.N ? src[j] : 0.f;
-        h[r] = make_float4(v[0], v[1], v[2], v[3]);
-      }
+    if (FULL || (has && r < rows)) {
+      if (VEC) h[r] = *reinterpret_cast<const float4*>(hp + r * hs);
+      else h[r] = load_quad_any(p.h, b0 + r, d, n0, p.D, p.N);
     }
   }
-  float a2[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    a2[j] = (has && n0 + j < p.N) ? p.A[(size_t)d * p.N + n0 + j] * kLog2e : 0.f;
   // the lane's own rows: q / PR * KR + i
   const float bias = (live && p.dt_bias) ? p.dt_bias[d] : 0.f;
   const float dsk = (live && p.dskip) ? p.dskip[d] : 0.f;
@@ -54,50 +44,63 @@ __global__ void __launch_bounds__(128) sel_step_kernel(const SelStepParams p) {
   for (int i = 0; i < KR; ++i) {
     const int r = q / PR * KR + i;
     de[i] = uu[i] = zz[i] = 0.f;
-    if (live && r < rows) {
+    if (FULL || (live && r < rows)) {
       const size_t b = b0 + r;
       uu[i] = Elem<T>::get(static_cast<const T*>(p.u)[b * p.ld_u + d]);
-      de[i] = step_size(Elem<T>::get(static_cast<const T*>(p.dt)[b * p.ld_dt + d]) + bias,
-                        p.softplus);
+      de[i] = Elem<T>::get(static_cast<const T*>(p.dt)[b * p.ld_dt + d]) + bias;
       if (p.z) zz[i] = Elem<T>::get(static_cast<const T*>(p.z)[b * p.ld_z + d]);
     }
   }
+  float4 a2 = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (has)
+    a2 = VEC ? *reinterpret_cast<const float4*>(p.A + (size_t)d * p.N + n0)
+             : load_quad_any(p.A, 0, d, n0, p.D, p.N);
+  a2 = scaled(a2, kLog2e);
+#pragma unroll
+  for (int i = 0; i < KR; ++i)
+    if (FULL || (live && q / PR * KR + i < rows)) de[i] = step_size(de[i], p.softplus);
+  const T* const pb = static_cast<const T*>(p.Bm) + b0 * p.ld_b + n0;
+  const T* const pc = static_cast<const T*>(p.Cm) + b0 * p.ld_c + n0;
   float y[kRows];
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int src = r / KR * PR;
-    const float der = __shfl_sync(0xffffffffu, de[r % KR], src, LN);
-    const float dur = der * __shfl_sync(0xffffffffu, uu[r % KR], src, LN);
-    Pack<T, 4> bv = zero_pack<T, 4>(), cv = zero_pack<T, 4>();
-    if (has && r < rows) {
-      const T* pb = static_cast<const T*>(p.Bm) + (b0 + r) * p.ld_b + n0;
-      const T* pc = static_cast<const T*>(p.Cm) + (b0 + r) * p.ld_c + n0;
-      if (VEC) {
-        bv = ld_pack<T, 4>(pb);
-        cv = ld_pack<T, 4>(pc);
-      } else {
+  for (int r0 = 0; r0 < kRows; r0 += kHalf) {
+    // the rows' B and C together, ahead of the stores that the loads could not pass
+    Pack<T, 4> bv[kHalf], cv[kHalf];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n0 + j < p.N) {
-            bv.load_one(j, pb);
-            cv.load_one(j, pc);
-          }
+    for (int i = 0; i < kHalf; ++i) {
+      const int r = r0 + i;
+      if (!FULL) {
+        bv[i].zero();
+        cv[i].zero();
+      }
+      if (FULL || (has && r < rows)) {
+        if (VEC) {
+          bv[i] = ld_pack<T, 4>(pb + r * p.ld_b);
+          cv[i] = ld_pack<T, 4>(pc + r * p.ld_c);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n0 + j < p.N) {
+              bv[i].load_one(j, pb + r * p.ld_b);
+              cv[i].load_one(j, pc + r * p.ld_c);
+            }
+        }
       }
     }
-    h[r].x = fmaf(ex2_approx(der * a2[0]), h[r].x, dur * bv.get(0));
-    h[r].y = fmaf(ex2_approx(der * a2[1]), h[r].y, dur * bv.get(1));
-    h[r].z = fmaf(ex2_approx(der * a2[2]), h[r].z, dur * bv.get(2));
-    h[r].w = fmaf(ex2_approx(der * a2[3]), h[r].w, dur * bv.get(3));
-    y[r] = fmaf(h[r].x, cv.get(0), h[r].y * cv.get(1)) +
-           fmaf(h[r].z, cv.get(2), h[r].w * cv.get(3));
-    if (has && r < rows) {
-      float* dst = p.h + ((b0 + r) * p.D + d) * p.N + n0;
-      if (VEC) *reinterpret_cast<float4*>(dst) = h[r];
-      else {
-        const float v[4] = {h[r].x, h[r].y, h[r].z, h[r].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n0 + j < p.N) dst[j] = v[j];
+    for (int i = 0; i < kHalf; ++i) {
+      const int r = r0 + i, src = r / KR * PR;
+      const float der = __shfl_sync(0xffffffffu, de[r % KR], src, LN);
+      const float dur = der * __shfl_sync(0xffffffffu, uu[r % KR], src, LN);
+      h[r].x = fmaf(ex2_approx(der * a2.x), h[r].x, dur * bv[i].get(0));
+      h[r].y = fmaf(ex2_approx(der * a2.y), h[r].y, dur * bv[i].get(1));
+      h[r].z = fmaf(ex2_approx(der * a2.z), h[r].z, dur * bv[i].get(2));
+      h[r].w = fmaf(ex2_approx(der * a2.w), h[r].w, dur * bv[i].get(3));
+      y[r] = fmaf(h[r].x, cv[i].get(0), h[r].y * cv[i].get(1)) +
+             fmaf(h[r].z, cv[i].get(2), h[r].w * cv[i].get(3));
+      if (FULL || (has && r < rows)) {
+        if (VEC) *reinterpret_cast<float4*>(hp + r * hs) = h[r];
+        else store_quad_any(h[r], p.h, b0 + r, d, n0, p.D, p.N);
       }
     }
   }
@@ -106,12 +109,24 @@ __global__ void __launch_bounds__(128) sel_step_kernel(const SelStepParams p) {
 #pragma unroll
     for (int i = 0; i < KR; ++i) {
       const int r = q / PR * KR + i;
-      if (r < rows) {
+      if (FULL || r < rows) {
         float v = fmaf(dsk, uu[i], y[i]);
         if (p.z) v *= silu_f(zz[i]);
         static_cast<T*>(p.y)[(b0 + r) * p.D + d] = Elem<T>::put(v);
       }
     }
+}
+
+template <typename T, int LN, bool VEC>
+__global__ void __launch_bounds__(128, 6) sel_step_kernel(const SelStepParams p) {
+  constexpr int CH = 128 / LN;   // channels per CTA
+  const int q = threadIdx.x % LN, d = (int)(blockIdx.x * CH + threadIdx.x / LN);
+  const size_t b0 = (size_t)blockIdx.y * kRows;
+  const int rows = (int)min((size_t)kRows, (size_t)p.B - b0);
+  if (VEC && rows == kRows && p.N == 4 * LN && (int)(blockIdx.x + 1) * CH <= p.D)
+    step_rows<T, LN, VEC, true>(p, q, d, b0, rows);
+  else
+    step_rows<T, LN, VEC, false>(p, q, d, b0, rows);
 }
 
 template <typename T, int LN>
@@ -138,7 +153,7 @@ cudaError_t step_lanes(const SelStepParams& p, bool vec, cudaStream_t s) {
 
 cudaError_t launch_sel_step(const SelStepParams& p, cudaStream_t s) {
   const int a = 4 * dsize(p.dtype);
-  const bool vec = p.N % 4 == 0 && aligned(p.h, 16) && aligned(p.Bm, a) && aligned(p.Cm, a) &&
+  const bool vec = p.N % 4 == 0 && aligned(p.h, 16) && aligned(p.A, 16) && aligned(p.Bm, a) && aligned(p.Cm, a) &&
                    p.ld_b % 4 == 0 && p.ld_c % 4 == 0;
   return p.dtype == M3_BF16 ? step_lanes<__nv_bfloat16>(p, vec, s) : step_lanes<float>(p, vec, s);
 }
