@@ -25,6 +25,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import scan as S
+from .norm import MAX_D, m3_rms_norm
 
 
 @dataclass
@@ -59,7 +60,14 @@ class MambaConfig:
 
 
 class RMSNorm(nn.Module):
-    """x * rsqrt(mean(x^2) + eps) * weight (mamba.py:82-89)."""
+    """x * rsqrt(mean(x^2) + eps) * weight (mamba.py:82-89).
+
+    ``use_kernel`` (class or instance attribute): run CUDA tensors of float32 or
+    bfloat16 on ``m3_rms_norm``, one launch forward and two backward instead of
+    torch's five and about ten.  Off by default, where results are torch's, bit
+    for bit; the kernel's differ by rounding (the order of its sums)."""
+
+    use_kernel = False
 
     def __init__(self, d: int, eps: float = 1e-5):
         super().__init__()
@@ -67,6 +75,10 @@ class RMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(d))
 
     def forward(self, x):
+        if (self.use_kernel and x.is_cuda and x.shape[-1] <= MAX_D
+                and x.dtype in (torch.float32, torch.bfloat16)):
+            return m3_rms_norm(x, self.weight, self.eps,
+                               out_dtype=torch.promote_types(x.dtype, self.weight.dtype))
         if not torch.is_grad_enabled():   # inference: torch's fused kernel, same formula
             return F.rms_norm(x, (x.shape[-1],), self.weight, self.eps)
         return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + self.eps) * self.weight

@@ -17,6 +17,8 @@ import torch.nn as nn
 
 from .graphs import StepGraph
 from .mamba import Mamba, MambaConfig
+from .norm import LayerNorm
+from .sampling import m3_sample
 
 
 class SearchMambaConfig(MambaConfig):
@@ -48,18 +50,19 @@ class SearchMamba(nn.Module):
         self.backbone = Mamba(config)
         d = config.d_model
         self.line_value_head = nn.Sequential(
-            nn.Linear(d, d), nn.GELU(), nn.LayerNorm(d),
+            nn.Linear(d, d), nn.GELU(), LayerNorm(d),
             nn.Linear(d, d // 2), nn.GELU(), nn.Linear(d // 2, 1))
         self.value_head = nn.Sequential(
-            nn.Linear(d, d), nn.GELU(), nn.LayerNorm(d), nn.Linear(d, 1))
+            nn.Linear(d, d), nn.GELU(), LayerNorm(d), nn.Linear(d, 1))
         self.continuation_head = nn.Sequential(
-            nn.Linear(d, d * 2), nn.GELU(), nn.LayerNorm(d * 2),
+            nn.Linear(d, d * 2), nn.GELU(), LayerNorm(d * 2),
             nn.Linear(d * 2, config.vocab_size))
         self.consistency_proj = nn.Sequential(
             nn.Linear(d, d), nn.GELU(), nn.Linear(d, eval_dim))
         self.apply(self._init_weights)
         self._node_graph = None
         self._line_graphs = {}
+        self._draw_graphs = {}
 
     def _init_weights(self, m):
         if isinstance(m, nn.Linear):
@@ -177,11 +180,44 @@ class SearchMamba(nn.Module):
         _, value, logits = g.step(int(move_token))
         return value.item(), logits.clone(), g.snapshot()
 
+    @torch.no_grad()
+    def sample_lines(self, board_encoding, uniforms, temperature=1.0, top_k=0, top_p=1.0,
+                     min_p=0.0):
+        """K lines of L moves drawn from the continuation head, in lockstep.
+
+        ``uniforms`` (K, L) float32 in [0, 1): the random number of every move, so
+        that the lines are a function of the arguments; the settings are those of
+        :func:`redpanda_b200.sampling.m3_sample`, one for all lines or one per
+        line.  Returns (moves (K, L) int64, values (K,)): the moves and the value
+        head's evaluation behind each line.  The step and the head run as one
+        captured graph for K lines, kept until ``release_graphs``."""
+        if uniforms.dim() != 2 or uniforms.shape[1] < 1:
+            raise ValueError("sample_lines: uniforms are (lines, moves)")
+        K, L = uniforms.shape
+        hidden, cache = self.prime_board(board_encoding)
+        if hidden.shape[0] != 1:
+            raise ValueError("sample_lines: one board")
+        g = self._draw_graphs.get(K)
+        if g is None:
+            g = self._draw_graphs[K] = StepGraph(self.backbone, K, head=self.continuation_head)
+        for (h, d), (h1, d1) in zip(g.cache, cache):   # broadcast the board's state
+            h.copy_(h1.expand_as(h))
+            d.copy_(d1.expand_as(d))
+        logits = self.continuation_head(hidden).expand(K, -1)
+        moves = []
+        for t in range(L):
+            move = m3_sample(logits, uniforms[:, t], temperature, top_k, top_p, min_p)
+            moves.append(move)
+            # -1: no candidate (all logits NaN); the step needs an id of the vocabulary
+            hidden, logits = g.step(move.clamp(min=0))
+        return torch.stack(moves, 1), torch.tanh(self.value_head(hidden)).squeeze(-1)
+
     def release_graphs(self):
-        """Drop the captured graphs (node evaluation, line batches); they are
-        captured again on next use -- call after changing the weights."""
+        """Drop the captured graphs (node evaluation, line batches, drawn lines);
+        they are captured again on next use -- call after changing the weights."""
         self._node_graph = None
         self._line_graphs = {}
+        self._draw_graphs = {}
 
     def dynamics_rollout(self, board_encoding, move_tokens):
         """Training rollout (search_mamba.py:252-273) as one causal scan.
