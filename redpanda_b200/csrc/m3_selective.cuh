@@ -61,11 +61,13 @@ __device__ __forceinline__ int sel_length(const int* lengths, int b, int L) {
 // where log(1 + t) is below half an ulp of x.
 constexpr float kLog2eLo = 0x1.4ae0cp-26f;      // log2(e) - kLog2e
 
+constexpr float kSoftplusShift = 7e-8f;
 __device__ __forceinline__ float exp_neg(float ax) {   // e^-ax, ax >= 0
   const float hi = -ax * kLog2e;
   const float lo = fmaf(-ax, kLog2eLo, fmaf(-ax, kLog2e, -hi));
   const float t = ex2_approx(hi);
-  return ax >= 126.f ? 0.f : fmaf(t * 0x1.62e43p-1f, lo, t);   // NaN passes
+  // + kSoftplusShift: the units' mean error of -5e-8 (ex2, then the division)
+  return ax >= 126.f ? 0.f : fmaf(t * 0x1.62e43p-1f, lo + kSoftplusShift, t);   // NaN passes
 }
 __device__ __forceinline__ float log1p_of(float t) {   // t in [0, 1]
   const float s = __fdividef(t, 2.f + t), q = s * s;
@@ -119,7 +121,14 @@ __device__ __forceinline__ void lane_sum(float* v, int q) {
   }
 }
 
-__device__ __forceinline__ float2 ex2_pair(float2 x) {
+// The gates exp(de A) of two states from a2 = A log2(e).  The MUFU unit's 2^x is
+// low by 2e-8 on average for x in [-1, -1e-4] (measured), a third of a last place
+// below 1; a slow state multiplies hundreds of gates, and dA, which weighs them
+// by age, was off by 4e-7 with one sign.  The shift of the argument by
+// 2e-8 log2(e) takes the mean out; 2^shift itself rounds to 1.
+constexpr float kGateShift = 2.9e-8f;
+__device__ __forceinline__ float2 gate_pair(float2 de, float2 a2) {
+  const float2 x = __ffma2_rn(de, a2, f2(kGateShift));
   return make_float2(ex2_approx(x.x), ex2_approx(x.y));
 }
 

@@ -262,7 +262,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
             const float2 de = f2(dd.x), deu = f2(dd.y);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-              h[k][j] = __ffma2_rn(ex2_pair(__fmul2_rn(de, a2[k][j])), h[k][j],
+              h[k][j] = __ffma2_rn(gate_pair(de, a2[k][j]), h[k][j],
                                    __fmul2_rn(deu, b2[j]));
           }
         }
@@ -287,7 +287,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
             float2 y2;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              ga[s][k][j] = ex2_pair(__fmul2_rn(de, a2[k][j]));
+              ga[s][k][j] = gate_pair(de, a2[k][j]);
               gh[s][k][j] = __fmul2_rn(ga[s][k][j], h[k][j]);
               h[k][j] = __ffma2_rn(deu, b2[j], gh[s][k][j]);
               y2 = j ? __ffma2_rn(h[k][j], c2[j], y2) : __fmul2_rn(h[k][j], c2[j]);
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(SelF<LN>::NT) sel_bwd_sum_kernel(const SelBwdP
 #pragma unroll
           for (int j = 0; j < 2; ++j)
             dh[k][2 * i + j] =
-                __fmul2_rn(ex2_pair(__fmul2_rn(de, a2[k][2 * i + j])),
+                __fmul2_rn(gate_pair(de, a2[k][2 * i + j]),
                            __ffma2_rn(gy, c2[j], dh[k][2 * i + j]));
         }
       }

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(SelF<LN>::NT) sel_fwd_kernel(const SelParams p
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int x = 2 * i + j;
-              const float2 a = ex2_pair(__fmul2_rn(de, a2[k][x]));
+              const float2 a = gate_pair(de, a2[k][x]);
               h[k][x] = __ffma2_rn(a, h[k][x], __fmul2_rn(du, b2[j]));
               if (!SUM)
                 ys[k] = x ? __ffma2_rn(h[k][x], c2[j], ys[k]) : __fmul2_rn(h[k][x], c2[j]);

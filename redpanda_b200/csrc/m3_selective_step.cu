@@ -92,10 +92,10 @@ __device__ __forceinline__ void step_rows(const SelStepParams& p, int q, int d, 
       const int r = r0 + i, src = r / KR * PR;
       const float der = __shfl_sync(0xffffffffu, de[r % KR], src, LN);
       const float dur = der * __shfl_sync(0xffffffffu, uu[r % KR], src, LN);
-      h[r].x = fmaf(ex2_approx(der * a2.x), h[r].x, dur * bv[i].get(0));
-      h[r].y = fmaf(ex2_approx(der * a2.y), h[r].y, dur * bv[i].get(1));
-      h[r].z = fmaf(ex2_approx(der * a2.z), h[r].z, dur * bv[i].get(2));
-      h[r].w = fmaf(ex2_approx(der * a2.w), h[r].w, dur * bv[i].get(3));
+      h[r].x = fmaf(ex2_approx(fmaf(der, a2.x, kGateShift)), h[r].x, dur * bv[i].get(0));
+      h[r].y = fmaf(ex2_approx(fmaf(der, a2.y, kGateShift)), h[r].y, dur * bv[i].get(1));
+      h[r].z = fmaf(ex2_approx(fmaf(der, a2.z, kGateShift)), h[r].z, dur * bv[i].get(2));
+      h[r].w = fmaf(ex2_approx(fmaf(der, a2.w, kGateShift)), h[r].w, dur * bv[i].get(3));
       y[r] = fmaf(h[r].x, cv[i].get(0), h[r].y * cv[i].get(1)) +
              fmaf(h[r].z, cv[i].get(2), h[r].w * cv[i].get(3));
       if (FULL || (has && r < rows)) {
