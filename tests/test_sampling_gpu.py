@@ -142,3 +142,35 @@ def test_sample_is_capturable():
         out = m3_sample(x, u, top_k=50, top_p=0.9)
     graph.replay()
     assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("V", [300, 8192, 40000])
+@pytest.mark.parametrize("kw", [dict(m=0.02), dict(p=0.9, m=0.001), dict(p=0.3), dict(p=0.99),
+                                dict(p=0.6, m=0.2), dict(p=1e-6), dict(m=1e-9)])
+def test_sample_borders_among_many_and_few_tokens(V, kw):
+    """Rows from peaked to flat, masked ones and ones with ties: the borders lie
+    within the first tokens of the order, behind them, or in a long tie."""
+    g = torch.Generator().manual_seed(V + 1)
+    rows = 12
+    logits = torch.randn(rows, V, generator=g) * torch.tensor(
+        [0.0, 0.01, 0.3, 1, 2, 3, 5, 8, 20, 3, 3, 1])[:, None]
+    logits[9] = logits[9].round()
+    logits[10] = (logits[10] * 2).round() / 2
+    logits[11][torch.rand(V, generator=g) < 0.97] = -float("inf")
+    T_ = np.random.RandomState(V).uniform(0.5, 1.6, rows)
+    _check(logits, torch.rand(rows, generator=g), T_, 0, kw.get("p", 1.0), kw.get("m", 0.0))
+
+
+def test_sample_border_on_a_token():
+    """top_p at, and a rounding beside, the cumulative weight of a token: decided
+    as the 64-bit definition decides it (equal weights make the sums exact)."""
+    V = 512
+    logits = torch.zeros(1, V)
+    for count in (1, 2, 128, 256, 511):
+        for p in (count / V, np.nextafter(np.float32(count / V), np.float32(2)),
+                  np.nextafter(np.float32(count / V), np.float32(0))):
+            p = float(np.float32(p))
+            w = O.kept_weights(logits[0].numpy(), 1.0, 0, p, 0.0)
+            last = int(np.nonzero(w)[0][-1])
+            got = m3_sample(logits.cuda(), torch.tensor([1.0]).cuda(), top_p=p)
+            assert got.item() == last
