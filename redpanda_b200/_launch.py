@@ -41,7 +41,7 @@ def device_index(*ts):
 
 def on_device(index):
     """Context in which device ``index`` is the current one."""
-    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def raw_stream(index):
@@ -86,6 +86,7 @@ def rows(t):
     r, n = t.shape
     if t.is_contiguous():
         return t, n
-    if t.stride(1) == 1 and (r == 1 or t.stride(0) >= n):
-        return t, (t.stride(0) if r > 1 else n)
+    s0, s1 = t.stride()
+    if s1 == 1 and (r == 1 or s0 >= n):
+        return t, (s0 if r > 1 else n)
     return t.contiguous(), n

@@ -42,6 +42,7 @@
 #include <stdint.h>
 
 #include "m3_api_util.h"
+#include "m3_math.cuh"
 #include "m3_ops.h"
 #include "m3_vec.cuh"
 
@@ -79,9 +80,7 @@ struct Shared {
   int ln;
   u64 found_base;
   int found;
-  float fmax;
   int imax;
-  unsigned n;
   float wm[32];
   int wi[32];
 };
@@ -108,14 +107,17 @@ __device__ u64 block_prefix(u64 v, u64* wsum, u64* total) {
   }
   if (lane == 31) wsum[warp] = s;
   __syncthreads();
-  u64 base = 0, all = 0;
-  for (int w = 0; w < NT / 32; ++w) {
-    if (w < warp) base += wsum[w];
-    all += wsum[w];
+  // every warp scans the warps' sums
+  u64 t = lane < NT / 32 ? wsum[lane] : 0;
+#pragma unroll
+  for (int m = 1; m < NT / 32; m <<= 1) {
+    const u64 o = __shfl_up_sync(0xffffffffu, t, m);
+    if (lane >= m) t += o;
   }
+  const u64 base = __shfl_sync(0xffffffffu, t, warp > 0 ? warp - 1 : 0);
+  *total = __shfl_sync(0xffffffffu, t, NT / 32 - 1);
   __syncthreads();
-  *total = all;
-  return base + s - v;
+  return (warp > 0 ? base : 0) + s - v;
 }
 
 // The bin where the running sum of the histogram (counts, or masses) first
@@ -176,14 +178,13 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
   const T* g = static_cast<const T*>(p.logits) + row * p.ld;
   const RowReader<T, CACHE> x{g, cache};
 
-  // ---- maximum (lowest index first) and candidates
+  // ---- maximum and candidates
   float m = -CUDART_INF_F;
-  int im = 0x7fffffff;
   unsigned cand = 0;
-  auto look = [&](int i, float v) -> float {
-    if (v > -CUDART_INF_F) ++cand;
-    else v = -CUDART_INF_F;   // NaN too
-    if (v > m) { m = v; im = i; }
+  auto look = [&](float v) -> float {
+    v = fmaxf(v, -CUDART_INF_F);   // NaN as -infinity
+    m = fmaxf(m, v);
+    cand += v > -CUDART_INF_F;
     return v;
   };
   constexpr int VW = 16 / (int)sizeof(T);
@@ -200,46 +201,60 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
       if (i < head) {
 #pragma unroll
         for (int j = 0; j < VW; j += 4) {
-          const float4 f = make_float4(look(i + j, v[k].get(j)), look(i + j + 1, v[k].get(j + 1)),
-                                       look(i + j + 2, v[k].get(j + 2)),
-                                       look(i + j + 3, v[k].get(j + 3)));
+          const float4 f = make_float4(look(v[k].get(j)), look(v[k].get(j + 1)),
+                                       look(v[k].get(j + 2)), look(v[k].get(j + 3)));
           if (CACHE) *reinterpret_cast<float4*>(cache + i + j) = f;
         }
       }
     }
   }
   for (int i = head + tid; i < V; i += NT) {
-    const float v = look(i, Elem<T>::get(g[i]));
+    const float v = look(Elem<T>::get(g[i]));
     if (CACHE) cache[i] = v;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, m, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, im, o);
-    if (om > m || (om == m && oi < im)) { m = om; im = oi; }
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     cand += __shfl_xor_sync(0xffffffffu, cand, o);
   }
-  if (tid == 0) { sh.n = 0; sh.ln = 0; }
-  if (tid < 32) sh.pow2[tid] = exp2((double)tid / 32);
-  if (lane == 0) { sh.wm[warp] = m; sh.wi[warp] = im; }
+  if (tid == 0) { sh.ln = 0; sh.imax = 0x7fffffff; }
+  if (lane == 0) { sh.wm[warp] = m; sh.wi[warp] = (int)cand; }
   __syncthreads();
-  if (lane == 0) atomicAdd(&sh.n, cand);
   float top = sh.wm[0];
-  int itop = sh.wi[0];
+  int ncand = sh.wi[0];
 #pragma unroll
-  for (int w = 1; w < NT / 32; ++w)
-    if (sh.wm[w] > top || (sh.wm[w] == top && sh.wi[w] < itop)) {
-      top = sh.wm[w];
-      itop = sh.wi[w];
+  for (int w = 1; w < NT / 32; ++w) {
+    top = fmaxf(top, sh.wm[w]);
+    ncand += sh.wi[w];
+  }
+  // every token, four at a time from the cache
+  auto for_each = [&](auto&& f) {
+    if (CACHE) {
+      const int whole = V & ~3;
+      for (int i = 4 * tid; i < whole; i += 4 * NT) {
+        const float4 v = *reinterpret_cast<const float4*>(cache + i);
+        f(i, v.x);
+        f(i + 1, v.y);
+        f(i + 2, v.z);
+        f(i + 3, v.w);
+      }
+      if (whole + tid < V) f(whole + tid, cache[whole + tid]);
+    } else {
+#pragma unroll 4
+      for (int i = tid; i < V; i += NT) f(i, x.at(i));
     }
-  __syncthreads();
-  const int ncand = (int)sh.n;
+  };
   const float temp = p.temperature ? p.temperature[row] : p.temperature0;
   const int k = p.top_k ? p.top_k[row] : p.top_k0;
-  if (ncand == 0 || !(temp > 0.f) || k == 1) {
-    if (tid == 0) p.out[row] = ncand == 0 ? -1 : itop;
+  if (ncand == 0 || !(temp > 0.f) || k == 1) {   // the first token of the order
+    for_each([&](int i, float v) {
+      if (v == top && ncand) atomicMin(&sh.imax, i);
+    });
+    __syncthreads();
+    if (tid == 0) p.out[row] = ncand ? sh.imax : -1;
     return;
   }
+  if (tid < 32) sh.pow2[tid] = exp2((double)tid / 32);   // a barrier stands before its use
   const float tp = p.top_p ? p.top_p[row] : p.top_p0;
   const double mp = fmin((double)(p.min_p ? p.min_p[row] : p.min_p0), 1.0);
   const double dtop = (double)top, unit = exp2((double)p.shift);
@@ -277,21 +292,6 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     return v == top ? 0 : d < (float)(kBins - 1) ? (int)d : kBins - 1;
   };
 
-  // every token, four at a time from the cache
-  auto for_each = [&](auto&& f) {
-    if (CACHE) {
-      for (int i = 4 * tid; i < V; i += 4 * NT) {
-        const float4 v = *reinterpret_cast<const float4*>(cache + i);
-        f(i, v.x);
-        if (i + 1 < V) f(i + 1, v.y);
-        if (i + 2 < V) f(i + 2, v.z);
-        if (i + 3 < V) f(i + 3, v.w);
-      }
-    } else {
-#pragma unroll 4
-      for (int i = tid; i < V; i += NT) f(i, x.at(i));
-    }
-  };
   auto clear = [&](int n, bool mass) {
     __syncthreads();
     for (int i = tid; i < n; i += NT) {
@@ -450,14 +450,20 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
 
   // ---- top-p and min-p among the first tokens of the order; false: not decided
   auto among_first = [&]() -> bool {
+    if (top == CUDART_INF_F) return false;
     clear(kBins, false);
+    // bins of this way, monotone in v like bin_of: from the weight's own exponent
     const float c2 = inv_t * 1.44269504f;
+    constexpr float kBinsPerPower = -kBinsPerUnit * 0.693147181f;
+    auto bin2 = [&](float v) -> int {
+      return (int)fminf((v - top) * c2 * kBinsPerPower, (float)(kBins - 1));
+    };
     float sum = 0.f;
-    for_each([&](int i, float v) {
-      if (v > -CUDART_INF_F) {
-        sum += v == top ? 1.f : exp2f((v - top) * c2);
-        atomicAdd(&sh.count[bin_of(v)], 1u);
-      }
+    for_each([&](int, float v) {
+      const float y = (v - top) * c2;
+      sum += ex2_approx(y);
+      if (v > -CUDART_INF_F)
+        atomicAdd(&sh.count[(int)fminf(y * kBinsPerPower, (float)(kBins - 1))], 1u);
     });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -488,8 +494,10 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     const int last = min(sh.found, bins - 1);
     const bool whole = last == bins - 1;   // min-p's tokens, or all, are gathered
     if (last < 0 || (tp >= 1.f && !whole)) return false;
+    // (the last bin takes every weight below e^-32: its test is not this one)
+    if (last == kBins - 1) return false;
     for_each([&](int i, float v) {
-      if (v > -CUDART_INF_F && bin_of(v) <= last) {
+      if (v > -CUDART_INF_F && (v - top) * c2 * kBinsPerPower < (float)(last + 1)) {
         const int at = atomicAdd(&sh.ln, 1);
         if (at < kLong) sh.li[at] = i;
       }
@@ -529,13 +537,13 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
         // the first token at which the running weight reaches `want`
         clear(kBins, true);
         for (int j = tid; j < n; j += NT)
-          if (sh.lw[j]) add64(sh, bin_of(x.at(sh.li[j])), sh.lw[j]);
+          if (sh.lw[j]) add64(sh, bin2(x.at(sh.li[j])), sh.lw[j]);
         __syncthreads();
         const u64 thr = want >= 1.0 ? (u64)ceil(want) : 1ull;
         find_bin<NT>(sh, true, kBins, thr);
         const int bin = sh.found;
         const u64 base = sh.found_base;
-        const int m = members([&](int i) { return bin_of(x.at(i)) == bin; });
+        const int m = members([&](int i) { return bin2(x.at(i)) == bin; });
         if (tid == 0) sh.found = -1;
         __syncthreads();
         if (tid < m) {

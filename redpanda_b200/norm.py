@@ -62,8 +62,8 @@ class _NormFn(torch.autograd.Function):
         if g.dtype is not out_dtype or not g.is_contiguous():
             g = g.to(out_dtype).contiguous()
         dx = torch.empty_like(x2, memory_format=torch.contiguous_format)
-        dwb = torch.empty((1 if bt is None else 2, d), device=x2.device)
-        dw, db = (dwb[0], None) if bt is None else dwb.unbind(0)
+        dw = torch.empty_like(w)
+        db = None if bt is None else torch.empty_like(w)
         if rows:
             lib = _lib.load()
             desc = NormDesc(rows, d, H.code(x2.dtype), H.code(out_dtype), rms, eps)
@@ -76,7 +76,9 @@ class _NormFn(torch.autograd.Function):
                     g.data_ptr(), dx.data_ptr(), dw.data_ptr(), H.ptr(db), ws.data_ptr(), nws,
                     H.raw_stream(dev)))
         else:
-            dwb.zero_()
+            dw.zero_()
+            if db is not None:
+                db.zero_()
         return (dx if len(shape) == 2 else dx.view(shape), dw if wt is torch.float32 else dw.to(wt),
                 db if bt is None or bt is torch.float32 else db.to(bt), None, None, None)
 

@@ -375,16 +375,21 @@ def m3_selective_step_(h, u_t, dt_t, A, B_t, C_t, D=None, z=None, dt_bias=None, 
         raise ValueError(f"{name}: B_t and C_t are (B, N) with A's N")
     if h.shape != (B, d, N) or h.dtype is not torch.float32 or not h.is_contiguous():
         raise ValueError(f"{name}: h is (B, D, N), float32 and contiguous (it is updated in place)")
-    prepared = _prepare(H.rows, u_t, dt_t, z, B_t, C_t)
+    ty = _common(u_t, dt_t, z, B_t, C_t)
     dev = H.device_index(h, u_t, dt_t, A, B_t, C_t, D, z, dt_bias)
-    ty = prepared[0][0].dtype
-    y = torch.empty_like(prepared[0][0], memory_format=torch.contiguous_format)
+    u2, lu = H.rows(_typed(u_t, ty))
+    d2, ld = H.rows(_typed(dt_t, ty))
+    z2, lz = (None, 0) if z is None else H.rows(_typed(z, ty))
+    b2, lb = H.rows(_typed(B_t, ty))
+    c2, lc = H.rows(_typed(C_t, ty))
+    y = torch.empty_like(u2, memory_format=torch.contiguous_format)
     if B == 0:
         return y
     a32, d32, b32 = H.f32(A), H.f32(D), H.f32(dt_bias)
+    args = SelArgs(u2.data_ptr(), lu, d2.data_ptr(), ld, H.ptr(z2), lz, b2.data_ptr(), lb,
+                   c2.data_ptr(), lc, a32.data_ptr(), H.ptr(d32), H.ptr(b32), None, None)
     with H.on_device(dev):
         _lib.check(_lib.load().m3_selective_step(
-            SelDesc(B, 1, d, N, H.code(ty), int(softplus)),
-            _sel_args(prepared, a32, d32, b32, None, None), h.data_ptr(), y.data_ptr(),
+            SelDesc(B, 1, d, N, H.code(ty), int(softplus)), args, h.data_ptr(), y.data_ptr(),
             H.raw_stream(dev)))
     return y
