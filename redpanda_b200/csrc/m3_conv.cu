@@ -21,6 +21,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "m3_api_util.h"
 #include "m3_math.cuh"
 #include "m3_ops.h"
@@ -184,12 +186,22 @@ __global__ void __launch_bounds__(32 * kWorkers, K <= 4 ? 2 : 1) conv_bwd_kernel
       const int tg = te > t0 ? min(te + K - 1, n) : t0;
       Pack<T, V> rx[kAhead], rg[kAhead];
       auto fetch = [&](int t) {
+        const T* px = in.x + (size_t)t * in.ld;
+        const T* pg = g + (size_t)t * p.D;
+        if (t + kAhead <= tg) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-          if (t + i < tg) {
-            rx[i] = ld_pack<T, V>(in.x + (size_t)(t + i) * in.ld);
-            rg[i] = ld_pack<T, V>(g + (size_t)(t + i) * p.D);
+          for (int i = 0; i < kAhead; ++i) {
+            rx[i] = ld_pack<T, V>(px + i * in.ld);
+            rg[i] = ld_pack<T, V>(pg + (size_t)i * p.D);
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i)
+            if (t + i < tg) {
+              rx[i] = ld_pack<T, V>(px + i * in.ld);
+              rg[i] = ld_pack<T, V>(pg + (size_t)i * p.D);
+            }
+        }
       };
       fetch(t0);
       Vals<V> win[K], gw[K];
@@ -210,6 +222,37 @@ __global__ void __launch_bounds__(32 * kWorkers, K <= 4 ? 2 : 1) conv_bwd_kernel
         for (int j = 0; j < V; ++j) o.put(j, a.get(j));
         st_pack<T, V>(dx + (size_t)s * p.D, o);
       };
+      // One step; WHOLE: inside the run, with a dx row to write (no conditions, so
+      // that the windows of a group of steps are renamed instead of moved).
+      auto step = [&](auto whole, const Pack<T, V>& px, const Pack<T, V>& pg, int t) {
+        constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) {
+          win[k] = win[k + 1];
+          gw[k] = gw[k + 1];
+        }
+        win[K - 1].from(px);
+        Vals<V> gt;
+        gt.from(pg);
+        if (p.silu) {
+          Vals<V> a = bias;
+#pragma unroll
+          for (int k = 0; k < K; ++k) a.fma(w[k], win[k]);
+#pragma unroll
+          for (int h = 0; h < Vals<V>::H; ++h) {
+            gt.v[h].x *= dsilu_f(a.v[h].x, sigmoid_f(a.v[h].x));
+            if (V > 1) gt.v[h].y *= dsilu_f(a.v[h].y, sigmoid_f(a.v[h].y));
+          }
+        }
+        gw[K - 1] = gt;
+        if (WHOLE || t < te) {   // halo steps belong to the next run
+#pragma unroll
+          for (int h = 0; h < Vals<V>::H; ++h) db.v[h] = __fadd2_rn(db.v[h], gt.v[h]);
+#pragma unroll
+          for (int k = 0; k < K; ++k) dw[k].fma(gt, win[k]);
+        }
+        if (WHOLE || t - (K - 1) >= t0) emit(t - (K - 1));
+      };
       for (int tb = t0; tb < tg; tb += kAhead) {
         Pack<T, V> cx[kAhead], cg[kAhead];
 #pragma unroll
@@ -218,37 +261,13 @@ __global__ void __launch_bounds__(32 * kWorkers, K <= 4 ? 2 : 1) conv_bwd_kernel
           cg[i] = rg[i];
         }
         fetch(tb + kAhead);
+        if (tb - (K - 1) >= t0 && tb + kAhead <= te) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int t = tb + i;
-          if (t < tg) {
+          for (int i = 0; i < kAhead; ++i) step(std::true_type(), cx[i], cg[i], tb + i);
+        } else {
 #pragma unroll
-            for (int k = 0; k < K - 1; ++k) {
-              win[k] = win[k + 1];
-              gw[k] = gw[k + 1];
-            }
-            win[K - 1].from(cx[i]);
-            Vals<V> gt;
-            gt.from(cg[i]);
-            if (p.silu) {
-              Vals<V> a = bias;
-#pragma unroll
-              for (int k = 0; k < K; ++k) a.fma(w[k], win[k]);
-#pragma unroll
-              for (int h = 0; h < Vals<V>::H; ++h) {
-                gt.v[h].x *= dsilu_f(a.v[h].x, sigmoid_f(a.v[h].x));
-                if (V > 1) gt.v[h].y *= dsilu_f(a.v[h].y, sigmoid_f(a.v[h].y));
-              }
-            }
-            gw[K - 1] = gt;
-            if (t < te) {   // halo steps belong to the next run
-#pragma unroll
-              for (int h = 0; h < Vals<V>::H; ++h) db.v[h] = __fadd2_rn(db.v[h], gt.v[h]);
-#pragma unroll
-              for (int k = 0; k < K; ++k) dw[k].fma(gt, win[k]);
-            }
-            if (t - (K - 1) >= t0) emit(t - (K - 1));
-          }
+          for (int i = 0; i < kAhead; ++i)
+            if (tb + i < tg) step(std::false_type(), cx[i], cg[i], tb + i);
         }
       }
       // the sequence's end: g past it is zero

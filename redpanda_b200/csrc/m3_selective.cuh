@@ -70,7 +70,7 @@ __device__ __forceinline__ float exp_neg(float ax) {   // e^-ax, ax >= 0
   return ax >= 126.f ? 0.f : fmaf(t * 0x1.62e43p-1f, lo + kSoftplusShift, t);   // NaN passes
 }
 __device__ __forceinline__ float log1p_of(float t) {   // t in [0, 1]
-  const float s = __fdividef(t, 2.f + t), q = s * s;
+  const float s = t * rcp_approx(2.f + t), q = s * s;
   float p = 1.f / 13.f;
   p = fmaf(p, q, 1.f / 11.f);
   p = fmaf(p, q, 1.f / 9.f);
@@ -91,7 +91,7 @@ __device__ __forceinline__ float step_size(float x, int softplus, float* slope) 
     *slope = 1.f;
     return x;
   }
-  const float t = exp_neg(fabsf(x)), r = __fdividef(1.f, 1.f + t);
+  const float t = exp_neg(fabsf(x)), r = rcp_approx(1.f + t);
   *slope = x > 0.f ? r : t * r;
   return fmaxf(x, 0.f) + log1p_of(t);
 }

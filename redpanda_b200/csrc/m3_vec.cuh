@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "m3_math.cuh"
+
 namespace m3 {
 
 template <typename T> struct Elem;
@@ -96,11 +98,21 @@ __device__ __forceinline__ Pack<T, V> zero_pack() {
 }
 
 // silu and its derivative in fp32: s = 1 / (1 + e^-x), silu = x s,
-// silu' = s (1 + x (1 - s)).  __expf and the fast division are within a few
-// fp32 ulp, below the rounding of a bf16 result and near that of an fp32 one;
-// e^-x overflows to infinity for x < -88, where s is 0 as it should be.
-__device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// silu' = s + x s (1 - s), on the MUFU unit (2^x and 1/x to a few fp32 ulp, below
+// the rounding of a bf16 result and near that of an fp32 one).  e^-x becomes
+// infinite for x < -88, where s is 0 as it should be.
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float sigmoid_f(float x) {
+  return rcp_approx(1.f + ex2_approx(x * -kLog2e));
+}
 __device__ __forceinline__ float silu_f(float x) { return x * sigmoid_f(x); }
-__device__ __forceinline__ float dsilu_f(float x, float s) { return s * (1.f + x * (1.f - s)); }
+__device__ __forceinline__ float dsilu_f(float x, float s) {
+  const float xs = x * s;
+  return fmaf(-xs, s, xs) + s;
+}
 
 }  // namespace m3
