@@ -142,12 +142,20 @@ __global__ void __launch_bounds__(128) conv_fwd_kernel(const ConvParams p) {
       for (int j = 0; j < V; ++j) o.put(j, p.silu ? silu_f(a.get(j)) : a.get(j));
       st_pack<T, V>(y + (size_t)tt * p.D, o);
     };
-    for (; t + kAheadFwd <= te; t += kAheadFwd) {
-      Pack<T, V> r[kAheadFwd];
+    // two groups of rows in flight: one computed on, one being loaded
+    Pack<T, V> r[kAheadFwd], next[kAheadFwd];
+    auto fetch = [&](Pack<T, V> (&q)[kAheadFwd], int at) {
+      const T* px = in.x + (size_t)at * in.ld;
 #pragma unroll
-      for (int i = 0; i < kAheadFwd; ++i) r[i] = ld_pack<T, V>(in.x + (size_t)(t + i) * in.ld);
+      for (int i = 0; i < kAheadFwd; ++i) q[i] = ld_pack<T, V>(px + i * in.ld);
+    };
+    if (t + kAheadFwd <= te) fetch(r, t);
+    for (; t + kAheadFwd <= te; t += kAheadFwd) {
+      if (t + 2 * kAheadFwd <= te) fetch(next, t + kAheadFwd);
 #pragma unroll
       for (int i = 0; i < kAheadFwd; ++i) one(r[i], t + i);
+#pragma unroll
+      for (int i = 0; i < kAheadFwd; ++i) r[i] = next[i];
     }
     for (; t < te; ++t) one(ld_pack<T, V>(in.x + (size_t)t * in.ld), t);
   }

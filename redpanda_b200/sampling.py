@@ -21,8 +21,9 @@ def _setting(name, v, lead, dtype, lo, hi):
             raise ValueError(f"m3_sample: {name} is a number or one per row")
         return (v if v.dtype is dtype else v.detach().to(dtype)).contiguous(), 0
     v = float(v)
-    if not lo <= v <= hi:
-        raise ValueError(f"m3_sample: {name} must lie in [{lo}, {hi}]")
+    if not lo <= v <= hi or (dtype is torch.int32 and v != int(v)):
+        raise ValueError(f"m3_sample: {name} must lie in [{lo}, {hi}]"
+                         + (" and be whole" if dtype is torch.int32 else ""))
     return None, v
 
 

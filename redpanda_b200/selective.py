@@ -49,7 +49,7 @@ def _lengths(name, lengths, B):
     if lengths.shape != (B,) or lengths.dtype.is_floating_point or lengths.dtype is torch.bool:
         raise ValueError(f"{name}: lengths are (B,) integers")
     if lengths.dtype is not torch.int32:
-        lengths = lengths.clamp(0, 2 ** 31 - 1).to(torch.int32)
+        lengths = lengths.to(torch.int64).clamp(0, 2 ** 31 - 1).to(torch.int32)
     return lengths.contiguous()
 
 

@@ -403,3 +403,56 @@ def test_in_place_steps_refuse_autograd_and_loose_states():
     with pytest.raises(ValueError, match="differentiable"):
         S.m3_selective_scan(e[:, None], e[:, None], A, b[:, None], b[:, None],
                             state=torch.zeros(2, 8, 4, **d, requires_grad=True))
+
+
+def test_steps_of_size_zero_leave_the_state():
+    """A gate of a step of size zero is one exactly, in the scan and the step
+    (masked steps within a chunk rest on it)."""
+    g = torch.Generator().manual_seed(91)
+    B, L, D, N = 2, 100, 40, 16
+    h0 = _rand(g, B, D, N).cuda()
+    zero, b = torch.zeros(B, L, D, device="cuda"), _rand(g, B, L, N).cuda()
+    A = -_rand(g, D, N, lo=0.1, hi=50.0).cuda()
+    _, h = S.m3_selective_scan_with_state(zero, zero, A, b, b, softplus=False, state=h0)
+    assert torch.equal(h, h0)
+    h = h0.clone()
+    S.m3_selective_step_(h, zero[:, 0], zero[:, 0], A, b[:, 0], b[:, 0], softplus=False)
+    assert torch.equal(h, h0)
+
+
+@pytest.mark.parametrize("kind", ["int64", "int16", "uint8", "far"])
+def test_lengths_of_other_integer_types_and_out_of_range(kind):
+    g = torch.Generator().manual_seed(92)
+    x, w = _rand(g, 3, 20, 8).cuda(), _rand(g, 8, 4).cuda()
+    n = torch.tensor([7, 20, 0])
+    given = torch.tensor([7, 2 ** 40, -5]) if kind == "far" else n.to(getattr(torch, kind))
+    ref = S.m3_causal_conv_with_state(x, w, lengths=n.to(torch.int32).cuda())
+    got = S.m3_causal_conv_with_state(x, w, lengths=given.cuda())
+    assert torch.equal(ref[0], got[0]) and torch.equal(ref[1], got[1])
+
+
+def test_calls_side_by_side_on_two_streams():
+    """Two scans and their backward passes at once: each has its own workspace."""
+    a, gr = _scan_inputs(1, 400, 64, 16, torch.float32, seed=95)
+    b, gb = _scan_inputs(1, 400, 64, 16, torch.float32, seed=96)
+    ref = [_run_scan(a, gr), _run_scan(b, gb)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s, (p, q) in zip(streams, ((a, gr), (b, gb))):
+            with torch.cuda.stream(s):
+                got.append(_run_scan(p, q))
+        torch.cuda.synchronize()
+        for r, o in zip(ref, got):
+            assert all(torch.equal(r[k], o[k]) for k in r)
+
+
+def test_double_backward_is_refused():
+    a, gr = _scan_inputs(1, 20, 16, 8, torch.float32, seed=97)
+    c = {k: _cuda(v) for k, v in a.items()}
+    c["u"].requires_grad_(True)
+    y = S.m3_selective_scan(**c)
+    (du,) = torch.autograd.grad((y * y).sum(), c["u"], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(du.sum(), c["u"])
