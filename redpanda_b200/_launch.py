@@ -9,6 +9,7 @@ import contextlib
 
 import torch
 
+from . import _lib
 from ._lib import M3_BF16, M3_F32
 
 _CODES = {torch.float32: M3_F32, torch.bfloat16: M3_BF16}
@@ -44,9 +45,26 @@ def on_device(index):
     return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
-def raw_stream(index):
-    """The device's current stream as the integer the C ABI takes."""
-    return torch._C._cuda_getCurrentRawStream(index)
+def launch(index, fn, *args):
+    """Call a library entry on device ``index`` and its current stream (the entry's
+    last argument); raises for a status other than 0."""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc)
+
+
+def once_differentiable(body):
+    """``torch.autograd.function.once_differentiable`` without its cost where no
+    second derivative can follow (autograd is off while the backward runs)."""
+    guarded = torch.autograd.function.once_differentiable(body)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else body(ctx, *grads)
+    return backward
 
 
 def f32(t):

@@ -9,14 +9,18 @@
 // earlier part), or are zero; steps at or past a row's length have y = 0 and
 // take no part in any gradient, and the new state ends at the length.
 //
-// Bound by memory: forward x in, y out; backward x and dy in, dx out.  A thread
-// owns a vector of channels and a run of TT steps and keeps the K rows of the
-// filter's window in registers, so each row is loaded once plus K-1 halo rows
-// per run (L1/L2 hits: the neighbouring run loads the same lines); rows are
-// fetched kAhead at a time before they are used.  The backward recomputes p
-// from x rather than storing it.  Weight gradients stay in registers over all
-// runs of a thread; a CTA joins its 8 workers per channel in order and writes
-// one partial, and a second launch adds the partials in a fixed order.
+// Bound by memory forward (x in, y out) and by instructions backward (x and dy
+// in, dx out, and silu' of every element: about 45 per element at first, a third
+// of them moves of the windows).  A thread owns a vector of channels and a run of
+// TT steps and keeps the K rows of the filter's window in registers, so each row
+// is loaded once plus K-1 halo rows per run (L1/L2 hits: the neighbouring run
+// loads the same lines); the next group of rows is in flight while the present
+// one is computed on.  Products are packed pairs of channels.  The backward
+// recomputes p from x rather than storing it.  Weight gradients stay in registers
+// over all runs of a thread; a CTA joins its 8 workers per channel in order and
+// writes one partial, and a second launch adds the partials in a fixed order.
+// 512 rows x 64 steps x 1536 channels, K = 4, bf16: 47 us forward (4.3 TB/s),
+// 84 us backward (3.6 TB/s); 60 and 186 us at first.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -80,14 +80,15 @@ struct ConvStepParams {
 };
 cudaError_t launch_conv_step(const ConvStepParams& p, cudaStream_t s);
 
-// Selective scan.  A lane group of `ln` threads shares a pair of channels, four
-// states per thread and channel; NP = 4 * ln states are kept per channel.
+// Selective scan.  In the backward a lane group of `ln` threads shares a pair of
+// channels, four states per thread and channel (the forward: half as many lanes,
+// eight states each); NP = 4 * ln states are kept per channel.
 constexpr int kMaxSelState = 128;
 constexpr int kSelSteps = 16;         // steps staged at a time = checkpoint interval
 
 inline int sel_lanes(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32; }
 inline int sel_threads(int ln) { return ln >= 16 ? 256 : 128; }
-inline int sel_tile(int ln) { return sel_threads(ln) / ln * 2; }   // channels per CTA
+inline int sel_tile(int ln) { return sel_threads(ln) / ln * 2; }   // channels per backward CTA
 
 struct SelParams {
   const void* u; const void* dt; const void* z;          // (B*L, ld), z may be nullptr

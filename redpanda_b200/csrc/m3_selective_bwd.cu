@@ -14,11 +14,14 @@
 // then each group of four steps is recomputed with its gates and gate-state
 // products in registers and taken back.  So a state costs 1.75 exponentials
 // here, about 16 packed FMA-pipe operations per two states, and no state but
-// the checkpoints moves through memory.
+// the checkpoints moves through memory.  256 rows x 64 steps x 1536 channels,
+// N = 32, bf16: 1041 us (1714 us at first), with no unit above 60 % busy (issue
+// 56 %, shared memory 57 %, FMA pipe 45 %, MUFU 36 %) and eleven warps per SM,
+// which the registers of four steps' gates and products leave room for.
 //
 // Sums over channels (dB, dC): pairs of channels in a thread, transposed
-// shuffles over a warp's lane groups, warps joined through shared memory in
-// order, channel tiles as partials that a second launch adds in order.  Sums
+// shuffles over a warp's lane groups (Order below), warps joined through shared
+// memory in order, channel tiles as partials that a second launch adds in order.  Sums
 // over rows (dA, dD, dbias) stay in registers over a CTA's rows, then partials
 // too.  No atomics: results do not depend on scheduling.
 //

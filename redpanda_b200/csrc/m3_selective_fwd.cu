@@ -1,16 +1,21 @@
 // Selective scan, forward (the recurrence stands in m3_selective.cuh).
 //
-// Bound by the exponentials: one per (step, channel, state) on the MUFU unit
-// (16 per SM and clock) beside four packed FMA-pipe operations per two states,
-// while u, dt, z and y move only once per (step, channel).  A CTA owns a tile
-// of channels of one row and walks its steps; raw inputs of the next kSelSteps
-// steps are loaded into registers while the present ones are computed.
+// Bound by the exponentials, one per (step, channel, state) on the MUFU unit (16
+// per SM and clock), with shared memory close behind: u, dt, z and y move only
+// once per (step, channel).  A CTA owns 64 channels (128 for N <= 8) of one row
+// and walks its steps kSelSteps at a time; the next steps' inputs are copied into
+// the threads' own slots by cp.async meanwhile, so no register waits for a load.
+// 256 rows x 64 steps x 1536 channels, N = 32, bf16: 277 us, of which the
+// exponentials alone are 180 us at the unit's rate (MUFU 69 %, shared memory
+// 54 % busy; 432 us at first, when bf16 pairs were unpacked where they were
+// loaded and softplus was the library's).
 //
 // With few rows (a single prompt) one pass over the steps would leave most SMs
 // idle, so the steps are split: a first launch gives every run its local end
 // state and the sum of its step sizes, a second joins them in order,
 //   h_in[s+1] = exp(A dsum[s]) h_in[s] + h_local[s],
-// and the scan proper then starts each run from its own h_in.
+// and the scan proper then starts each run from its own h_in.  One row of 4096
+// steps x 1024 channels, N = 16, bf16: 29 + 9 + 37 us.
 #include "m3_api_util.h"
 #include "m3_selective.cuh"
 

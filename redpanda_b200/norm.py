@@ -21,20 +21,17 @@ from ._lib import NormDesc
 MAX_D = 32768           # longest row of the kernels
 
 
-def _forward(x2, ld, w, b, eps, rms, out_dtype, stats):
+def _forward(x2, ld, w, b, desc, out_dtype, stats):
+    """y and, with ``stats``, one buffer of rstd and (layer norm) the means."""
     rows, d = x2.shape
-    dev = x2.get_device()
     y = (torch.empty_like(x2) if out_dtype is x2.dtype and ld == d
          else torch.empty((rows, d), device=x2.device, dtype=out_dtype))
-    # one buffer: rstd, then (layer norm) the means
-    st = torch.empty((1 if rms else 2, rows), device=x2.device) if stats else None
+    st = torch.empty((1 if desc.rms else 2, rows), device=x2.device) if stats else None
     if rows:
         rstd = st.data_ptr() if stats else None
-        mean = rstd + 4 * rows if stats and not rms else None
-        with H.on_device(dev):
-            _lib.check(_lib.load().m3_norm_fwd(
-                NormDesc(rows, d, H.code(x2.dtype), H.code(out_dtype), rms, eps), x2.data_ptr(),
-                ld, w.data_ptr(), H.ptr(b), y.data_ptr(), mean, rstd, H.raw_stream(dev)))
+        mean = rstd + 4 * rows if stats and not desc.rms else None
+        H.launch(x2.get_device(), _lib.load().m3_norm_fwd, desc, x2.data_ptr(), ld, w.data_ptr(),
+                 H.ptr(b), y.data_ptr(), mean, rstd)
     return y, st
 
 
@@ -46,35 +43,34 @@ class _NormFn(torch.autograd.Function):
         d = x.shape[-1]
         x2, ld = H.rows(x if x.dim() == 2 else x.reshape(-1, d))
         w = H.f32(weight)
-        y, st = _forward(x2, ld, w, H.f32(bias), eps, rms, out_dtype, True)
+        desc = NormDesc(x2.shape[0], d, H.code(x2.dtype), H.code(out_dtype), rms, eps)
+        y, st = _forward(x2, ld, w, H.f32(bias), desc, out_dtype, True)
         ctx.save_for_backward(x2, w, st)
-        ctx.cfg = (ld, eps, rms, out_dtype, x.shape, weight.dtype,
+        ctx.cfg = (ld, desc, out_dtype, x.shape, weight.dtype,
                    None if bias is None else bias.dtype)
         return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @H.once_differentiable
     def backward(ctx, g):
         x2, w, st = ctx.saved_tensors
-        ld, eps, rms, out_dtype, shape, wt, bt = ctx.cfg
-        rows, d = x2.shape
-        dev = x2.get_device()
+        ld, desc, out_dtype, shape, wt, bt = ctx.cfg
         if g.dtype is not out_dtype or not g.is_contiguous():
             g = g.to(out_dtype).contiguous()
         dx = torch.empty_like(x2, memory_format=torch.contiguous_format)
         dw = torch.empty_like(w)
         db = None if bt is None else torch.empty_like(w)
+        rows = desc.rows
         if rows:
             lib = _lib.load()
-            desc = NormDesc(rows, d, H.code(x2.dtype), H.code(out_dtype), rms, eps)
+            dev = x2.get_device()
             with H.on_device(dev):
                 nws = lib.m3_norm_bwd_workspace_bytes(desc)
-                ws = torch.empty(nws, device=x2.device, dtype=torch.uint8)
-                rstd = st.data_ptr()
-                _lib.check(lib.m3_norm_bwd(
-                    desc, x2.data_ptr(), ld, w.data_ptr(), None if rms else rstd + 4 * rows, rstd,
-                    g.data_ptr(), dx.data_ptr(), dw.data_ptr(), H.ptr(db), ws.data_ptr(), nws,
-                    H.raw_stream(dev)))
+            ws = torch.empty(nws, device=x2.device, dtype=torch.uint8)
+            rstd = st.data_ptr()
+            H.launch(dev, lib.m3_norm_bwd, desc, x2.data_ptr(), ld, w.data_ptr(),
+                     None if desc.rms else rstd + 4 * rows, rstd, g.data_ptr(), dx.data_ptr(),
+                     dw.data_ptr(), H.ptr(db), ws.data_ptr(), nws)
         else:
             dw.zero_()
             if db is not None:
@@ -98,7 +94,8 @@ def _norm(name, x, weight, bias, eps, rms, out_dtype):
     if H.needs_grad(x, weight, bias):
         return _NormFn.apply(x, weight, bias, eps, rms, out_dtype)
     x2, ld = H.rows(x if x.dim() == 2 else x.reshape(-1, d))
-    y = _forward(x2, ld, H.f32(weight), H.f32(bias), eps, rms, out_dtype, False)[0]
+    desc = NormDesc(x2.shape[0], d, H.code(x2.dtype), H.code(out_dtype), rms, eps)
+    y = _forward(x2, ld, H.f32(weight), H.f32(bias), desc, out_dtype, False)[0]
     return y if x.dim() == 2 else y.view(x.shape)
 
 

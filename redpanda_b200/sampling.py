@@ -63,8 +63,7 @@ def m3_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         return out
     x, ld = H.rows(logits if lead else logits.unsqueeze(0))
     u = uniform.contiguous()
-    with H.on_device(dev):
-        _lib.check(_lib.load().m3_sample(
-            SampleDesc(rows, V, code, t0, int(k0), p0, m0), x.data_ptr(), ld, u.data_ptr(),
-            H.ptr(t), H.ptr(k), H.ptr(p), H.ptr(m), out.data_ptr(), H.raw_stream(dev)))
+    H.launch(dev, _lib.load().m3_sample, SampleDesc(rows, V, code, t0, int(k0), p0, m0),
+             x.data_ptr(), ld, u.data_ptr(), H.ptr(t), H.ptr(k), H.ptr(p), H.ptr(m),
+             out.data_ptr())
     return out

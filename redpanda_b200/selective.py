@@ -95,11 +95,9 @@ def _conv_fwd(x, ld, w, b, state, lengths, silu, want_state):
         if out is not None:
             out.copy_(state) if state is not None else out.zero_()
         return y, out
-    dev = x.get_device()
-    with H.on_device(dev):
-        _lib.check(_lib.load().m3_causal_conv_fwd(
-            ConvDesc(B, L, D, K, H.code(x.dtype), silu), x.data_ptr(), ld, w.data_ptr(), H.ptr(b),
-            H.ptr(state), H.ptr(lengths), y.data_ptr(), H.ptr(out), H.raw_stream(dev)))
+    H.launch(x.get_device(), _lib.load().m3_causal_conv_fwd,
+             ConvDesc(B, L, D, K, H.code(x.dtype), silu), x.data_ptr(), ld, w.data_ptr(), H.ptr(b),
+             H.ptr(state), H.ptr(lengths), y.data_ptr(), H.ptr(out))
     return y, out
 
 
@@ -120,7 +118,7 @@ class _ConvFn(torch.autograd.Function):
         return y, out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @H.once_differentiable
     def backward(ctx, g, _):
         if g is None:
             return (None,) * 7
@@ -143,11 +141,10 @@ class _ConvFn(torch.autograd.Function):
             desc = ConvDesc(B, L, D, K, H.code(x.dtype), silu)
             with H.on_device(dev):
                 nws = lib.m3_causal_conv_bwd_workspace_bytes(desc)
-                ws = torch.empty(nws, device=x.device, dtype=torch.uint8)
-                _lib.check(lib.m3_causal_conv_bwd(
-                    desc, x.data_ptr(), ld, w.data_ptr(), H.ptr(b), H.ptr(state), H.ptr(lengths),
-                    g.data_ptr(), dx.data_ptr(), dw.data_ptr(), H.ptr(db), ws.data_ptr(), nws,
-                    H.raw_stream(dev)))
+            ws = torch.empty(nws, device=x.device, dtype=torch.uint8)
+            H.launch(dev, lib.m3_causal_conv_bwd, desc, x.data_ptr(), ld, w.data_ptr(), H.ptr(b),
+                     H.ptr(state), H.ptr(lengths), g.data_ptr(), dx.data_ptr(), dw.data_ptr(),
+                     H.ptr(db), ws.data_ptr(), nws)
         return dx, _typed(dw, wt), _typed(db, bt), None, None, None, None
 
 
@@ -198,10 +195,8 @@ def m3_causal_conv_step_(state, x_t, weight, bias=None, silu=True):
         return y
     x2, ld = H.rows(x_t)
     w, b = H.f32(weight), H.f32(bias)
-    with H.on_device(dev):
-        _lib.check(_lib.load().m3_causal_conv_step(
-            ConvDesc(B, 1, D, K, code, int(silu)), state.data_ptr(), x2.data_ptr(), ld,
-            w.data_ptr(), H.ptr(b), y.data_ptr(), H.raw_stream(dev)))
+    H.launch(dev, _lib.load().m3_causal_conv_step, ConvDesc(B, 1, D, K, code, int(silu)),
+             state.data_ptr(), x2.data_ptr(), ld, w.data_ptr(), H.ptr(b), y.data_ptr())
     return y
 
 
@@ -242,11 +237,11 @@ def _scan_fwd(prepared, A, Dskip, dt_bias, state, lengths, softplus, want_state,
             nck = lib.m3_selective_ckpt_floats(desc)
             ckpt = torch.empty(nck, device=u.device) if nck else None
         nws = lib.m3_selective_fwd_workspace_bytes(desc)
-        if nws:
-            ws = torch.empty(nws, device=u.device, dtype=torch.uint8)
-        _lib.check(lib.m3_selective_fwd(
-            desc, _sel_args(prepared, A, Dskip, dt_bias, state, lengths), y.data_ptr(), H.ptr(h),
-            H.ptr(ckpt), H.ptr(ws), nws, H.raw_stream(dev)))
+    if nws:
+        ws = torch.empty(nws, device=u.device, dtype=torch.uint8)
+    H.launch(dev, lib.m3_selective_fwd, desc,
+             _sel_args(prepared, A, Dskip, dt_bias, state, lengths), y.data_ptr(), H.ptr(h),
+             H.ptr(ckpt), H.ptr(ws), nws)
     return y, h, ckpt
 
 
@@ -273,7 +268,7 @@ class _SelectiveScanFn(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @H.once_differentiable
     def backward(ctx, g, _):
         if g is None:
             return (None,) * 12
@@ -306,9 +301,9 @@ class _SelectiveScanFn(torch.autograd.Function):
             index = u.get_device()
             with H.on_device(index):
                 nws = lib.m3_selective_bwd_workspace_bytes(desc)
-                ws = torch.empty(nws, device=dev, dtype=torch.uint8)
-                _lib.check(lib.m3_selective_bwd(desc, args, g.data_ptr(), H.ptr(ckpt), grads,
-                                                ws.data_ptr(), nws, H.raw_stream(index)))
+            ws = torch.empty(nws, device=dev, dtype=torch.uint8)
+            H.launch(index, lib.m3_selective_bwd, desc, args, g.data_ptr(), H.ptr(ckpt), grads,
+                     ws.data_ptr(), nws)
         out = (du, ddt, dA, dB, dC, dD, dz, dbias)
         return (*(_typed(t, ty) for t, ty in zip(out, types)), None, None, None, None)
 
@@ -388,8 +383,6 @@ def m3_selective_step_(h, u_t, dt_t, A, B_t, C_t, D=None, z=None, dt_bias=None, 
     a32, d32, b32 = H.f32(A), H.f32(D), H.f32(dt_bias)
     args = SelArgs(u2.data_ptr(), lu, d2.data_ptr(), ld, H.ptr(z2), lz, b2.data_ptr(), lb,
                    c2.data_ptr(), lc, a32.data_ptr(), H.ptr(d32), H.ptr(b32), None, None)
-    with H.on_device(dev):
-        _lib.check(_lib.load().m3_selective_step(
-            SelDesc(B, 1, d, N, H.code(ty), int(softplus)), args, h.data_ptr(), y.data_ptr(),
-            H.raw_stream(dev)))
+    H.launch(dev, _lib.load().m3_selective_step, SelDesc(B, 1, d, N, H.code(ty), int(softplus)),
+             args, h.data_ptr(), y.data_ptr())
     return y
