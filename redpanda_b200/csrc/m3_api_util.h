@@ -47,7 +47,7 @@ inline int check_device() {
 }
 
 // Lets a kernel use `smem` bytes of dynamic shared memory, once per device and
-// kernel.
+// kernel; one value per kernel, so that calls from several threads agree.
 struct OncePerDevice {
   std::atomic<int> value[kMaxDevices] = {};
 };

@@ -677,7 +677,9 @@ template <typename T, int NT, bool CACHE>
 cudaError_t sample_typed(const SampleParams& p, cudaStream_t s) {
   constexpr auto* kern = sample_kernel<T, NT, CACHE>;
   const int smem = ((int)sizeof(Shared) + 15) / 16 * 16 + (CACHE ? (p.V + 3) / 4 * 16 : 0);
-  const cudaError_t e = allow_smem<kern>(smem);
+  // the most that any row length takes: calls side by side set one value
+  constexpr int most = ((int)sizeof(Shared) + 15) / 16 * 16 + (CACHE ? kCacheMax * 4 : 0);
+  const cudaError_t e = allow_smem<kern>(most);
   if (e != cudaSuccess) return e;
   kern<<<p.rows, NT, smem, s>>>(p);
   return cudaGetLastError();

@@ -174,3 +174,22 @@ def test_sample_border_on_a_token():
             last = int(np.nonzero(w)[0][-1])
             got = m3_sample(logits.cuda(), torch.tensor([1.0]).cuda(), top_p=p)
             assert got.item() == last
+
+
+def test_sample_from_threads_with_different_lengths():
+    """Row lengths that need different amounts of shared memory, side by side."""
+    from concurrent.futures import ThreadPoolExecutor
+    g = torch.Generator().manual_seed(41)
+    work = [(torch.randn(3, V, generator=g).cuda(), torch.rand(3, generator=g).cuda())
+            for V in (12000, 32768, 5000, 30000, 16000, 25000)]
+
+    def run(w):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = [m3_sample(*w, top_k=40, top_p=0.9) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+        return torch.stack(out)
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(len(work)) as pool:
+        got = list(pool.map(run, work))
+    for w, o in zip(work, got):
+        assert (o == m3_sample(*w, top_k=40, top_p=0.9)).all()
