@@ -165,8 +165,19 @@ __device__ __forceinline__ void set_pairs(float2* h, float4 v) {
 __device__ __forceinline__ float4 quad_of(const float2* h) {
   return make_float4(h[0].x, h[0].y, h[1].x, h[1].y);
 }
-__device__ __forceinline__ float4 scaled(float4 v, float a) {
-  return make_float4(v.x * a, v.y * a, v.z * a, v.w * a);
+// A to powers of 2.  A below -1e38 (-infinity among them) counts as that: its gate
+// is 0 at any step size, but 1 where the step size is 0 (a step past the length).
+__device__ __forceinline__ float power_of(float a) {
+  const float v = a * kLog2e;
+  return v < -1e38f ? -1e38f : v;   // NaN stays
+}
+__device__ __forceinline__ float4 powers_of(float4 a) {
+  return make_float4(power_of(a.x), power_of(a.y), power_of(a.z), power_of(a.w));
+}
+// A run's gate 2^e on a state: a zero stays, even where growth over the whole run
+// (A > 0) overflows.
+__device__ __forceinline__ float carry_over(float e, float h, float sum) {
+  return h == 0.f ? sum : fmaf(ex2_approx(e), h, sum);
 }
 
 // ------------------------------------------------------------- staged rows

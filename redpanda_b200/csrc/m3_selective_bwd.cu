@@ -189,7 +189,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const float4 v = load_quad_any(p.A, 0, c0 + cc2[k], n0, p.D, p.N);
-    set_pairs(a2[k], reorder(scaled(v, kLog2e), pr, el));
+    set_pairs(a2[k], reorder(powers_of(v), pr, el));
     dA[k][0] = dA[k][1] = make_float2(0.f, 0.f);
   }
   // a thread's staged elements share their columns
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(SelF<LN>::NT) sel_bwd_sum_kernel(const SelBwdP
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
       set_pairs(a2[k] + 2 * i,
-                scaled(load_quad_any(p.A, 0, c + k, n0 + 4 * i, p.D, p.N), kLog2e));
+                powers_of(load_quad_any(p.A, 0, c + k, n0 + 4 * i, p.D, p.N)));
       dh[k][2 * i] = dh[k][2 * i + 1] = make_float2(0.f, 0.f);
     }
   float bias[M::VW], dsum[2] = {0.f, 0.f};
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(128) sel_join_bwd_kernel(const SelBwdParams bp
   if (i >= total) return;
   const int n = (int)(i % NP);
   const long long bd = i / NP;
-  const float a2 = n < p.N ? p.A[(size_t)(bd % p.D) * p.N + n] * kLog2e : 0.f;
+  const float a2 = n < p.N ? power_of(p.A[(size_t)(bd % p.D) * p.N + n]) : 0.f;
   const long long sd = (long long)p.B * p.D;
   float v = 0.f;
   constexpr int U = 8;   // runs whose summaries are loaded ahead of the chain
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(128) sel_join_bwd_kernel(const SelBwdParams bp
 #pragma unroll
     for (int k = 0; k < U; ++k)
       if (s0 - k > 0) {
-        v = fmaf(ex2_approx(d[k] * a2), v, x[k]);
+        v = carry_over(d[k] * a2, v, x[k]);
         bp.qin[(s0 - k - 1) * total + i] = v;
       }
   }

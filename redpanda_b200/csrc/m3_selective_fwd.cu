@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(SelF<LN>::NT) sel_fwd_kernel(const SelParams p
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
       set_pairs(a2[k] + 2 * i,
-                scaled(load_quad_any(p.A, 0, c + k, n0 + 4 * i, p.D, p.N), kLog2e));
+                powers_of(load_quad_any(p.A, 0, c + k, n0 + 4 * i, p.D, p.N)));
       set_pairs(h[k] + 2 * i,
                 SUM ? make_float4(0.f, 0.f, 0.f, 0.f)
                     : p.hin != nullptr && split > 0
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(128) sel_join_kernel(const SelParams p, int NP
   const int d = (int)(bd % p.D);
   float h = 0.f, a2 = 0.f;
   if (n < p.N) {
-    a2 = p.A[(size_t)d * p.N + n] * kLog2e;
+    a2 = power_of(p.A[(size_t)d * p.N + n]);
     if (p.h0 != nullptr) h = p.h0[bd * p.N + n];
   }
   const long long sd = (long long)p.B * p.D;
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(128) sel_join_kernel(const SelParams p, int NP
 #pragma unroll
     for (int k = 0; k < U; ++k)
       if (s0 + k + 1 < p.splits) {
-        h = fmaf(ex2_approx(d[k] * a2), h, x[k]);
+        h = carry_over(d[k] * a2, h, x[k]);
         p.hin[(s0 + k + 1) * total + i] = h;
       }
   }

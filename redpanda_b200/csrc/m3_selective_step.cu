@@ -56,7 +56,7 @@ __device__ __forceinline__ void step_rows(const SelStepParams& p, int q, int d, 
   if (has)
     a2 = VEC ? *reinterpret_cast<const float4*>(p.A + (size_t)d * p.N + n0)
              : load_quad_any(p.A, 0, d, n0, p.D, p.N);
-  a2 = scaled(a2, kLog2e);
+  a2 = powers_of(a2);
 #pragma unroll
   for (int i = 0; i < KR; ++i)
     if (FULL || (live && q / PR * KR + i < rows)) de[i] = step_size(de[i], p.softplus);

@@ -456,3 +456,43 @@ def test_double_backward_is_refused():
     (du,) = torch.autograd.grad((y * y).sum(), c["u"], create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(du.sum(), c["u"])
+
+
+def _growing(seed):
+    a, gr = _scan_inputs(1, 2000, 64, 16, torch.float32, gate=False, skip=False, bias=False,
+                         seed=seed)
+    a["A"] = a["A"].abs() / 160 + 0.95          # 0.95 to 1.05
+    a["dt"] = torch.full_like(a["dt"], 4.0)
+    return a, gr
+
+
+def test_growth_over_empty_runs_keeps_zeros():
+    """A > 0: a state that is zero over a long part stays zero there, although the
+    part's whole growth is past float32; its gradient, from the back, too."""
+    a, _ = _growing(51)
+    a["u"][:, :-8] = 0
+    with torch.no_grad():
+        y, h = S.m3_selective_scan_with_state(**{k: _cuda(v) for k, v in a.items()},
+                                              softplus=False)
+    ref, mag = O.scan(**a, sp=False), O.scan(**a, sp=False, magnitude=True)
+    # the 8 steps that are not empty: 10 roundings each, the sum over the states
+    for got, k in ((y, "y"), (h, "h")):
+        assert ((got.cpu().double() - ref[k]).abs() <= (20 * 8 + 16 + 64) * O.E * mag[k]).all()
+    a, gr = _growing(52)
+    a["u"].zero_()
+    gr[:, 8:] = 0
+    _check_scan(a, gr, _run_scan(a, gr, softplus=False), softplus=False)
+
+
+@pytest.mark.parametrize("low", [-float("inf"), -3e38])
+def test_gates_of_the_lowest_values_are_zero_up_to_the_length(low):
+    """A column of A at the type's lowest values forgets at every step, and the
+    state behind a length that ends inside a chunk is the one at the length."""
+    a, _ = _scan_inputs(2, 13, 8, 4, torch.float32, seed=52)
+    a["lengths"] = torch.tensor([13, 5], dtype=torch.int32)
+    a["A"][:, 1] = low
+    y, h = S.m3_selective_scan_with_state(**{k: _cuda(v) for k, v in a.items()})
+    b = dict(a, A=a["A"].clone())
+    b["A"][:, 1] = -1e6          # exp(-1e6 de) is 0 for every step size here
+    y1, h1 = S.m3_selective_scan_with_state(**{k: _cuda(v) for k, v in b.items()})
+    assert torch.equal(y, y1) and torch.equal(h, h1) and h.isfinite().all()
