@@ -19,6 +19,10 @@ def _setting(name, v, lead, dtype, lo, hi):
     if torch.is_tensor(v) and v.dim():
         if v.shape != lead:
             raise ValueError(f"m3_sample: {name} is a number or one per row")
+        if dtype is torch.int32 and v.dtype is not dtype:
+            if v.dtype.is_floating_point or v.dtype is torch.bool:
+                raise ValueError(f"m3_sample: {name} per row is a tensor of integers")
+            v = v.to(torch.int64).clamp(0, 2 ** 31 - 1)
         return (v if v.dtype is dtype else v.detach().to(dtype)).contiguous(), 0
     v = float(v)
     if not lo <= v <= hi or (dtype is torch.int32 and v != int(v)):
@@ -40,7 +44,7 @@ def m3_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     times their total.  Temperature 0 takes the largest logit, the lowest index
     among equals.  A row without candidates gives -1.
 
-    Each setting is a number or a tensor of one per row (float32; int32 for
+    Each setting is a number or a tensor of one per row (float32; integers for
     top_k).  Values in tensors are not checked: a temperature that is negative or
     NaN counts as 0, top_k below 0 as 0, top_p that is NaN or below 0 as 0, min_p
     above 1 or NaN as 1.  V <= 262144."""

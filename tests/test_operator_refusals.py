@@ -64,6 +64,7 @@ def test_cpu_tensors_are_refused():
     lambda: m3_sample(z(2, 8), z(2), top_k=-1),
     lambda: m3_sample(z(2, 8), z(2), top_k=2.5),
     lambda: m3_sample(z(2, 8), z(2), top_k=z(3, dtype=torch.int32)),
+    lambda: m3_sample(z(2, 8), z(2), top_k=z(2)),
     lambda: m3_sample(z(1, 262145), z(1)),
 ])
 def test_bad_arguments_raise_value_errors(call):

@@ -193,3 +193,14 @@ def test_sample_from_threads_with_different_lengths():
         got = list(pool.map(run, work))
     for w, o in zip(work, got):
         assert (o == m3_sample(*w, top_k=40, top_p=0.9)).all()
+
+
+def test_sample_top_k_of_other_integer_types():
+    """Counts past 32 bits keep every token, negative ones too; none wraps."""
+    g = torch.Generator().manual_seed(42)
+    x, u = torch.randn(4, 100, generator=g).cuda(), torch.rand(4, generator=g).cuda()
+    want = m3_sample(x, u, top_k=torch.tensor([0, 0, 3, 0], dtype=torch.int32).cuda())
+    got = m3_sample(x, u, top_k=torch.tensor([2 ** 32 + 1, -2 ** 32 + 1, 3, 2 ** 40]).cuda())
+    assert torch.equal(got, want)
+    assert torch.equal(m3_sample(x, u, top_k=torch.tensor([0, 0, 3, 0], dtype=torch.uint8).cuda()),
+                       want)
