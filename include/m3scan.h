@@ -449,7 +449,9 @@ M3_API int m3_scan_bwd_noalloc(const m3_scan_desc* desc,
  * Row-strided inputs: row r starts at base + r * ld elements; a (B, L, .)
  * tensor has the rows b * L + t.  Arithmetic, states and sums are fp32 (64-bit
  * where stated); outputs are rounded once to their element type.  All results
- * are independent of scheduling (no floating-point atomics). */
+ * are independent of scheduling (no floating-point atomics).  Batch, seqlen and
+ * d_inner are at most 2^30 each; for the selective scan the products batch *
+ * seqlen and batch * d_inner are below 2^31 and d_inner below 2^24. */
 
 typedef struct m3_norm_desc {
   int64_t rows;       /* >= 1 */

@@ -24,6 +24,14 @@ def code(dtype):
     return c
 
 
+MAX_SIZE = 2 ** 30      # rows, steps and channels of one call (32-bit in the library)
+
+
+def check_sizes(name, *sizes):
+    if max(sizes) > MAX_SIZE:
+        raise ValueError(f"{name}: sizes of at most {MAX_SIZE} each")
+
+
 def device_index(*ts):
     """Index of the CUDA device that every tensor (None: skipped) is on."""
     dev = -1

@@ -18,6 +18,12 @@ int status(cudaError_t e) {
   return M3_ERR_LAUNCH;
 }
 
+// sizes that the kernels' 32-bit roundings up to tiles could pass 2^31 with
+bool too_large(int a, int b, int c) {
+  constexpr int most = 1 << 30;
+  return a > most || b > most || c > most;
+}
+
 int check_norm(const m3_norm_desc* d) {
   if (!d) return M3_ERR_NULL;
   if (d->rows < 1 || d->d < 1 || !(d->eps >= 0.f)) return M3_ERR_SHAPE;
@@ -29,6 +35,7 @@ int check_norm(const m3_norm_desc* d) {
 int check_conv(const m3_conv_desc* d) {
   if (!d) return M3_ERR_NULL;
   if (d->batch < 1 || d->seqlen < 1 || d->d_inner < 1 || d->width < 1) return M3_ERR_SHAPE;
+  if (too_large(d->batch, d->seqlen, d->d_inner)) return M3_ERR_SHAPE;
   if ((double)d->batch * d->seqlen * d->d_inner > 128.0 * 2147483647.0) return M3_ERR_SHAPE;
   if (!dtype_ok(d->dtype)) return M3_ERR_DTYPE;
   if (d->width > kMaxConvWidth) return M3_ERR_UNSUPPORTED;
@@ -40,6 +47,7 @@ int check_sel(const m3_sel_desc* d) {
   if (d->batch < 1 || d->seqlen < 1 || d->d_inner < 1 || d->d_state < 1) return M3_ERR_SHAPE;
   if (!dtype_ok(d->dtype)) return M3_ERR_DTYPE;
   if (d->d_state > kMaxSelState) return M3_ERR_UNSUPPORTED;
+  if (too_large(d->batch, d->seqlen, d->d_inner)) return M3_ERR_SHAPE;
   // grids: rows x channel tiles, state quads of the joins
   const double tiles = (double)(d->d_inner + 15) / 16;
   if (tiles > 65535.0 * 16 || (double)d->batch * tiles > 2147483647.0 ||

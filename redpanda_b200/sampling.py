@@ -53,6 +53,8 @@ def m3_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     V, lead = logits.shape[-1], logits.shape[:-1]
     if V > MAX_VOCAB:
         raise ValueError(f"m3_sample: at most {MAX_VOCAB} logits per row")
+    if lead:
+        H.check_sizes("m3_sample", lead[0])
     if uniform.shape != lead or uniform.dtype != torch.float32:
         raise ValueError("m3_sample: uniform is float32, one number per row")
     code = H.code(logits.dtype)

@@ -75,7 +75,8 @@ def _check_conv(name, x, weight, bias, state, lengths):
     if x.dim() != 3 or x.shape[-1] < 1:
         raise ValueError(f"{name}: x is (B, L, D)")
     H.code(x.dtype)
-    B, _, D = x.shape
+    B, L, D = x.shape
+    H.check_sizes(name, B, L, D)
     _check_filter(name, D, weight, bias)
     if state is not None and (state.shape != (B, weight.shape[1] - 1, D)
                               or state.dtype is not x.dtype):
@@ -183,6 +184,7 @@ def m3_causal_conv_step_(state, x_t, weight, bias=None, silu=True):
     if x_t.dim() != 2 or x_t.shape[1] < 1:
         raise ValueError(f"{name}: x_t is (B, D)")
     B, D = x_t.shape
+    H.check_sizes(name, B, D)
     _check_filter(name, D, weight, bias)
     K = weight.shape[1]
     if state.shape != (B, K - 1, D) or state.dtype is not x_t.dtype or not state.is_contiguous():
@@ -313,6 +315,7 @@ def _scan(name, u, dt, A, Bm, Cm, D, z, dt_bias, softplus, state, lengths, want_
             (z is not None and z.shape != u.shape):
         raise ValueError(f"{name}: u, dt and z are (B, L, D)")
     B, L, d = u.shape
+    H.check_sizes(name, B, L, d)
     _check_params(name, d, A, D, dt_bias)
     N = A.shape[1]
     if Bm.shape != (B, L, N) or Cm.shape != (B, L, N):
@@ -364,6 +367,7 @@ def m3_selective_step_(h, u_t, dt_t, A, B_t, C_t, D=None, z=None, dt_bias=None, 
             (z is not None and z.shape != u_t.shape):
         raise ValueError(f"{name}: u_t, dt_t and z are (B, D)")
     B, d = u_t.shape
+    H.check_sizes(name, B, d)
     _check_params(name, d, A, D, dt_bias)
     N = A.shape[1]
     if B_t.shape != (B, N) or C_t.shape != (B, N):

@@ -65,6 +65,15 @@ def test_cpu_tensors_are_refused():
     lambda: m3_sample(z(2, 8), z(2), top_k=2.5),
     lambda: m3_sample(z(2, 8), z(2), top_k=z(3, dtype=torch.int32)),
     lambda: m3_sample(z(2, 8), z(2), top_k=z(2)),
+    # sizes that 32 bits would cut short
+    lambda: m3_sample(z(1, 1).expand(2 ** 32 + 1, 1), z(1).expand(2 ** 32 + 1)),
+    lambda: S.m3_causal_conv(z(1, 1, 1).expand(1, 2 ** 32 + 5, 1), z(1, 1)),
+    lambda: S.m3_causal_conv_step_(z(1, 0, 1).expand(2 ** 31, 0, 1),
+                                   z(1, 1).expand(2 ** 31, 1), z(1, 1)),
+    lambda: S.m3_selective_scan(*2 * [z(1, 1, 1).expand(1, 2 ** 32 + 5, 1)], z(1, 1),
+                                *2 * [z(1, 1, 1).expand(1, 2 ** 32 + 5, 1)]),
+    lambda: S.m3_selective_step_(z(1, 1, 1).expand(2 ** 31, 1, 1), *2 * [z(1, 1).expand(2 ** 31, 1)],
+                                 z(1, 1), *2 * [z(1, 1).expand(2 ** 31, 1)]),
     lambda: m3_sample(z(1, 262145), z(1)),
 ])
 def test_bad_arguments_raise_value_errors(call):
@@ -110,6 +119,8 @@ def test_c_entries_validate_before_device_work():
     def conv(B=1, L=4, D=8, K=4, ty=0, x=p, ld=8, st=n, y=p + 512, so=n):
         return lib.m3_causal_conv_fwd(_lib.ConvDesc(B, L, D, K, ty, 1), x, ld, p, n, st, n, y, so, n)
     assert [conv(B=0), conv(L=0), conv(D=0), conv(K=0), conv(ld=7)] == [2] * 5
+    big = (1 << 30) + 1
+    assert [conv(B=big), conv(L=big), conv(D=big, ld=big)] == [2] * 3
     assert [conv(K=9), conv(ty=2), conv(x=n), conv(x=p + 1)] == [4, 3, 1, 5]
     assert [conv(y=p), conv(st=p + 1024, so=p + 1024)] == [11, 11]
     c = _lib.ConvDesc(1, 4, 8, 4, 0, 1)
@@ -125,6 +136,8 @@ def test_c_entries_validate_before_device_work():
     def sel(B=1, L=4, D=8, Ns=2, ty=0, a=None, y=p, h=n, ws=n, nws=0):
         return lib.m3_selective_fwd(_lib.SelDesc(B, L, D, Ns, ty, 1), a or args(), y, h, n, ws, nws, n)
     assert [sel(B=0), sel(L=0), sel(D=0), sel(Ns=0)] == [2] * 4
+    assert [sel(L=big), sel(L=2 ** 31 - 1), sel(B=big),
+            sel(D=2 ** 31 - 1, a=args(u_ld=2 ** 31, dt_ld=2 ** 31))] == [2] * 4
     assert [sel(ty=3), sel(Ns=129, a=args(B_ld=129, C_ld=129)), sel(y=n)] == [3, 4, 1]
     assert [sel(a=args(u=n)), sel(a=args(A=n)), sel(a=args(u_ld=7)), sel(a=args(B_ld=1)),
             sel(a=args(u=p + 2)), sel(a=args(z=p, z_ld=4))] == [1, 1, 2, 2, 5, 2]
