@@ -76,7 +76,8 @@ class RMSNorm(nn.Module):
 
     def forward(self, x):
         if (self.use_kernel and x.is_cuda and x.shape[-1] <= MAX_D
-                and x.dtype in (torch.float32, torch.bfloat16)):
+                and x.dtype in (torch.float32, torch.bfloat16)
+                and self.weight.dtype in (torch.float32, torch.bfloat16)):
             return m3_rms_norm(x, self.weight, self.eps,
                                out_dtype=torch.promote_types(x.dtype, self.weight.dtype))
         if not torch.is_grad_enabled():   # inference: torch's fused kernel, same formula

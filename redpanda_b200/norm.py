@@ -128,5 +128,7 @@ class LayerNorm(nn.LayerNorm):
         if (self.use_kernel and x.is_cuda and x.dtype in (torch.float32, torch.bfloat16)
                 and self.weight is not None and len(self.normalized_shape) == 1
                 and self.normalized_shape[0] <= MAX_D):
-            return m3_layer_norm(x, self.weight, self.bias, self.eps)
+            # autocast: torch's layer norm gives float32 there
+            wide = torch.float32 if torch.is_autocast_enabled("cuda") else None
+            return m3_layer_norm(x, self.weight, self.bias, self.eps, out_dtype=wide)
         return super().forward(x)

@@ -191,8 +191,8 @@ class SearchMamba(nn.Module):
         line.  Returns (moves (K, L) int64, values (K,)): the moves and the value
         head's evaluation behind each line.  The step and the head run as one
         captured graph for K lines, kept until ``release_graphs``."""
-        if uniforms.dim() != 2 or uniforms.shape[1] < 1:
-            raise ValueError("sample_lines: uniforms are (lines, moves)")
+        if uniforms.dim() != 2 or uniforms.numel() == 0:
+            raise ValueError("sample_lines: uniforms are (lines, moves), one of each at least")
         K, L = uniforms.shape
         hidden, cache = self.prime_board(board_encoding)
         if hidden.shape[0] != 1:

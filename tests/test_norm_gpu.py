@@ -181,3 +181,17 @@ def test_layer_norm_module():
     m.use_kernel = True
     assert torch.equal(m(x), N.m3_layer_norm(x, m.weight, m.bias, m.eps))
     assert set(m.state_dict()) == {"weight", "bias"}
+
+
+def test_layer_norm_module_under_autocast():
+    """float32 results under autocast, as torch's layer norm, for bfloat16 inputs."""
+    m = N.LayerNorm(64).cuda()
+    x = torch.randn(10, 64, generator=torch.Generator().manual_seed(8)).cuda().bfloat16()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        ref = m(x)
+        m.use_kernel = True
+        got = m(x)
+    assert got.dtype == ref.dtype == torch.float32
+    # sums of 64 terms in either order and a dozen roundings: each side is off by
+    # at most (64 + 12) 2^-24 of |y| + max |x - mean| rstd < 8, twice
+    assert (got - ref).abs().max().item() <= 2 * 76 * 2 ** -24 * 16

@@ -229,3 +229,11 @@ def test_model_norms_on_the_kernels():
             N.LayerNorm.use_kernel = False
     for a, b in zip(ref, got):
         assert (a - b).abs().max() <= 5e-6 * max(1.0, a.abs().max().item())
+
+
+def test_sample_lines_needs_a_line_and_a_move():
+    m = _search()
+    board = torch.randint(0, 96, (12,), device="cuda")
+    for shape in ((0, 3), (3, 0), (3,)):
+        with pytest.raises(ValueError):
+            m.sample_lines(board, torch.zeros(shape, device="cuda"))
