@@ -28,6 +28,7 @@
 // Few rows: the steps are split over CTAs as in the forward, with the state's
 // gradient at each run's end from per-run summaries joined from the back.
 #include "m3_api_util.h"
+#include "m3_pdl.cuh"
 #include "m3_selective.cuh"
 
 namespace m3 {
@@ -202,6 +203,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
     dD[j] = dbias[j] = 0.f;
   }
 
+  pdl_wait();   // every CTA: the join's results, and the end of what it waited for
   for (size_t b = bg; b < (size_t)p.B; b += bp.bgroups) {
     const int n = sel_length(p.lengths, (int)b, p.L);
     const size_t rows = b * p.L;
@@ -438,6 +440,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
   }
   // partials over this CTA's rows: dA, then dD and dbias of each channel
   constexpr int PW = G::NP + 2;
+  pdl_launch_dependents();   // not before: waiting CTAs would take room
   float* part = bp.part_a + (size_t)blockIdx.y * p.D * PW;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
@@ -494,6 +497,7 @@ __global__ void __launch_bounds__(SelF<LN>::NT) sel_bwd_sum_kernel(const SelBwdP
   const size_t b = blockIdx.x / tiles;
   const int split = blockIdx.y + 1;
   const int ch0 = split * p.cps, ch1 = min(ch0 + p.cps, p.nch);
+  pdl_launch_dependents();
   const int n = sel_length(p.lengths, (int)b, p.L);
   const RowPtrs<T> rp(bp, b * p.L);
   const bool gate = rp.z != nullptr;
@@ -592,10 +596,15 @@ __global__ void __launch_bounds__(128) sel_join_bwd_kernel(const SelBwdParams bp
   const SelParams& p = bp.f;
   const long long total = (long long)p.B * p.D * NP;
   const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
-  if (i >= total) return;
+  pdl_launch_dependents();
+  if (i >= total) {
+    pdl_wait();
+    return;
+  }
   const int n = (int)(i % NP);
   const long long bd = i / NP;
   const float a2 = n < p.N ? power_of(p.A[(size_t)(bd % p.D) * p.N + n]) : 0.f;
+  pdl_wait();
   const long long sd = (long long)p.B * p.D;
   float v = 0.f;
   constexpr int U = 8;   // runs whose summaries are loaded ahead of the chain
@@ -624,6 +633,8 @@ __global__ void __launch_bounds__(128) sel_reduce_bc_kernel(const SelBwdParams b
   const long long rows = (long long)p.B * p.L;
   const int per = 2 * NP / 4;
   const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
   if (i >= rows * per) return;
   const long long row = i / per;
   const int x = (int)(i % per) * 4, which = x / NP, n0 = x % NP;
@@ -656,6 +667,7 @@ __global__ void __launch_bounds__(128) sel_reduce_a_kernel(const SelBwdParams bp
   const SelParams& p = bp.f;
   const int pw = NP + 2;
   const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
+  pdl_wait();
   if (i >= (long long)p.D * pw) return;
   const int n = (int)(i % pw);
   const long long d = i / pw;
@@ -684,15 +696,22 @@ cudaError_t bwd_typed(const SelBwdParams& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const unsigned wtiles = (unsigned)((p.f.D + W::DT - 1) / W::DT);
     sum<<<dim3(wtiles * p.f.B, p.f.splits - 1), W::NT, wide, s>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
     const long long total = (long long)p.f.B * p.f.D * G::NP;
-    sel_join_bwd_kernel<<<(unsigned)((total + 127) / 128), 128, 0, s>>>(p, G::NP);
+    e = launch_maybe_pdl(true, sel_join_bwd_kernel, dim3((unsigned)((total + 127) / 128)),
+                         dim3(128), 0, s, p, (int)G::NP);
+    if (e != cudaSuccess) return e;
   }
-  main<<<dim3(tiles, p.workers), G::NT, smem, s>>>(p);
+  e = launch_maybe_pdl(p.f.splits > 1, main, dim3(tiles, p.workers), dim3(G::NT), smem, s, p);
+  if (e != cudaSuccess) return e;
   const long long quads = (long long)p.f.B * p.f.L * (2 * G::NP / 4);
-  sel_reduce_bc_kernel<T><<<(unsigned)((quads + 127) / 128), 128, 0, s>>>(p, tiles, G::NP);
+  e = launch_maybe_pdl(true, sel_reduce_bc_kernel<T>, dim3((unsigned)((quads + 127) / 128)),
+                       dim3(128), 0, s, p, (int)tiles, (int)G::NP);
+  if (e != cudaSuccess) return e;
   const long long na = (long long)p.f.D * (G::NP + 2);
-  sel_reduce_a_kernel<<<(unsigned)((na + 127) / 128), 128, 0, s>>>(p, G::NP);
-  return cudaGetLastError();
+  return launch_maybe_pdl(true, sel_reduce_a_kernel, dim3((unsigned)((na + 127) / 128)), dim3(128),
+                          0, s, p, (int)G::NP);
 }
 
 template <typename T>
