@@ -30,6 +30,7 @@
 #include "m3_api_util.h"
 #include "m3_math.cuh"
 #include "m3_ops.h"
+#include "m3_pdl.cuh"
 #include "m3_vec.cuh"
 
 namespace m3 {
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(32 * kWorkers, K <= 4 ? 2 : 1) conv_bwd_kernel
         st_pack<T, V>(dx + (size_t)s * p.D, zero_pack<T, V>());
     }
   }
+  pdl_launch_dependents();
   for (int k = 0; k < kWorkers; ++k) {   // workers add in order
     if (wk == k)
 #pragma unroll
@@ -323,6 +325,7 @@ __global__ void __launch_bounds__(256) conv_reduce_kernel(const float* part, int
   const int cx = threadIdx.x & 31, k = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + cx, tap = blockIdx.y;
   float a = 0.f;
+  pdl_wait();
   if (c < D) {
     const float* q = part + (size_t)tap * D + c;
     for (int i = k; i < n; i += 8) a += q[(size_t)i * (K + 1) * D];
@@ -425,9 +428,9 @@ struct BwdLaunch {
     conv_bwd_kernel<T, V, K><<<grid, 32 * kWorkers, 0, s>>>(p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    conv_reduce_kernel<<<dim3((unsigned)((p.D + 31) / 32), (unsigned)(K + 1)), 256, 0, s>>>(
-        p.part, p.workers, p.D, K, p.dw, p.db);
-    return cudaGetLastError();
+    return launch_maybe_pdl(true, conv_reduce_kernel,
+                            dim3((unsigned)((p.D + 31) / 32), (unsigned)(K + 1)), dim3(256), 0, s,
+                            (const float*)p.part, p.workers, p.D, K, p.dw, p.db);
   }
 };
 

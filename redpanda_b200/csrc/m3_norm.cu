@@ -29,6 +29,7 @@
 
 #include "m3_api_util.h"
 #include "m3_ops.h"
+#include "m3_pdl.cuh"
 #include "m3_vec.cuh"
 
 namespace m3 {
@@ -228,6 +229,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_bwd_kernel(const NormBwdParam
     cx = nx;
     cg = ng;
   }
+  pdl_launch_dependents();
   // the CTA's partial of dw (and db)
   float* part = p.part + (size_t)blockIdx.x * 2 * d;
   if constexpr (WARP) {
@@ -269,6 +271,7 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* part, in
   const int c = blockIdx.x * 32 + cx;
   const int which = blockIdx.y;   // 0: dw, 1: db
   float a = 0.f;
+  pdl_wait();
   if (c < d) {
     const float* q = part + (size_t)which * d + c;
 #pragma unroll 4
@@ -369,9 +372,9 @@ struct LaunchBwd {
     else norm_bwd_kernel<TX, TY, VEC, NV, WARP, MAXT, MINB, false><<<ctas, nt, 0, s>>>(p);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    norm_reduce_kernel<<<dim3((p.d + 31) / 32, p.db != nullptr ? 2 : 1), 1024, 0, s>>>(
-        p.part, ctas, p.d, p.dw, p.db);
-    return cudaGetLastError();
+    return launch_maybe_pdl(true, norm_reduce_kernel,
+                            dim3((p.d + 31) / 32, p.db != nullptr ? 2 : 1), dim3(1024), 0, s,
+                            (const float*)p.part, ctas, p.d, p.dw, p.db);
   }
 };
 
