@@ -53,7 +53,7 @@ namespace {
 typedef unsigned long long u64;
 constexpr int kBins = 1024;
 constexpr float kBinsPerUnit = 32.f;
-constexpr int kCacheMax = 32768;   // floats of a row kept in shared memory
+constexpr int kCacheMax = 32768;   // logits of a row kept in shared memory
 constexpr int kList = 256;         // tokens ranked by comparing all pairs
 constexpr int kLong = 1024;        // tokens gathered around a top-p or min-p border
 // Relative error of a sum of fp32 weights against the exact one: the argument's
@@ -156,23 +156,32 @@ struct Cut {
   }
 };
 
-// The row: cached floats, or the logits themselves (NaN as -infinity).
+// The row: cached in its own type, where two bytes a token hold two more CTAs per
+// SM than four, or the logits themselves (NaN as -infinity).
 template <typename T, bool CACHE>
 struct RowReader {
   const T* g;
-  const float* s;
+  const T* s;
   __device__ __forceinline__ float at(int i) const {
-    if (CACHE) return s[i];
+    if (CACHE) return Elem<T>::get(s[i]);
     const float v = Elem<T>::get(g[i]);
     return v > -CUDART_INF_F ? v : -CUDART_INF_F;
   }
 };
 
+__device__ __forceinline__ void cache_four(float* p, float4 f) {
+  *reinterpret_cast<float4*>(p) = f;
+}
+__device__ __forceinline__ void cache_four(__nv_bfloat16* p, float4 f) {
+  __nv_bfloat162 v[2] = {__floats2bfloat162_rn(f.x, f.y), __floats2bfloat162_rn(f.z, f.w)};
+  *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+}
+
 template <typename T, int NT, bool CACHE>
 __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
-  float* cache = reinterpret_cast<float*>(raw + (sizeof(Shared) + 15) / 16 * 16);
+  T* cache = reinterpret_cast<T*>(raw + (sizeof(Shared) + 15) / 16 * 16);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const size_t row = blockIdx.x;
   const int V = p.V;
@@ -204,14 +213,14 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
         for (int j = 0; j < VW; j += 4) {
           const float4 f = make_float4(look(v[k].get(j)), look(v[k].get(j + 1)),
                                        look(v[k].get(j + 2)), look(v[k].get(j + 3)));
-          if (CACHE) *reinterpret_cast<float4*>(cache + i + j) = f;
+          if (CACHE) cache_four(cache + i + j, f);
         }
       }
     }
   }
   for (int i = head + tid; i < V; i += NT) {
     const float v = look(Elem<T>::get(g[i]));
-    if (CACHE) cache[i] = v;
+    if (CACHE) cache[i] = Elem<T>::put(v);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -233,13 +242,11 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     if (CACHE) {
       const int whole = V & ~3;
       for (int i = 4 * tid; i < whole; i += 4 * NT) {
-        const float4 v = *reinterpret_cast<const float4*>(cache + i);
-        f(i, v.x);
-        f(i + 1, v.y);
-        f(i + 2, v.z);
-        f(i + 3, v.w);
+        const Pack<T, 4> v = ld_pack<T, 4>(cache + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f(i + j, v.get(j));
       }
-      if (whole + tid < V) f(whole + tid, cache[whole + tid]);
+      if (whole + tid < V) f(whole + tid, x.at(whole + tid));
     } else {
 #pragma unroll 4
       for (int i = tid; i < V; i += NT) f(i, x.at(i));
@@ -676,9 +683,9 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
 template <typename T, int NT, bool CACHE>
 cudaError_t sample_typed(const SampleParams& p, cudaStream_t s) {
   constexpr auto* kern = sample_kernel<T, NT, CACHE>;
-  const int smem = ((int)sizeof(Shared) + 15) / 16 * 16 + (CACHE ? (p.V + 3) / 4 * 16 : 0);
+  const int smem = ((int)sizeof(Shared) + 15) / 16 * 16 + (CACHE ? (p.V + 3) / 4 * 4 * (int)sizeof(T) : 0);
   // the most that any row length takes: calls side by side set one value
-  constexpr int most = ((int)sizeof(Shared) + 15) / 16 * 16 + (CACHE ? kCacheMax * 4 : 0);
+  constexpr int most = ((int)sizeof(Shared) + 15) / 16 * 16 + (CACHE ? kCacheMax * (int)sizeof(T) : 0);
   const cudaError_t e = allow_smem<kern>(most);
   if (e != cudaSuccess) return e;
   kern<<<p.rows, NT, smem, s>>>(p);
