@@ -35,8 +35,11 @@
 //    ordered key.
 // Measured for 4096 rows of 8192 bf16 logits, top-p and min-p of their own per
 // row, half of them with k = 1: 589 us with every way by digits and the
-// library's exponential, 164 us without the gathered lists, 105 us now (the row's bytes alone: 10 us; it
-// is bound by instructions, about 20 per token of a row with a top-p).
+// library's exponential, 164 us without the gathered lists, 105 us with the
+// row cached as floats, 91 us now (the row's bytes alone: 10 us; it is bound by
+// instructions, about 70 per token on average).  Shorter lists (kLong 512) or
+// fewer bins (512) free room for another CTA but leave more rows to the next way:
+// 100 and 96 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
