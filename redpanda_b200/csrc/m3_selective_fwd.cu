@@ -6,8 +6,8 @@
 // and walks its steps kSelSteps at a time; the next steps' inputs are copied into
 // the threads' own slots by cp.async meanwhile, so no register waits for a load.
 // 256 rows x 64 steps x 1536 channels, N = 32, bf16: 277 us, of which the
-// exponentials alone are 180 us at the unit's rate (MUFU 69 %, shared memory
-// 54 % busy; 432 us at first, when bf16 pairs were unpacked where they were
+// exponentials alone are 180 us at the unit's rate (MUFU 74 %, shared memory
+// 64 % busy; 432 us at first, when bf16 pairs were unpacked where they were
 // loaded and softplus was the library's).
 //
 // With few rows (a single prompt) one pass over the steps would leave most SMs
