@@ -265,7 +265,8 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     if (tid == 0) p.out[row] = ncand ? sh.imax : -1;
     return;
   }
-  if (tid < 32) sh.pow2[tid] = exp2((double)tid / 32);   // a barrier stands before its use
+  if (tid < 32) sh.pow2[tid] = exp2((double)tid / 32);
+  __syncthreads();   // the draw without any cut evaluates weights at once
   const float tp = p.top_p ? p.top_p[row] : p.top_p0;
   const double mp = fmin((double)(p.min_p ? p.min_p[row] : p.min_p0), 1.0);
   const double dtop = (double)top, unit = exp2((double)p.shift);
