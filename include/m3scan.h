@@ -590,7 +590,7 @@ typedef struct m3_sample_desc {
  * holders weigh 1 and the others 0), ordered by x descending, then index:
  *   top_k   keeps the first k (<= 0: all)
  *   top_p   of those, the shortest prefix with at least top_p of their weight,
- *           one token at least (>= 1: all)
+ *           one token at least (>= 1: all; negative or NaN: as 0, one token)
  *   min_p   of those, the tokens with w_i >= min(min_p, 1)
  * and the token is the smallest index whose cumulative weight over the kept
  * tokens, in index order, exceeds uniform * their total (the last kept one when

@@ -267,7 +267,9 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
   }
   if (tid < 32) sh.pow2[tid] = exp2((double)tid / 32);
   __syncthreads();   // the draw without any cut evaluates weights at once
-  const float tp = p.top_p ? p.top_p[row] : p.top_p0;
+  // NaN and negative as 0, the first token: each of the ways below compares tp in
+  // its own direction
+  const float tp = fmaxf(p.top_p ? p.top_p[row] : p.top_p0, 0.f);
   const double mp = fmin((double)(p.min_p ? p.min_p[row] : p.min_p0), 1.0);
   const double dtop = (double)top, unit = exp2((double)p.shift);
   const double scale = CUDART_L2E / (double)temp;   // to powers of 2
@@ -638,7 +640,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     u64 total;
     block_prefix<NT>(mine, sh.wsum, &total);
     const double want = ceil((double)tp * (double)total);
-    const u64 thr = want >= 1.0 ? (u64)want : 1ull;   // NaN and p <= 0: the first token
+    const u64 thr = want >= 1.0 ? (u64)want : 1ull;   // p = 0: the first token
     find_bin<NT>(sh, true, kBins, thr);
     select(true, thr, sh.found, sh.found_base);
   }

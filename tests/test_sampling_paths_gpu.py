@@ -4,6 +4,7 @@ that are not numbers, borders in large vocabularies."""
 import pytest
 import torch
 
+from redpanda_b200.sampling import m3_sample
 from test_sampling_gpu import T, _check
 
 pytestmark = pytest.mark.gpu
@@ -26,3 +27,30 @@ def test_sample_without_cuts_sets_up_its_own_tables(rows, V, dtype):
     for kw in (dict(), dict(T_=0.7), dict(k=V + 5)):
         _overwrite_shared_memory()
         _check(logits, torch.rand(rows, generator=g), **kw)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [7, 255, 256, 257, 700, 1024, 1025, 8192, 40000])
+def test_sample_top_p_that_is_no_number_takes_the_first_token(V, dtype):
+    """top_p of NaN, or below 0, per row counts as 0, whatever the number of
+    candidates and the other settings: the first token of the order."""
+    g = torch.Generator().manual_seed(V)
+    rows = 6
+    logits = (torch.randn(rows, V, generator=g) * 0.5).to(T[dtype])
+    logits[1] = 0.25                       # ties: the lowest index
+    logits[2, :V // 2] = -float("inf")
+    most = logits.float() == logits.float().max(1, keepdim=True).values
+    want = torch.where(most, torch.arange(V), V).min(1).values
+    assert want[1] == 0
+    x, u = logits.cuda(), torch.full((rows,), 0.999).cuda()
+    for bad in (float("nan"), -0.5, -float("inf"), 0.0):
+        p = torch.full((rows,), bad).cuda()
+        for kw in (dict(), dict(top_k=3), dict(top_k=V - 1), dict(min_p=1e-4), dict(min_p=0.3),
+                   dict(temperature=0.5), dict(temperature=50.0, min_p=0.01)):
+            got = m3_sample(x, u, top_p=p, **kw)
+            assert torch.equal(got.cpu(), want), (bad, kw)
+    # beside rows with a top_p of their own, whose draws stay theirs
+    p = torch.tensor([0.5, float("nan")] * 3).cuda()
+    ref = m3_sample(x, u, top_p=0.5, min_p=1e-4)
+    got = m3_sample(x, u, top_p=p, min_p=1e-4).cpu()
+    assert torch.equal(got[::2], ref[::2].cpu()) and torch.equal(got[1::2], want[1::2])
