@@ -8,6 +8,7 @@ device, no copy or cast of what already has the kernels' layout and type.
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import M3_BF16, M3_F32
@@ -84,6 +85,15 @@ def f32(t):
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def refuse_tangents(name, *ts):
+    """Raise for a tensor that carries a forward-mode tangent: the kernels have
+    reverse-mode derivatives only, and would return a result without one."""
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode derivative")
 
 
 def needs_grad(*ts):

@@ -90,6 +90,7 @@ def _norm(name, x, weight, bias, eps, rms, out_dtype):
         raise ValueError(f"{name}: eps must not be negative")
     out_dtype = x.dtype if out_dtype is None else out_dtype
     H.code(x.dtype), H.code(out_dtype)      # TypeError for another element type
+    H.refuse_tangents(name, x, weight, bias)
     H.device_index(x, weight, bias)
     if H.needs_grad(x, weight, bias):
         return _NormFn.apply(x, weight, bias, eps, rms, out_dtype)
@@ -104,7 +105,7 @@ def m3_layer_norm(x, weight, bias=None, eps=1e-5, out_dtype=None):
 
     x float32 or bfloat16 (rows may be strided); weight and bias (d,) of any
     float type, used in float32; the result has ``out_dtype`` (default x's).
-    Differentiable in x, weight and bias (once)."""
+    Differentiable in x, weight and bias (once, in reverse mode)."""
     return _norm("m3_layer_norm", x, weight, bias, eps, 0, out_dtype)
 
 

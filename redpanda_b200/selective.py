@@ -18,8 +18,8 @@ last K-1 input rows (B, K-1, D) in x's element type and h (B, D, N) float32.
 past a row's length are not read, their outputs and gradients are zero, and the
 state is the one at the length.  Arithmetic and states are float32, each output
 is rounded once, and sums run in a fixed order.  Outputs are differentiable
-(once); the states are not, neither as input nor as output.  There is no CPU
-path: every op raises on CPU tensors.
+(once, in reverse mode); the states are not, neither as input nor as output.
+There is no CPU path: every op raises on CPU tensors.
 """
 
 import torch
@@ -83,6 +83,7 @@ def _check_conv(name, x, weight, bias, state, lengths):
         raise ValueError(f"{name}: the state is (B, K - 1, D) in x's element type")
     _fixed_state(name, state)
     lens = _lengths(name, lengths, B)
+    H.refuse_tangents(name, x, weight, bias, state)
     H.device_index(x, weight, bias, state, lens)
     return lens
 
@@ -191,6 +192,7 @@ def m3_causal_conv_step_(state, x_t, weight, bias=None, silu=True):
         raise ValueError(f"{name}: the state is (B, K - 1, D), contiguous (it is updated in "
                          "place) and of x_t's element type")
     code = H.code(x_t.dtype)
+    H.refuse_tangents(name, x_t, state, weight, bias)
     dev = H.device_index(x_t, state, weight, bias)
     y = torch.empty_like(x_t, memory_format=torch.contiguous_format)
     if B == 0:
@@ -325,6 +327,7 @@ def _scan(name, u, dt, A, Bm, Cm, D, z, dt_bias, softplus, state, lengths, want_
     _common(u, dt, z, Bm, Cm)
     _fixed_state(name, state)
     lens = _lengths(name, lengths, B)
+    H.refuse_tangents(name, u, dt, A, Bm, Cm, D, z, dt_bias, state)
     H.device_index(u, dt, A, Bm, Cm, D, z, dt_bias, state, lens)
     if H.needs_grad(u, dt, A, Bm, Cm, D, z, dt_bias):
         return _SelectiveScanFn.apply(u, dt, A, Bm, Cm, D, z, dt_bias, state, lens, int(softplus),
@@ -375,6 +378,7 @@ def m3_selective_step_(h, u_t, dt_t, A, B_t, C_t, D=None, z=None, dt_bias=None, 
     if h.shape != (B, d, N) or h.dtype is not torch.float32 or not h.is_contiguous():
         raise ValueError(f"{name}: h is (B, D, N), float32 and contiguous (it is updated in place)")
     ty = _common(u_t, dt_t, z, B_t, C_t)
+    H.refuse_tangents(name, h, u_t, dt_t, A, B_t, C_t, D, z, dt_bias)
     dev = H.device_index(h, u_t, dt_t, A, B_t, C_t, D, z, dt_bias)
     u2, lu = H.rows(_typed(u_t, ty))
     d2, ld = H.rows(_typed(dt_t, ty))
