@@ -23,6 +23,7 @@ There is no CPU path: every op raises on CPU tensors.
 """
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from . import _launch as H
@@ -201,6 +202,7 @@ def m3_causal_conv_step_(state, x_t, weight, bias=None, silu=True):
     w, b = H.f32(weight), H.f32(bias)
     H.launch(dev, _lib.load().m3_causal_conv_step, ConvDesc(B, 1, D, K, code, int(silu)),
              state.data_ptr(), x2.data_ptr(), ld, w.data_ptr(), H.ptr(b), y.data_ptr())
+    increment_version(state)    # a backward pass that has saved it raises
     return y
 
 
@@ -393,4 +395,5 @@ def m3_selective_step_(h, u_t, dt_t, A, B_t, C_t, D=None, z=None, dt_bias=None, 
                    c2.data_ptr(), lc, a32.data_ptr(), H.ptr(d32), H.ptr(b32), None, None)
     H.launch(dev, _lib.load().m3_selective_step, SelDesc(B, 1, d, N, H.code(ty), int(softplus)),
              args, h.data_ptr(), y.data_ptr())
+    increment_version(h)
     return y
