@@ -59,10 +59,20 @@ constexpr float kBinsPerUnit = 32.f;
 constexpr int kCacheMax = 32768;   // logits of a row kept in shared memory
 constexpr int kList = 256;         // tokens ranked by comparing all pairs
 constexpr int kLong = 1024;        // tokens gathered around a top-p or min-p border
-// Relative error of a sum of fp32 weights against the exact one: the argument's
-// rounding, (2 + 30) 2^-23 for weights above 2^-30, and the sum's, 40 2^-24,
-// doubled.
-constexpr double kSumError = 1.6e-5;
+// Bound on the relative error of the fp32 total of a row's weights, in steps of
+// e = 2^-24 and to first order.
+//  - The exponent y = (x - max) c, c = log2(e) / T, passes 4.3 roundings (the
+//    difference, 1 / T, log2(e) itself, two products), so a weight 2^y is off by
+//    ln 2 * 4.3 |y| e < 3 |y| e.  Over the weights' own distribution the mean of |y|
+//    is its entropy less log2 of the total (which is 1 at least): at most log2 V
+//    <= 18, so 54 e of the total.
+//  - ex2.approx: 4 e.  The exact weights' own rounding to integers: below e.
+//  - The additions that a weight passes: its thread's (V / NT, 5 more where four
+//    neighbours go together), 5 shuffles, NT / 32 warps.
+template <int NT>
+__device__ __forceinline__ double sum_error(int V) {
+  return (54 + 4 + 1 + V / NT + 5 + 5 + NT / 32) * 0x1p-24;
+}
 
 // A key whose unsigned order is x descending.
 __device__ __forceinline__ unsigned desc_key(float x) {
@@ -543,7 +553,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     };
     Cut c;
     if (tp < 1.f) {
-      const double want = (double)tp * (double)all * unit, slack = kSumError * want + 1.0;
+      const double want = (double)tp * (double)all * unit, slack = sum_error<NT>(V) * want + 1.0;
       if ((double)got < want + slack) {
         if (!whole || (double)got > want - slack) return false;
         // top-p's border is behind min-p's: everything gathered stays

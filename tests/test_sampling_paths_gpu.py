@@ -1,9 +1,11 @@
 """m3_sample where its ways of deciding a row meet: rows without any cut, settings
 that are not numbers, borders in large vocabularies."""
 
+import numpy as np
 import pytest
 import torch
 
+import seq_oracle as O
 from redpanda_b200.sampling import m3_sample
 from test_sampling_gpu import T, _check
 
@@ -54,3 +56,29 @@ def test_sample_top_p_that_is_no_number_takes_the_first_token(V, dtype):
     ref = m3_sample(x, u, top_p=0.5, min_p=1e-4)
     got = m3_sample(x, u, top_p=p, min_p=1e-4).cpu()
     assert torch.equal(got[::2], ref[::2].cpu()) and torch.equal(got[1::2], want[1::2])
+
+
+@pytest.mark.parametrize("V,rows", [(262144, 1), (262144, 5), (32768, 1), (32768, 400), (4100, 3)])
+@pytest.mark.parametrize("T_", [1.0, 0.7])
+def test_sample_top_p_border_beside_a_token_before_a_long_tail(V, rows, T_):
+    """top_p a little below and above the share of a prefix: 600 tokens of falling
+    weight before a tail of equal weights that are no power of two, whose fp32 sum
+    rounds one way.  u = 1 draws the last kept token, as the 64-bit definition
+    counts them."""
+    heads = 600
+    x = torch.full((V,), float(np.log(0.7) - np.log(V - heads) + np.log(heads)))
+    x[:heads] = -torch.arange(heads) * 1e-3
+    x = x * T_
+    w = O.kept_weights(x.numpy(), float(np.float32(T_)), 0, 1.0, 0.0)
+    cum = np.cumsum(w[:heads]) / w.sum()
+    ps, want = [], []
+    for j in (0, 1, 99, 300, 599):
+        for off in (-1e-4, -3e-5, -1e-5, -2e-6, -2e-7, 2e-7, 2e-6, 1e-5, 3e-5, 1e-4):
+            p = float(np.float32(cum[j] * (1 + off)))
+            kept = O.kept_weights(x.numpy(), float(np.float32(T_)), 0, p, 0.0)
+            ps.append(p)
+            want.append(int(np.nonzero(kept)[0][-1]))
+    logits = x.cuda()
+    for p, n in zip(ps, want):
+        got = m3_sample(logits.expand(rows, V), torch.ones(rows).cuda(), temperature=T_, top_p=p)
+        assert (got == n).all(), (p, n, got)
