@@ -15,12 +15,16 @@ MAX_VOCAB = 262144
 
 
 def _setting(name, v, lead, dtype, lo, hi):
-    """(array or None, scalar) of a setting given as one number or one per row."""
-    if torch.is_tensor(v) and v.dim():
+    """(array or None, scalar) of a setting given as one number or one per row; a
+    number on the GPU stays there, as one per row, and is not waited for."""
+    whole = torch.is_tensor(v) and not (v.dtype.is_floating_point or v.dtype is torch.bool)
+    if torch.is_tensor(v) and (v.dim() or (v.is_cuda and (whole or dtype is not torch.int32))):
+        if v.dim() == 0:
+            v = v.expand(lead)
         if v.shape != lead:
             raise ValueError(f"m3_sample: {name} is a number or one per row")
         if dtype is torch.int32 and v.dtype is not dtype:
-            if v.dtype.is_floating_point or v.dtype is torch.bool:
+            if not whole:
                 raise ValueError(f"m3_sample: {name} per row is a tensor of integers")
             v = v.to(torch.int64).clamp(0, 2 ** 31 - 1)
         return (v if v.dtype is dtype else v.detach().to(dtype)).contiguous(), 0
@@ -44,10 +48,11 @@ def m3_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     times their total.  Temperature 0 takes the largest logit, the lowest index
     among equals.  A row without candidates gives -1.
 
-    Each setting is a number or a tensor of one per row (float32; integers for
-    top_k).  Values in tensors are not checked: a temperature that is negative or
-    NaN counts as 0, top_k below 0 as 0, top_p that is NaN or below 0 as 0, min_p
-    above 1 or NaN as 1.  V <= 262144."""
+    Each setting is a number (rounded to float32), or a tensor of one per row or,
+    0-dim, of one for all (float32; integers for top_k).  Values in tensors on the
+    GPU are not checked: a temperature that is negative or NaN counts as 0, top_k
+    below 0 as 0, top_p that is NaN or below 0 as 0, min_p above 1 or NaN as 1.
+    V <= 262144."""
     if logits.dim() not in (1, 2) or logits.shape[-1] < 1:
         raise ValueError("m3_sample: logits are (V,) or (rows, V)")
     V, lead = logits.shape[-1], logits.shape[:-1]

@@ -82,3 +82,37 @@ def test_sample_top_p_border_beside_a_token_before_a_long_tail(V, rows, T_):
     for p, n in zip(ps, want):
         got = m3_sample(logits.expand(rows, V), torch.ones(rows).cuda(), temperature=T_, top_p=p)
         assert (got == n).all(), (p, n, got)
+
+
+@pytest.fixture
+def _no_waiting():
+    torch.cuda.set_sync_debug_mode("error")
+    yield
+    torch.cuda.set_sync_debug_mode("default")
+
+
+@pytest.mark.parametrize("shape", [(5, 900), (900,), (0, 900)])
+def test_sample_settings_of_one_number_on_the_gpu(shape, _no_waiting):
+    """0-dim tensors on the GPU: the draw of the same numbers, without a wait for
+    the GPU, and so in a captured graph, where a later value takes part."""
+    g = torch.Generator("cuda").manual_seed(9)
+    x = torch.randn(shape, device="cuda", generator=g) * 2
+    u = torch.rand(shape[:-1], device="cuda", generator=g)
+    new = lambda v, t: torch.full((), v, device="cuda", dtype=t)  # noqa: E731
+    kw = dict(temperature=new(0.75, torch.float64), top_k=new(30, torch.int64),
+              top_p=new(0.875, torch.float32), min_p=new(0.015625, torch.bfloat16))
+    ref = m3_sample(x, u, temperature=0.75, top_k=30, top_p=0.875, min_p=0.015625)
+    got = m3_sample(x, u, **kw)
+    assert got.shape == ref.shape == u.shape
+    torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(got, ref)
+    if x.numel() == 0:
+        return
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m3_sample(x, u, **kw)
+    graph.replay()
+    assert torch.equal(out, ref)
+    kw["top_k"].fill_(1)
+    graph.replay()
+    assert torch.equal(out, x.argmax(-1))
