@@ -564,7 +564,10 @@ typedef struct m3_sel_grads {
 } m3_sel_grads;
 
 /* Backward of m3_selective_fwd: g (B, L, D) the gradient of y, ckpt the
- * forward's.  The states get no gradient. */
+ * forward's.  The states get no gradient.  The batch is taken in slabs of rows
+ * whose partials of d_B and d_C (0.5, 2, 8, 16, 64 bytes per step and channel for
+ * up to 8, 16, 32, 64, 128 states) fill 2 GB, or in larger ones of the rows that
+ * one wave of CTAs walks. */
 M3_API size_t m3_selective_bwd_workspace_bytes(const m3_sel_desc* desc);
 M3_API int m3_selective_bwd(const m3_sel_desc* desc, const m3_sel_args* args, const void* g,
             const float* ckpt, const m3_sel_grads* grads, void* workspace,

@@ -68,8 +68,13 @@ int time_splits(int nch, long long ctas, long long want) {
   return (nch + cps - 1) / cps;
 }
 
+// The backward's partials of dB and dC: rows are taken in slabs of this many
+// bytes, or of the rows that one wave of CTAs walks where those need more.
+constexpr size_t kSelSlabBytes = (size_t)2 << 30;
+
 struct SelLayout {
   int splits, cps, nch, np, tiles, bgroups, workers;
+  int slab;                            // rows of the batch that the backward takes at a time
   size_t hin, hsum, dsum;              // the time split's buffers (backward: qin, qsum)
   size_t bc, a;                        // the backward's partials
   size_t total;
@@ -96,6 +101,13 @@ bool sel_layout(const m3_sel_desc* d, bool backward, SelLayout* l) {
   long long bg = wave / ((long long)l->tiles * l->splits);
   if (bg > d->batch) bg = d->batch;
   if (bg < 1) bg = 1;
+  const size_t row_bc = (size_t)l->tiles * d->seqlen * 2 * l->np * 4;
+  long long slab = (long long)(kSelSlabBytes / row_bc);
+  if (slab < bg) slab = bg;
+  if (slab > d->batch) slab = d->batch;
+  const long long slabs = (d->batch + slab - 1) / slab;
+  l->slab = (int)((d->batch + slabs - 1) / slabs);   // of equal size
+  if (bg > l->slab) bg = l->slab;
   l->bgroups = (int)bg;
   l->workers = l->bgroups * l->splits;
   const size_t run = round256((size_t)l->splits * d->batch * d->d_inner * l->np * 4);
@@ -106,7 +118,7 @@ bool sel_layout(const m3_sel_desc* d, bool backward, SelLayout* l) {
   l->bc = l->splits > 1 ? 2 * run + sums : 0;
   l->total = l->bc;
   if (backward) {
-    l->a = l->bc + round256((size_t)l->tiles * d->batch * d->seqlen * 2 * l->np * 4);
+    l->a = l->bc + round256(l->slab * row_bc);
     l->total = l->a + round256((size_t)l->workers * d->d_inner * (l->np + 2) * 4);
   }
   return true;
@@ -360,6 +372,7 @@ int m3_selective_bwd(const m3_sel_desc* desc, const m3_sel_args* args, const voi
   }
   p.workers = l.workers;
   p.bgroups = l.bgroups;
+  p.nb = l.slab;
   p.vec_g = desc->d_inner % (16 / e) == 0 && aligned(g, 16) && aligned(grads->d_u, 16) &&
             aligned(grads->d_dt, 16) && aligned(grads->d_z, 16);
   return status(launch_sel_bwd(p, static_cast<cudaStream_t>(stream)));

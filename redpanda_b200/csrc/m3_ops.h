@@ -122,7 +122,8 @@ struct SelBwdParams {
   void* du; void* ddt; void* dz;                         // (B, L, D)
   void* dB; void* dC;                                    // (B, L, N)
   float* dA; float* dD; float* dbias;                    // (D, N), (D,), (D,)
-  float* part_bc;                                        // (G, B*L, 2, NP)
+  int b0, nb;                                            // rows of a slab (launcher: the first)
+  float* part_bc;                                        // (G, nb*L, 2, NP)
   float* part_a;                                         // (workers, D, NP + 2)
   int workers;                                           // CTAs along the batch and the splits
   int bgroups;                                           // workers / splits

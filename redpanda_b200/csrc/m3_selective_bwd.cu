@@ -21,9 +21,11 @@
 //
 // Sums over channels (dB, dC): pairs of channels in a thread, transposed
 // shuffles over a warp's lane groups (Order below), warps joined through shared
-// memory in order, channel tiles as partials that a second launch adds in order.  Sums
-// over rows (dA, dD, dbias) stay in registers over a CTA's rows, then partials
-// too.  No atomics: results do not depend on scheduling.
+// memory in order, channel tiles as partials that a second launch adds in order.
+// Sums over rows (dA, dD, dbias) stay in registers over a CTA's rows, then partials
+// too.  No atomics: results do not depend on scheduling.  The channel tiles'
+// partials are 8 NP bytes per tile and step (NP the padded states), so a large
+// batch is taken in slabs of rows that share one buffer.
 //
 // Few rows: the steps are split over CTAs as in the forward, with the state's
 // gradient at each run's end from per-run summaries joined from the back.
@@ -204,7 +206,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
   }
 
   pdl_wait();   // every CTA: the join's results, and the end of what it waited for
-  for (size_t b = bg; b < (size_t)p.B; b += bp.bgroups) {
+  for (size_t b = (size_t)bp.b0 + bg; b < (size_t)bp.b0 + bp.nb; b += bp.bgroups) {
     const int n = sel_length(p.lengths, (int)b, p.L);
     const size_t rows = b * p.L;
     const RowPtrs<T> rp(bp, rows);
@@ -406,7 +408,7 @@ sel_bwd_kernel(const SelBwdParams bp) {
 #pragma unroll
           for (int w = 1; w < Sm::NW; ++w) v += sm.BC[sub & 1][s][w][x];
           if (t < n)
-            bp.part_bc[((size_t)blockIdx.x * p.B * p.L + rows + t) * 2 * G::NP + x] = v;
+            bp.part_bc[(((size_t)blockIdx.x * bp.nb + (b - bp.b0)) * p.L + t) * 2 * G::NP + x] = v;
         }
       }
       // the last group's barrier is behind every write of sm.R
@@ -438,7 +440,8 @@ sel_bwd_kernel(const SelBwdParams bp) {
       __syncthreads();   // sm.D and sm.R are written again
     }
   }
-  // partials over this CTA's rows: dA, then dD and dbias of each channel
+  // partials over this CTA's rows: dA, then dD and dbias of each channel; a later
+  // slab's rows are added to those of the slabs before
   constexpr int PW = G::NP + 2;
   pdl_launch_dependents();   // not before: waiting CTAs would take room
   float* part = bp.part_a + (size_t)blockIdx.y * p.D * PW;
@@ -450,6 +453,11 @@ sel_bwd_kernel(const SelBwdParams bp) {
       float4 v = quad_of(dA[k]);
       if (el) v = make_float4(v.y, v.x, v.w, v.z);
       if (pr) v = make_float4(v.z, v.w, v.x, v.y);
+      if (bp.b0) {
+        const float2 a = *reinterpret_cast<const float2*>(o);
+        const float2 c = *reinterpret_cast<const float2*>(o + 2);
+        v = make_float4(a.x + v.x, a.y + v.y, c.x + v.z, c.y + v.w);
+      }
       *reinterpret_cast<float2*>(o) = make_float2(v.x, v.y);
       *reinterpret_cast<float2*>(o + 2) = make_float2(v.z, v.w);
     }
@@ -468,7 +476,10 @@ sel_bwd_kernel(const SelBwdParams bp) {
     const int which = e / G::DT, x = e % G::DT;
     float v = 0.f;
     for (int i = 0; i < RPT; ++i) v += red[(i * 2 + which) * G::DT + x];
-    if (c0 + x < p.D) part[(size_t)(c0 + x) * PW + G::NP + which] = v;
+    if (c0 + x < p.D) {
+      float* o = part + (size_t)(c0 + x) * PW + G::NP + which;
+      *o = bp.b0 ? *o + v : v;
+    }
   }
 }
 
@@ -630,7 +641,7 @@ template <typename T>
 __global__ void __launch_bounds__(128) sel_reduce_bc_kernel(const SelBwdParams bp, int tiles,
                                                             int NP) {
   const SelParams& p = bp.f;
-  const long long rows = (long long)p.B * p.L;
+  const long long rows = (long long)bp.nb * p.L, row0 = (long long)bp.b0 * p.L;
   const int per = 2 * NP / 4;
   const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
   pdl_launch_dependents();
@@ -640,7 +651,7 @@ __global__ void __launch_bounds__(128) sel_reduce_bc_kernel(const SelBwdParams b
   const int x = (int)(i % per) * 4, which = x / NP, n0 = x % NP;
   if (n0 >= p.N) return;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (row % p.L < sel_length(p.lengths, (int)(row / p.L), p.L)) {
+  if (row % p.L < sel_length(p.lengths, bp.b0 + (int)(row / p.L), p.L)) {
     const float* src = bp.part_bc + row * 2 * NP + x;
 #pragma unroll 8
     for (int t = 0; t < tiles; ++t) {
@@ -648,7 +659,7 @@ __global__ void __launch_bounds__(128) sel_reduce_bc_kernel(const SelBwdParams b
       s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
   }
-  T* o = static_cast<T*>(which ? bp.dC : bp.dB) + row * p.N + n0;
+  T* o = static_cast<T*>(which ? bp.dC : bp.dB) + (row0 + row) * p.N + n0;
   const float v[4] = {s.x, s.y, s.z, s.w};
   if (p.N % 4 == 0) {
     Pack<T, 4> r;
@@ -681,7 +692,8 @@ __global__ void __launch_bounds__(128) sel_reduce_a_kernel(const SelBwdParams bp
 }
 
 template <typename T, int LN>
-cudaError_t bwd_typed(const SelBwdParams& p, cudaStream_t s) {
+cudaError_t bwd_typed(const SelBwdParams& p0, cudaStream_t s) {
+  SelBwdParams p = p0;
   using G = Sel<LN>;
   const unsigned tiles = (unsigned)((p.f.D + G::DT - 1) / G::DT);
   constexpr int smem = (int)sizeof(BwdSmem<T, LN>);
@@ -703,12 +715,17 @@ cudaError_t bwd_typed(const SelBwdParams& p, cudaStream_t s) {
                          dim3(128), 0, s, p, (int)G::NP);
     if (e != cudaSuccess) return e;
   }
-  e = launch_maybe_pdl(p.f.splits > 1, main, dim3(tiles, p.workers), dim3(G::NT), smem, s, p);
-  if (e != cudaSuccess) return e;
-  const long long quads = (long long)p.f.B * p.f.L * (2 * G::NP / 4);
-  e = launch_maybe_pdl(true, sel_reduce_bc_kernel<T>, dim3((unsigned)((quads + 127) / 128)),
-                       dim3(128), 0, s, p, (int)tiles, (int)G::NP);
-  if (e != cudaSuccess) return e;
+  // slab by slab of the batch: the pass, and the sum of its partials of dB and dC
+  for (p.b0 = 0; p.b0 < p.f.B; p.b0 += p0.nb) {
+    p.nb = p.f.B - p.b0 < p0.nb ? p.f.B - p.b0 : p0.nb;
+    e = launch_maybe_pdl(p.f.splits > 1 && p.b0 == 0, main, dim3(tiles, p.workers), dim3(G::NT),
+                         smem, s, p);
+    if (e != cudaSuccess) return e;
+    const long long quads = (long long)p.nb * p.f.L * (2 * G::NP / 4);
+    e = launch_maybe_pdl(true, sel_reduce_bc_kernel<T>, dim3((unsigned)((quads + 127) / 128)),
+                         dim3(128), 0, s, p, (int)tiles, (int)G::NP);
+    if (e != cudaSuccess) return e;
+  }
   const long long na = (long long)p.f.D * (G::NP + 2);
   return launch_maybe_pdl(true, sel_reduce_a_kernel, dim3((unsigned)((na + 127) / 128)), dim3(128),
                           0, s, p, (int)G::NP);
