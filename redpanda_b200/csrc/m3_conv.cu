@@ -20,7 +20,9 @@
 // over all runs of a thread; a CTA joins its 8 workers per channel in order and
 // writes one partial, and a second launch adds the partials in a fixed order.
 // 512 rows x 64 steps x 1536 channels, K = 4, bf16: 47 us forward (4.3 TB/s),
-// 84 us backward (3.6 TB/s); 60 and 186 us at first.
+// 84 us backward (3.6 TB/s); 60 and 186 us at first.  In fp32: 66 us forward (6.1
+// TB/s), 222 us backward (2.7 TB/s), whose filter of four taps does not fit the 128
+// registers of two CTAs per SM (424 bytes per thread in local memory).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

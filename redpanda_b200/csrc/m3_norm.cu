@@ -6,14 +6,17 @@
 //                  dw = sum over rows of g xh,  db = sum over rows of g
 //
 // Bound by memory: forward reads x and writes y, backward reads x and g and
-// writes dx.  So every row is read once and stays in registers between the
-// statistics and the output, 8 elements per thread (32 past 8192): few
-// registers, so many rows in flight.  Up to 256 elements (in the forward, which
-// holds less, up to 1024 at up to 32 per lane: no barriers, 74 us against 92 us
-// for 131072 x 768 bf16) a warp holds a row and a CTA four of them; longer rows
-// have a CTA of their own.  The variance is
-// taken from the centred values in registers (no cancellation of mean(x^2) -
-// mu^2).  The grid is persistent: weights stay in registers over a CTA's rows,
+// writes dx.  So every row is read once and stays on the SM between the
+// statistics and the output, 8 elements per thread in registers: few of them, so
+// many rows in flight.  Rows past 8192 take 32 elements per thread, more than the
+// registers of 512 or 1024 threads hold beside the next row: part of them lies in
+// local memory (4096 x 16384 fp32, RMS: 101 us forward, 272 us backward, 1.2 and 2.2
+// times its bytes; 4096 x 8192: 47 and 87 us).  Up to 256 elements (in the forward,
+// which holds less, up to 1024 at up to 32 per lane: no barriers, 74 us against 92
+// us for 131072 x 768 bf16) a warp holds a row and a CTA four of them; longer rows
+// have a CTA of their own.  The variance is taken from the centred values (no
+// cancellation of mean(x^2) - mu^2).  The grid is persistent: weights stay with a
+// thread over a CTA's rows,
 // the next row's loads are issued before the present row is reduced, and the
 // backward keeps the weight gradients of its columns in registers over all its
 // rows.  Each CTA writes one partial row of dw (and db); a second launch adds

@@ -16,7 +16,7 @@
 // here, about 16 packed FMA-pipe operations per two states, and no state but
 // the checkpoints moves through memory.  256 rows x 64 steps x 1536 channels,
 // N = 32, bf16: 1041 us (1714 us at first), with no unit above 60 % busy (issue
-// 56 %, shared memory 57 %, FMA pipe 45 %, MUFU 36 %) and eleven warps per SM,
+// 56 %, shared memory 59 %, FMA pipe 45 %, MUFU 37 %) and eleven warps per SM,
 // which the registers of four steps' gates and products leave room for.
 //
 // Sums over channels (dB, dC): pairs of channels in a thread, transposed
@@ -159,10 +159,14 @@ __device__ __forceinline__ void bwd_fetch(BwdSmem<T, LN>& sm, const SelBwdParams
   copies_commit();
 }
 
-// Registers per thread: three CTAs per SM pay for N in 17..32 (1081 us against
-// 1214 us with the two that 255 registers allow, 256 rows x 64 steps x 1536
-// channels, N = 32, bf16), not for N <= 16 (306 us against 329 us, 2 x 4001 x
-// 1536, N = 16, fp32).
+// Registers per thread: three CTAs of 128 threads per SM pay for N in 17..32 (1081
+// us against 1214 us with the two that 255 registers allow, 256 rows x 64 steps x
+// 1536 channels, N = 32, bf16), not for N <= 16: 672 us against 692 us with three at
+// N = 16, 470 us against 619 us at N = 8 (the same rows, bf16), and 306 us against
+// 329 us (2 x 4001 x 1536, N = 16, fp32).  Above 32 states a CTA has 256 threads, one
+// per SM: two are slower at N = 128 (64 rows, bf16: 2292 us against 2461 us; fp32:
+// 1933 us against 2132 us) and at N = 64 in fp32 (128 rows: 1253 us against 1391 us),
+// and faster at N = 64 in bf16 (1290 us against 1099 us), which the rule leaves out.
 template <int LN> constexpr int bwd_min_ctas() { return LN == 8 ? 3 : 1; }
 
 template <typename T, int LN>
@@ -618,7 +622,9 @@ __global__ void __launch_bounds__(128) sel_join_bwd_kernel(const SelBwdParams bp
   pdl_wait();
   const long long sd = (long long)p.B * p.D;
   float v = 0.f;
-  constexpr int U = 8;   // runs whose summaries are loaded ahead of the chain
+  // runs whose summaries are loaded ahead of the chain (32, as forward: 3 to 7 us of
+  // 180 to 480 us saved in bf16, between 6 us saved and 11 us lost in fp32)
+  constexpr int U = 8;
   for (int s0 = p.splits - 1; s0 > 0; s0 -= U) {
     float d[U], x[U];
 #pragma unroll
