@@ -26,7 +26,8 @@ def _forward(x2, ld, w, b, desc, out_dtype, stats):
     rows, d = x2.shape
     y = (torch.empty_like(x2) if out_dtype is x2.dtype and ld == d
          else torch.empty((rows, d), device=x2.device, dtype=out_dtype))
-    st = torch.empty((1 if desc.rms else 2, rows), device=x2.device) if stats else None
+    st = (torch.empty((1 if desc.rms else 2, rows), device=x2.device, dtype=torch.float32)
+          if stats else None)
     if rows:
         rstd = st.data_ptr() if stats else None
         mean = rstd + 4 * rows if stats and not desc.rms else None

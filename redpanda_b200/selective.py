@@ -230,7 +230,7 @@ def _scan_fwd(prepared, A, Dskip, dt_bias, state, lengths, softplus, want_state,
     B, L, D = u.shape
     N = A.shape[1]
     y = torch.empty_like(u, memory_format=torch.contiguous_format)
-    h = torch.empty((B, D, N), device=u.device) if want_state else None
+    h = torch.empty((B, D, N), device=u.device, dtype=torch.float32) if want_state else None
     if B == 0 or L == 0:
         if h is not None:
             h.copy_(state) if state is not None else h.zero_()
@@ -241,7 +241,7 @@ def _scan_fwd(prepared, A, Dskip, dt_bias, state, lengths, softplus, want_state,
     with H.on_device(dev):
         if want_ckpt:
             nck = lib.m3_selective_ckpt_floats(desc)
-            ckpt = torch.empty(nck, device=u.device) if nck else None
+            ckpt = torch.empty(nck, device=u.device, dtype=torch.float32) if nck else None
         nws = lib.m3_selective_fwd_workspace_bytes(desc)
     if nws:
         ws = torch.empty(nws, device=u.device, dtype=torch.uint8)
