@@ -513,7 +513,8 @@ class Mamba3Block(nn.Module):
         """Functional O(1) step (mamba.py:427-498): returns (out, (h, dBu_t))."""
         cfg = self.config
         if state is None:
-            h = torch.zeros(x_t.shape[0], cfg.d_inner, cfg.d_state, device=x_t.device)
+            h = torch.zeros(x_t.shape[0], cfg.d_inner, cfg.d_state, device=x_t.device,
+                            dtype=torch.float32)
             state = (h, torch.zeros_like(h))
         else:
             state = tuple(s.detach().to(torch.float32).clone(

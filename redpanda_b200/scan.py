@@ -89,15 +89,14 @@ def _require_cuda(*ts):
 
 def pad_params(A_real, A_imag, track, n_rot, n_state, d_inner, device):
     """(D, N) fp32 parameter tensors in the layout of triton_scan.py:325-335."""
+    def none():
+        return torch.zeros(d_inner, n_state, device=device, dtype=torch.float32)
     if A_real is not None:
         Ar_p = F.pad(A_real, (0, n_state - A_real.shape[-1]))
-        Ai_p = (F.pad(A_imag, (0, n_state - A_imag.shape[-1]))
-                if A_imag is not None else torch.zeros(d_inner, n_state, device=device))
+        Ai_p = F.pad(A_imag, (0, n_state - A_imag.shape[-1])) if A_imag is not None else none()
     else:
-        Ar_p = torch.zeros(d_inner, n_state, device=device)
-        Ai_p = torch.zeros(d_inner, n_state, device=device)
-    Tk_p = (F.pad(track, (n_rot, 0))
-            if track is not None else torch.zeros(d_inner, n_state, device=device))
+        Ar_p, Ai_p = none(), none()
+    Tk_p = F.pad(track, (n_rot, 0)) if track is not None else none()
     return Ar_p, Ai_p, Tk_p
 
 
@@ -257,7 +256,7 @@ class _FusedScanFn(torch.autograd.Function):
         desc = ScanDesc(B, L, D, N, int(n_rot), M3_BF16, M3_BF16, int(direction))
         y = torch.empty(B, L, D, device=dev, dtype=y_dtype)
         nck = lib.m3_scan_ckpt_floats(desc) if want_ckpt else 0
-        ckpt = torch.empty(nck, device=dev) if nck else None
+        ckpt = torch.empty(nck, device=dev, dtype=torch.float32) if nck else None
         with torch.cuda.device(dev):
             rc = lib.m3_scan_fwd_fused(desc, int(P), dt.data_ptr(), x_dbl.data_ptr(),
                                        x_dbl.shape[-1], int(off_b), int(off_c),
