@@ -76,6 +76,29 @@ def once_differentiable(body):
     return backward
 
 
+# the saved-tensor hooks in force, None without any
+_hooks = getattr(torch._C._autograd, "_top_saved_tensors_default_hooks", lambda ignore: True)
+
+
+def save(ctx, *ts):
+    """Save tensors for the backward pass, and their types and shapes where hooks
+    may give back others (``ctx.hooked``, else None)."""
+    ctx.save_for_backward(*ts)
+    ctx.hooked = None if _hooks(True) is None else [
+        None if t is None else (t.dtype, t.shape) for t in ts]
+
+
+def check_saved(ctx, ts, g):
+    """Refuse saved tensors of another type, shape or device than forward; their
+    layout may be another, and the caller looks at it again.  ``g``: the incoming
+    gradient."""
+    for t, like in zip(ts, ctx.hooked or ()):
+        if t is not None and (t.dtype, t.shape) != like:
+            raise RuntimeError("m3 ops: saved-tensor hooks have to give back the element type and "
+                               "shape that they were given")
+    device_index(g, *ts)
+
+
 def f32(t):
     """A parameter as contiguous float32 (itself when it is)."""
     if t is None or (t.dtype is torch.float32 and t.is_contiguous()):

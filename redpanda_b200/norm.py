@@ -46,7 +46,7 @@ class _NormFn(torch.autograd.Function):
         w = H.f32(weight)
         desc = NormDesc(x2.shape[0], d, H.code(x2.dtype), H.code(out_dtype), rms, eps)
         y, st = _forward(x2, ld, w, H.f32(bias), desc, out_dtype, True)
-        ctx.save_for_backward(x2, w, st)
+        H.save(ctx, x2, w, st)
         ctx.cfg = (ld, desc, out_dtype, x.shape, weight.dtype,
                    None if bias is None else bias.dtype)
         return y if x.dim() == 2 else y.view(x.shape)
@@ -56,6 +56,9 @@ class _NormFn(torch.autograd.Function):
     def backward(ctx, g):
         x2, w, st = ctx.saved_tensors
         ld, desc, out_dtype, shape, wt, bt = ctx.cfg
+        if ctx.hooked is not None or x2.stride(0) != ld:
+            H.check_saved(ctx, (x2, w, st), g)
+            (x2, ld), w, st = H.rows(x2), w.contiguous(), st.contiguous()
         if g.dtype is not out_dtype or not g.is_contiguous():
             g = g.to(out_dtype).contiguous()
         dx = torch.empty_like(x2, memory_format=torch.contiguous_format)

@@ -63,6 +63,10 @@ def _typed(t, dtype):
     return t if t is None or t.dtype is dtype else t.to(dtype)
 
 
+def _contiguous(ts):
+    return [None if t is None else t.contiguous() for t in ts]
+
+
 # ---------------------------------------------------------------- convolution
 
 def _check_filter(name, D, weight, bias):
@@ -113,7 +117,7 @@ class _ConvFn(torch.autograd.Function):
         w, b = H.f32(weight), H.f32(bias)
         st = None if state is None else state.contiguous()
         y, out = _conv_fwd(x2, ld, w, b, st, lengths, silu, want_state)
-        ctx.save_for_backward(x2, w, b, st, lengths)
+        H.save(ctx, x2, w, b, st, lengths)
         ctx.cfg = (ld, silu, weight.dtype, None if bias is None else bias.dtype)
         ctx.set_materialize_grads(False)
         if out is not None:
@@ -125,8 +129,12 @@ class _ConvFn(torch.autograd.Function):
     def backward(ctx, g, _):
         if g is None:
             return (None,) * 7
-        x, w, b, state, lengths = ctx.saved_tensors
+        x, w, b, state, lengths = ts = ctx.saved_tensors
         ld, silu, wt, bt = ctx.cfg
+        if ctx.hooked is not None or x.stride(1) != ld:
+            H.check_saved(ctx, ts, g)
+            x, ld = H.seq_rows(x)
+            w, b, state, lengths = _contiguous(ts[1:])
         B, L, D = x.shape
         K = w.shape[1]
         if g.dtype is not x.dtype or not g.is_contiguous():
@@ -265,7 +273,7 @@ class _SelectiveScanFn(torch.autograd.Function):
         prepared = _prepare(H.seq_rows, u, dt, z, Bm, Cm)
         a32, d32, b32, st = H.f32(A), H.f32(Dskip), H.f32(dt_bias), H.f32(state)
         y, h, ckpt = _scan_fwd(prepared, a32, d32, b32, st, lengths, softplus, want_state, True)
-        ctx.save_for_backward(*(t for t, _ in prepared), a32, d32, b32, st, lengths, ckpt)
+        H.save(ctx, *(t for t, _ in prepared), a32, d32, b32, st, lengths, ckpt)
         ctx.cfg = ([ld for _, ld in prepared], softplus,
                    [None if t is None else t.dtype for t in (u, dt, A, Bm, Cm, Dskip, z, dt_bias)])
         ctx.set_materialize_grads(False)
@@ -278,8 +286,14 @@ class _SelectiveScanFn(torch.autograd.Function):
     def backward(ctx, g, _):
         if g is None:
             return (None,) * 12
-        u, dt, z, Bm, Cm, A, Dskip, dt_bias, state, lengths, ckpt = ctx.saved_tensors
+        ts = ctx.saved_tensors
         lds, softplus, types = ctx.cfg
+        if ctx.hooked is not None or any(t is not None and t.stride(1) != ld
+                                         for t, ld in zip(ts, lds)):
+            H.check_saved(ctx, ts, g)
+            seqs, lds = zip(*((None, 0) if t is None else H.seq_rows(t) for t in ts[:5]))
+            ts = (*seqs, *_contiguous(ts[5:]))
+        u, dt, z, Bm, Cm, A, Dskip, dt_bias, state, lengths, ckpt = ts
         B, L, D = u.shape
         N = A.shape[1]
         dev, ty = u.device, u.dtype
