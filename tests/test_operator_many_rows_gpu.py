@@ -1,4 +1,4 @@
-"""Batches that the backward passes walk in several rounds: a CTA (or warp) takes
+"""Batches that the backward passes walk in several turns: a CTA (or warp) takes
 more than two rows or runs, with a remainder, so that what it carries from one to
 the next -- fetched inputs, sums of the parameters' gradients, the gradient of the
 state -- is compared with the definition in 64 bits."""
@@ -131,7 +131,7 @@ def test_scan_over_many_rows(B, L, D, Ns, opt, dtype):
 
 
 def test_scan_over_many_rows_split_along_time():
-    """Long rows, split along time, and more of them than one round holds."""
+    """Long rows, split along time, and more of them than one turn holds."""
     a, gr = _scan_inputs(130, 1500, 20, 8, torch.float32, ragged=True, state=True, seed=7)
     a["lengths"][::3], a["lengths"][1::5] = 1500, 0
     _check_scan(a, gr, _run_scan(a, gr))
