@@ -56,3 +56,39 @@ def test_backward_in_slabs_equals_the_parts(dtype):
         else:
             ref = one[k].double() + two[k].double()
             assert (ref > 0).all() and ((v.double() - ref).abs() <= tol * ref).all(), k
+
+
+def test_backward_in_slabs_of_rows_that_are_split_along_time():
+    """Two rows so long that each is a slab, their steps split over CTAs, against
+    either row alone (another split).  All terms are positive (the step sizes'
+    gradient is left out) and gates below e^-0.5 forget within 60 steps to 1e-13,
+    so each side is off by at most (20 * 60 + N + 64) e beside the sums over D
+    channels (dB, dC) and B L steps (the parameters)."""
+    B, L, D, N = 2, 44000, 1536, 64
+    assert 48 * L * 2 * 64 * 4 > 1 << 30
+    assert _workspace(B, L, D, N, 1) < 3 << 30
+    g = torch.Generator("cuda").manual_seed(5)
+    pos = lambda *s: torch.rand(*s, device="cuda", generator=g)  # noqa: E731
+    bf = torch.bfloat16
+    a = dict(u=pos(B, L, D).to(bf), A=-1 - pos(D, N), Bm=pos(B, L, N).to(bf),
+             Cm=pos(B, L, N).to(bf), D=pos(D))
+    dt, gr = (0.5 + pos(B, L, D)).to(bf), pos(B, L, D).to(bf)
+    n = torch.tensor([L, L - 1234], device="cuda", dtype=torch.int32)
+
+    def run(lo, hi):
+        x = {k: (v[lo:hi] if v.dim() == 3 else v).detach().requires_grad_(True)
+             for k, v in a.items()}
+        y = S.m3_selective_scan(dt=dt[lo:hi], **x, softplus=False, lengths=n[lo:hi])
+        return dict(zip(x, torch.autograd.grad(y, list(x.values()), gr[lo:hi])))
+    whole, rows = run(0, B), [run(i, i + 1) for i in range(B)]
+    k, half = 20 * 60 + N + 64, 2.0 ** -8          # half a step of bf16, on each side
+    for name, v in whole.items():
+        if v.dim() == 3:
+            tol = 2 * ((k + D) * E + half)
+            for i in range(B):
+                p, q = v[i].float(), rows[i][name][0].float()
+                assert ((p - q).abs() <= tol * q).all(), name
+                assert (q[:n[i]] > 0).all() and not q[n[i]:].any(), name
+        else:
+            ref = rows[0][name].double() + rows[1][name].double()
+            assert ((v.double() - ref).abs() <= 2 * (k + B * L) * E * ref).all(), name
