@@ -578,6 +578,48 @@ M3_API int m3_selective_bwd(const m3_sel_desc* desc, const m3_sel_args* args, co
 M3_API int m3_selective_step(const m3_sel_desc* desc, const m3_sel_args* args, float* h, void* y,
             void* stream);
 
+typedef struct m3_gated_desc {
+  int32_t batch;      /* B >= 1 */
+  int32_t seqlen;     /* L >= 1; 1 for the step */
+  int32_t d_inner;    /* D >= 1 */
+  int32_t dtype;      /* element type of x, rg, ig, y and their gradients */
+  float c;            /* > 0, finite */
+} m3_gated_desc;
+
+typedef struct m3_gated_args {
+  const void* x;  int64_t ld_x;     /* (B*L, ld_x), D columns: the input */
+  const void* rg; int64_t ld_r;     /* (B*L, ld_r): recurrence gate before its sigmoid */
+  const void* ig; int64_t ld_i;     /* (B*L, ld_i): input gate before its sigmoid */
+  const float* decay;               /* (D,) */
+  const float* state;               /* (B, D) the state before the first step, or NULL: zero */
+  const int32_t* lengths;           /* (B,) or NULL: all L; clamped to [0, L] */
+} m3_gated_args;
+
+/* Gated linear recurrence, per row b and channel d:
+ *   a_t = exp(-c softplus(decay) sigmoid(rg_t)),
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(ig_t) x_t,   y_t = h_t
+ *   y       (B, L, D); zero at steps at or past a row's length, whose inputs are
+ *           not read
+ *   h_last  (B, D) float32 or NULL: the state at each row's length (not state)
+ *   ckpt    m3_gated_ckpt_floats() floats for the backward (the state in front of
+ *           every 8 steps), 8-byte aligned, or NULL */
+M3_API size_t m3_gated_ckpt_floats(const m3_gated_desc* desc);
+M3_API int m3_gated_fwd(const m3_gated_desc* desc, const m3_gated_args* args, void* y,
+            float* h_last, float* ckpt, void* stream);
+
+/* Backward: g (B, L, D) the gradient of y, ckpt the forward's; d_x, d_rg, d_ig
+ * (B, L, D), zero at steps at or past a length; d_decay (D,) float32, summed in a
+ * fixed order.  The states get no gradient. */
+M3_API size_t m3_gated_bwd_workspace_bytes(const m3_gated_desc* desc);
+M3_API int m3_gated_bwd(const m3_gated_desc* desc, const m3_gated_args* args, const void* g,
+            const float* ckpt, void* d_x, void* d_rg, void* d_ig, float* d_decay,
+            void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token per row (seqlen 1), in place on h (B, D) float32; y (B, D).
+ * args->state and args->lengths must be NULL. */
+M3_API int m3_gated_step(const m3_gated_desc* desc, const m3_gated_args* args, float* h, void* y,
+            void* stream);
+
 typedef struct m3_sample_desc {
   int32_t rows;         /* >= 1 */
   int32_t vocab;        /* V, 1..262144 */

@@ -66,6 +66,19 @@ class SelGrads(ctypes.Structure):
                                   "d_dt_bias")]
 
 
+class GatedDesc(ctypes.Structure):
+    """``m3_gated_desc``."""
+    _fields_ = [("batch", _I), ("seqlen", _I), ("d_inner", _I), ("dtype", _I),
+                ("c", ctypes.c_float)]
+
+
+class GatedArgs(ctypes.Structure):
+    """``m3_gated_args``."""
+    _fields_ = [(n, t) for a, ld in (("x", "ld_x"), ("rg", "ld_r"), ("ig", "ld_i"))
+                for n, t in ((a, _P), (ld, ctypes.c_int64))] + [
+        (n, _P) for n in ("decay", "state", "lengths")]
+
+
 class SampleDesc(ctypes.Structure):
     """``m3_sample_desc``."""
     _fields_ = [("rows", _I), ("vocab", _I), ("dtype", _I), ("temperature", ctypes.c_float),
@@ -78,6 +91,8 @@ _N = ctypes.POINTER(NormDesc)
 _C = ctypes.POINTER(ConvDesc)
 _E = ctypes.POINTER(SelDesc)
 _A = ctypes.POINTER(SelArgs)
+_G = ctypes.POINTER(GatedDesc)
+_GA = ctypes.POINTER(GatedArgs)
 
 SIGNATURES = {
     "m3_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -143,6 +158,11 @@ SIGNATURES = {
     "m3_selective_bwd_workspace_bytes": (_Z, [_E]),
     "m3_selective_bwd": (ctypes.c_int, [_E, _A, _P, _P, ctypes.POINTER(SelGrads), _P, _Z, _P]),
     "m3_selective_step": (ctypes.c_int, [_E, _A, _P, _P, _P]),
+    "m3_gated_ckpt_floats": (_Z, [_G]),
+    "m3_gated_fwd": (ctypes.c_int, [_G, _GA, _P, _P, _P, _P]),
+    "m3_gated_bwd_workspace_bytes": (_Z, [_G]),
+    "m3_gated_bwd": (ctypes.c_int, [_G, _GA, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "m3_gated_step": (ctypes.c_int, [_G, _GA, _P, _P, _P]),
     "m3_sample": (ctypes.c_int, [ctypes.POINTER(SampleDesc), _P, ctypes.c_int64, _P, _P, _P, _P,
                                  _P, _P, _P]),
 }

@@ -57,6 +57,36 @@ int check_sel(const m3_sel_desc* d) {
   return M3_OK;
 }
 
+int check_gated(const m3_gated_desc* d) {
+  if (!d) return M3_ERR_NULL;
+  if (d->batch < 1 || d->seqlen < 1 || d->d_inner < 1 || !(d->c > 0.f) || d->c > 3e38f)
+    return M3_ERR_SHAPE;
+  if (!dtype_ok(d->dtype)) return M3_ERR_DTYPE;
+  if (too_large(d->batch, d->seqlen, d->d_inner)) return M3_ERR_SHAPE;
+  return M3_OK;
+}
+
+// Fills what the gated recurrence's forward and backward share; returns a status.
+int fill_gated(const m3_gated_desc* d, const m3_gated_args* a, bool backward, GatedParams* p) {
+  const int e = dsize(d->dtype);
+  if (!a || !a->x || !a->rg || !a->ig || !a->decay) return M3_ERR_NULL;
+  if (a->ld_x < d->d_inner || a->ld_r < d->d_inner || a->ld_i < d->d_inner) return M3_ERR_SHAPE;
+  if (!aligned(a->x, e) || !aligned(a->rg, e) || !aligned(a->ig, e) || !aligned(a->decay, 4) ||
+      !aligned(a->state, 4) || !aligned(a->lengths, 4))
+    return M3_ERR_ALIGN;
+  const int rc = check_device();
+  if (rc != M3_OK) return rc;
+  p->x = a->x; p->rg = a->rg; p->ig = a->ig;
+  p->ld_x = a->ld_x; p->ld_r = a->ld_r; p->ld_i = a->ld_i;
+  p->decay = a->decay; p->c = d->c; p->h0 = a->state; p->lengths = a->lengths;
+  p->B = d->batch; p->L = d->seqlen; p->D = d->d_inner; p->dtype = d->dtype;
+  const int v = 16 / e;
+  p->vec = d->d_inner % v == 0 && a->ld_x % v == 0 && a->ld_r % v == 0 && a->ld_i % v == 0 &&
+           aligned(a->x, 16) && aligned(a->rg, 16) && aligned(a->ig, 16);
+  gated_plan(p->B, p->L, p->D, p->dtype, backward, device_sms(), &p->warps, &p->splits, &p->rows);
+  return M3_OK;
+}
+
 // Few rows are split along time into runs, of four chunks at least.  The
 // summaries of the runs cost about three quarters of another pass, so fewer
 // than three runs do not pay.
@@ -399,6 +429,87 @@ int m3_selective_step(const m3_sel_desc* desc, const m3_sel_args* args, float* h
   p.A = f.A; p.dskip = f.dskip; p.dt_bias = f.dt_bias; p.y = y;
   p.B = f.B; p.D = f.D; p.N = f.N; p.dtype = f.dtype; p.softplus = f.softplus;
   return status(launch_sel_step(p, static_cast<cudaStream_t>(stream)));
+}
+
+size_t m3_gated_ckpt_floats(const m3_gated_desc* desc) {
+  if (check_gated(desc) != M3_OK) return 0;
+  return (size_t)desc->batch * gated_segments(desc->seqlen) * desc->d_inner;
+}
+
+int m3_gated_fwd(const m3_gated_desc* desc, const m3_gated_args* args, void* y, float* h_last,
+                 float* ckpt, void* stream) {
+  int rc = check_gated(desc);
+  if (rc != M3_OK) return rc;
+  if (!args || !y) return M3_ERR_NULL;
+  if (!aligned(y, dsize(desc->dtype)) || !aligned(h_last, 4) || !aligned(ckpt, 8))
+    return M3_ERR_ALIGN;
+  if ((h_last && h_last == args->state) || y == args->x || y == args->rg || y == args->ig)
+    return M3_ERR_ALIAS;
+  GatedParams p;
+  memset(&p, 0, sizeof(p));
+  if ((rc = fill_gated(desc, args, false, &p)) != M3_OK) return rc;
+  p.vec = p.vec && aligned(y, 16);
+  p.y = y; p.h_last = h_last; p.ckpt = ckpt;
+  return status(launch_gated_fwd(p, static_cast<cudaStream_t>(stream)));
+}
+
+size_t m3_gated_bwd_workspace_bytes(const m3_gated_desc* desc) {
+  const int sms = device_sms();
+  if (check_gated(desc) != M3_OK || sms <= 0) return 0;
+  int warps, splits, rows;
+  gated_plan(desc->batch, desc->seqlen, desc->d_inner, desc->dtype, true, sms, &warps, &splits,
+             &rows);
+  return (size_t)rows * splits * desc->d_inner * 4;
+}
+
+int m3_gated_bwd(const m3_gated_desc* desc, const m3_gated_args* args, const void* g,
+                 const float* ckpt, void* d_x, void* d_rg, void* d_ig, float* d_decay,
+                 void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_gated(desc);
+  if (rc != M3_OK) return rc;
+  if (!args || !g || !ckpt || !d_x || !d_rg || !d_ig || !d_decay) return M3_ERR_NULL;
+  const int e = dsize(desc->dtype);
+  if (!aligned(g, e) || !aligned(d_x, e) || !aligned(d_rg, e) || !aligned(d_ig, e) ||
+      !aligned(ckpt, 8) || !aligned(d_decay, 4) || !aligned(workspace, 4))
+    return M3_ERR_ALIGN;
+  for (void* o : {d_x, d_rg, d_ig})
+    if (o == args->x || o == args->rg || o == args->ig || o == g) return M3_ERR_ALIAS;
+  GatedBwdParams q;
+  memset(&q, 0, sizeof(q));
+  if ((rc = fill_gated(desc, args, true, &q.f)) != M3_OK) return rc;
+  if (!workspace || workspace_bytes < m3_gated_bwd_workspace_bytes(desc)) return M3_ERR_WORKSPACE;
+  q.f.vec = q.f.vec && aligned(g, 16) && aligned(d_x, 16) && aligned(d_rg, 16) &&
+            aligned(d_ig, 16);
+  q.f.ckpt = const_cast<float*>(ckpt);
+  q.g = g; q.dx = d_x; q.drg = d_rg; q.dig = d_ig; q.ddecay = d_decay;
+  q.part = static_cast<float*>(workspace);
+  return status(launch_gated_bwd(q, static_cast<cudaStream_t>(stream)));
+}
+
+int m3_gated_step(const m3_gated_desc* desc, const m3_gated_args* args, float* h, void* y,
+                  void* stream) {
+  int rc = check_gated(desc);
+  if (rc != M3_OK) return rc;
+  if (!args || !h || !y || !args->x || !args->rg || !args->ig || !args->decay) return M3_ERR_NULL;
+  if (desc->seqlen != 1 || args->ld_x < desc->d_inner || args->ld_r < desc->d_inner ||
+      args->ld_i < desc->d_inner)
+    return M3_ERR_SHAPE;
+  if (args->state || args->lengths) return M3_ERR_UNSUPPORTED;
+  const int e = dsize(desc->dtype);
+  if (!aligned(args->x, e) || !aligned(args->rg, e) || !aligned(args->ig, e) || !aligned(y, e) ||
+      !aligned(args->decay, 4) || !aligned(h, 4))
+    return M3_ERR_ALIGN;
+  if (y == h || y == args->x || y == args->rg || y == args->ig || h == args->x || h == args->rg ||
+      h == args->ig)
+    return M3_ERR_ALIAS;
+  if ((rc = check_device()) != M3_OK) return rc;
+  GatedStepParams p;
+  memset(&p, 0, sizeof(p));
+  p.h = h; p.x = args->x; p.rg = args->rg; p.ig = args->ig;
+  p.ld_x = args->ld_x; p.ld_r = args->ld_r; p.ld_i = args->ld_i;
+  p.decay = args->decay; p.c = desc->c; p.y = y;
+  p.B = desc->batch; p.D = desc->d_inner; p.dtype = desc->dtype; p.sms = device_sms();
+  return status(launch_gated_step(p, static_cast<cudaStream_t>(stream)));
 }
 
 int m3_sample(const m3_sample_desc* desc, const void* logits, int64_t ld, const float* uniform,

@@ -1,0 +1,186 @@
+// Gated linear recurrence, backward.  Formulas of the forward: m3_gated.cuh.
+//
+//   q_t   = g_t + a_{t+1} q_{t+1}                        (gradient of h_t)
+//   dx_t  = q m i,   dig_t = q m x i (1 - i)
+//   e_t   = q l (a h_{t-1} - (a^2 / m) i x)              (l times the gradient of l)
+//   drg_t = e (1 - r),   ddecay = sigmoid(decay) / softplus(decay) sum e
+// l / m is finite where l goes to 0 (a gate far closed), the gradient of l itself
+// is not, so only the product is formed.
+//
+// As in the forward a warp holds 8 steps, the CTA's warps (the cluster's CTAs)
+// consecutive runs, and the passes go from the sequence's end to its start.  The
+// forward's checkpoint in front of every run gives h_{t-1} in fp32 (y in bf16
+// would put its rounding on e); a thread computes forward what multiplies q in
+// each gradient, then joins the runs behind its own and walks back with q.
+// ddecay stays in registers over all steps of a thread; each CTA writes one partial
+// per channel, and a second launch adds them in a fixed order.
+#include "m3_gated.cuh"
+
+#include "m3_api_util.h"
+#include "m3_ops.h"
+#include "m3_pdl.cuh"
+
+namespace m3 {
+namespace {
+
+__device__ __forceinline__ int row_length(const int* lengths, int b, int L) {
+  if (lengths == nullptr) return L;
+  const int n = lengths[b];
+  return n < 0 ? 0 : n > L ? L : n;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256, 2) gated_bwd_kernel(const GatedBwdParams q) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ Joint joint;
+  constexpr int TS = kGatedSteps;
+  using St = Stage<T, 4>;
+  const GatedParams& p = q.f;
+  const int lane = threadIdx.x, w = threadIdx.y, W = blockDim.y, S = p.splits;
+  const int rank = blockIdx.x % S, c0 = blockIdx.x / S * kGatedTile, c = c0 + 2 * lane;
+  const int left = p.D - c, D = p.D, L = p.L, span = S * W * TS;
+  const int at0 = (rank * W + w) * TS;
+  const bool vec = p.vec != 0;
+  char* buf = smem + w * St::kBytes;
+  St st{{static_cast<const T*>(p.x), static_cast<const T*>(p.rg), static_cast<const T*>(p.ig),
+         static_cast<const T*>(q.g)},
+        {p.ld_x, p.ld_r, p.ld_i, D}};
+  const float2 dec = load_pair(p.decay + c, left);
+  const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
+  float2 sum = f2(0.f);
+  int flip = 0;
+  if (S > 1) cluster_sync();                         // every CTA runs before its memory is written
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const int n = row_length(p.lengths, b, L);
+    const long long base = (long long)b * L;
+    T* dx = static_cast<T*>(q.dx) + (size_t)base * D + c;
+    T* dr = static_cast<T*>(q.drg) + (size_t)base * D + c;
+    T* di = static_cast<T*>(q.dig) + (size_t)base * D + c;
+    const int passes = (n + span - 1) / span;
+    // steps of passes that are wholly past the length
+    for (int t0 = passes * span + at0; t0 < L; t0 += span)
+      for (int i = 0; i < TS && t0 + i < L; ++i) {
+        store_pair(dx + (size_t)(t0 + i) * D, f2(0.f), left, vec);
+        store_pair(dr + (size_t)(t0 + i) * D, f2(0.f), left, vec);
+        store_pair(di + (size_t)(t0 + i) * D, f2(0.f), left, vec);
+      }
+    float2 carry = f2(0.f);                          // a_{t+1} q_{t+1}
+    int t0 = (passes - 1) * span + at0;
+    if (passes > 0) st.issue(buf, base, t0, n, c0, D, vec);
+    for (int k0 = passes; k0 > 0; --k0, t0 -= span) {
+      float2 a[TS], X[TS], I[TS], A[TS], R[TS], g[TS];
+      float2 h = f2(0.f);
+      if (t0 < n) h = load_pair(p.ckpt + ((size_t)b * ((L + TS - 1) / TS) + t0 / TS) * D + c, left);
+      St::wait();
+#pragma unroll
+      for (int i = 0; i < TS; ++i) {
+        const float2 x = St::get(buf, 0, i), r = sigmoid2(St::get(buf, 1, i)),
+                     u = sigmoid2(St::get(buf, 2, i));
+        g[i] = St::get(buf, 3, i);
+        const float2 l = mul2(k, r);
+        float2 m, inv;
+        decay2(l, a[i], m);
+        root2(m, m, inv);
+        const float2 ah = mul2(a[i], h), ux = mul2(u, x);
+        X[i] = mul2(m, u);
+        h = fma2(m, ux, ah);
+        const float2 am = mul2(mul2(a[i], a[i]), inv);
+        A[i] = mul2(l, fma2(mul2(am, f2(-1.f)), ux, ah));
+        R[i] = fma2(r, f2(-1.f), f2(1.f));
+        I[i] = mul2(mul2(X[i], x), fma2(u, f2(-1.f), f2(1.f)));
+        if (t0 + i >= n) {                           // the state stays, nothing has a gradient
+          a[i] = f2(1.f);
+          g[i] = X[i] = I[i] = A[i] = f2(0.f);
+        }
+      }
+      Run run{f2(1.f), f2(0.f)};                     // v = a (g + v), from the last step
+#pragma unroll
+      for (int i = TS - 1; i >= 0; --i) {
+        run.V = mul2(a[i], add2(g[i], run.V));
+        run.P = mul2(a[i], run.P);
+      }
+      __syncwarp();
+      if (k0 > 1) st.issue(buf, base, t0 - span, n, c0, D, vec);
+      float2 v = join(joint, flip, run, W - 1 - w, W, S - 1 - rank, S, carry);
+      flip ^= 1;
+      float2 part = f2(0.f);
+#pragma unroll
+      for (int i = TS - 1; i >= 0; --i) {
+        const float2 qt = add2(g[i], v), e = mul2(qt, A[i]);
+        v = mul2(a[i], qt);
+        part = add2(part, e);
+        if (t0 + i < L) {
+          store_pair(dx + (size_t)(t0 + i) * D, mul2(qt, X[i]), left, vec);
+          store_pair(dr + (size_t)(t0 + i) * D, mul2(e, R[i]), left, vec);
+          store_pair(di + (size_t)(t0 + i) * D, mul2(qt, I[i]), left, vec);
+        }
+      }
+      sum = add2(sum, part);
+    }
+  }
+  pdl_launch_dependents();
+  // the CTA's partial: warps in order
+  __syncthreads();
+  float2* s = reinterpret_cast<float2*>(&joint);
+  s[w * 32 + lane] = sum;
+  __syncthreads();
+  if (w == 0) {
+    float2 v = s[lane];
+    for (int i = 1; i < W; ++i) v = add2(v, s[i * 32 + lane]);
+    store_pair(q.part + ((size_t)blockIdx.y * S + rank) * D + c, v, left, false);
+  }
+}
+
+// ddecay[c] = sigmoid(decay) / softplus(decay) * the sum of the CTAs' partials: 32
+// columns per CTA, 32 strided sums each, joined in order.
+__global__ void __launch_bounds__(1024) gated_reduce_kernel(const float* part, int n, int D,
+                                                            const float* decay, float* out) {
+  __shared__ float s[32][33];
+  const int cx = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + cx;
+  float a = 0.f;
+  pdl_wait();
+  if (c < D)
+    for (int i = k; i < n; i += 32) a += part[(size_t)i * D + c];
+  s[k][cx] = a;
+  __syncthreads();
+  float v = s[cx][k];
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  const int cc = blockIdx.x * 32 + k;
+  if (cx == 0 && cc < D) {
+    const float d = decay[cc], e = expf(-fabsf(d));
+    // both go as e^d far below 0, where their ratio is 1
+    out[cc] = d < -15.f ? v : v * ((d < 0.f ? e : 1.f) / (1.f + e)) / softplus_f(d);
+  }
+}
+
+template <typename T>
+cudaError_t bwd_impl(const GatedBwdParams& q, cudaStream_t s) {
+  const GatedParams& p = q.f;
+  const cudaError_t e = allow_smem<gated_bwd_kernel<T>>(8 * Stage<T, 4>::kBytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.D + kGatedTile - 1) / kGatedTile * p.splits), p.rows);
+  cfg.blockDim = dim3(32, p.warps);
+  cfg.dynamicSmemBytes = p.warps * Stage<T, 4>::kBytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.splits > 1 ? 1 : 0;
+  const cudaError_t r = cudaLaunchKernelEx(&cfg, gated_bwd_kernel<T>, q);
+  if (r != cudaSuccess) return r;
+  return launch_maybe_pdl(true, gated_reduce_kernel, dim3((p.D + 31) / 32), dim3(1024), 0, s,
+                          (const float*)q.part, p.rows * p.splits, p.D, p.decay, q.ddecay);
+}
+
+}  // namespace
+
+cudaError_t launch_gated_bwd(const GatedBwdParams& q, cudaStream_t s) {
+  return q.f.dtype == M3_BF16 ? bwd_impl<__nv_bfloat16>(q, s) : bwd_impl<float>(q, s);
+}
+
+}  // namespace m3

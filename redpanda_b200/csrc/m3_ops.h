@@ -160,4 +160,43 @@ struct SampleParams {
 };
 cudaError_t launch_sample(const SampleParams& p, cudaStream_t s);
 
+// Gated linear recurrence: see m3_gated.cuh.
+struct GatedParams {
+  const void* x; const void* rg; const void* ig;         // (B*L, ld)
+  long long ld_x, ld_r, ld_i;
+  const float* decay; float c;                           // (D,)
+  const float* h0;                                       // (B, D) or nullptr
+  const int* lengths;                                    // (B,) or nullptr
+  void* y;                                               // (B, L, D)
+  float* h_last;                                         // (B, D) or nullptr
+  float* ckpt;                                           // (B, segments, D) or nullptr
+  int B, L, D;
+  int dtype;
+  int warps, splits, rows;                               // gated_plan: per CTA, per cluster, grid
+  int vec;                                               // 16-byte loads, vector stores
+};
+struct GatedBwdParams {
+  GatedParams f;                                         // y, h_last unused
+  const void* g;                                         // (B, L, D)
+  void* dx; void* drg; void* dig;                        // (B, L, D)
+  float* ddecay;                                         // (D,)
+  float* part;                                           // (rows * splits, D)
+};
+int gated_segments(int L);                               // checkpoints per row and channel
+// warps per CTA, CTAs along time and along the batch
+void gated_plan(int B, int L, int D, int dtype, bool backward, int sms, int* warps, int* splits,
+                int* rows);
+cudaError_t launch_gated_fwd(const GatedParams& p, cudaStream_t s);
+cudaError_t launch_gated_bwd(const GatedBwdParams& p, cudaStream_t s);
+
+struct GatedStepParams {
+  float* h;                                              // (B, D), updated in place
+  const void* x; const void* rg; const void* ig;         // (B, ld)
+  long long ld_x, ld_r, ld_i;
+  const float* decay; float c;
+  void* y;                                               // (B, D)
+  int B, D, dtype, sms;
+};
+cudaError_t launch_gated_step(const GatedStepParams& p, cudaStream_t s);
+
 }  // namespace m3
