@@ -482,6 +482,53 @@ M3_API int m3_norm_bwd(const m3_norm_desc* desc, const void* x, int64_t ld_x, co
             const float* mean, const float* rstd, const void* g, void* dx, float* dw, float* db,
             void* workspace, size_t workspace_bytes, void* stream);
 
+typedef struct m3_add_norm_desc {
+  int64_t rows;       /* >= 1 */
+  int32_t d;          /* 1..32768 */
+  int32_t dtype_x;    /* element type of the branch x and of dx */
+  int32_t dtype_s;    /* element type of the residual stream: res, s, gs, ds */
+  int32_t dtype_y;    /* element type of y and gy */
+  float eps;          /* >= 0 */
+} m3_add_norm_desc;
+
+/* The residual's addition and the RMS norm behind it (mamba.py:591-595 and 82-89):
+ *   s = x + res, rounded to dtype_s;  y = s * rstd * w, rstd = 1 / sqrt(mean(s^2) + eps)
+ *   x (rows, ld_x), res (rows, ld_r), w (d,) float32, y and s (rows, d), rstd
+ *   (rows,) float32 for the backward, or NULL.  s may be res when ld_r == d, or x
+ *   when ld_x == d and both have one element type. */
+M3_API int m3_add_norm_fwd(const m3_add_norm_desc* desc, const void* x, int64_t ld_x,
+            const void* res, int64_t ld_r, const float* w, void* y, void* s, float* rstd,
+            void* stream);
+
+/* Backward: s (rows, ld_s) and rstd of the forward, gy (rows, d) the gradient of
+ * y, gs (rows, d) that of s or NULL (zero).  ds (rows, d) is the gradient of res;
+ * dx (rows, d) that of x where dtype_x is not dtype_s, else NULL (ds serves).  dw
+ * (d,) float32, summed over the rows in a fixed order. */
+M3_API size_t m3_add_norm_bwd_workspace_bytes(const m3_add_norm_desc* desc);
+M3_API int m3_add_norm_bwd(const m3_add_norm_desc* desc, const void* s, int64_t ld_s,
+            const float* w, const float* rstd, const void* gy, const void* gs, void* ds, void* dx,
+            float* dw, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct m3_norm8_desc {
+  int64_t rows;       /* >= 1 */
+  int32_t d;          /* 1..32768 */
+  int32_t group;      /* columns per scale: 32, 64 or 128 that divide d, or 0: a row */
+  int32_t dtype_x;    /* element type of x */
+  int32_t dtype_s;    /* element type of res and s */
+  int32_t e4m3;       /* non-zero: 8-bit floats (largest value 448), else int8 (127) */
+  float eps;          /* >= 0 */
+} m3_norm8_desc;
+
+/* y = the RMS norm of x, or of s = x + res rounded to dtype_s, in 8 bits:
+ *   scale = max(max |y| / top, 2^-126) over a row or a group of columns,
+ *   q = y / scale rounded to nearest even and held to [-top, top]
+ *   x (rows, ld_x), res (rows, ld_r) or NULL, w (d,) float32, q (rows, d) bytes,
+ *   scale (rows,) or (rows, d / group) float32, s (rows, d), not used without res.
+ * A group with a NaN has the scale NaN.  With groups, rows and pointers aligned to
+ * 4 elements (q to 4 bytes). */
+M3_API int m3_norm8_fwd(const m3_norm8_desc* desc, const void* x, int64_t ld_x, const void* res,
+            int64_t ld_r, const float* w, void* q, float* scale, void* s, void* stream);
+
 typedef struct m3_conv_desc {
   int32_t batch;      /* B >= 1 */
   int32_t seqlen;     /* L >= 1; 1 for the step */

@@ -41,6 +41,18 @@ class NormDesc(ctypes.Structure):
                 ("rms", _I), ("eps", ctypes.c_float)]
 
 
+class AddNormDesc(ctypes.Structure):
+    """``m3_add_norm_desc``."""
+    _fields_ = [("rows", ctypes.c_int64), ("d", _I), ("dtype_x", _I), ("dtype_s", _I),
+                ("dtype_y", _I), ("eps", ctypes.c_float)]
+
+
+class Norm8Desc(ctypes.Structure):
+    """``m3_norm8_desc``."""
+    _fields_ = [("rows", ctypes.c_int64), ("d", _I), ("group", _I), ("dtype_x", _I),
+                ("dtype_s", _I), ("e4m3", _I), ("eps", ctypes.c_float)]
+
+
 class ConvDesc(ctypes.Structure):
     """``m3_conv_desc``."""
     _fields_ = [("batch", _I), ("seqlen", _I), ("d_inner", _I), ("width", _I), ("dtype", _I),
@@ -88,6 +100,7 @@ class SampleDesc(ctypes.Structure):
 _D = ctypes.POINTER(ScanDesc)
 _S = ctypes.POINTER(StepDesc)
 _N = ctypes.POINTER(NormDesc)
+_AN = ctypes.POINTER(AddNormDesc)
 _C = ctypes.POINTER(ConvDesc)
 _E = ctypes.POINTER(SelDesc)
 _A = ctypes.POINTER(SelArgs)
@@ -147,6 +160,13 @@ SIGNATURES = {
     "m3_norm_bwd_workspace_bytes": (_Z, [_N]),
     "m3_norm_bwd": (ctypes.c_int, [_N, _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _Z,
                                    _P]),
+    "m3_add_norm_fwd": (ctypes.c_int, [_AN, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, _P, _P,
+                                       _P, _P]),
+    "m3_add_norm_bwd_workspace_bytes": (_Z, [_AN]),
+    "m3_add_norm_bwd": (ctypes.c_int, [_AN, _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P, _P, _P,
+                                       _Z, _P]),
+    "m3_norm8_fwd": (ctypes.c_int, [ctypes.POINTER(Norm8Desc), _P, ctypes.c_int64, _P,
+                                    ctypes.c_int64, _P, _P, _P, _P, _P]),
     "m3_causal_conv_fwd": (ctypes.c_int, [_C, _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P, _P]),
     "m3_causal_conv_bwd_workspace_bytes": (_Z, [_C]),
     "m3_causal_conv_bwd": (ctypes.c_int, [_C, _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P, _P,

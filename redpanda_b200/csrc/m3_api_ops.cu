@@ -32,6 +32,14 @@ int check_norm(const m3_norm_desc* d) {
   return M3_OK;
 }
 
+int check_add_norm(const m3_add_norm_desc* d) {
+  if (!d) return M3_ERR_NULL;
+  if (d->rows < 1 || d->d < 1 || !(d->eps >= 0.f)) return M3_ERR_SHAPE;
+  if (!dtype_ok(d->dtype_x) || !dtype_ok(d->dtype_s) || !dtype_ok(d->dtype_y)) return M3_ERR_DTYPE;
+  if (d->d > kMaxNormD) return M3_ERR_UNSUPPORTED;
+  return M3_OK;
+}
+
 int check_conv(const m3_conv_desc* d) {
   if (!d) return M3_ERR_NULL;
   if (d->batch < 1 || d->seqlen < 1 || d->d_inner < 1 || d->width < 1) return M3_ERR_SHAPE;
@@ -236,6 +244,97 @@ int m3_norm_bwd(const m3_norm_desc* desc, const void* x, int64_t ld_x, const flo
   p.dtype_x = desc->dtype_x; p.dtype_y = desc->dtype_y; p.rms = desc->rms != 0;
   p.sms = device_sms();
   return status(launch_norm_bwd(p, static_cast<cudaStream_t>(stream)));
+}
+
+int m3_add_norm_fwd(const m3_add_norm_desc* desc, const void* x, int64_t ld_x, const void* res,
+                    int64_t ld_r, const float* w, void* y, void* sum, float* rstd, void* stream) {
+  int rc = check_add_norm(desc);
+  if (rc != M3_OK) return rc;
+  if (ld_x < desc->d || ld_r < desc->d) return M3_ERR_SHAPE;
+  if (!x || !res || !w || !y || !sum) return M3_ERR_NULL;
+  if (!aligned(x, dsize(desc->dtype_x)) || !aligned(res, dsize(desc->dtype_s)) ||
+      !aligned(sum, dsize(desc->dtype_s)) || !aligned(y, dsize(desc->dtype_y)) ||
+      !aligned(w, 4) || !aligned(rstd, 4))
+    return M3_ERR_ALIGN;
+  if (y == x || y == res || y == sum || (sum == res && ld_r != desc->d) ||
+      (sum == x && (ld_x != desc->d || desc->dtype_x != desc->dtype_s)))
+    return M3_ERR_ALIAS;
+  if ((rc = check_device()) != M3_OK) return rc;
+  AddNormParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = x; p.ld_x = ld_x; p.res = res; p.ld_r = ld_r; p.w = w; p.y = y; p.s = sum; p.rstd = rstd;
+  p.rows = desc->rows; p.d = desc->d;
+  p.dtype_x = desc->dtype_x; p.dtype_s = desc->dtype_s; p.dtype_y = desc->dtype_y;
+  p.eps = desc->eps;
+  p.sms = device_sms();
+  return status(launch_add_norm_fwd(p, static_cast<cudaStream_t>(stream)));
+}
+
+size_t m3_add_norm_bwd_workspace_bytes(const m3_add_norm_desc* desc) {
+  const int sms = device_sms();
+  if (check_add_norm(desc) != M3_OK || sms <= 0) return 0;
+  return (size_t)norm_bwd_ctas(desc->rows, desc->d, sms) * 2 * desc->d * 4;
+}
+
+int m3_add_norm_bwd(const m3_add_norm_desc* desc, const void* sum, int64_t ld_s, const float* w,
+                    const float* rstd, const void* gy, const void* gs, void* ds, void* dx,
+                    float* dw, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_add_norm(desc);
+  if (rc != M3_OK) return rc;
+  if (ld_s < desc->d) return M3_ERR_SHAPE;
+  const bool same = desc->dtype_x == desc->dtype_s;
+  if (!sum || !w || !rstd || !gy || !ds || !dw || (!same && !dx)) return M3_ERR_NULL;
+  if (same && dx) return M3_ERR_UNSUPPORTED;   // it is ds
+  const int es = dsize(desc->dtype_s);
+  if (!aligned(sum, es) || !aligned(gs, es) || !aligned(ds, es) ||
+      !aligned(dx, dsize(desc->dtype_x)) || !aligned(gy, dsize(desc->dtype_y)) ||
+      !aligned(w, 4) || !aligned(rstd, 4) || !aligned(dw, 4) || !aligned(workspace, 4))
+    return M3_ERR_ALIGN;
+  if (ds == sum || ds == gy || (dx && (dx == sum || dx == gy || dx == gs || dx == ds)))
+    return M3_ERR_ALIAS;
+  if ((rc = check_device()) != M3_OK) return rc;
+  if (!workspace || workspace_bytes < m3_add_norm_bwd_workspace_bytes(desc))
+    return M3_ERR_WORKSPACE;
+  AddNormBwdParams p;
+  memset(&p, 0, sizeof(p));
+  p.s = sum; p.ld_s = ld_s; p.w = w; p.rstd = rstd; p.gy = gy; p.gs = gs; p.ds = ds; p.dx = dx;
+  p.dw = dw; p.part = static_cast<float*>(workspace);
+  p.rows = desc->rows; p.d = desc->d;
+  p.dtype_x = desc->dtype_x; p.dtype_s = desc->dtype_s; p.dtype_y = desc->dtype_y;
+  p.sms = device_sms();
+  return status(launch_add_norm_bwd(p, static_cast<cudaStream_t>(stream)));
+}
+
+int m3_norm8_fwd(const m3_norm8_desc* desc, const void* x, int64_t ld_x, const void* res,
+                 int64_t ld_r, const float* w, void* q, float* scale, void* sum, void* stream) {
+  if (!desc) return M3_ERR_NULL;
+  const int g = desc->group;
+  if (desc->rows < 1 || desc->d < 1 || !(desc->eps >= 0.f)) return M3_ERR_SHAPE;
+  if (g != 0 && ((g != 32 && g != 64 && g != 128) || desc->d % g != 0)) return M3_ERR_SHAPE;
+  if (!dtype_ok(desc->dtype_x) || !dtype_ok(desc->dtype_s)) return M3_ERR_DTYPE;
+  if (desc->d > kMaxNormD) return M3_ERR_UNSUPPORTED;
+  if (ld_x < desc->d || (res && ld_r < desc->d)) return M3_ERR_SHAPE;
+  if (!x || !w || !q || !scale || (res && !sum)) return M3_ERR_NULL;
+  const int ex = dsize(desc->dtype_x), es = dsize(desc->dtype_s), v = g ? 4 : 1;
+  if (!aligned(x, v * ex) || !aligned(res, v * es) || (res && !aligned(sum, v * es)) ||
+      !aligned(q, v) || !aligned(w, 4) || !aligned(scale, 4) || ld_x % v != 0 ||
+      (res && ld_r % v != 0))
+    return M3_ERR_ALIGN;
+  if (q == x || q == res || (res && (q == sum || (sum == res && ld_r != desc->d) ||
+                                     (sum == x && (ld_x != desc->d || ex != es)))))
+    return M3_ERR_ALIAS;
+  const int rc = check_device();
+  if (rc != M3_OK) return rc;
+  Norm8Params p;
+  memset(&p, 0, sizeof(p));
+  p.x = x; p.ld_x = ld_x; p.res = res; p.ld_r = ld_r; p.w = w;
+  p.q = static_cast<unsigned char*>(q);
+  p.scale = scale; p.s = res ? sum : nullptr;
+  p.rows = desc->rows; p.d = desc->d; p.group = g;
+  p.dtype_x = desc->dtype_x; p.dtype_s = desc->dtype_s; p.e4m3 = desc->e4m3 != 0;
+  p.eps = desc->eps;
+  p.sms = device_sms();
+  return status(launch_norm8(p, static_cast<cudaStream_t>(stream)));
 }
 
 int m3_causal_conv_fwd(const m3_conv_desc* desc, const void* x, int64_t ld_x, const float* w,

@@ -38,6 +38,55 @@ struct NormBwdParams {
 int norm_bwd_ctas(long long rows, int d, int sms);   // partials
 cudaError_t launch_norm_bwd(const NormBwdParams& p, cudaStream_t s);
 
+// RMS norm of the residual stream with the branch's addition: s = x + res.
+struct AddNormParams {
+  const void* x; long long ld_x;      // (rows, ld_x), the branch
+  const void* res; long long ld_r;    // (rows, ld_r), the stream
+  const float* w;                     // (d,)
+  void* y;                            // (rows, d)
+  void* s;                            // (rows, d) of the stream's type
+  float* rstd;                        // (rows,) or nullptr
+  long long rows; int d;
+  int dtype_x, dtype_s, dtype_y;
+  float eps;
+  int sms;
+};
+cudaError_t launch_add_norm_fwd(const AddNormParams& p, cudaStream_t s);
+
+struct AddNormBwdParams {
+  const void* s; long long ld_s;      // (rows, ld_s)
+  const float* w; const float* rstd;
+  const void* gy;                     // (rows, d) of dtype_y
+  const void* gs;                     // (rows, d) of dtype_s or nullptr: zero
+  void* ds;                           // (rows, d) of dtype_s
+  void* dx;                           // (rows, d) of dtype_x, or nullptr: ds serves
+  float* dw;                          // (d,)
+  float* part;                        // (norm_bwd_ctas, 2, d), the first of each pair used
+  long long rows; int d;
+  int dtype_x, dtype_s, dtype_y;
+  int sms;
+};
+cudaError_t launch_add_norm_bwd(const AddNormBwdParams& p, cudaStream_t s);
+// out[c] = sum over n partials part[(i * 2 + which) * d + c], in a fixed order (db may be nullptr)
+cudaError_t launch_norm_reduce(const float* part, int n, int d, float* dw, float* db,
+                               cudaStream_t s);
+
+// The RMS norm (of x, or of s = x + res) in 8 bits with scales.
+struct Norm8Params {
+  const void* x; long long ld_x;      // (rows, ld_x)
+  const void* res; long long ld_r;    // (rows, ld_r) of dtype_s, or nullptr
+  const float* w;                     // (d,)
+  unsigned char* q;                   // (rows, d)
+  float* scale;                       // (rows, d / group), or (rows,) for group 0
+  void* s;                            // (rows, d) of dtype_s, unused without res
+  long long rows; int d, group;
+  int dtype_x, dtype_s;
+  int e4m3;                           // else int8
+  float eps;
+  int sms;
+};
+cudaError_t launch_norm8(const Norm8Params& p, cudaStream_t s);
+
 constexpr int kMaxConvWidth = 8;
 
 struct ConvParams {

@@ -3,6 +3,10 @@
 * ``m3_layer_norm`` -- (x - mean) * rsqrt(var + eps) * weight + bias over the
   last dimension (the heads of redpanda/engine/search_mamba.py:60-83)
 * ``m3_rms_norm`` -- x * rsqrt(mean(x^2) + eps) * weight (mamba.py:82-89)
+* ``m3_add_rms_norm`` -- the residual's addition and the RMS norm behind it
+  (mamba.py:591-595, 82-89): (norm(x + residual), x + residual)
+* ``m3_rms_norm_8bit`` -- the RMS norm, with or without that addition, in 8 bits
+  with a scale per row or group of columns, for a projection of 8-bit operands
 * ``LayerNorm`` -- ``torch.nn.LayerNorm`` that runs ``m3_layer_norm`` on CUDA
   tensors when its class attribute ``use_kernel`` is set
 
@@ -16,7 +20,7 @@ import torch.nn as nn
 
 from . import _lib
 from . import _launch as H
-from ._lib import NormDesc
+from ._lib import AddNormDesc, Norm8Desc, NormDesc
 
 MAX_D = 32768           # longest row of the kernels
 
@@ -117,6 +121,156 @@ def m3_rms_norm(x, weight, eps=1e-5, out_dtype=None):
     """x * rsqrt(mean(x^2) + eps) * weight over the last dimension; arguments as
     :func:`m3_layer_norm`."""
     return _norm("m3_rms_norm", x, weight, None, eps, 1, out_dtype)
+
+
+def _add_forward(x2, lx, r2, lr, w, desc, out_dtype, stats):
+    """(y, s, rstd or None) of rows."""
+    rows, d = r2.shape
+    y = torch.empty((rows, d), device=x2.device, dtype=out_dtype)
+    s = torch.empty((rows, d), device=x2.device, dtype=r2.dtype)
+    st = torch.empty(rows, device=x2.device, dtype=torch.float32) if stats else None
+    if rows:
+        H.launch(x2.get_device(), _lib.load().m3_add_norm_fwd, desc, x2.data_ptr(), lx,
+                 r2.data_ptr(), lr, w.data_ptr(), y.data_ptr(), s.data_ptr(), H.ptr(st))
+    return y, s, st
+
+
+class _AddNormFn(torch.autograd.Function):
+    """Addition and norm with the analytic backward (m3_add_norm_fwd / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, out_dtype):
+        d = x.shape[-1]
+        x2, lx = H.rows(x if x.dim() == 2 else x.reshape(-1, d))
+        r2, lr = H.rows(residual if x.dim() == 2 else residual.reshape(-1, d))
+        w = H.f32(weight)
+        desc = AddNormDesc(x2.shape[0], d, H.code(x2.dtype), H.code(r2.dtype), H.code(out_dtype),
+                           eps)
+        y, s, st = _add_forward(x2, lx, r2, lr, w, desc, out_dtype, True)
+        y, s = y.view(x.shape), s.view(x.shape)
+        H.save(ctx, s, w, st)
+        ctx.cfg = (desc, x.dtype, out_dtype, weight.dtype)
+        ctx.set_materialize_grads(False)
+        return y, s
+
+    @staticmethod
+    @H.once_differentiable
+    def backward(ctx, gy, gs):
+        if gy is None and gs is None:
+            return (None,) * 5
+        desc, xt, yt, wt = ctx.cfg
+        s, w, st = ts = ctx.saved_tensors
+        if ctx.hooked is not None:
+            H.check_saved(ctx, ts, gs if gy is None else gy)
+        shape, d = s.shape, s.shape[-1]
+        (s2, ls), w, st = H.rows(s.reshape(-1, d)), w.contiguous(), st.contiguous()
+        if gs is not None and (gs.dtype is not s.dtype or not gs.is_contiguous()):
+            gs = gs.to(s.dtype).contiguous()
+        if gy is None:      # the norm's result was not used
+            return (gs if xt is gs.dtype else gs.to(xt)), gs, None, None, None
+        if gy.dtype is not yt or not gy.is_contiguous():
+            gy = gy.to(yt).contiguous()
+        ds = torch.empty(shape, device=s.device, dtype=s.dtype)
+        dx = None if xt is s.dtype else torch.empty(shape, device=s.device, dtype=xt)
+        dw = torch.empty_like(w)
+        if desc.rows:
+            lib = _lib.load()
+            dev = s.get_device()
+            with H.on_device(dev):
+                nws = lib.m3_add_norm_bwd_workspace_bytes(desc)
+            ws = torch.empty(nws, device=s.device, dtype=torch.uint8)
+            H.launch(dev, lib.m3_add_norm_bwd, desc, s2.data_ptr(), ls, w.data_ptr(),
+                     st.data_ptr(), gy.data_ptr(), H.ptr(gs), ds.data_ptr(), H.ptr(dx),
+                     dw.data_ptr(), ws.data_ptr(), nws)
+        else:
+            dw.zero_()
+        return (ds if dx is None else dx), ds, (dw if wt is torch.float32 else dw.to(wt)), None, \
+            None
+
+
+def _check_rows(name, x, weight, residual, eps):
+    d = x.shape[-1] if x.dim() else 0
+    if d < 1 or weight.shape != (d,):
+        raise ValueError(f"{name}: weight of the length of x's last dimension")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"{name}: the residual has x's shape")
+    if d > MAX_D:
+        raise ValueError(f"{name}: rows of at most {MAX_D} elements")
+    eps = float(eps)
+    if not eps >= 0:
+        raise ValueError(f"{name}: eps must not be negative")
+    H.code(x.dtype), H.code(x.dtype if residual is None else residual.dtype)
+    return d, eps
+
+
+def m3_add_rms_norm(x, residual, weight, eps=1e-5, out_dtype=None):
+    """(y, s): s = x + residual, the residual stream behind a layer, and y = its RMS
+    norm, the next layer's input; x and residual (..., d), d <= 32768.
+
+    x (a layer's output) and residual float32 or bfloat16 each, rows may be strided;
+    s has the residual's element type, and y is the norm of s as rounded to it; y
+    has ``out_dtype`` (default: the residual's).  weight (d,) of any float type,
+    used in float32.  Differentiable in x, residual and weight (once, in reverse
+    mode); the gradients of y and s reach x and the residual as one sum."""
+    name = "m3_add_rms_norm"
+    d, eps = _check_rows(name, x, weight, residual, eps)
+    out_dtype = residual.dtype if out_dtype is None else out_dtype
+    H.code(out_dtype)
+    H.refuse_tangents(name, x, residual, weight)
+    H.device_index(x, residual, weight)
+    if H.needs_grad(x, residual, weight):
+        return _AddNormFn.apply(x, residual, weight, eps, out_dtype)
+    x2, lx = H.rows(x if x.dim() == 2 else x.reshape(-1, d))
+    r2, lr = H.rows(residual if x.dim() == 2 else residual.reshape(-1, d))
+    desc = AddNormDesc(x2.shape[0], d, H.code(x2.dtype), H.code(r2.dtype), H.code(out_dtype), eps)
+    y, s, _ = _add_forward(x2, lx, r2, lr, H.f32(weight), desc, out_dtype, False)
+    return (y, s) if x.dim() == 2 else (y.view(x.shape), s.view(x.shape))
+
+
+def _grouped_rows(t, d, group):
+    """H.rows of (..., d), copied where groups need vectors of 4 and it has none."""
+    t2, ld = H.rows(t if t.dim() == 2 else t.reshape(-1, d))
+    if group and (ld % 4 or t2.data_ptr() % (4 * t2.element_size())):
+        t2, ld = t2.clone(memory_format=torch.contiguous_format), d
+    return t2, ld
+
+
+def m3_rms_norm_8bit(x, weight, residual=None, eps=1e-5, dtype=torch.float8_e4m3fn, group=None):
+    """The RMS norm in 8 bits: (q, scale), or with ``residual`` (q, scale, s) where
+    s = x + residual as in :func:`m3_add_rms_norm` and q is its norm.
+
+    x (and residual) (..., d) float32 or bfloat16; ``dtype``: torch.float8_e4m3fn or
+    torch.int8; ``group``: 32, 64 or 128 columns per scale (they have to divide d),
+    or None, one scale per row.  q (..., d) and scale (..., 1) or (..., d / group)
+    float32 stand for y = q * scale, with scale = max(max|y| / 448, 2^-126) (int8:
+    127) over the group, y in float32, q = y / scale rounded to nearest even.  A
+    group with a NaN has the scale NaN.  Inference only."""
+    name = "m3_rms_norm_8bit"
+    d, eps = _check_rows(name, x, weight, residual, eps)
+    if dtype not in (torch.float8_e4m3fn, torch.int8):
+        raise TypeError(f"{name}: dtype is torch.float8_e4m3fn or torch.int8")
+    if group not in (None, 32, 64, 128) or (group and d % group):
+        raise ValueError(f"{name}: group is None, 32, 64 or 128 and divides d")
+    if H.needs_grad(x, weight, residual):
+        raise ValueError(f"{name} has no derivative: call it under torch.no_grad()")
+    H.refuse_tangents(name, x, weight, residual)
+    dev = H.device_index(x, weight, residual)
+    x2, lx = _grouped_rows(x, d, group)
+    r2, lr = (None, 0) if residual is None else _grouped_rows(residual, d, group)
+    rows = x2.shape[0]
+    q = torch.empty(x.shape, device=x.device, dtype=dtype)
+    scale = torch.empty((*x.shape[:-1], d // group if group else 1), device=x.device,
+                        dtype=torch.float32)
+    s = None if r2 is None else torch.empty(x.shape, device=x.device, dtype=r2.dtype)
+    if rows:
+        w = H.f32(weight)
+        H.launch(dev, _lib.load().m3_norm8_fwd,
+                 Norm8Desc(rows, d, group or 0, H.code(x2.dtype),
+                           H.code(x2.dtype if r2 is None else r2.dtype),
+                           dtype is torch.float8_e4m3fn, eps),
+                 x2.data_ptr(), lx, H.ptr(r2), lr, w.data_ptr(), q.data_ptr(), scale.data_ptr(),
+                 H.ptr(s))
+    return (q, scale) if s is None else (q, scale, s)
 
 
 class LayerNorm(nn.LayerNorm):
