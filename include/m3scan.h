@@ -289,6 +289,39 @@ M3_API int m3_rows_linear(int32_t rows, int32_t d_in, int32_t d_out, const float
             int32_t silu, float* out0, int64_t ld0, float* out1, int64_t ld1,
             int32_t overlap, void* stream);
 
+typedef struct m3_rows_q4_desc {
+  int32_t rows;       /* 1..8 */
+  int32_t d_in;       /* 1..65536 */
+  int32_t d_out;      /* >= 1 */
+  int32_t group;      /* columns per scale: 32, 64 or 128 */
+  int32_t center;     /* non-zero: a center beside each scale */
+  int32_t dtype;      /* element type of x, residual, out0 and out1 */
+  int32_t split;      /* columns of out0 */
+  int32_t silu;       /* non-zero: silu on the columns of out0 */
+  float eps;          /* of the norm */
+} m3_rows_q4_desc;
+
+/* m3_rows_linear with weights of 4 bits: out = act(residual + (bias + xn W^T)),
+ *   W[o,k] = scale[o,k/group] (q[o,k] - 8) + center[o,k/group],  q in 0..15,
+ * in fp32 (inputs are not rounded), each output rounded once; the norm, split,
+ * residual and overlap as above (the codes and scales are the weights that overlap
+ * is about).  Sums in a fixed order.
+ *   codes   (tiles, blocks, 32, 4) 32-bit words, 16-byte aligned: tiles of 16
+ *           outputs, blocks of 64 columns; both numbers rounded up, the columns to
+ *           whole groups of 128 where group is 128.  Word j of lane l of a block
+ *           holds, in bits 4 (h + 2 v + 4 e) up, the code of output l / 4 + 8 h and
+ *           column 16 j + 8 v + 2 (l % 4) + e of the tile and block (h, v, e: 0, 1).
+ *   scales  (tiles, groups, 8) of two outputs each, l and l + 8: bf16 pairs of
+ *           scale and center (64 bits) with center, else their two scales (32
+ *           bits); 8- or 4-byte aligned; groups cover the rounded-up columns
+ *   x (rows, ld_x); norm_w (d_in,) float32 or NULL; bias (d_out,) float32 or NULL;
+ *   residual (rows, ld_r) or NULL: it may be out0 itself (same stride, split ==
+ *   d_out), no other overlap of an output with an input. */
+M3_API int m3_rows_linear_q4(const m3_rows_q4_desc* desc, const void* x, int64_t ld_x,
+            const float* norm_w, const void* codes, const void* scales, const float* bias,
+            const void* residual, int64_t ld_r, void* out0, int64_t ld0, void* out1, int64_t ld1,
+            int32_t overlap, void* stream);
+
 /* m3_xdt_proj: x_dbl = u W_x^T + b_x  (rows, n_x; mamba.py:454) and
  * dt = x_dbl[:, :dt_rank] W_dt^T  (rows, d_inner; dt_proj without its bias,
  * mamba.py:463 -- m3_step_gated_fused / m3_step_inputs add it) in one launch.

@@ -91,6 +91,12 @@ class GatedArgs(ctypes.Structure):
         (n, _P) for n in ("decay", "state", "lengths")]
 
 
+class RowsQ4Desc(ctypes.Structure):
+    """``m3_rows_q4_desc``."""
+    _fields_ = [(n, _I) for n in ("rows", "d_in", "d_out", "group", "center", "dtype", "split",
+                                  "silu")] + [("eps", ctypes.c_float)]
+
+
 class SampleDesc(ctypes.Structure):
     """``m3_sample_desc``."""
     _fields_ = [("rows", _I), ("vocab", _I), ("dtype", _I), ("temperature", ctypes.c_float),
@@ -134,6 +140,9 @@ SIGNATURES = {
     "m3_rows_linear": (ctypes.c_int, [_I, _I, _I, _P, ctypes.c_int64, _P, ctypes.c_float, _P,
                                       _P, _P, ctypes.c_int64, _I, _I, _P, ctypes.c_int64, _P,
                                       ctypes.c_int64, _I, _P]),
+    "m3_rows_linear_q4": (ctypes.c_int, [ctypes.POINTER(RowsQ4Desc), _P, ctypes.c_int64, _P, _P,
+                                         _P, _P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P,
+                                         ctypes.c_int64, _I, _P]),
     "m3_xdt_proj": (ctypes.c_int, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P]),
     "m3_step_inputs_bwd_workspace_bytes": (_Z, [_S, _I]),
     "m3_step_inputs_bwd": (ctypes.c_int, [_S, _I, _P, ctypes.c_int64, _P, ctypes.c_int64, _I,

@@ -8,6 +8,7 @@
 #include "m3_api_util.h"
 #include "m3_common.cuh"
 #include "m3_internal.h"
+#include "m3_ops.h"
 #include "m3_tiles.h"
 #include "m3scan.h"
 
@@ -692,6 +693,55 @@ int m3_rows_linear(int32_t rows, int32_t d_in, int32_t d_out, const float* x, in
   p.vec = aligned(x, 16) && ld_x % 4 == 0 && (!norm_w || aligned(norm_w, 16));
   cudaError_t e = launch_rows_linear(p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? M3_OK : M3_ERR_LAUNCH;
+}
+
+int m3_rows_linear_q4(const m3_rows_q4_desc* desc, const void* x, int64_t ld_x,
+                      const float* norm_w, const void* codes, const void* scales,
+                      const float* bias, const void* residual, int64_t ld_r, void* out0,
+                      int64_t ld0, void* out1, int64_t ld1, int32_t overlap, void* stream) {
+  if (!desc) return M3_ERR_NULL;
+  const int rows = desc->rows, d_in = desc->d_in, d_out = desc->d_out, split = desc->split;
+  if (rows < 1 || d_in < 1 || d_out < 1 || d_out > 1 << 30 || split < 0 || split > d_out ||
+      (norm_w && !(desc->eps >= 0.f)))
+    return M3_ERR_SHAPE;
+  if (desc->group != 32 && desc->group != 64 && desc->group != 128) return M3_ERR_SHAPE;
+  if (!dtype_ok(desc->dtype)) return M3_ERR_DTYPE;
+  if (rows > kQ4Rows || d_in > kQ4MaxIn) return M3_ERR_UNSUPPORTED;
+  if (!x || !codes || !scales || (split > 0 && !out0) || (split < d_out && !out1))
+    return M3_ERR_NULL;
+  if (ld_x < d_in || (residual && ld_r < d_out) || (split > 0 && ld0 < split) ||
+      (split < d_out && ld1 < d_out - split))
+    return M3_ERR_SHAPE;
+  const int e = dsize(desc->dtype);
+  if (!aligned(codes, 16) || !aligned(scales, desc->center ? 8 : 4) || !aligned(x, e) ||
+      !aligned(norm_w, 4) || !aligned(bias, 4) || !aligned(residual, e) ||
+      (split > 0 && !aligned(out0, e)) || (split < d_out && !aligned(out1, e)))
+    return M3_ERR_ALIGN;
+  // CTAs stage x and write outputs in any order; only the residual's own place may
+  // be written
+  auto span = [&](int64_t ld, int64_t width) { return (size_t)((rows - 1) * ld + width) * e; };
+  const size_t xs = span(ld_x, d_in), rs = residual ? span(ld_r, d_out) : 0;
+  const size_t s0 = split > 0 ? span(ld0, split) : 0, s1 = split < d_out ? span(ld1, d_out - split) : 0;
+  const bool in_place = residual && residual == out0 && ld_r == ld0 && split == d_out;
+  if ((s0 && (spans_overlap(x, xs, out0, s0) ||
+              (residual && !in_place && spans_overlap(residual, rs, out0, s0)))) ||
+      (s1 && (spans_overlap(x, xs, out1, s1) ||
+              (residual && spans_overlap(residual, rs, out1, s1)))))
+    return M3_ERR_ALIAS;
+  const int rc = check_device();
+  if (rc != M3_OK) return rc;
+  RowsQ4Params p;
+  memset(&p, 0, sizeof(p));
+  p.x = x; p.ld_x = ld_x; p.norm_w = norm_w; p.eps = desc->eps;
+  p.codes = static_cast<const uint4*>(codes); p.scales = scales; p.bias = bias;
+  p.residual = residual; p.ld_r = ld_r; p.out0 = out0; p.ld0 = ld0; p.out1 = out1; p.ld1 = ld1;
+  p.rows = rows; p.d_in = d_in; p.d_out = d_out; p.split = split; p.silu = desc->silu != 0;
+  p.group = desc->group; p.center = desc->center != 0; p.dtype = desc->dtype;
+  p.pdl = overlap != 0;
+  p.sms = device_sms();
+  p.vec = aligned(x, 2 * e) && ld_x % 2 == 0 && aligned(norm_w, 8);
+  return launch_rows_q4(p, static_cast<cudaStream_t>(stream)) == cudaSuccess ? M3_OK
+                                                                             : M3_ERR_LAUNCH;
 }
 
 int m3_xdt_proj(int32_t rows, int32_t d_inner, int32_t n_x, int32_t dt_rank, const float* u,

@@ -248,4 +248,23 @@ struct GatedStepParams {
 };
 cudaError_t launch_gated_step(const GatedStepParams& p, cudaStream_t s);
 
+// Product of a few rows with 4-bit weights (m3_gemv4.cu).
+constexpr int kQ4Rows = 8;
+constexpr int kQ4MaxIn = 65536;
+struct RowsQ4Params {
+  const void* x; long long ld_x;                         // (rows, d_in)
+  const float* norm_w; float eps;                        // RMS norm weight or nullptr
+  const uint4* codes;                                    // (tiles, blocks, 32): see m3_gemv4.cu
+  const void* scales;                                    // (tiles, groups, 8) words
+  const float* bias;                                     // (d_out,) or nullptr
+  const void* residual; long long ld_r;                  // (rows, d_out) or nullptr
+  void* out0; long long ld0;
+  void* out1; long long ld1;
+  int rows, d_in, d_out, split, silu, group, center, dtype;
+  int pdl, sms;
+  int vec;                                               // pairs of x and norm_w may be loaded
+  int mw, kw, chunk;                                     // set by the launcher
+};
+cudaError_t launch_rows_q4(const RowsQ4Params& p, cudaStream_t s);
+
 }  // namespace m3
