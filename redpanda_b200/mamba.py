@@ -25,7 +25,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import scan as S
-from .norm import MAX_D, m3_rms_norm
+from .norm import MAX_D, m3_add_rms_norm, m3_rms_norm
+from .quant import Q4Weight, m3_rows_linear_q4
 
 
 @dataclass
@@ -124,6 +125,8 @@ class Mamba3Block(nn.Module):
     # matrix-vector products, where launch latency, not arithmetic, sets the
     # time.  0 disables it.
     small_step_max_batch = 8
+    # 4-bit weights of the small-batch step (Mamba.quantize_step_), by projection
+    step_q4 = None
 
     def __init__(self, config: MambaConfig):
         super().__init__()
@@ -483,14 +486,16 @@ class Mamba3Block(nn.Module):
           (``m3_rows_linear``, mamba.py:497, 591-595).
 
         Same arithmetic as ``step_fused_`` except the projections' summation
-        order (their products are not cuBLAS GEMMs here)."""
+        order (their products are not cuBLAS GEMMs here) and, after
+        ``Mamba.quantize_step_``, the 4-bit weights of the projections named there
+        (``m3_rows_linear_q4``)."""
         cfg = self.config
         d_in, n, p = cfg.d_inner, cfg.d_state, cfg.mimo_p
+        linear = self._step_linear
         # each launch may start while the one before it finishes (programmatic
         # dependent launches; no kernel of the step writes a weight)
-        u, z = S.m3_rows_linear(x, self.in_proj.weight, self.in_proj.bias, norm.weight,
-                                norm.eps, split=d_in, silu=True, overlap=True)
-        x_dbl, _ = S.m3_rows_linear(u, self.x_proj.weight, self.x_proj.bias, overlap=True)
+        u, z = linear("in_proj", x, norm.weight, norm.eps, split=d_in, silu=True)
+        x_dbl, _ = linear("x_proj", u)
         bw = self.b_norm.weight if cfg.use_bcnorm else None
         cw = self.c_norm.weight if cfg.use_bcnorm else None
         eps = self.b_norm.eps if cfg.use_bcnorm else 0.0
@@ -505,9 +510,19 @@ class Mamba3Block(nn.Module):
                                              dt_bias=self.dt_proj.bias)
             g = S.m3_step_gated_(state, delta, u, bc, cc, self.step_params(), cfg.n_rot_state,
                                  z, self.D)
-        S.m3_rows_linear(g, self.out_proj.weight, self.out_proj.bias, residual=x, out0=x,
-                         overlap=True)
+        linear("out_proj", g, residual=x, out0=x)
         return x
+
+    def _step_linear(self, name, x, norm_weight=None, eps=0.0, **kw):
+        """A projection of the small-batch step: its weight, or the 4-bit one."""
+        proj = getattr(self, name)
+        q = None if self.step_q4 is None else self.step_q4.get(name)
+        if q is None:
+            return S.m3_rows_linear(x, proj.weight, proj.bias, norm_weight, eps, overlap=True,
+                                    **kw)
+        if q[1] != (proj.weight.data_ptr(), proj.weight._version):
+            raise RuntimeError(f"{name}'s weight has changed: call quantize_step_ again")
+        return m3_rows_linear_q4(x, q[0], proj.bias, norm_weight, eps, overlap=True, **kw)
 
     def step(self, x_t, state=None):
         """Functional O(1) step (mamba.py:427-498): returns (out, (h, dBu_t))."""
@@ -530,7 +545,15 @@ def _state_pair(entry):
 
 
 class Mamba(nn.Module):
-    """Embedding + Mamba3Block layers + final norm (mamba.py:503-620)."""
+    """Embedding + Mamba3Block layers + final norm (mamba.py:503-620).
+
+    ``fuse_add_norm`` (class or instance attribute): in training, run each layer's
+    residual addition and the next layer's norm as one launch each way
+    (``m3_add_rms_norm``) on CUDA streams of float32 or bfloat16.  Off by default,
+    where results are torch's; the kernel's norms differ by rounding.  Not used
+    with ``grad_checkpoint``, whose layers hold their norm."""
+
+    fuse_add_norm = False
 
     def __init__(self, config: MambaConfig):
         super().__init__()
@@ -554,6 +577,8 @@ class Mamba(nn.Module):
 
     def forward(self, input_ids, input_embeds=None):
         x = input_embeds if input_embeds is not None else self.embedding(input_ids)
+        if self._add_norm_ok(x):
+            return self._forward_add_norm(x)
         for layer in self.layers:
             mixer, norm = layer["mixer"], layer["norm"]
             if self.grad_checkpoint and self.training and x.requires_grad:
@@ -564,6 +589,53 @@ class Mamba(nn.Module):
             else:
                 x = x + mixer(norm(x))
         return self.norm_f(x)
+
+    def _add_norm_ok(self, x):
+        types = (torch.float32, torch.bfloat16)
+        return (self.fuse_add_norm and torch.is_grad_enabled() and x.is_cuda
+                and not (self.grad_checkpoint and self.training) and x.dtype in types
+                and self.config.d_model <= MAX_D
+                and all(n.weight.dtype in types for n in self._norms()))
+
+    def _norms(self):
+        return [layer["norm"] for layer in self.layers] + [self.norm_f]
+
+    def _forward_add_norm(self, x):
+        """``forward`` with each residual addition and the norm behind it in one
+        kernel: the same values up to the norms' rounding."""
+        norms = self._norms()
+
+        def out_type(norm):   # RMSNorm's; in a bf16 layer what autocast's in_proj casts it to
+            if _bf16_layer() and norm is not self.norm_f:
+                return torch.bfloat16
+            return torch.promote_types(x.dtype, norm.weight.dtype)
+        if not len(self.layers):
+            return self.norm_f(x)
+        h = m3_rms_norm(x, norms[0].weight, norms[0].eps, out_dtype=out_type(norms[0]))
+        for layer, norm in zip(self.layers, norms[1:]):
+            h, x = m3_add_rms_norm(layer["mixer"](h), x, norm.weight, norm.eps,
+                                   out_dtype=out_type(norm))
+        return h
+
+    def quantize_step_(self, group=64, names=("in_proj", "out_proj"), center=True):
+        """Hold 4-bit weights (:class:`redpanda_b200.quant.Q4Weight`) of the named
+        projections ("in_proj", "x_proj", "out_proj") for the small-batch step:
+        ``step_fused_`` on at most ``Mamba3Block.small_step_max_batch`` rows, and
+        step graphs captured from now on.  Larger batches, priming and training keep
+        the full weights.  The copies are of the present weights: a step after the
+        weights have changed raises until this is called again.  ``names=()`` goes
+        back to the full weights.  Returns the model."""
+        names = tuple(names)
+        if not set(names) <= {"in_proj", "x_proj", "out_proj"}:
+            raise ValueError("quantize_step_: names are of in_proj, x_proj, out_proj")
+        for layer in self.layers:
+            mixer = layer["mixer"]
+            held = {}
+            for name in names:
+                w = getattr(mixer, name).weight
+                held[name] = (Q4Weight.quantize(w, group, center), (w.data_ptr(), w._version))
+            mixer.step_q4 = held or None
+        return self
 
     def init_cache(self, batch_size, device):
         return [None] * len(self.layers)
