@@ -682,7 +682,7 @@ typedef struct m3_gated_args {
  *           not read
  *   h_last  (B, D) float32 or NULL: the state at each row's length (not state)
  *   ckpt    m3_gated_ckpt_floats() floats for the backward (the state in front of
- *           every 8 steps), 8-byte aligned, or NULL */
+ *           every 4 steps), 8-byte aligned, or NULL */
 M3_API size_t m3_gated_ckpt_floats(const m3_gated_desc* desc);
 M3_API int m3_gated_fwd(const m3_gated_desc* desc, const m3_gated_args* args, void* y,
             float* h_last, float* ckpt, void* stream);

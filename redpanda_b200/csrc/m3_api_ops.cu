@@ -91,7 +91,7 @@ int fill_gated(const m3_gated_desc* d, const m3_gated_args* a, bool backward, Ga
   const int v = 16 / e;
   p->vec = d->d_inner % v == 0 && a->ld_x % v == 0 && a->ld_r % v == 0 && a->ld_i % v == 0 &&
            aligned(a->x, 16) && aligned(a->rg, 16) && aligned(a->ig, 16);
-  gated_plan(p->B, p->L, p->D, p->dtype, backward, device_sms(), &p->warps, &p->splits, &p->rows);
+  gated_plan(p->B, p->L, p->D, backward, device_sms(), p);
   return M3_OK;
 }
 
@@ -555,10 +555,9 @@ int m3_gated_fwd(const m3_gated_desc* desc, const m3_gated_args* args, void* y, 
 size_t m3_gated_bwd_workspace_bytes(const m3_gated_desc* desc) {
   const int sms = device_sms();
   if (check_gated(desc) != M3_OK || sms <= 0) return 0;
-  int warps, splits, rows;
-  gated_plan(desc->batch, desc->seqlen, desc->d_inner, desc->dtype, true, sms, &warps, &splits,
-             &rows);
-  return (size_t)rows * splits * desc->d_inner * 4;
+  GatedParams p;
+  gated_plan(desc->batch, desc->seqlen, desc->d_inner, true, sms, &p);
+  return (size_t)p.rows * p.splits * desc->d_inner * 4;
 }
 
 int m3_gated_bwd(const m3_gated_desc* desc, const m3_gated_args* args, const void* g,

@@ -6,8 +6,9 @@
 // A decay near 1 is what these layers are made of, and an error of a counts
 // 1 / (1 - a) times in the state, so a and 1 - a^2 both come from p = e^l - 1
 // computed to its own precision: a = 1 + p, 1 - a^2 = -p (2 + p).  e^l - 1 is
-// 2^n e^f - 1 with l = n ln 2 + f (Cody and Waite's two-part ln 2), |f| <= 0.35,
-// and the Taylor sum of e^f - 1 to f^7 (next term below 2e-8 of f).  On the MUFU
+// 2^n e^f - 1 with l = n ln 2 + f, |f| <= 0.35, and e^f - 1 = f + f^2 q(f), q of
+// degree 4: this project's own least-squares fit on Chebyshev nodes, weighted for
+// e^f - 1's relative error, which is 1.6e-8 at most.  On the MUFU
 // unit's ex2 instead, whose results are low by 2e-8 on average, a state would be
 // low by that times 1 / (1 - a): 2e-5 at a = 0.999.
 //
@@ -23,13 +24,31 @@
 
 namespace m3 {
 
-constexpr int kGatedSteps = 8;        // steps per thread at a time = checkpoint interval
-constexpr int kGatedTile = 64;        // channels per CTA: two per lane
+constexpr int kGatedCkpt = 4;         // steps between the backward's checkpoints
+#ifndef M3_W
+#define M3_W 8
+#endif
+#ifndef M3_TF
+#define M3_TF 8
+#endif
+#ifndef M3_TB
+#define M3_TB 4
+#endif
+#ifndef M3_GB
+#define M3_GB 2
+#endif
+constexpr int kGatedFwdSteps = M3_TF, kGatedBwdSteps = M3_TB;   // of a thread at a time
+constexpr int kGatedWarps = M3_W;        // of a CTA, at most
 
+#ifdef M3_SCALAR
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
+#else
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return __ffma2_rn(b, f2(-1.f), a); }
+#endif
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN stays NaN
   float y;
@@ -41,8 +60,10 @@ __device__ __forceinline__ float rsqrt_approx(float x) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float2 sigmoid2(float2 x) {
-  return make_float2(sigmoid_f(x.x), sigmoid_f(x.y));
+__device__ __forceinline__ float2 sigmoid2(float2 x) {   // sigmoid_f, packed
+  const float2 t = mul2(x, f2(-kLog2e));
+  const float2 u = add2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), f2(1.f));
+  return make_float2(rcp_approx(u.x), rcp_approx(u.y));
 }
 
 // log(1 + e^x), of the decay parameter: once per thread
@@ -50,33 +71,42 @@ __device__ __forceinline__ float softplus_f(float x) {
   return x > 20.f ? x : log1pf(expf(x));
 }
 
-// a = e^l and p = e^l - 1 for l <= 0 (l below -87: as -87, where a is 2e-38)
+// a = e^l and p = e^l - 1 for l <= 0 (l below -87: as -87, where a is 2e-38).  NEAR:
+// l >= -kNear, where n is 0; the same bits with half the instructions.
+constexpr float kNear = 0.34f;        // below ln(2) / 2
+template <bool NEAR>
 __device__ __forceinline__ void decay2(float2 l, float2& a, float2& p) {
-  constexpr float kLn2Hi = 0x1.62e4p-1f;          // ln 2 to 16 bits: n times it is exact
-  constexpr float kLn2Lo = 0x1.7f7d1cp-20f;       // ln 2 - kLn2Hi
-  l = make_float2(max_nan(l.x, -87.f), max_nan(l.y, -87.f));
-  const float2 j = fma2(l, f2(kLog2e), f2(kMagic));
-  const float2 n = add2(j, f2(-kMagic));
-  float2 f = fma2(n, f2(-kLn2Hi), l);
-  f = fma2(n, f2(-kLn2Lo), f);
-  float2 q = fma2(f, f2(1.f / 5040.f), f2(1.f / 720.f));
-  q = fma2(q, f, f2(1.f / 120.f));
-  q = fma2(q, f, f2(1.f / 24.f));
-  q = fma2(q, f, f2(1.f / 6.f));
+  constexpr float kLn2 = 0x1.62e430p-1f;          // off by 2e-9, which n times is a's error
+  float2 f = l, j;
+  if (!NEAR) {
+    l = make_float2(max_nan(l.x, -87.f), max_nan(l.y, -87.f));
+    j = fma2(l, f2(kLog2e), f2(kMagic));
+    f = fma2(add2(j, f2(-kMagic)), f2(-kLn2), l);
+  }
+  float2 q = fma2(f, f2(0x1.6d9956p-10f), f2(0x1.122838p-7f));
+  q = fma2(q, f, f2(0x1.555486p-5f));
+  q = fma2(q, f, f2(0x1.5554b0p-3f));
   q = fma2(q, f, f2(0.5f));
   const float2 e = fma2(mul2(f, f), q, f);        // e^f - 1
-  // 2^n: the low bits of j hold n
-  const float2 s = make_float2(
-      __uint_as_float((__float_as_uint(j.x) << 23) + 0x3f800000u),
-      __uint_as_float((__float_as_uint(j.y) << 23) + 0x3f800000u));
-  a = fma2(s, e, s);
-  p = fma2(s, e, add2(s, f2(-1.f)));
+  if (NEAR) {
+    a = add2(e, f2(1.f));
+    p = e;
+  } else {
+    // 2^n: the low bits of j hold n
+    const float2 s = make_float2(
+        __uint_as_float((__float_as_uint(j.x) << 23) + 0x3f800000u),
+        __uint_as_float((__float_as_uint(j.y) << 23) + 0x3f800000u));
+    a = fma2(s, e, s);
+    p = fma2(s, e, add2(s, f2(-1.f)));
+  }
 }
 
-// m = sqrt(-p (2 + p)) and 1 / m (finite where m is 0)
+// m = sqrt(-p (2 + p)) and 1 / m, finite where m is 0 (1e-37 is far below what m
+// can be but for that: 2 |l| is 1e-37 where the gate is 1e-38)
 __device__ __forceinline__ void root2(float2 p, float2& m, float2& inv) {
   const float2 v = mul2(p, fma2(p, f2(-1.f), f2(-2.f)));
-  inv = make_float2(rsqrt_approx(fmaxf(v.x, 1e-37f)), rsqrt_approx(fmaxf(v.y, 1e-37f)));
+  const float2 w = add2(v, f2(1e-37f));
+  inv = make_float2(rsqrt_approx(w.x), rsqrt_approx(w.y));
   m = mul2(v, inv);
 }
 
@@ -89,47 +119,68 @@ __device__ __forceinline__ void then(Run& first, const Run& next) {   // first, 
   first.P = mul2(next.P, first.P);
 }
 
-// ------------------------------------------------------------------ staging
-// A warp's rows of NA arrays, kGatedSteps steps of kGatedTile channels each, as
-// they lie in memory.  Each warp copies and reads its own rows only.
-template <typename T, int NA>
-struct Stage {
-  static constexpr int kRow = kGatedTile * (int)sizeof(T);         // bytes
-  static constexpr int kBytes = NA * kGatedSteps * kRow;           // per warp
-  const T* src[NA]; long long ld[NA];
+// ------------------------------------------------------------------ layout
+// LC lanes hold a run of TS steps, two channels each; a warp holds 32 / LC
+// consecutive runs of a tile of 2 LC channels.
+template <int LC, int TS> struct Lanes {
+  static constexpr int kSub = 32 / LC, kTile = 2 * LC, kSteps = TS * kSub;
+};
 
-  // rows t0 .. of row `base` (b L), those below `n`; channels c0 .. below D
-  __device__ __forceinline__ void issue(char* buf, long long base, int t0, int n, int c0, int D,
-                                        bool vec) const {
+// A warp's rows of NA arrays: kSteps steps of a tile, row (i, sub) (step i of run
+// sub) at i * kSub + sub, so that lanes read neighbouring words.  Each warp copies
+// and reads its own rows only; rows past the length and channels past D are not
+// copied, and what lies there is not used.
+template <typename T, int NA, int LC, int TS>
+struct Stage {
+  using La = Lanes<LC, TS>;
+  static constexpr int kRow = La::kTile * (int)sizeof(T);          // bytes
+  static constexpr int kArray = La::kSteps * kRow;
+  static constexpr int kBytes = NA * kArray;                       // per warp
+  static constexpr int V = 16 / (int)sizeof(T), PR = La::kTile / V, RI = 32 / PR;
+  const T* p[NA];                    // of step t0 of the row: this lane's first piece
+
+  // rows t0 .. below n; channels c0 .. below D
+  __device__ __forceinline__ void issue(char* buf, const long long (&ld)[NA], int t0, int n,
+                                        int c0, int D, bool vec) const {
     const int lane = threadIdx.x;
     if (vec) {
-      constexpr int V = 16 / (int)sizeof(T), PR = kGatedTile / V;
+      const int row = lane / PR, c = lane % PR * V;
+      if (c0 + c < D) {
 #pragma unroll
-      for (int k = 0; k < NA; ++k)
+        for (int i = 0; i < La::kSteps / RI; ++i) {
+          const int rr = i * RI + row;
+          if (t0 + rr < n) {
+            const int at = (rr % TS * La::kSub + rr / TS) * kRow + c * (int)sizeof(T);
+            const unsigned s = (unsigned)__cvta_generic_to_shared(buf) + at;
 #pragma unroll
-        for (int i = 0; i < kGatedSteps * PR / 32; ++i) {
-          const int at = i * 32 + lane, t = t0 + at / PR, c = c0 + at % PR * V;
-          const bool ok = t < n && c < D;
-          const T* g = src[k] + (ok ? (size_t)(base + t) * ld[k] + c : 0);
-          const unsigned s = (unsigned)__cvta_generic_to_shared(buf + k * kGatedSteps * kRow +
-                                                                at * 16);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(g),
-                       "r"(ok ? 16 : 0)
-                       : "memory");
+            for (int k = 0; k < NA; ++k)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s + k * kArray),
+                           "l"(p[k] + (long long)(i * RI) * ld[k])
+                           : "memory");
+          }
         }
+      }
       asm volatile("cp.async.commit_group;" ::: "memory");
     } else {
-      const int c = c0 + 2 * lane;
+      const int sub = lane / LC, c = c0 + lane % LC * 2;
 #pragma unroll
       for (int k = 0; k < NA; ++k)
-        for (int i = 0; i < kGatedSteps; ++i) {
-          const bool ok = t0 + i < n;
-          const T* g = src[k] + (ok ? (size_t)(base + t0 + i) * ld[k] + c : 0);
-          T* s = reinterpret_cast<T*>(buf + (k * kGatedSteps + i) * kRow) + 2 * lane;
-          s[0] = ok && c < D ? g[0] : T(0.f);
-          s[1] = ok && c + 1 < D ? g[1] : T(0.f);
-        }
+        for (int i = 0; i < TS; ++i)
+          if (t0 + sub * TS + i < n) {
+            const T* g = p[k] + (long long)(sub * TS + i) * ld[k];
+            T* s = reinterpret_cast<T*>(buf + k * kArray + (i * La::kSub + sub) * kRow) +
+                   lane % LC * 2;
+            if (c < D) s[0] = g[0];
+            if (c + 1 < D) s[1] = g[1];
+          }
     }
+  }
+  // p[k] for the row that starts at `row` (b L + t0)
+  __device__ __forceinline__ void at(int k, const void* base, long long row, long long ld, int c0,
+                                     bool vec) {
+    const int lane = threadIdx.x;
+    p[k] = static_cast<const T*>(base) + (row + (vec ? lane / PR : 0)) * ld + c0 +
+           (vec ? lane % PR * V : lane % LC * 2);
   }
   static __device__ __forceinline__ void wait() {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -137,8 +188,8 @@ struct Stage {
   }
   // the lane's pair of step i of array k
   static __device__ __forceinline__ float2 get(const char* buf, int k, int i) {
-    const Pack<T, 2> v = ld_pack<T, 2>(reinterpret_cast<const T*>(buf + (k * kGatedSteps + i) * kRow) +
-                                       2 * threadIdx.x);
+    const Pack<T, 2> v = ld_pack<T, 2>(
+        reinterpret_cast<const T*>(buf + k * kArray + i * La::kSub * kRow) + 2 * threadIdx.x);
     return make_float2(v.get(0), v.get(1));
   }
 };
@@ -164,53 +215,98 @@ __device__ __forceinline__ float2 load_pair(const float* p, int left) {
 }
 
 // ------------------------------------------------------------------ joins
-// The CTA's warps and, for S > 1, the cluster's CTAs hold consecutive runs of
-// steps (`order`: this warp's place in the CTA's order, `rank` this CTA's in the
-// cluster's).  Every thread folds the runs ahead of its own onto the value
-// `carry` before the first, and carry moves behind the last.  Two buffers in turn:
-// one CTA barrier (and one cluster barrier) per call.
+// A warp's runs, the CTA's warps and, for S > 1, the cluster's CTAs hold
+// consecutive steps, forwards (DIR 1) or backwards (-1): w and rank are this warp's
+// and CTA's places in that order.  A warp folds the runs ahead of its own onto the
+// value before the first; the last warp passes the value behind all of them on to
+// the next call.  Two buffers in turn: one CTA barrier (and one cluster barrier) per
+// call.
+template <int LC>
 struct Joint {
-  float4 warp[2][8][32];
-  float4 cta[2][8][32];
+  float4 warp[2][kGatedWarps][LC];
+  float4 cta[2][8][LC];
+  float2 carry[2][LC];
 };
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
 }
+__device__ __forceinline__ float2 shfl2(float2 v, int from) {
+  return make_float2(__shfl_sync(0xffffffffu, v.x, from & 31),
+                     __shfl_sync(0xffffffffu, v.y, from & 31));
+}
+__device__ __forceinline__ Run as_run(const float4& v) {
+  return Run{make_float2(v.x, v.y), make_float2(v.z, v.w)};
+}
 
-__device__ __forceinline__ float2 join(Joint& j, int flip, const Run& mine, int order, int warps,
-                                       int rank, int S, float2& carry) {
-  const int lane = threadIdx.x;
-  j.warp[flip][order][lane] = make_float4(mine.P.x, mine.P.y, mine.V.x, mine.V.y);
-  __syncthreads();
-  Run all{f2(1.f), f2(0.f)}, ahead = all;
-  for (int w = 0; w < warps; ++w) {
-    if (w == order) ahead = all;
-    const float4 v = j.warp[flip][w][lane];
-    then(all, Run{make_float2(v.x, v.y), make_float2(v.z, v.w)});
+// The value in front of this run.  first: `carry` is the value in front of all, else
+// the last call's.  On return carry is the value behind all, in the last warp's last
+// run's lanes.
+template <int LC, int DIR>
+__device__ __forceinline__ float2 join(Joint<LC>& j, int flip, const Run& mine, int w, int warps,
+                                       int rank, int S, bool first, float2& carry) {
+  constexpr int kSub = 32 / LC;
+  const int lane = threadIdx.x, cl = lane % LC;
+  const int sub = DIR > 0 ? lane / LC : kSub - 1 - lane / LC;     // this run's place in the warp
+  Run upto = mine, ahead{f2(1.f), f2(0.f)};                       // through this run; ahead of it
+  if (kSub > 1) {
+#pragma unroll
+    for (int s = 1; s < kSub; s *= 2) {
+      Run f{shfl2(upto.P, lane - DIR * s * LC), shfl2(upto.V, lane - DIR * s * LC)};
+      if (sub >= s) {
+        then(f, upto);
+        upto = f;
+      }
+    }
+    const Run f{shfl2(upto.P, lane - DIR * LC), shfl2(upto.V, lane - DIR * LC)};
+    if (sub > 0) ahead = f;
   }
-  float2 start = carry;
-  if (S > 1) {
-    for (int peer = threadIdx.y; peer < S; peer += warps) {
-      unsigned a = (unsigned)__cvta_generic_to_shared(&j.cta[flip][rank][lane]), to;
+  if (sub == kSub - 1)
+    j.warp[flip][w][cl] = make_float4(upto.P.x, upto.P.y, upto.V.x, upto.V.y);
+  __syncthreads();
+  float2 c = first ? carry : j.carry[flip][cl];
+  if (S == 1) {
+    for (int k = 0; k < w; ++k) {
+      const Run f = as_run(j.warp[flip][k][cl]);
+      c = fma2(f.P, c, f.V);
+    }
+    if (w == warps - 1) {
+      carry = fma2(upto.P, c, upto.V);
+      if (sub == kSub - 1) j.carry[flip ^ 1][cl] = carry;
+    }
+    return kSub > 1 ? fma2(ahead.P, c, ahead.V) : c;
+  }
+  Run before{f2(1.f), f2(0.f)};
+  for (int k = 0; k < w; ++k) then(before, as_run(j.warp[flip][k][cl]));
+  if (w == warps - 1 && sub == kSub - 1) {
+    Run all = before;
+    then(all, upto);
+    for (int peer = 0; peer < S; ++peer) {
+      const unsigned a = (unsigned)__cvta_generic_to_shared(&j.cta[flip][rank][cl]);
+      unsigned to;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(a), "r"(peer));
       asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(all.P.x),
                    "f"(all.P.y), "f"(all.V.x), "f"(all.V.y)
                    : "memory");
     }
-    cluster_sync();
-    float2 c = carry;
-    for (int k = 0; k < S; ++k) {
-      if (k == rank) start = c;
-      const float4 v = j.cta[flip][k][lane];
-      c = fma2(make_float2(v.x, v.y), c, make_float2(v.z, v.w));
-    }
-    carry = c;
-  } else {
-    carry = fma2(all.P, carry, all.V);
   }
-  return fma2(ahead.P, start, ahead.V);
+  __syncwarp();
+  cluster_sync();
+  for (int k = 0; k < rank; ++k) {
+    const Run f = as_run(j.cta[flip][k][cl]);
+    c = fma2(f.P, c, f.V);
+  }
+  if (w == warps - 1) {
+    carry = c;
+    for (int k = rank; k < S; ++k) {
+      const Run f = as_run(j.cta[flip][k][cl]);
+      carry = fma2(f.P, carry, f.V);
+    }
+    if (sub == kSub - 1) j.carry[flip ^ 1][cl] = carry;
+  }
+  c = fma2(before.P, c, before.V);
+  return kSub > 1 ? fma2(ahead.P, c, ahead.V) : c;
 }
 
 }  // namespace m3

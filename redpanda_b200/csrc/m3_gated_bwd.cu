@@ -16,6 +16,8 @@
 // per channel, and a second launch adds them in a fixed order.
 #include "m3_gated.cuh"
 
+#include <type_traits>
+
 #include "m3_api_util.h"
 #include "m3_ops.h"
 #include "m3_pdl.cuh"
@@ -29,104 +31,142 @@ __device__ __forceinline__ int row_length(const int* lengths, int b, int L) {
   return n < 0 ? 0 : n > L ? L : n;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256, 2) gated_bwd_kernel(const GatedBwdParams q) {
+template <typename T, int LC, int TS>
+__global__ void __launch_bounds__(32 * kGatedWarps, M3_GB)
+    gated_bwd_kernel(const GatedBwdParams q) {
   extern __shared__ __align__(16) char smem[];
-  __shared__ Joint joint;
-  constexpr int TS = kGatedSteps;
-  using St = Stage<T, 4>;
+  __shared__ Joint<LC> joint;
+  static_assert(TS == kGatedCkpt, "a run starts at a checkpoint");
+  using St = Stage<T, 4, LC, TS>;
+  using La = Lanes<LC, TS>;
   const GatedParams& p = q.f;
-  const int lane = threadIdx.x, w = threadIdx.y, W = blockDim.y, S = p.splits;
-  const int rank = blockIdx.x % S, c0 = blockIdx.x / S * kGatedTile, c = c0 + 2 * lane;
-  const int left = p.D - c, D = p.D, L = p.L, span = S * W * TS;
-  const int at0 = (rank * W + w) * TS;
+  const int lane = threadIdx.x, w = __shfl_sync(0xffffffffu, threadIdx.y, 0), W = blockDim.y;
+  const int S = p.splits, rank = blockIdx.x % S;
+  const int c0 = blockIdx.x / S * La::kTile, c = c0 + lane % LC * 2;
+  const int left = p.D - c, D = p.D, L = p.L, span = S * W * La::kSteps;
+  const int tw0 = (rank * W + w) * La::kSteps, own = lane / LC * TS;   // of the warp; of the run
   const bool vec = p.vec != 0;
+  const long long ld[4] = {p.ld_x, p.ld_r, p.ld_i, D};
   char* buf = smem + w * St::kBytes;
-  St st{{static_cast<const T*>(p.x), static_cast<const T*>(p.rg), static_cast<const T*>(p.ig),
-         static_cast<const T*>(q.g)},
-        {p.ld_x, p.ld_r, p.ld_i, D}};
+  St st;
   const float2 dec = load_pair(p.decay + c, left);
   const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
+  const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
   float2 sum = f2(0.f);
   int flip = 0;
   if (S > 1) cluster_sync();                         // every CTA runs before its memory is written
-  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
-    const int n = row_length(p.lengths, b, L);
+  // the copies of a row's first pass, its last steps, start while the row before it
+  // is finished
+  auto start = [&](int b, int n) {
+    const int tw = (n - 1) / span * span + tw0;
+    const long long row = (long long)b * L + tw;
+    st.at(0, p.x, row, ld[0], c0, vec);
+    st.at(1, p.rg, row, ld[1], c0, vec);
+    st.at(2, p.ig, row, ld[2], c0, vec);
+    st.at(3, q.g, row, ld[3], c0, vec);
+    st.issue(buf, ld, tw, n, c0, D, vec);
+  };
+  int n = row_length(p.lengths, blockIdx.y, L), n2;
+  if (n > 0) start(blockIdx.y, n);
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y, n = n2) {
+    const int nb = b + gridDim.y;
+    n2 = nb < p.B ? row_length(p.lengths, nb, L) : 0;
+    if (n == 0 && n2 > 0) start(nb, n2);
     const long long base = (long long)b * L;
-    T* dx = static_cast<T*>(q.dx) + (size_t)base * D + c;
-    T* dr = static_cast<T*>(q.drg) + (size_t)base * D + c;
-    T* di = static_cast<T*>(q.dig) + (size_t)base * D + c;
     const int passes = (n + span - 1) / span;
     // steps of passes that are wholly past the length
-    for (int t0 = passes * span + at0; t0 < L; t0 += span)
+    for (int t0 = passes * span + tw0 + own; t0 - tw0 - own < L; t0 += span)
       for (int i = 0; i < TS && t0 + i < L; ++i) {
-        store_pair(dx + (size_t)(t0 + i) * D, f2(0.f), left, vec);
-        store_pair(dr + (size_t)(t0 + i) * D, f2(0.f), left, vec);
-        store_pair(di + (size_t)(t0 + i) * D, f2(0.f), left, vec);
+        const size_t at = (size_t)(base + t0 + i) * D + c;
+        store_pair(static_cast<T*>(q.dx) + at, f2(0.f), left, vec);
+        store_pair(static_cast<T*>(q.drg) + at, f2(0.f), left, vec);
+        store_pair(static_cast<T*>(q.dig) + at, f2(0.f), left, vec);
       }
     float2 carry = f2(0.f);                          // a_{t+1} q_{t+1}
-    int t0 = (passes - 1) * span + at0;
-    if (passes > 0) st.issue(buf, base, t0, n, c0, D, vec);
-    for (int k0 = passes; k0 > 0; --k0, t0 -= span) {
-      float2 a[TS], X[TS], I[TS], A[TS], R[TS], g[TS];
-      float2 h = f2(0.f);
-      if (t0 < n) h = load_pair(p.ckpt + ((size_t)b * ((L + TS - 1) / TS) + t0 / TS) * D + c, left);
+    int tw = (passes - 1) * span + tw0;
+    size_t at = (size_t)(base + tw + own) * D + c;
+    const float* ck = p.ckpt + ((size_t)b * ((L + TS - 1) / TS) + (tw + own) / TS) * D + c;
+    float2 h = tw + own < n ? load_pair(ck, left) : f2(0.f);
+    for (int k0 = passes; k0 > 0; --k0, tw -= span) {
+      const int t0 = tw + own;
       St::wait();
+      // FAST: every step of the warp is one of the sequence, and no decay is far from 1
+      auto pass = [&](auto fast) {
+        constexpr bool FAST = decltype(fast)::value;
+        float2 a[TS], X[TS], I[TS], A[TS], R[TS], g[TS];
 #pragma unroll
-      for (int i = 0; i < TS; ++i) {
-        const float2 x = St::get(buf, 0, i), r = sigmoid2(St::get(buf, 1, i)),
-                     u = sigmoid2(St::get(buf, 2, i));
-        g[i] = St::get(buf, 3, i);
-        const float2 l = mul2(k, r);
-        float2 m, inv;
-        decay2(l, a[i], m);
-        root2(m, m, inv);
-        const float2 ah = mul2(a[i], h), ux = mul2(u, x);
-        X[i] = mul2(m, u);
-        h = fma2(m, ux, ah);
-        const float2 am = mul2(mul2(a[i], a[i]), inv);
-        A[i] = mul2(l, fma2(mul2(am, f2(-1.f)), ux, ah));
-        R[i] = fma2(r, f2(-1.f), f2(1.f));
-        I[i] = mul2(mul2(X[i], x), fma2(u, f2(-1.f), f2(1.f)));
-        if (t0 + i >= n) {                           // the state stays, nothing has a gradient
-          a[i] = f2(1.f);
-          g[i] = X[i] = I[i] = A[i] = f2(0.f);
+        for (int i = 0; i < TS; ++i) {
+          const float2 x = St::get(buf, 0, i), r = sigmoid2(St::get(buf, 1, i)),
+                       u = sigmoid2(St::get(buf, 2, i));
+          g[i] = St::get(buf, 3, i);
+          const float2 l = mul2(k, r);
+          float2 m, inv;
+          decay2<FAST>(l, a[i], m);
+          root2(m, m, inv);
+          const float2 ah = mul2(a[i], h), ux = mul2(u, x);
+          X[i] = mul2(m, u);
+          h = fma2(m, ux, ah);
+          const float2 am = mul2(mul2(a[i], a[i]), inv);
+          A[i] = mul2(l, fma2(mul2(am, f2(-1.f)), ux, ah));
+          R[i] = fma2(r, f2(-1.f), f2(1.f));
+          I[i] = mul2(mul2(X[i], x), fma2(u, f2(-1.f), f2(1.f)));
+          if (!FAST && t0 + i >= n) {                // the state stays, nothing has a gradient
+            a[i] = f2(1.f);
+            g[i] = X[i] = I[i] = A[i] = R[i] = f2(0.f);
+          }
         }
-      }
-      Run run{f2(1.f), f2(0.f)};                     // v = a (g + v), from the last step
+        Run run{f2(1.f), f2(0.f)};                   // v = a (g + v), from the last step
 #pragma unroll
-      for (int i = TS - 1; i >= 0; --i) {
-        run.V = mul2(a[i], add2(g[i], run.V));
-        run.P = mul2(a[i], run.P);
-      }
-      __syncwarp();
-      if (k0 > 1) st.issue(buf, base, t0 - span, n, c0, D, vec);
-      float2 v = join(joint, flip, run, W - 1 - w, W, S - 1 - rank, S, carry);
+        for (int i = TS - 1; i >= 0; --i) {
+          run.V = mul2(a[i], add2(g[i], run.V));
+          run.P = mul2(a[i], run.P);
+        }
+        __syncwarp();
+        if (k0 > 1) {
+#pragma unroll
+          for (int z = 0; z < 4; ++z) st.p[z] -= (long long)span * ld[z];
+          st.issue(buf, ld, tw - span, n, c0, D, vec);
+          ck -= (size_t)(span / TS) * D;
+          h = load_pair(ck, left);                   // every pass but the last is full
+        } else if (n2 > 0) {
+          start(nb, n2);
+        }
+        float2 v = join<LC, -1>(joint, flip, run, W - 1 - w, W, S - 1 - rank, S, k0 == passes,
+                                carry);
+        float2 part = f2(0.f);
+#pragma unroll
+        for (int i = TS - 1; i >= 0; --i) {
+          const float2 qt = add2(g[i], v), e = mul2(qt, A[i]);
+          v = mul2(a[i], qt);
+          part = add2(part, e);
+          if (FAST || t0 + i < L) {
+            const size_t o = at + (size_t)i * D;
+            store_pair(static_cast<T*>(q.dx) + o, mul2(qt, X[i]), left, vec);
+            store_pair(static_cast<T*>(q.drg) + o, mul2(e, R[i]), left, vec);
+            store_pair(static_cast<T*>(q.dig) + o, mul2(qt, I[i]), left, vec);
+          }
+        }
+        sum = add2(sum, part);
+      };
+      if (near && tw + La::kSteps <= n) pass(std::true_type());
+      else pass(std::false_type());
       flip ^= 1;
-      float2 part = f2(0.f);
-#pragma unroll
-      for (int i = TS - 1; i >= 0; --i) {
-        const float2 qt = add2(g[i], v), e = mul2(qt, A[i]);
-        v = mul2(a[i], qt);
-        part = add2(part, e);
-        if (t0 + i < L) {
-          store_pair(dx + (size_t)(t0 + i) * D, mul2(qt, X[i]), left, vec);
-          store_pair(dr + (size_t)(t0 + i) * D, mul2(e, R[i]), left, vec);
-          store_pair(di + (size_t)(t0 + i) * D, mul2(qt, I[i]), left, vec);
-        }
-      }
-      sum = add2(sum, part);
+      at -= (size_t)span * D;
     }
   }
   pdl_launch_dependents();
-  // the CTA's partial: warps in order
+  // the CTA's partial: the runs of a warp, then the warps, in order
+#pragma unroll
+  for (int s = LC; s < 32; s *= 2)
+    sum = add2(sum, make_float2(__shfl_xor_sync(0xffffffffu, sum.x, s),
+                                __shfl_xor_sync(0xffffffffu, sum.y, s)));
   __syncthreads();
   float2* s = reinterpret_cast<float2*>(&joint);
-  s[w * 32 + lane] = sum;
+  if (lane < LC) s[w * LC + lane] = sum;
   __syncthreads();
-  if (w == 0) {
+  if (w == 0 && lane < LC) {
     float2 v = s[lane];
-    for (int i = 1; i < W; ++i) v = add2(v, s[i * 32 + lane]);
+    for (int i = 1; i < W; ++i) v = add2(v, s[i * LC + lane]);
     store_pair(q.part + ((size_t)blockIdx.y * S + rank) * D + c, v, left, false);
   }
 }
@@ -155,32 +195,39 @@ __global__ void __launch_bounds__(1024) gated_reduce_kernel(const float* part, i
   }
 }
 
-template <typename T>
+template <typename T, int LC>
 cudaError_t bwd_impl(const GatedBwdParams& q, cudaStream_t s) {
+  constexpr int TS = kGatedBwdSteps, kBytes = Stage<T, 4, LC, TS>::kBytes, kTile = 2 * LC;
   const GatedParams& p = q.f;
-  const cudaError_t e = allow_smem<gated_bwd_kernel<T>>(8 * Stage<T, 4>::kBytes);
+  const cudaError_t e = allow_smem<gated_bwd_kernel<T, LC, TS>>(kGatedWarps * kBytes);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.D + kGatedTile - 1) / kGatedTile * p.splits), p.rows);
+  cfg.gridDim = dim3((unsigned)((p.D + kTile - 1) / kTile * p.splits), p.rows);
   cfg.blockDim = dim3(32, p.warps);
-  cfg.dynamicSmemBytes = p.warps * Stage<T, 4>::kBytes;
+  cfg.dynamicSmemBytes = p.warps * kBytes;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = p.splits > 1 ? 1 : 0;
-  const cudaError_t r = cudaLaunchKernelEx(&cfg, gated_bwd_kernel<T>, q);
+  const cudaError_t r = cudaLaunchKernelEx(&cfg, gated_bwd_kernel<T, LC, TS>, q);
   if (r != cudaSuccess) return r;
   return launch_maybe_pdl(true, gated_reduce_kernel, dim3((p.D + 31) / 32), dim3(1024), 0, s,
                           (const float*)q.part, p.rows * p.splits, p.D, p.decay, q.ddecay);
 }
 
+template <typename T>
+cudaError_t bwd_lanes(const GatedBwdParams& q, cudaStream_t s) {
+  if (q.f.lanes == 32) return bwd_impl<T, 32>(q, s);
+  return q.f.lanes == 16 ? bwd_impl<T, 16>(q, s) : bwd_impl<T, 8>(q, s);
+}
+
 }  // namespace
 
 cudaError_t launch_gated_bwd(const GatedBwdParams& q, cudaStream_t s) {
-  return q.f.dtype == M3_BF16 ? bwd_impl<__nv_bfloat16>(q, s) : bwd_impl<float>(q, s);
+  return q.f.dtype == M3_BF16 ? bwd_lanes<__nv_bfloat16>(q, s) : bwd_lanes<float>(q, s);
 }
 
 }  // namespace m3

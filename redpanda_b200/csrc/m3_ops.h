@@ -221,7 +221,7 @@ struct GatedParams {
   float* ckpt;                                           // (B, segments, D) or nullptr
   int B, L, D;
   int dtype;
-  int warps, splits, rows;                               // gated_plan: per CTA, per cluster, grid
+  int lanes, warps, splits, rows;                        // per run, per CTA, per cluster; grid
   int vec;                                               // 16-byte loads, vector stores
 };
 struct GatedBwdParams {
@@ -232,9 +232,8 @@ struct GatedBwdParams {
   float* part;                                           // (rows * splits, D)
 };
 int gated_segments(int L);                               // checkpoints per row and channel
-// warps per CTA, CTAs along time and along the batch
-void gated_plan(int B, int L, int D, int dtype, bool backward, int sms, int* warps, int* splits,
-                int* rows);
+// sets lanes, warps, splits and rows
+void gated_plan(int B, int L, int D, bool backward, int sms, GatedParams* p);
 cudaError_t launch_gated_fwd(const GatedParams& p, cudaStream_t s);
 cudaError_t launch_gated_bwd(const GatedBwdParams& p, cudaStream_t s);
 

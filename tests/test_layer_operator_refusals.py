@@ -269,4 +269,4 @@ def test_c_entries_validate_before_device_work():
 def test_checkpoint_floats():
     f = lambda B, L, D: _lib.load().m3_gated_ckpt_floats(  # noqa: E731
         _lib.GatedDesc(B, L, D, 0, 8.0))
-    assert f(2, 1, 8) == 16 and f(2, 8, 8) == 16 and f(2, 9, 8) == 32 and f(1, 0, 8) == 0
+    assert f(2, 1, 8) == 16 and f(2, 4, 8) == 16 and f(2, 9, 8) == 48 and f(1, 0, 8) == 0
