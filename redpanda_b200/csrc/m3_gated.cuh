@@ -25,30 +25,12 @@
 namespace m3 {
 
 constexpr int kGatedCkpt = 4;         // steps between the backward's checkpoints
-#ifndef M3_W
-#define M3_W 8
-#endif
-#ifndef M3_TF
-#define M3_TF 8
-#endif
-#ifndef M3_TB
-#define M3_TB 4
-#endif
-#ifndef M3_GB
-#define M3_GB 2
-#endif
-constexpr int kGatedFwdSteps = M3_TF, kGatedBwdSteps = M3_TB;   // of a thread at a time
-constexpr int kGatedWarps = M3_W;        // of a CTA, at most
+constexpr int kGatedFwdSteps = 8, kGatedBwdSteps = 4;   // of a thread at a time
+constexpr int kGatedWarps = 8;                          // of a CTA, at most
 
-#ifdef M3_SCALAR
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
-#else
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-#endif
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN stays NaN
   float y;
@@ -130,7 +112,7 @@ template <int LC, int TS> struct Lanes {
 // sub) at i * kSub + sub, so that lanes read neighbouring words.  Each warp copies
 // and reads its own rows only; rows past the length and channels past D are not
 // copied, and what lies there is not used.
-template <typename T, int NA, int LC, int TS>
+template <typename T, int NA, int LC, int TS, bool VEC>
 struct Stage {
   using La = Lanes<LC, TS>;
   static constexpr int kRow = La::kTile * (int)sizeof(T);          // bytes
@@ -141,9 +123,9 @@ struct Stage {
 
   // rows t0 .. below n; channels c0 .. below D
   __device__ __forceinline__ void issue(char* buf, const long long (&ld)[NA], int t0, int n,
-                                        int c0, int D, bool vec) const {
+                                        int c0, int D) const {
     const int lane = threadIdx.x;
-    if (vec) {
+    if constexpr (VEC) {
       const int row = lane / PR, c = lane % PR * V;
       if (c0 + c < D) {
 #pragma unroll
@@ -176,14 +158,15 @@ struct Stage {
     }
   }
   // p[k] for the row that starts at `row` (b L + t0)
-  __device__ __forceinline__ void at(int k, const void* base, long long row, long long ld, int c0,
-                                     bool vec) {
+  __device__ __forceinline__ void at(int k, const void* base, long long row, long long ld, int c0) {
     const int lane = threadIdx.x;
-    p[k] = static_cast<const T*>(base) + (row + (vec ? lane / PR : 0)) * ld + c0 +
-           (vec ? lane % PR * V : lane % LC * 2);
+    p[k] = static_cast<const T*>(base) + (row + (VEC ? lane / PR : 0)) * ld + c0 +
+           (VEC ? lane % PR * V : lane % LC * 2);
   }
+  // all but the last LEFT calls of issue are complete
+  template <int LEFT = 0>
   static __device__ __forceinline__ void wait() {
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
     __syncwarp();
   }
   // the lane's pair of step i of array k
@@ -196,14 +179,12 @@ struct Stage {
 
 // A lane's pair of channels in a (.., D) array, element by element where a pair
 // may be cut or is not aligned.
-template <typename T>
-__device__ __forceinline__ void store_pair(T* p, float2 v, int left, bool vec) {
-  if (vec) {
+template <bool VEC, typename T>
+__device__ __forceinline__ void store_pair(T* p, float2 v, int left) {
+  if constexpr (VEC) {
     if (left > 0) {
-      Pack<T, 2> o;
-      o.put(0, v.x);
-      o.put(1, v.y);
-      st_pack<T, 2>(p, o);
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v);
+      else *reinterpret_cast<float2*>(p) = v;
     }
   } else {
     if (left > 0) p[0] = Elem<T>::put(v.x);
@@ -223,10 +204,26 @@ __device__ __forceinline__ float2 load_pair(const float* p, int left) {
 // call.
 template <int LC>
 struct Joint {
-  float4 warp[2][kGatedWarps][LC];
-  float4 cta[2][8][LC];
-  float2 carry[2][LC];
+  float4* warp;      // (2, warps, LC)
+  float4* cta;       // (2, S, LC), for S > 1
+  float2* carry;     // (2, LC)
+  int warps, S;
+  // in shared memory behind the warps' stages
+  __device__ __forceinline__ Joint(char* at, int warps, int S) : warps(warps), S(S) {
+    warp = reinterpret_cast<float4*>(at);
+    cta = warp + 2 * warps * LC;
+    carry = reinterpret_cast<float2*>(cta + (S > 1 ? 2 * S * LC : 0));
+  }
+  __device__ __forceinline__ float4& run(int flip, int k, int cl) const {
+    return warp[(flip * warps + k) * LC + cl];
+  }
+  __device__ __forceinline__ float4& part(int flip, int k, int cl) const {
+    return cta[(flip * S + k) * LC + cl];
+  }
 };
+inline int joint_bytes(int lanes, int warps, int S) {
+  return lanes * (32 * warps + (S > 1 ? 32 * S : 0) + 16);
+}
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
@@ -244,8 +241,9 @@ __device__ __forceinline__ Run as_run(const float4& v) {
 // the last call's.  On return carry is the value behind all, in the last warp's last
 // run's lanes.
 template <int LC, int DIR>
-__device__ __forceinline__ float2 join(Joint<LC>& j, int flip, const Run& mine, int w, int warps,
-                                       int rank, int S, bool first, float2& carry) {
+__device__ __forceinline__ float2 join(const Joint<LC>& j, int flip, const Run& mine, int w, int rank,
+                                       bool first, float2& carry) {
+  const int warps = j.warps, S = j.S;
   constexpr int kSub = 32 / LC;
   const int lane = threadIdx.x, cl = lane % LC;
   const int sub = DIR > 0 ? lane / LC : kSub - 1 - lane / LC;     // this run's place in the warp
@@ -263,27 +261,27 @@ __device__ __forceinline__ float2 join(Joint<LC>& j, int flip, const Run& mine, 
     if (sub > 0) ahead = f;
   }
   if (sub == kSub - 1)
-    j.warp[flip][w][cl] = make_float4(upto.P.x, upto.P.y, upto.V.x, upto.V.y);
+    j.run(flip, w, cl) = make_float4(upto.P.x, upto.P.y, upto.V.x, upto.V.y);
   __syncthreads();
-  float2 c = first ? carry : j.carry[flip][cl];
+  float2 c = first ? carry : j.carry[flip * LC + cl];
   if (S == 1) {
     for (int k = 0; k < w; ++k) {
-      const Run f = as_run(j.warp[flip][k][cl]);
+      const Run f = as_run(j.run(flip, k, cl));
       c = fma2(f.P, c, f.V);
     }
     if (w == warps - 1) {
       carry = fma2(upto.P, c, upto.V);
-      if (sub == kSub - 1) j.carry[flip ^ 1][cl] = carry;
+      if (sub == kSub - 1) j.carry[(flip ^ 1) * LC + cl] = carry;
     }
     return kSub > 1 ? fma2(ahead.P, c, ahead.V) : c;
   }
   Run before{f2(1.f), f2(0.f)};
-  for (int k = 0; k < w; ++k) then(before, as_run(j.warp[flip][k][cl]));
+  for (int k = 0; k < w; ++k) then(before, as_run(j.run(flip, k, cl)));
   if (w == warps - 1 && sub == kSub - 1) {
     Run all = before;
     then(all, upto);
     for (int peer = 0; peer < S; ++peer) {
-      const unsigned a = (unsigned)__cvta_generic_to_shared(&j.cta[flip][rank][cl]);
+      const unsigned a = (unsigned)__cvta_generic_to_shared(&j.part(flip, rank, cl));
       unsigned to;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(a), "r"(peer));
       asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(all.P.x),
@@ -294,16 +292,16 @@ __device__ __forceinline__ float2 join(Joint<LC>& j, int flip, const Run& mine, 
   __syncwarp();
   cluster_sync();
   for (int k = 0; k < rank; ++k) {
-    const Run f = as_run(j.cta[flip][k][cl]);
+    const Run f = as_run(j.part(flip, k, cl));
     c = fma2(f.P, c, f.V);
   }
   if (w == warps - 1) {
     carry = c;
     for (int k = rank; k < S; ++k) {
-      const Run f = as_run(j.cta[flip][k][cl]);
+      const Run f = as_run(j.part(flip, k, cl));
       carry = fma2(f.P, carry, f.V);
     }
-    if (sub == kSub - 1) j.carry[flip ^ 1][cl] = carry;
+    if (sub == kSub - 1) j.carry[(flip ^ 1) * LC + cl] = carry;
   }
   c = fma2(before.P, c, before.V);
   return kSub > 1 ? fma2(ahead.P, c, ahead.V) : c;

@@ -31,13 +31,32 @@ __device__ __forceinline__ int row_length(const int* lengths, int b, int L) {
   return n < 0 ? 0 : n > L ? L : n;
 }
 
-template <typename T, int LC, int TS>
-__global__ void __launch_bounds__(32 * kGatedWarps, M3_GB)
+// What multiplies q in the gradients of a step, and the step of h
+struct Factors {
+  float2 a, X, I, A, R;
+};
+template <bool FAST>
+__device__ __forceinline__ Factors factors(float2 k, float2 x, float2 rg, float2 ig, float2& h) {
+  const float2 r = sigmoid2(rg), u = sigmoid2(ig), l = mul2(k, r);
+  float2 m, inv;
+  Factors f;
+  decay2<FAST>(l, f.a, m);
+  root2(m, m, inv);
+  const float2 ah = mul2(f.a, h), ux = mul2(u, x), am = mul2(mul2(f.a, f.a), inv);
+  f.X = mul2(m, u);
+  h = fma2(m, ux, ah);
+  f.A = mul2(l, fma2(mul2(am, f2(-1.f)), ux, ah));
+  f.R = fma2(r, f2(-1.f), f2(1.f));
+  f.I = mul2(mul2(f.X, x), fma2(u, f2(-1.f), f2(1.f)));
+  return f;
+}
+
+template <typename T, int LC, int TS, bool VEC>
+__global__ void __launch_bounds__(256, 2)
     gated_bwd_kernel(const GatedBwdParams q) {
   extern __shared__ __align__(16) char smem[];
-  __shared__ Joint<LC> joint;
   static_assert(TS == kGatedCkpt, "a run starts at a checkpoint");
-  using St = Stage<T, 4, LC, TS>;
+  using St = Stage<T, 4, LC, TS, VEC>;
   using La = Lanes<LC, TS>;
   const GatedParams& p = q.f;
   const int lane = threadIdx.x, w = __shfl_sync(0xffffffffu, threadIdx.y, 0), W = blockDim.y;
@@ -45,9 +64,9 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GB)
   const int c0 = blockIdx.x / S * La::kTile, c = c0 + lane % LC * 2;
   const int left = p.D - c, D = p.D, L = p.L, span = S * W * La::kSteps;
   const int tw0 = (rank * W + w) * La::kSteps, own = lane / LC * TS;   // of the warp; of the run
-  const bool vec = p.vec != 0;
   const long long ld[4] = {p.ld_x, p.ld_r, p.ld_i, D};
   char* buf = smem + w * St::kBytes;
+  const Joint<LC> joint(smem + W * St::kBytes, W, S);
   St st;
   const float2 dec = load_pair(p.decay + c, left);
   const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
@@ -60,11 +79,11 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GB)
   auto start = [&](int b, int n) {
     const int tw = (n - 1) / span * span + tw0;
     const long long row = (long long)b * L + tw;
-    st.at(0, p.x, row, ld[0], c0, vec);
-    st.at(1, p.rg, row, ld[1], c0, vec);
-    st.at(2, p.ig, row, ld[2], c0, vec);
-    st.at(3, q.g, row, ld[3], c0, vec);
-    st.issue(buf, ld, tw, n, c0, D, vec);
+    st.at(0, p.x, row, ld[0], c0);
+    st.at(1, p.rg, row, ld[1], c0);
+    st.at(2, p.ig, row, ld[2], c0);
+    st.at(3, q.g, row, ld[3], c0);
+    st.issue(buf, ld, tw, n, c0, D);
   };
   int n = row_length(p.lengths, blockIdx.y, L), n2;
   if (n > 0) start(blockIdx.y, n);
@@ -78,9 +97,9 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GB)
     for (int t0 = passes * span + tw0 + own; t0 - tw0 - own < L; t0 += span)
       for (int i = 0; i < TS && t0 + i < L; ++i) {
         const size_t at = (size_t)(base + t0 + i) * D + c;
-        store_pair(static_cast<T*>(q.dx) + at, f2(0.f), left, vec);
-        store_pair(static_cast<T*>(q.drg) + at, f2(0.f), left, vec);
-        store_pair(static_cast<T*>(q.dig) + at, f2(0.f), left, vec);
+        store_pair<VEC>(static_cast<T*>(q.dx) + at, f2(0.f), left);
+        store_pair<VEC>(static_cast<T*>(q.drg) + at, f2(0.f), left);
+        store_pair<VEC>(static_cast<T*>(q.dig) + at, f2(0.f), left);
       }
     float2 carry = f2(0.f);                          // a_{t+1} q_{t+1}
     int tw = (passes - 1) * span + tw0;
@@ -96,20 +115,10 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GB)
         float2 a[TS], X[TS], I[TS], A[TS], R[TS], g[TS];
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const float2 x = St::get(buf, 0, i), r = sigmoid2(St::get(buf, 1, i)),
-                       u = sigmoid2(St::get(buf, 2, i));
+          const Factors f = factors<FAST>(k, St::get(buf, 0, i), St::get(buf, 1, i),
+                                          St::get(buf, 2, i), h);
           g[i] = St::get(buf, 3, i);
-          const float2 l = mul2(k, r);
-          float2 m, inv;
-          decay2<FAST>(l, a[i], m);
-          root2(m, m, inv);
-          const float2 ah = mul2(a[i], h), ux = mul2(u, x);
-          X[i] = mul2(m, u);
-          h = fma2(m, ux, ah);
-          const float2 am = mul2(mul2(a[i], a[i]), inv);
-          A[i] = mul2(l, fma2(mul2(am, f2(-1.f)), ux, ah));
-          R[i] = fma2(r, f2(-1.f), f2(1.f));
-          I[i] = mul2(mul2(X[i], x), fma2(u, f2(-1.f), f2(1.f)));
+          a[i] = f.a, X[i] = f.X, I[i] = f.I, A[i] = f.A, R[i] = f.R;
           if (!FAST && t0 + i >= n) {                // the state stays, nothing has a gradient
             a[i] = f2(1.f);
             g[i] = X[i] = I[i] = A[i] = R[i] = f2(0.f);
@@ -125,14 +134,13 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GB)
         if (k0 > 1) {
 #pragma unroll
           for (int z = 0; z < 4; ++z) st.p[z] -= (long long)span * ld[z];
-          st.issue(buf, ld, tw - span, n, c0, D, vec);
+          st.issue(buf, ld, tw - span, n, c0, D);
           ck -= (size_t)(span / TS) * D;
           h = load_pair(ck, left);                   // every pass but the last is full
         } else if (n2 > 0) {
           start(nb, n2);
         }
-        float2 v = join<LC, -1>(joint, flip, run, W - 1 - w, W, S - 1 - rank, S, k0 == passes,
-                                carry);
+        float2 v = join<LC, -1>(joint, flip, run, W - 1 - w, S - 1 - rank, k0 == passes, carry);
         float2 part = f2(0.f);
 #pragma unroll
         for (int i = TS - 1; i >= 0; --i) {
@@ -141,9 +149,9 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GB)
           part = add2(part, e);
           if (FAST || t0 + i < L) {
             const size_t o = at + (size_t)i * D;
-            store_pair(static_cast<T*>(q.dx) + o, mul2(qt, X[i]), left, vec);
-            store_pair(static_cast<T*>(q.drg) + o, mul2(e, R[i]), left, vec);
-            store_pair(static_cast<T*>(q.dig) + o, mul2(qt, I[i]), left, vec);
+            store_pair<VEC>(static_cast<T*>(q.dx) + o, mul2(qt, X[i]), left);
+            store_pair<VEC>(static_cast<T*>(q.drg) + o, mul2(e, R[i]), left);
+            store_pair<VEC>(static_cast<T*>(q.dig) + o, mul2(qt, I[i]), left);
           }
         }
         sum = add2(sum, part);
@@ -161,13 +169,13 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GB)
     sum = add2(sum, make_float2(__shfl_xor_sync(0xffffffffu, sum.x, s),
                                 __shfl_xor_sync(0xffffffffu, sum.y, s)));
   __syncthreads();
-  float2* s = reinterpret_cast<float2*>(&joint);
+  float2* s = reinterpret_cast<float2*>(smem);
   if (lane < LC) s[w * LC + lane] = sum;
   __syncthreads();
   if (w == 0 && lane < LC) {
     float2 v = s[lane];
     for (int i = 1; i < W; ++i) v = add2(v, s[i * LC + lane]);
-    store_pair(q.part + ((size_t)blockIdx.y * S + rank) * D + c, v, left, false);
+    store_pair<false>(q.part + ((size_t)blockIdx.y * S + rank) * D + c, v, left);
   }
 }
 
@@ -195,11 +203,18 @@ __global__ void __launch_bounds__(1024) gated_reduce_kernel(const float* part, i
   }
 }
 
-template <typename T, int LC>
-cudaError_t bwd_impl(const GatedBwdParams& q, cudaStream_t s) {
-  constexpr int TS = kGatedBwdSteps, kBytes = Stage<T, 4, LC, TS>::kBytes, kTile = 2 * LC;
+cudaError_t reduce(const GatedBwdParams& q, cudaStream_t s) {
   const GatedParams& p = q.f;
-  const cudaError_t e = allow_smem<gated_bwd_kernel<T, LC, TS>>(kGatedWarps * kBytes);
+  return launch_maybe_pdl(true, gated_reduce_kernel, dim3((p.D + 31) / 32), dim3(1024), 0, s,
+                          (const float*)q.part, p.rows * p.splits, p.D, p.decay, q.ddecay);
+}
+
+template <typename T, int LC, bool VEC>
+cudaError_t bwd_impl(const GatedBwdParams& q, cudaStream_t s) {
+  constexpr int TS = kGatedBwdSteps, kBytes = Stage<T, 4, LC, TS, VEC>::kBytes, kTile = 2 * LC;
+  const GatedParams& p = q.f;
+  const cudaError_t e = allow_smem<gated_bwd_kernel<T, LC, TS, VEC>>(
+      kGatedWarps * kBytes + joint_bytes(LC, kGatedWarps, 8));
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -208,26 +223,26 @@ cudaError_t bwd_impl(const GatedBwdParams& q, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.D + kTile - 1) / kTile * p.splits), p.rows);
   cfg.blockDim = dim3(32, p.warps);
-  cfg.dynamicSmemBytes = p.warps * kBytes;
+  cfg.dynamicSmemBytes = p.warps * kBytes + joint_bytes(LC, p.warps, p.splits);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = p.splits > 1 ? 1 : 0;
-  const cudaError_t r = cudaLaunchKernelEx(&cfg, gated_bwd_kernel<T, LC, TS>, q);
-  if (r != cudaSuccess) return r;
-  return launch_maybe_pdl(true, gated_reduce_kernel, dim3((p.D + 31) / 32), dim3(1024), 0, s,
-                          (const float*)q.part, p.rows * p.splits, p.D, p.decay, q.ddecay);
+  const cudaError_t r = cudaLaunchKernelEx(&cfg, gated_bwd_kernel<T, LC, TS, VEC>, q);
+  return r != cudaSuccess ? r : reduce(q, s);
 }
 
-template <typename T>
+template <typename T, bool VEC>
 cudaError_t bwd_lanes(const GatedBwdParams& q, cudaStream_t s) {
-  if (q.f.lanes == 32) return bwd_impl<T, 32>(q, s);
-  return q.f.lanes == 16 ? bwd_impl<T, 16>(q, s) : bwd_impl<T, 8>(q, s);
+  if (q.f.lanes == 32) return bwd_impl<T, 32, VEC>(q, s);
+  return q.f.lanes == 16 ? bwd_impl<T, 16, VEC>(q, s) : bwd_impl<T, 8, VEC>(q, s);
 }
 
 }  // namespace
 
 cudaError_t launch_gated_bwd(const GatedBwdParams& q, cudaStream_t s) {
-  return q.f.dtype == M3_BF16 ? bwd_lanes<__nv_bfloat16>(q, s) : bwd_lanes<float>(q, s);
+  if (q.f.dtype == M3_BF16)
+    return q.f.vec ? bwd_lanes<__nv_bfloat16, true>(q, s) : bwd_lanes<__nv_bfloat16, false>(q, s);
+  return q.f.vec ? bwd_lanes<float, true>(q, s) : bwd_lanes<float, false>(q, s);
 }
 
 }  // namespace m3

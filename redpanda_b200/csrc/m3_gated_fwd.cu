@@ -14,15 +14,6 @@
 #include "m3_api_util.h"
 #include "m3_ops.h"
 
-#ifndef M3_GF
-#define M3_GF 3
-#endif
-#ifndef M3_GS
-#define M3_GS 8
-#endif
-#ifndef M3_GL
-#define M3_GL 8
-#endif
 namespace m3 {
 namespace {
 
@@ -32,20 +23,19 @@ __device__ __forceinline__ int row_length(const int* lengths, int b, int L) {
   return n < 0 ? 0 : n > L ? L : n;
 }
 
-template <typename T, int LC, int TS>
-__global__ void __launch_bounds__(32 * kGatedWarps, M3_GF) gated_fwd_kernel(const GatedParams p) {
+template <typename T, int LC, int TS, bool VEC>
+__global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) {
   extern __shared__ __align__(16) char smem[];
-  __shared__ Joint<LC> joint;
-  using St = Stage<T, 3, LC, TS>;
+  using St = Stage<T, 3, LC, TS, VEC>;
   using La = Lanes<LC, TS>;
   const int lane = threadIdx.x, w = __shfl_sync(0xffffffffu, threadIdx.y, 0), W = blockDim.y;
   const int S = p.splits, rank = blockIdx.x % S;
   const int c0 = blockIdx.x / S * La::kTile, c = c0 + lane % LC * 2;
   const int left = p.D - c, D = p.D, L = p.L, span = S * W * La::kSteps;
   const int tw0 = (rank * W + w) * La::kSteps, own = lane / LC * TS;   // of the warp; of the run
-  const bool vec = p.vec != 0;
   const long long ld[3] = {p.ld_x, p.ld_r, p.ld_i};
   char* buf = smem + w * St::kBytes;
+  const Joint<LC> joint(smem + W * St::kBytes, W, S);
   St st;
   const float2 dec = load_pair(p.decay + c, left);
   const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
@@ -55,10 +45,10 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GF) gated_fwd_kernel(cons
   // the copies of a row's first pass start while the row before it is finished
   auto start = [&](int b, int n) {
     const long long row = (long long)b * L + tw0;
-    st.at(0, p.x, row, ld[0], c0, vec);
-    st.at(1, p.rg, row, ld[1], c0, vec);
-    st.at(2, p.ig, row, ld[2], c0, vec);
-    st.issue(buf, ld, tw0, n, c0, D, vec);
+    st.at(0, p.x, row, ld[0], c0);
+    st.at(1, p.rg, row, ld[1], c0);
+    st.at(2, p.ig, row, ld[2], c0);
+    st.issue(buf, ld, tw0, n, c0, D);
   };
   int n = row_length(p.lengths, blockIdx.y, L), n2;
   if (n > 0) start(blockIdx.y, n);
@@ -69,7 +59,7 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GF) gated_fwd_kernel(cons
     if (n == 0) {
       if (n2 > 0) start(nb, n2);
       if (p.h_last != nullptr && rank == 0 && w == 0 && lane < LC)
-        store_pair(p.h_last + (size_t)b * D + c, carry, left, false);
+        store_pair<false>(p.h_last + (size_t)b * D + c, carry, left);
     }
     int tw = tw0;
     T* y = static_cast<T*>(p.y) + ((size_t)b * L + tw0 + own) * D + c;
@@ -103,18 +93,18 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GF) gated_fwd_kernel(cons
         if (s0 + span < n) {
 #pragma unroll
           for (int q = 0; q < 3; ++q) st.p[q] += (long long)span * ld[q];
-          st.issue(buf, ld, tw + span, n, c0, D, vec);
+          st.issue(buf, ld, tw + span, n, c0, D);
         } else if (n2 > 0) {
           start(nb, n2);
         }
-        float2 h = join<LC, 1>(joint, flip, run, w, W, rank, S, s0 == 0, carry);
+        float2 h = join<LC, 1>(joint, flip, run, w, rank, s0 == 0, carry);
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
           if (i % kGatedCkpt == 0 && ck != nullptr && (FAST || t0 + i < n))
-            store_pair(ck + (size_t)(i / kGatedCkpt) * D, h, left, D % 2 == 0);
+            store_pair<VEC>(ck + (size_t)(i / kGatedCkpt) * D, h, left);
           h = fma2(a[i], h, v[i]);
-          if (FAST) store_pair(y + (size_t)i * D, h, left, vec);
-          else if (t0 + i < L) store_pair(y + (size_t)i * D, t0 + i < n ? h : f2(0.f), left, vec);
+          if (FAST) store_pair<VEC>(y + (size_t)i * D, h, left);
+          else if (t0 + i < L) store_pair<VEC>(y + (size_t)i * D, t0 + i < n ? h : f2(0.f), left);
         }
       };
       if (near && tw + La::kSteps <= n) pass(std::true_type());
@@ -124,12 +114,101 @@ __global__ void __launch_bounds__(32 * kGatedWarps, M3_GF) gated_fwd_kernel(cons
       if (ck != nullptr) ck += (size_t)(span / kGatedCkpt) * D;
     }
     if (n > 0 && p.h_last != nullptr && rank == 0 && w == W - 1 && lane >= 32 - LC)
-      store_pair(p.h_last + (size_t)b * D + c, carry, left, false);
+      store_pair<false>(p.h_last + (size_t)b * D + c, carry, left);
     for (; tw - tw0 < L; tw += span) {               // steps past the length
       for (int i = 0; i < TS && tw + own + i < L; ++i)
-        store_pair(y + (size_t)i * D, f2(0.f), left, vec);
+        store_pair<VEC>(y + (size_t)i * D, f2(0.f), left);
       y += (size_t)span * D;
     }
+  }
+}
+
+// Many rows: a warp walks 64 channels of a row by itself, so that there is nothing
+// to join; the CTA's warps are workers of their own.  Two buffers of 4 steps.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParams p) {
+  extern __shared__ __align__(16) char smem[];
+  constexpr int TS = 4;
+  static_assert(TS == kGatedCkpt, "a pass starts at a checkpoint");
+  using St = Stage<T, 3, 32, TS, VEC>;
+  const int lane = threadIdx.x, w = threadIdx.y;
+  const int c0 = blockIdx.x * 64, c = c0 + lane * 2, left = p.D - c, D = p.D, L = p.L;
+  const long long ld[3] = {p.ld_x, p.ld_r, p.ld_i};
+  char* buf = smem + w * 2 * St::kBytes;
+  St st;
+  const int step = gridDim.y * blockDim.y;
+  int b = blockIdx.y * blockDim.y + w, nb, n, tn = 0;   // (nb, tn): the pass that is copied next
+  if (b >= p.B) return;
+  auto at = [&](int row) {
+    st.at(0, p.x, (long long)row * L, ld[0], c0);
+    st.at(1, p.rg, (long long)row * L, ld[1], c0);
+    st.at(2, p.ig, (long long)row * L, ld[2], c0);
+  };
+  nb = b;
+  int nn = n = row_length(p.lengths, b, L);             // the length of nb
+  at(b);
+  int put = 0, get = 0;
+  // copies the next pass, of this row or of the next that has one
+  auto ahead = [&] {
+    while (tn >= nn && nb < p.B) {
+      nb += step;
+      tn = 0;
+      if (nb < p.B) {
+        nn = row_length(p.lengths, nb, L);
+        at(nb);
+      }
+    }
+    if (nb < p.B) {
+      st.issue(buf + put * St::kBytes, ld, tn, nn, c0, D);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) st.p[q] += TS * ld[q];
+      tn += TS;
+      put ^= 1;
+    } else {
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  ahead();
+  const float2 dec = load_pair(p.decay + c, left);
+  const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
+  const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
+  for (; b < p.B; b += step) {
+    n = row_length(p.lengths, b, L);
+    float2 h = p.h0 != nullptr ? load_pair(p.h0 + (size_t)b * D + c, left) : f2(0.f);
+    T* y = static_cast<T*>(p.y) + (size_t)b * L * D + c;
+    float* ck = p.ckpt == nullptr ? nullptr : p.ckpt + (size_t)b * ((L + TS - 1) / TS) * D + c;
+    for (int t0 = 0; t0 < n; t0 += TS) {
+      ahead();
+      St::template wait<1>();
+      const char* from = buf + get * St::kBytes;
+      get ^= 1;
+      if (ck != nullptr) {
+        store_pair<VEC>(ck, h, left);
+        ck += D;
+      }
+      auto pass = [&](auto fast) {
+        constexpr bool FAST = decltype(fast)::value;
+#pragma unroll
+        for (int i = 0; i < TS; ++i) {
+          const float2 x = St::get(from, 0, i), r = sigmoid2(St::get(from, 1, i)),
+                       g = sigmoid2(St::get(from, 2, i));
+          float2 a, m, inv;
+          decay2<FAST>(mul2(k, r), a, m);
+          root2(m, m, inv);
+          const float2 v = fma2(a, h, mul2(mul2(m, g), x));
+          if (FAST || t0 + i < n) {
+            h = v;
+            store_pair<VEC>(y, h, left);
+            y += D;
+          }
+        }
+      };
+      if (near && t0 + TS <= n) pass(std::true_type());
+      else pass(std::false_type());
+      __syncwarp();
+    }
+    if (p.h_last != nullptr) store_pair<false>(p.h_last + (size_t)b * D + c, h, left);
+    for (int t = n; t < L; ++t, y += D) store_pair<VEC>(y, f2(0.f), left);
   }
 }
 
@@ -183,10 +262,11 @@ cudaError_t step_impl(const GatedStepParams& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-template <typename T, int LC>
+template <typename T, int LC, bool VEC>
 cudaError_t fwd_impl(const GatedParams& p, cudaStream_t s) {
-  constexpr int TS = kGatedFwdSteps, kBytes = Stage<T, 3, LC, TS>::kBytes, kTile = 2 * LC;
-  const cudaError_t e = allow_smem<gated_fwd_kernel<T, LC, TS>>(kGatedWarps * kBytes);
+  constexpr int TS = kGatedFwdSteps, kBytes = Stage<T, 3, LC, TS, VEC>::kBytes, kTile = 2 * LC;
+  const cudaError_t e = allow_smem<gated_fwd_kernel<T, LC, TS, VEC>>(
+      kGatedWarps * kBytes + joint_bytes(LC, kGatedWarps, 8));
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -195,17 +275,27 @@ cudaError_t fwd_impl(const GatedParams& p, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((p.D + kTile - 1) / kTile * p.splits), p.rows);
   cfg.blockDim = dim3(32, p.warps);
-  cfg.dynamicSmemBytes = p.warps * kBytes;
+  cfg.dynamicSmemBytes = p.warps * kBytes + joint_bytes(LC, p.warps, p.splits);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = p.splits > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, gated_fwd_kernel<T, LC, TS>, p);
+  return cudaLaunchKernelEx(&cfg, gated_fwd_kernel<T, LC, TS, VEC>, p);
 }
 
-template <typename T>
+template <typename T, bool VEC>
+cudaError_t fwd_rows(const GatedParams& p, cudaStream_t s) {
+  constexpr int kBytes = 2 * Stage<T, 3, 32, 4, VEC>::kBytes;
+  const cudaError_t e = allow_smem<gated_rows_fwd_kernel<T, VEC>>(4 * kBytes);
+  if (e != cudaSuccess) return e;
+  gated_rows_fwd_kernel<T, VEC><<<dim3((p.D + 63) / 64, p.rows), dim3(32, p.warps), p.warps * kBytes, s>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, bool VEC>
 cudaError_t fwd_lanes(const GatedParams& p, cudaStream_t s) {
-  if (p.lanes == 32) return fwd_impl<T, 32>(p, s);
-  return p.lanes == 16 ? fwd_impl<T, 16>(p, s) : fwd_impl<T, 8>(p, s);
+  if (p.solo) return fwd_rows<T, VEC>(p, s);
+  if (p.lanes == 32) return fwd_impl<T, 32, VEC>(p, s);
+  return p.lanes == 16 ? fwd_impl<T, 16, VEC>(p, s) : fwd_impl<T, 8, VEC>(p, s);
 }
 
 }  // namespace
@@ -213,28 +303,36 @@ cudaError_t fwd_lanes(const GatedParams& p, cudaStream_t s) {
 int gated_segments(int L) { return (L + kGatedCkpt - 1) / kGatedCkpt; }
 
 void gated_plan(int B, int L, int D, bool backward, int sms, GatedParams* p) {
-  const int per = backward ? M3_GB : M3_GF;                 // CTAs per SM
   const int ts = backward ? kGatedBwdSteps : kGatedFwdSteps, segs = (L + ts - 1) / ts;
-  const long long wave = (long long)per * sms;
-  const int warps = segs < kGatedWarps ? segs : kGatedWarps;
+  const long long wave = (backward ? 16LL : 24LL) * sms;    // warps that are resident
+  const long long tiles64 = (D + 63) / 64;
+  p->lanes = 32;
+  p->splits = 1;
+  p->solo = !backward && tiles64 * B >= wave;
+  if (p->solo) {                                            // a row per warp
+    p->warps = 4;
+    p->rows = B / 4 + (B % 4 != 0) < 65535 ? (B + 3) / 4 : 65535;
+    return;
+  }
+  int warps = 2;
+  while (warps < kGatedWarps && tiles64 * B * warps * 2 <= wave) warps *= 2;
+  if (warps > segs) warps = segs;
+  p->warps = warps;
+  const long long slots = wave / warps;
   // Of the tile widths and time splits whose every CTA has a pass of its own, the one
   // with most CTAs in one wave; wide tiles and few splits among equals.
-  int lanes = 32, S = 1;
   auto tiles = [&](int l) { return (long long)(D + 2 * l - 1) / (2 * l); };
   long long most = tiles(32) * B;
-  for (int l = 32; l >= M3_GL; l /= 2)
-    for (int k = 1; k <= M3_GS; ++k) {
+  for (int l = 32; l >= 8; l /= 2)
+    for (int k = 1; k <= 8; ++k) {
       const long long ctas = tiles(l) * B * k;
-      if (ctas <= wave && ctas > most && segs >= (long long)k * warps * (32 / l)) {
+      if (ctas <= slots && ctas > most && segs >= (long long)k * warps * (32 / l)) {
         most = ctas;
-        lanes = l;
-        S = k;
+        p->lanes = l;
+        p->splits = k;
       }
     }
-  p->lanes = lanes;
-  p->warps = warps;
-  p->splits = S;
-  long long gy = B, cap = wave / (tiles(lanes) * S);
+  long long gy = B, cap = slots / (tiles(p->lanes) * p->splits);
   if (cap < 1) cap = 1;
   if (cap > 65535) cap = 65535;
   if (gy > cap) {
@@ -245,7 +343,9 @@ void gated_plan(int B, int L, int D, bool backward, int sms, GatedParams* p) {
 }
 
 cudaError_t launch_gated_fwd(const GatedParams& p, cudaStream_t s) {
-  return p.dtype == M3_BF16 ? fwd_lanes<__nv_bfloat16>(p, s) : fwd_lanes<float>(p, s);
+  if (p.dtype == M3_BF16)
+    return p.vec ? fwd_lanes<__nv_bfloat16, true>(p, s) : fwd_lanes<__nv_bfloat16, false>(p, s);
+  return p.vec ? fwd_lanes<float, true>(p, s) : fwd_lanes<float, false>(p, s);
 }
 
 cudaError_t launch_gated_step(const GatedStepParams& p, cudaStream_t s) {

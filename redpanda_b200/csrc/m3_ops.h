@@ -222,6 +222,7 @@ struct GatedParams {
   int B, L, D;
   int dtype;
   int lanes, warps, splits, rows;                        // per run, per CTA, per cluster; grid
+  int solo;                                              // a warp walks its rows by itself
   int vec;                                               // 16-byte loads, vector stores
 };
 struct GatedBwdParams {
