@@ -13,6 +13,8 @@
 namespace m3 {
 namespace {
 
+constexpr int kFrom = 2048;
+
 template <typename TX, typename TS, typename TY, int VEC, int NV, bool WARP, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) add_norm_bwd_kernel(const AddNormBwdParams p) {
   constexpr int E = VEC * NV;
@@ -116,7 +118,7 @@ struct Launch {
   cudaStream_t s;
   template <int VEC, int NV, bool WARP, int MAXT, int MINB>
   cudaError_t operator()(int nt) {
-    const int ctas = norm_bwd_ctas(p.rows, p.d, p.sms);
+    const int ctas = add_norm_bwd_ctas(p.rows, p.d, p.sms);
     add_norm_bwd_kernel<TX, TS, TY, VEC, NV, WARP, MAXT, MINB><<<ctas, nt, 0, s>>>(p);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
@@ -126,6 +128,14 @@ struct Launch {
 
 }  // namespace
 
+// 768 threads per SM at 80 registers, 512 at 128 where a thread holds 16 elements
+int add_norm_bwd_ctas(long long rows, int d, int sms) {
+  const int rpc = d <= 256 ? 4 : 1, nt = d <= 256 ? 128 : add_threads(d, kFrom);
+  const int per = d <= kFrom ? 768 / nt : nt <= 512 ? 512 / nt : 1;
+  const long long want = (rows + rpc - 1) / rpc, cap = (long long)sms * per;
+  return (int)(want < cap ? want : cap);
+}
+
 cudaError_t launch_add_norm_bwd(const AddNormBwdParams& p, cudaStream_t s) {
   const int ex = dsize(p.dtype_x), es = dsize(p.dtype_s), ey = dsize(p.dtype_y);
   auto ok = [&](int v) {
@@ -134,7 +144,7 @@ cudaError_t launch_add_norm_bwd(const AddNormBwdParams& p, cudaStream_t s) {
   };
   const int vec = ex + es + ey < 12 && ok(8) ? 8 : ok(4) ? 4 : 1;
   return with_types(p.dtype_x, p.dtype_s, p.dtype_y, [&](auto tx, auto ts, auto ty) {
-    return norm_dispatch(p.d, vec, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
+    return add_dispatch(p.d, vec, kFrom, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
   });
 }
 

@@ -11,6 +11,8 @@
 namespace m3 {
 namespace {
 
+constexpr int kFrom = 2048;
+
 template <typename TX, typename TS, typename TY, int VEC, int NV, bool WARP, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) add_norm_fwd_kernel(const AddNormParams p) {
   constexpr int E = VEC * NV;
@@ -79,7 +81,9 @@ struct Launch {
   cudaError_t operator()(int nt) {
     const int rpc = WARP ? MAXT / 32 : 1;
     const long long want = (p.rows + rpc - 1) / rpc;
-    const long long cap = (long long)p.sms * (WARP ? MINB : norm_per_sm(p.d, nt));
+    const int per = WARP ? MINB : add_resident<add_norm_fwd_kernel<TX, TS, TY, VEC, NV, WARP, MAXT, MINB>>(nt);
+    if (per <= 0) return cudaErrorInvalidConfiguration;
+    const long long cap = (long long)p.sms * per;
     const int grid = (int)(want < cap ? want : cap);
     add_norm_fwd_kernel<TX, TS, TY, VEC, NV, WARP, MAXT, MINB><<<grid, nt, 0, s>>>(p);
     return cudaGetLastError();
@@ -96,7 +100,7 @@ cudaError_t launch_add_norm_fwd(const AddNormParams& p, cudaStream_t s) {
   };
   const int vec = ex + es + ey < 12 && ok(8) ? 8 : ok(4) ? 4 : 1;
   return with_types(p.dtype_x, p.dtype_s, p.dtype_y, [&](auto tx, auto ts, auto ty) {
-    return norm_dispatch(p.d, vec, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
+    return add_dispatch(p.d, vec, kFrom, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
   });
 }
 

@@ -40,24 +40,29 @@ __device__ __forceinline__ float row_max(float v, float (*red)[64], int& flip) {
   return v;
 }
 
-template <bool E4M3>
-__device__ __forceinline__ unsigned code8(float y) {
-  if (E4M3) return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-  int i = __float2int_rn(y);
-  i = i < -127 ? -127 : i > 127 ? 127 : i;
-  return (unsigned)i & 0xffu;
-}
-
-template <int VEC>
-__device__ __forceinline__ void store8(unsigned char* p, const unsigned (&b)[VEC]) {
-  if constexpr (VEC == 8)
-    *reinterpret_cast<uint2*>(p) =
-        make_uint2(b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24,
-                   b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24);
-  else if constexpr (VEC == 4)
-    *reinterpret_cast<unsigned*>(p) = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
-  else
-    *p = (unsigned char)b[0];
+// Codes of VEC values, the first in the lowest byte; one instruction per pair for
+// e4m3 (which holds the result to 448), one per value for int8.
+template <bool E4M3, int VEC>
+__device__ __forceinline__ void store8(unsigned char* p, const float (&v)[VEC]) {
+  unsigned b[(VEC + 3) / 4] = {};
+#pragma unroll
+  for (int j = 0; j < VEC; j += 2) {
+    unsigned two;
+    if (E4M3) {
+      two = __nv_cvt_float2_to_fp8x2(make_float2(v[j], VEC > 1 ? v[j + (VEC > 1)] : 0.f),
+                                     __NV_SATFINITE, __NV_E4M3);
+    } else {
+      auto one = [](float x) {
+        const int i = __float2int_rn(x);
+        return (unsigned)(i < -127 ? -127 : i > 127 ? 127 : i) & 0xffu;
+      };
+      two = one(v[j]) | (VEC > 1 ? one(v[j + (VEC > 1)]) << 8 : 0u);
+    }
+    b[j / 4] |= two << (j % 4 * 8);
+  }
+  if constexpr (VEC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(b[0], b[1]);
+  else if constexpr (VEC == 4) *reinterpret_cast<unsigned*>(p) = b[0];
+  else *p = (unsigned char)b[0];
 }
 
 template <typename TX, typename TS, bool E4M3, int VEC, int NV, bool WARP, int MAXT, int MINB>
@@ -138,12 +143,14 @@ __global__ void __launch_bounds__(MAXT, MINB) norm8_kernel(const Norm8Params p) 
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * tpr + t) * VEC;
-      const float scale = nan_max(__fdiv_rn(top[i], kTop), 0x1p-126f);
+      // the quotient as a product with the scale's reciprocal: two roundings of 2^-24
+      // where a division has one, a thousandth of the step of any code
+      const float scale = nan_max(top[i] * (1.f / kTop), 0x1p-126f), inv = rcp_approx(scale);
       if (c < d) {
-        unsigned b[VEC];
+        float u[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) b[j] = code8<E4M3>(__fdiv_rn(v[i * VEC + j], scale));
-        store8<VEC>(qr + c, b);
+        for (int j = 0; j < VEC; ++j) u[j] = v[i * VEC + j] * inv;
+        store8<E4M3, VEC>(qr + c, u);
         if (p.group == 0) {
           if (c == 0) p.scale[r] = scale;
         } else if (c % p.group == 0) {
@@ -163,11 +170,15 @@ struct Launch {
   cudaError_t operator()(int nt) {
     const int rpc = WARP ? MAXT / 32 : 1;
     const long long want = (p.rows + rpc - 1) / rpc;
-    const long long cap = (long long)p.sms * (WARP ? MINB : norm_per_sm(p.d, nt));
-    const int grid = (int)(want < cap ? want : cap);
-    if (p.e4m3) norm8_kernel<TX, TS, true, VEC, NV, WARP, MAXT, MINB><<<grid, nt, 0, s>>>(p);
-    else norm8_kernel<TX, TS, false, VEC, NV, WARP, MAXT, MINB><<<grid, nt, 0, s>>>(p);
-    return cudaGetLastError();
+    auto go = [&](auto e4m3) -> cudaError_t {
+      constexpr auto* kern = norm8_kernel<TX, TS, decltype(e4m3)::value, VEC, NV, WARP, MAXT, MINB>;
+      const int per = WARP ? MINB : add_resident<kern>(nt);
+      if (per <= 0) return cudaErrorInvalidConfiguration;
+      const long long cap = (long long)p.sms * per;
+      kern<<<(int)(want < cap ? want : cap), nt, 0, s>>>(p);
+      return cudaGetLastError();
+    };
+    return p.e4m3 ? go(std::true_type()) : go(std::false_type());
   }
 };
 
@@ -182,7 +193,7 @@ cudaError_t launch_norm8(const Norm8Params& p, cudaStream_t s) {
   const int vec = ok(8) ? 8 : ok(4) ? 4 : 1;
   if (p.group != 0 && vec == 1) return cudaErrorInvalidValue;   // refused by the entry
   return with_types(p.dtype_x, p.dtype_s, M3_F32, [&](auto tx, auto ts, auto) {
-    return norm_dispatch(p.d, vec, Launch<decltype(tx), decltype(ts)>{p, s});
+    return add_dispatch(p.d, vec, 1024, Launch<decltype(tx), decltype(ts)>{p, s});
   });
 }
 

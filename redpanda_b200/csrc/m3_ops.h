@@ -61,11 +61,12 @@ struct AddNormBwdParams {
   void* ds;                           // (rows, d) of dtype_s
   void* dx;                           // (rows, d) of dtype_x, or nullptr: ds serves
   float* dw;                          // (d,)
-  float* part;                        // (norm_bwd_ctas, 2, d), the first of each pair used
+  float* part;                        // (add_norm_bwd_ctas, 2, d), the first of each pair used
   long long rows; int d;
   int dtype_x, dtype_s, dtype_y;
   int sms;
 };
+int add_norm_bwd_ctas(long long rows, int d, int sms);   // partials
 cudaError_t launch_add_norm_bwd(const AddNormBwdParams& p, cudaStream_t s);
 // out[c] = sum over n partials part[(i * 2 + which) * d + c], in a fixed order (db may be nullptr)
 cudaError_t launch_norm_reduce(const float* part, int n, int d, float* dw, float* db,
