@@ -20,7 +20,8 @@
 // A warp takes MT tiles of 16 outputs; the CTA's warps split tiles (mw) and the
 // columns (kw), whose totals are added in order.  Codes are laid out once so that a
 // lane's 16 bytes are its operand of four instructions (64 columns).  Inputs are
-// staged in shared memory as the instruction's fragments, `chunk` columns at a time.
+// staged in shared memory as the instruction's fragments, `chunk` columns at a time;
+// codes and scales come through a ring of asynchronous copies per warp.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -32,8 +33,6 @@
 
 namespace m3 {
 namespace {
-
-constexpr int kAhead = 4;          // blocks of 64 columns in flight per warp
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], unsigned b0,
                                          unsigned b1) {
@@ -82,6 +81,11 @@ __device__ __forceinline__ float below(float v) {   // v without its top 16 bits
   return t == v ? 0.f : v - t;
 }
 
+// The inputs' fragments of two instructions (32 columns of k): a lane's 16 bytes
+// (b0, b1 of each) at (pair of instructions, column of the operand, lane % 4).  Only
+// the `cols` columns in use are kept; lanes of others read the last one's, and their
+// results are not used.
+//
 // Stages the columns from k0 of every row: fragments, the groups' sums of the
 // inputs and the squares' sums of every unit of U columns.
 template <typename T, int NB, int G, bool CENTER>
@@ -89,28 +93,41 @@ __device__ void stage(const RowsQ4Params& p, int k0, int units, unsigned* frag, 
                       float* sq, int parts) {
   constexpr int U = G > 64 ? G : 64;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int cols = parts * p.rows;
   const T* x = static_cast<const T*>(p.x);
   for (int u = warp; u < units; u += warps) {
-    for (int r = 0; r < p.rows; ++r) {
+    // every row's loads before any is used
+    float2 v[kQ4Rows][U / 64], w[U / 64];
+#pragma unroll
+    for (int h = 0; h < U / 64; ++h) {
+      const int k = k0 + u * U + h * 64 + 2 * lane, left = p.d_in - k, at = left > 0 ? k : 0;
+#pragma unroll
+      for (int r = 0; r < kQ4Rows; ++r)
+        if (r < p.rows) v[r][h] = load2(x + (size_t)r * p.ld_x + at, left, p.vec != 0);
+      if (p.norm_w != nullptr) w[h] = load2(p.norm_w + at, left, p.vec != 0);
+    }
+#pragma unroll
+    for (int r = 0; r < kQ4Rows; ++r) {
+      if (r >= p.rows) break;
       float sum = 0.f, ss = 0.f;
 #pragma unroll
       for (int h = 0; h < U / 64; ++h) {
-        const int in = u * U + h * 64 + 2 * lane, k = k0 + in, left = p.d_in - k;
-        float2 v = load2(x + (size_t)r * p.ld_x + (left > 0 ? k : 0), left, p.vec != 0);
+        const int in = u * U + h * 64 + 2 * lane;
+        float2 y = v[r][h];
         if (p.norm_w != nullptr) {
-          ss = fmaf(v.x, v.x, fmaf(v.y, v.y, ss));
-          const float2 w = load2(p.norm_w + (left > 0 ? k : 0), left, p.vec != 0);
-          v.x *= w.x;
-          v.y *= w.y;
+          ss = fmaf(y.x, y.x, fmaf(y.y, y.y, ss));
+          y.x *= w[h].x;
+          y.y *= w[h].y;
         }
-        if (CENTER) sum += v.x + v.y;
+        if (CENTER) sum += y.x + y.y;
         // instruction k / 16; pairs t and (half) t + 4 of its 16 columns
         const int ks = in >> 4, half = lane >> 2 & 1, t = lane & 3;
-        for (int s = 0; s < parts; ++s) {
-          const int col = s * p.rows + r;
-          frag[(((ks >> 1) * NB + (col >> 3)) * 32 + (col & 7) * 4 + t) * 4 + (ks & 1) * 2 + half] =
-              top_halves(v);
-          if (s + 1 < parts) v = make_float2(below(v.x), below(v.y));
+        unsigned* f = frag + (((ks >> 1) * cols + r) * 4 + t) * 4 + (ks & 1) * 2 + half;
+        *f = top_halves(y);
+        if (parts == 3) {
+          y = make_float2(below(y.x), below(y.y));
+          f[p.rows * 16] = top_halves(y);
+          f[p.rows * 32] = top_halves(make_float2(below(y.x), below(y.y)));
         }
       }
       if (CENTER) {
@@ -126,104 +143,124 @@ __device__ void stage(const RowsQ4Params& p, int k0, int units, unsigned* frag, 
   }
 }
 
-// shared memory: fragments, then the groups' sums, then the squares' sums of all units
-struct Layout {
-  int xs, sq, total;               // bytes
+// A warp's ring of units in flight: MT tiles' codes, then their scales.
+template <int MT, int G, bool CENTER>
+struct Ring {
+  static constexpr int U = G > 64 ? G : 64, BU = U / 64, GU = U / G;   // columns, blocks, groups
+  static constexpr int kScale = GU * 8 * (CENTER ? 8 : 4);             // bytes per tile and unit
+  static constexpr int kSlot = MT * (BU * 512 + kScale);
+  static constexpr int kSlots = MT * BU == 1 ? 8 : MT * BU == 2 ? 6 : 4;
 };
-__host__ __device__ inline Layout layout(int NB, int G, bool center, int chunk, int units,
-                                         bool norm) {
+
+// shared memory: the warps' rings, the fragments, the groups' sums, and the squares'
+// sums of all units; the totals lie over rings and fragments at the end
+struct Layout {
+  int frag, xs, sq, total;         // bytes
+};
+template <int NB, int MT, int G, bool CENTER>
+__host__ __device__ inline Layout layout(int warps, int cols, int chunk, int units, bool norm) {
+  using R = Ring<MT, G, CENTER>;
   Layout l;
-  l.xs = chunk * 16 * NB;
-  l.sq = l.xs + (center ? chunk / G * 8 * NB * 4 : 0);
+  l.frag = warps * R::kSlots * R::kSlot;
+  l.xs = l.frag + chunk * 2 * cols;
+  l.sq = l.xs + (CENTER ? chunk / G * 8 * NB * 4 : 0);
   l.total = l.sq + (norm ? units * kQ4Rows * 4 : 0);
   return l;
 }
 
+__device__ __forceinline__ void copy16(char* to, const char* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   (unsigned)__cvta_generic_to_shared(to)),
+               "l"(from)
+               : "memory");
+}
+
 template <typename T, int NB, int MT, int G, bool CENTER>
 __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
-  constexpr int U = G > 64 ? G : 64, BU = U / 64, GU = U / G;   // a unit's columns, blocks, groups
-  constexpr int NU = kAhead / BU / MT < 1 ? 1 : kAhead / BU / MT;   // units of a batch
+  using R = Ring<MT, G, CENTER>;
+  constexpr int U = R::U, BU = R::BU, GU = R::GU;
   extern __shared__ __align__(16) char smem[];
   __shared__ float s_rstd[kQ4Rows];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int mw = warp % p.mw, kw = warp / p.mw;
-  const int units = (p.d_in + U - 1) / U, per = (units + p.kw - 1) / p.kw;
+  const int units = (p.d_in + U - 1) / U, per = (units - kw + p.kw - 1) / p.kw;   // of this warp
+  const int parts = sizeof(T) == 4 || p.norm_w != nullptr ? 3 : 1, cols = parts * p.rows;
   const int chunk_units = p.chunk / U, per_chunk = chunk_units / p.kw;
-  const Layout lay = layout(NB, G, CENTER, p.chunk, units, p.norm_w != nullptr);
-  unsigned* frag = reinterpret_cast<unsigned*>(smem);
+  const Layout lay = layout<NB, MT, G, CENTER>(p.mw * p.kw, cols, p.chunk, units,
+                                               p.norm_w != nullptr);
+  char* ring = smem + warp * R::kSlots * R::kSlot;
+  unsigned* frag = reinterpret_cast<unsigned*>(smem + lay.frag);
   float* xs = reinterpret_cast<float*>(smem + lay.xs);
   float* sq = reinterpret_cast<float*>(smem + lay.sq);
-  const int parts = sizeof(T) == 4 || p.norm_w != nullptr ? 3 : 1;
-  const int tiles = (p.d_out + 15) / 16;
-  const int tile0 = (blockIdx.x * p.mw + mw) * MT;
+  const int tiles = (p.d_out + 15) / 16, tile0 = (blockIdx.x * p.mw + mw) * MT;
   pdl_launch_dependents();
 
-  uint4 w[MT][NU][BU];
-  uint2 sc[MT][NU][GU];
-  auto load = [&](int i0) {
+  // This warp's units kw, kw + p.kw, ..: the next one to copy.  A tile past the last is
+  // the last once more; its results are not stored.
+  const char* codes[MT];
+  const char* scales[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < MT; ++m) {
+    const size_t at = (size_t)min(tile0 + m, tiles - 1) * units + kw;
+    codes[m] = reinterpret_cast<const char*>(p.codes) + at * (BU * 512) + lane * 16;
+    scales[m] = static_cast<const char*>(p.scales) + at * R::kScale + lane * 16;
+  }
+  int put = 0, slot_in = 0;
+  auto copy = [&] {
+    if (put < per) {
+      char* to = ring + slot_in * R::kSlot + lane * 16;
 #pragma unroll
-      for (int n = 0; n < NU; ++n) {
-        const int u = (i0 + n) * p.kw + kw;
-        const bool ok = i0 + n < per && u < units && tile0 + m < tiles;
+      for (int m = 0; m < MT; ++m) {
 #pragma unroll
-        for (int b = 0; b < BU; ++b)
-          w[m][n][b] = ok ? __ldg(p.codes + ((size_t)(tile0 + m) * units * BU + u * BU + b) * 32 +
-                                  lane)
-                          : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int g = 0; g < GU; ++g) {
-          const size_t at = ((size_t)(tile0 + m) * units * GU + u * GU + g) * 8 + (lane >> 2);
-          sc[m][n][g] = make_uint2(0, 0);
-          if (ok) {
-            if (CENTER) sc[m][n][g] = __ldg(static_cast<const uint2*>(p.scales) + at);
-            else sc[m][n][g].x = __ldg(static_cast<const unsigned*>(p.scales) + at);
-          }
-        }
+        for (int b = 0; b < BU; ++b) copy16(to + (m * BU + b) * 512, codes[m] + b * 512);
+        if (lane < R::kScale / 16) copy16(to + MT * BU * 512 + m * R::kScale, scales[m]);
+        codes[m] += (size_t)p.kw * (BU * 512);
+        scales[m] += (size_t)p.kw * R::kScale;
       }
+      ++put;
+      slot_in = slot_in + 1 == R::kSlots ? 0 : slot_in + 1;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  load(0);
+#pragma unroll
+  for (int i = 0; i < R::kSlots - 1; ++i) copy();
   pdl_wait();
   if (CENTER)   // the columns of the inputs' lower parts have no sum of their own
     for (int i = threadIdx.x; i < p.chunk / G * 8 * NB; i += blockDim.x) xs[i] = 0.f;
 
+  int at[NB];                                        // of the lane's fragments
+#pragma unroll
+  for (int c = 0; c < NB; ++c) at[c] = (min(c * 8 + (lane >> 2), cols - 1) * 4 + (lane & 3)) * 4;
   float tot[MT][NB][4] = {};
-  for (int i0 = 0; i0 < per; i0 += NU) {
-    const int in = i0 % per_chunk;
-    if (in == 0) {
-      const int u0 = i0 * p.kw;
-      __syncthreads();
-      stage<T, NB, G, CENTER>(p, u0 * U, min(chunk_units, units - u0), frag, xs, sq, parts);
-      __syncthreads();
-    }
-    uint4 cw[MT][NU][BU];
-    uint2 cs[MT][NU][GU];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < NU; ++n) {
-#pragma unroll
-        for (int b = 0; b < BU; ++b) cw[m][n][b] = w[m][n][b];
-#pragma unroll
-        for (int g = 0; g < GU; ++g) cs[m][n][g] = sc[m][n][g];
-      }
-    load(i0 + NU);
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      const int u = (in + n) * p.kw + kw;            // in the chunk
-      if (i0 + n >= per || (i0 + n) * p.kw + kw >= units) break;
+  int slot = 0;
+  for (int i0 = 0; i0 * p.kw < units; i0 += per_chunk) {   // chunks of the columns
+    const int u0 = i0 * p.kw;
+    __syncthreads();
+    stage<T, NB, G, CENTER>(p, u0 * U, min(chunk_units, units - u0), frag, xs, sq, parts);
+    __syncthreads();
+    const int end = min(per, i0 + per_chunk);
+    for (int i = i0; i < end; ++i) {
+      copy();
+      asm volatile("cp.async.wait_group %0;" ::"n"(R::kSlots - 1) : "memory");
+      __syncwarp();
+      const char* from = ring + slot * R::kSlot;
+      slot = slot + 1 == R::kSlots ? 0 : slot + 1;
+      const int u = (i - i0) * p.kw + kw;            // in the chunk
+      const unsigned* fu = frag + u * (U / 32) * cols * 16;
       float acc[MT][NB][4];
 #pragma unroll
-      for (int b = 0; b < BU; ++b)
+      for (int b = 0; b < BU; ++b) {
+        uint4 w[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          w[m] = *reinterpret_cast<const uint4*>(from + (m * BU + b) * 512 + lane * 16);
 #pragma unroll
         for (int jp = 0; jp < 2; ++jp) {             // two instructions' worth of columns
           const bool first = G < 64 || (b == 0 && jp == 0), last = G < 64 || (b == BU - 1 && jp == 1);
           uint4 f[NB];
 #pragma unroll
           for (int c = 0; c < NB; ++c)
-            f[c] = *reinterpret_cast<const uint4*>(
-                frag + (((u * (U / 32) + b * 2 + jp) * NB + c) * 32 + lane) * 4);
+            f[c] = *reinterpret_cast<const uint4*>(fu + (b * 2 + jp) * cols * 16 + at[c]);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             if (first)
@@ -231,23 +268,26 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
               for (int c = 0; c < NB; ++c)
                 acc[m][c][0] = acc[m][c][1] = acc[m][c][2] = acc[m][c][3] = 0.f;
             unsigned a[4];
-            unpack(jp ? cw[m][n][b].z : cw[m][n][b].x, a);
+            unpack(jp ? w[m].z : w[m].x, a);
 #pragma unroll
             for (int c = 0; c < NB; ++c) mma16816(acc[m][c], a, f[c].x, f[c].y);
-            unpack(jp ? cw[m][n][b].w : cw[m][n][b].y, a);
+            unpack(jp ? w[m].w : w[m].y, a);
 #pragma unroll
             for (int c = 0; c < NB; ++c) mma16816(acc[m][c], a, f[c].z, f[c].w);
             if (last) {
-              const uint2 s2 = cs[m][n][G < 64 ? jp : 0];
+              const int g = G < 64 ? jp : 0;
+              const char* sp = from + MT * BU * 512 + m * R::kScale;
               float s0, s1, c0 = 0.f, c1 = 0.f;      // of outputs lane / 4 and lane / 4 + 8
               if (CENTER) {
+                const uint2 s2 = reinterpret_cast<const uint2*>(sp)[g * 8 + (lane >> 2)];
                 s0 = __uint_as_float(s2.x << 16);
                 c0 = __uint_as_float(s2.x & 0xffff0000u);
                 s1 = __uint_as_float(s2.y << 16);
                 c1 = __uint_as_float(s2.y & 0xffff0000u);
               } else {
-                s0 = __uint_as_float(s2.x << 16);
-                s1 = __uint_as_float(s2.x & 0xffff0000u);
+                const unsigned s2 = reinterpret_cast<const unsigned*>(sp)[g * 8 + (lane >> 2)];
+                s0 = __uint_as_float(s2 << 16);
+                s1 = __uint_as_float(s2 & 0xffff0000u);
               }
 #pragma unroll
               for (int c = 0; c < NB; ++c) {
@@ -257,7 +297,7 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
                 tot[m][c][3] = fmaf(s1, acc[m][c][3], tot[m][c][3]);
                 if (CENTER) {
                   const float2 v = *reinterpret_cast<const float2*>(
-                      xs + (u * GU + (G < 64 ? jp : 0)) * (8 * NB) + c * 8 + 2 * (lane & 3));
+                      xs + (u * GU + g) * (8 * NB) + c * 8 + 2 * (lane & 3));
                   tot[m][c][0] = fmaf(c0, v.x, tot[m][c][0]);
                   tot[m][c][1] = fmaf(c0, v.y, tot[m][c][1]);
                   tot[m][c][2] = fmaf(c1, v.x, tot[m][c][2]);
@@ -267,6 +307,8 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
             }
           }
         }
+      }
+      __syncwarp();                                  // before the slot is copied to again
     }
   }
 
@@ -289,7 +331,8 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int o = (mw * MT + m) * 16 + (lane >> 2) + (i >> 1) * 8;
-        red[((size_t)kw * outs + o) * (8 * NB) + c * 8 + 2 * (lane & 3) + (i & 1)] = tot[m][c][i];
+        red[((size_t)kw * outs + o) * (8 * NB + 1) + c * 8 + 2 * (lane & 3) + (i & 1)] =
+            tot[m][c][i];
       }
   __syncthreads();
   for (int i = threadIdx.x; i < outs * p.rows; i += blockDim.x) {
@@ -297,7 +340,8 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
     if (out >= p.d_out) continue;
     float v = 0.f;
     for (int s = parts - 1; s >= 0; --s)             // the smallest part first
-      for (int k = 0; k < p.kw; ++k) v += red[((size_t)k * outs + o) * (8 * NB) + s * p.rows + r];
+      for (int k = 0; k < p.kw; ++k)
+        v += red[((size_t)k * outs + o) * (8 * NB + 1) + s * p.rows + r];
     if (p.norm_w != nullptr) v *= s_rstd[r];
     if (p.bias != nullptr) v += p.bias[out];
     if (p.residual != nullptr)
@@ -313,20 +357,24 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
 
 template <typename T, int NB, int MT, int G, bool CENTER>
 cudaError_t launch(RowsQ4Params p, cudaStream_t s) {
-  constexpr int U = G > 64 ? G : 64, BU = U / 64;
-  constexpr int NU = kAhead / BU / MT < 1 ? 1 : kAhead / BU / MT;
+  constexpr int U = G > 64 ? G : 64;
   constexpr int kSmem = 112 << 10;                   // two CTAs per SM
   const int units = (p.d_in + U - 1) / U;
   const bool norm = p.norm_w != nullptr;
-  // as many columns at a time as fit, a whole number of batches of every warp; at
-  // kw = 1 and d_in = kQ4MaxIn one batch and the squares' sums take 45 KB
-  auto bytes = [&](int chunk) { return layout(NB, G, CENTER, chunk, units, norm).total; };
-  while (p.kw > 1 && bytes(p.kw * NU * U) > kSmem) --p.kw;
-  const int step = p.kw * NU * U;
+  const int cols = p.rows * (sizeof(T) == 4 || norm ? 3 : 1);
+  // As many columns at a time as fit, a whole number of units of every warp, of fewer
+  // warps where one unit of each does not fit (at one warp along the columns it does:
+  // the rings' 68 KB, 128 columns' 7 KB and 32 KB of squares' sums at d_in = kQ4MaxIn).
+  auto bytes = [&](int chunk) {
+    return layout<NB, MT, G, CENTER>(p.mw * p.kw, cols, chunk, units, norm).total;
+  };
+  while (p.kw > 1 && bytes(p.kw * U) > kSmem) --p.kw;
+  const int step = p.kw * U;
   int chunk = (units * U + step - 1) / step * step;
   while (chunk > step && bytes(chunk) > kSmem) chunk -= step;
   p.chunk = chunk;
-  const int red = p.kw * 16 * MT * p.mw * 8 * NB * 4, smem = bytes(chunk) > red ? bytes(chunk) : red;
+  const int red = p.kw * 16 * MT * p.mw * (8 * NB + 1) * 4;
+  const int smem = bytes(chunk) > red ? bytes(chunk) : red;
   const cudaError_t e = allow_smem<rows_q4_kernel<T, NB, MT, G, CENTER>>(kSmem);
   if (e != cudaSuccess) return e;
   const int grid = (p.d_out + 16 * MT * p.mw - 1) / (16 * MT * p.mw);
@@ -352,11 +400,11 @@ cudaError_t with_type(RowsQ4Params p, cudaStream_t s) {
   const int nb = (p.rows * parts + 7) / 8, unit = p.group > 64 ? p.group : 64;
   const int units = (p.d_in + unit - 1) / unit;
   const long long tiles = (p.d_out + 15) / 16;
-  // Warps along the columns while tiles are few, along the outputs where they fill
-  // the GPU twice over: fewer copies of the inputs are staged.
+  // Warps along the columns while tiles are few, along the outputs where there are more
+  // than one wave of CTAs: fewer copies of the inputs are staged.
   int mt = 1, mw = 1;
-  if (tiles >= 4LL * p.sms) mt = 2;
-  while (mw < 4 && tiles >= 4LL * p.sms * mt * mw) mw *= 2;
+  if (tiles > 2LL * p.sms) mt = 2;
+  while (mw < 8 && tiles > 2LL * p.sms * mt * mw) mw *= 2;
   p.mw = mw;
   p.kw = 8 / mw < units ? 8 / mw : units;
   switch (nb * 2 + (mt - 1)) {
