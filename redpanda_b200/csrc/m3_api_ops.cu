@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include "m3_api_util.h"
+#include "m3_internal.h"
 #include "m3_ops.h"
 #include "m3scan.h"
 
@@ -92,6 +93,7 @@ int fill_gated(const m3_gated_desc* d, const m3_gated_args* a, bool backward, Ga
   p->vec = d->d_inner % v == 0 && a->ld_x % v == 0 && a->ld_r % v == 0 && a->ld_i % v == 0 &&
            aligned(a->x, 16) && aligned(a->rg, 16) && aligned(a->ig, 16);
   gated_plan(p->B, p->L, p->D, backward, device_sms(), p);
+  if (p->splits > 1) p->err = device_err_ptr();
   return M3_OK;
 }
 

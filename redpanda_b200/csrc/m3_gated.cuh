@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "m3_bulk.cuh"
 #include "m3_math.cuh"
 #include "m3_vec.cuh"
 
@@ -200,20 +201,31 @@ __device__ __forceinline__ float2 load_pair(const float* p, int left) {
 // consecutive steps, forwards (DIR 1) or backwards (-1): w and rank are this warp's
 // and CTA's places in that order.  A warp folds the runs ahead of its own onto the
 // value before the first; the last warp passes the value behind all of them on to
-// the next call.  Two buffers in turn: one CTA barrier (and one cluster barrier) per
-// call.
+// the next call.  Two buffers in turn: one CTA barrier per call.
+//
+// The cluster's CTAs write their runs into each other's shared memory, counted by
+// an mbarrier of the receiver's (two in turn, S x LC x 16 bytes each time).  A
+// cluster barrier there would wait for every store to memory before it (prompt of
+// 16384 x 1024: 51 against XX us).  A slot is written again two calls later, by a CTA
+// that by then has this CTA's run of the call between, which was sent after every
+// warp here had read the slot.  The wait is bounded: after kMbarMaxPolls polls the
+// thread sets `dead`, waits no more, and the kernel records M3_ERR_DEVICE.
 template <int LC>
 struct Joint {
   float4* warp;      // (2, warps, LC)
   float4* cta;       // (2, S, LC), for S > 1
   float2* carry;     // (2, LC)
+  uint64_t* bar;     // (2), for S > 1
   int warps, S;
   // in shared memory behind the warps' stages
   __device__ __forceinline__ Joint(char* at, int warps, int S) : warps(warps), S(S) {
     warp = reinterpret_cast<float4*>(at);
     cta = warp + 2 * warps * LC;
     carry = reinterpret_cast<float2*>(cta + (S > 1 ? 2 * S * LC : 0));
+    bar = reinterpret_cast<uint64_t*>(carry + 2 * LC);
   }
+  // every CTA of the cluster runs, and its barriers are set up, before any is written to
+  __device__ __forceinline__ void start() const;
   __device__ __forceinline__ float4& run(int flip, int k, int cl) const {
     return warp[(flip * warps + k) * LC + cl];
   }
@@ -222,12 +234,27 @@ struct Joint {
   }
 };
 inline int joint_bytes(int lanes, int warps, int S) {
-  return lanes * (32 * warps + (S > 1 ? 32 * S : 0) + 16);
+  return lanes * (32 * warps + (S > 1 ? 32 * S : 0) + 16) + 16;
 }
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
+}
+template <int LC>
+__device__ __forceinline__ void Joint<LC>::start() const {
+  if (S == 1) return;
+  if (threadIdx.x + threadIdx.y == 0) {
+    mbar_init(bar, 1);
+    mbar_init(bar + 1, 1);
+    mbar_fence_init();
+  }
+  cluster_sync();
+}
+__device__ __forceinline__ unsigned peer_addr(const void* p, int peer) {
+  unsigned to;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_addr(p)), "r"(peer));
+  return to;
 }
 __device__ __forceinline__ float2 shfl2(float2 v, int from) {
   return make_float2(__shfl_sync(0xffffffffu, v.x, from & 31),
@@ -237,12 +264,13 @@ __device__ __forceinline__ Run as_run(const float4& v) {
   return Run{make_float2(v.x, v.y), make_float2(v.z, v.w)};
 }
 
-// The value in front of this run.  first: `carry` is the value in front of all, else
-// the last call's.  On return carry is the value behind all, in the last warp's last
+// The value in front of this run; turn: the call's number.  first: `carry` is the value
+// in front of all, else the last call's.  On return carry is the value behind all, in the last warp's last
 // run's lanes.
 template <int LC, int DIR>
-__device__ __forceinline__ float2 join(const Joint<LC>& j, int flip, const Run& mine, int w, int rank,
-                                       bool first, float2& carry) {
+__device__ __forceinline__ float2 join(const Joint<LC>& j, int turn, const Run& mine, int w, int rank,
+                                       bool first, float2& carry, bool& dead) {
+  const int flip = turn & 1;
   const int warps = j.warps, S = j.S;
   constexpr int kSub = 32 / LC;
   const int lane = threadIdx.x, cl = lane % LC;
@@ -277,20 +305,22 @@ __device__ __forceinline__ float2 join(const Joint<LC>& j, int flip, const Run& 
   }
   Run before{f2(1.f), f2(0.f)};
   for (int k = 0; k < w; ++k) then(before, as_run(j.run(flip, k, cl)));
-  if (w == warps - 1 && sub == kSub - 1) {
-    Run all = before;
-    then(all, upto);
-    for (int peer = 0; peer < S; ++peer) {
-      const unsigned a = (unsigned)__cvta_generic_to_shared(&j.part(flip, rank, cl));
-      unsigned to;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(a), "r"(peer));
-      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(all.P.x),
-                   "f"(all.P.y), "f"(all.V.x), "f"(all.V.y)
-                   : "memory");
+  if (w == warps - 1) {
+    if (lane == 0) mbar_arrive_expect_tx(j.bar + flip, S * LC * 16);
+    if (sub == kSub - 1) {
+      Run all = before;
+      then(all, upto);
+      for (int peer = 0; peer < S; ++peer)
+        asm volatile(
+            "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 "
+            "[%0], {%1, %2, %3, %4}, [%5];" ::"r"(peer_addr(&j.part(flip, rank, cl), peer)),
+            "f"(all.P.x), "f"(all.P.y), "f"(all.V.x), "f"(all.V.y),
+            "r"(peer_addr(j.bar + flip, peer))
+            : "memory");
     }
+    __syncwarp();
   }
-  __syncwarp();
-  cluster_sync();
+  if (!dead) dead = !mbar_wait(j.bar + flip, turn >> 1 & 1);
   for (int k = 0; k < rank; ++k) {
     const Run f = as_run(j.part(flip, k, cl));
     c = fma2(f.P, c, f.V);

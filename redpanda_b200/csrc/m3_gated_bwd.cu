@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "m3_api_util.h"
+#include "m3_common.cuh"
 #include "m3_ops.h"
 #include "m3_pdl.cuh"
 
@@ -72,8 +73,9 @@ __global__ void __launch_bounds__(256, 2)
   const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
   const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
   float2 sum = f2(0.f);
-  int flip = 0;
-  if (S > 1) cluster_sync();                         // every CTA runs before its memory is written
+  int turn = 0;
+  bool dead = false;
+  joint.start();
   // the copies of a row's first pass, its last steps, start while the row before it
   // is finished
   auto start = [&](int b, int n) {
@@ -140,7 +142,8 @@ __global__ void __launch_bounds__(256, 2)
         } else if (n2 > 0) {
           start(nb, n2);
         }
-        float2 v = join<LC, -1>(joint, flip, run, W - 1 - w, S - 1 - rank, k0 == passes, carry);
+        float2 v = join<LC, -1>(joint, turn, run, W - 1 - w, S - 1 - rank, k0 == passes, carry,
+                                    dead);
         float2 part = f2(0.f);
 #pragma unroll
         for (int i = TS - 1; i >= 0; --i) {
@@ -158,10 +161,12 @@ __global__ void __launch_bounds__(256, 2)
       };
       if (near && tw + La::kSteps <= n) pass(std::true_type());
       else pass(std::false_type());
-      flip ^= 1;
+      ++turn;
       at -= (size_t)span * D;
     }
   }
+  if (S > 1) cluster_sync();                         // nobody writes to a CTA that has left
+  if (dead) set_err(p.err, M3_ERR_DEVICE);
   pdl_launch_dependents();
   // the CTA's partial: the runs of a warp, then the warps, in order
 #pragma unroll

@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "m3_api_util.h"
+#include "m3_common.cuh"
 #include "m3_ops.h"
 
 namespace m3 {
@@ -40,8 +41,9 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
   const float2 dec = load_pair(p.decay + c, left);
   const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
   const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
-  int flip = 0;
-  if (S > 1) cluster_sync();                         // every CTA runs before its memory is written
+  int turn = 0;
+  bool dead = false;
+  joint.start();
   // the copies of a row's first pass start while the row before it is finished
   auto start = [&](int b, int n) {
     const long long row = (long long)b * L + tw0;
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
         } else if (n2 > 0) {
           start(nb, n2);
         }
-        float2 h = join<LC, 1>(joint, flip, run, w, rank, s0 == 0, carry);
+        float2 h = join<LC, 1>(joint, turn, run, w, rank, s0 == 0, carry, dead);
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
           if (i % kGatedCkpt == 0 && ck != nullptr && (FAST || t0 + i < n))
@@ -109,7 +111,7 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
       };
       if (near && tw + La::kSteps <= n) pass(std::true_type());
       else pass(std::false_type());
-      flip ^= 1;
+      ++turn;
       y += (size_t)span * D;
       if (ck != nullptr) ck += (size_t)(span / kGatedCkpt) * D;
     }
@@ -121,6 +123,8 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
       y += (size_t)span * D;
     }
   }
+  if (S > 1) cluster_sync();                         // nobody writes to a CTA that has left
+  if (dead) set_err(p.err, M3_ERR_DEVICE);
 }
 
 // Many rows: a warp walks 64 channels of a row by itself, so that there is nothing

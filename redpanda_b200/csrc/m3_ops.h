@@ -225,6 +225,7 @@ struct GatedParams {
   int lanes, warps, splits, rows;                        // per run, per CTA, per cluster; grid
   int solo;                                              // a warp walks its rows by itself
   int vec;                                               // 16-byte loads, vector stores
+  int* err;                                              // the device's error word
 };
 struct GatedBwdParams {
   GatedParams f;                                         // y, h_last unused

@@ -56,10 +56,13 @@ def _forward(prepared, decay, c, state, lengths, want_state, want_ckpt):
     return y, h, ckpt
 
 
-def _prepare(seq, *ts):
+def _prepare(seq, x, r, i):
     """(tensor, row stride) of each activation in their common element type."""
-    ty = _common(*ts)
-    return [seq(_typed(t, ty)) for t in ts]
+    ty = x.dtype
+    if r.dtype is not ty or i.dtype is not ty:
+        ty = torch.float32
+        x, r, i = _typed(x, ty), _typed(r, ty), _typed(i, ty)
+    return seq(x), seq(r), seq(i)
 
 
 class _GatedScanFn(torch.autograd.Function):
@@ -113,11 +116,12 @@ class _GatedScanFn(torch.autograd.Function):
 
 
 def _check(name, x, rgate, igate, decay, c, dims):
-    what = "(B, L, D)" if dims == 3 else "(B, D)"
-    if x.dim() != dims or x.shape[-1] < 1 or rgate.shape != x.shape or igate.shape != x.shape:
+    shape = x.shape
+    if len(shape) != dims or shape[-1] < 1 or rgate.shape != shape or igate.shape != shape:
+        what = "(B, L, D)" if dims == 3 else "(B, D)"
         raise ValueError(f"{name}: x, rgate and igate are {what}")
-    H.check_sizes(name, *x.shape)
-    if decay.shape != x.shape[-1:]:
+    H.check_sizes(name, *shape)
+    if decay.shape != shape[-1:]:
         raise ValueError(f"{name}: decay is (D,)")
     c = float(c)
     if not 0 < c < math.inf:
@@ -167,17 +171,19 @@ def m3_gated_step_(h, x_t, rgate_t, igate_t, decay, c=8.0):
     if H.needs_grad(h, x_t, rgate_t, igate_t, decay):
         raise ValueError(f"{name} works in place: call it under torch.no_grad()")
     c = _check(name, x_t, rgate_t, igate_t, decay, c, 2)
-    B, D = x_t.shape
-    if h.shape != (B, D) or h.dtype is not torch.float32 or not h.is_contiguous():
+    shape = x_t.shape
+    if h.shape != shape or h.dtype is not torch.float32 or not h.is_contiguous():
         raise ValueError(f"{name}: h is (B, D), float32 and contiguous (it is updated in place)")
     H.refuse_tangents(name, h, x_t, rgate_t, igate_t, decay)
     dev = H.device_index(h, x_t, rgate_t, igate_t, decay)
     prepared = _prepare(H.rows, x_t, rgate_t, igate_t)
     x = prepared[0][0]
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    B, D = shape
     if B == 0:
         return y
+    d32 = H.f32(decay)
     H.launch(dev, _lib.load().m3_gated_step, GatedDesc(B, 1, D, H.code(x.dtype), c),
-             _args(prepared, H.f32(decay), None, None), h.data_ptr(), y.data_ptr())
+             _args(prepared, d32, None, None), h.data_ptr(), y.data_ptr())
     increment_version(h)
     return y

@@ -23,6 +23,7 @@ from . import _launch as H
 from ._lib import AddNormDesc, Norm8Desc, NormDesc
 
 MAX_D = 32768           # longest row of the kernels
+_DENSE = torch.contiguous_format
 
 
 def _forward(x2, ld, w, b, desc, out_dtype, stats):
@@ -125,13 +126,14 @@ def m3_rms_norm(x, weight, eps=1e-5, out_dtype=None):
 
 def _add_forward(x2, lx, r2, lr, w, desc, out_dtype, stats):
     """(y, s, rstd or None) of rows."""
-    rows, d = r2.shape
-    y = torch.empty((rows, d), device=x2.device, dtype=out_dtype)
-    s = torch.empty((rows, d), device=x2.device, dtype=r2.dtype)
+    s = torch.empty_like(r2, memory_format=_DENSE)
+    y = torch.empty_like(r2, dtype=out_dtype, memory_format=_DENSE)
+    rows = desc.rows
     st = torch.empty(rows, device=x2.device, dtype=torch.float32) if stats else None
     if rows:
         H.launch(x2.get_device(), _lib.load().m3_add_norm_fwd, desc, x2.data_ptr(), lx,
-                 r2.data_ptr(), lr, w.data_ptr(), y.data_ptr(), s.data_ptr(), H.ptr(st))
+                 r2.data_ptr(), lr, w.data_ptr(), y.data_ptr(), s.data_ptr(),
+                 st.data_ptr() if stats else None)
     return y, s, st
 
 
@@ -189,17 +191,17 @@ class _AddNormFn(torch.autograd.Function):
 
 
 def _check_rows(name, x, weight, residual, eps):
-    d = x.shape[-1] if x.dim() else 0
-    if d < 1 or weight.shape != (d,):
+    shape = x.shape
+    d = shape[-1] if shape else 0
+    if d < 1 or weight.shape != shape[-1:]:
         raise ValueError(f"{name}: weight of the length of x's last dimension")
-    if residual is not None and residual.shape != x.shape:
+    if residual is not None and residual.shape != shape:
         raise ValueError(f"{name}: the residual has x's shape")
     if d > MAX_D:
         raise ValueError(f"{name}: rows of at most {MAX_D} elements")
     eps = float(eps)
     if not eps >= 0:
         raise ValueError(f"{name}: eps must not be negative")
-    H.code(x.dtype), H.code(x.dtype if residual is None else residual.dtype)
     return d, eps
 
 
@@ -214,17 +216,19 @@ def m3_add_rms_norm(x, residual, weight, eps=1e-5, out_dtype=None):
     mode); the gradients of y and s reach x and the residual as one sum."""
     name = "m3_add_rms_norm"
     d, eps = _check_rows(name, x, weight, residual, eps)
-    out_dtype = residual.dtype if out_dtype is None else out_dtype
-    H.code(out_dtype)
+    xt, st = x.dtype, residual.dtype
+    out_dtype = st if out_dtype is None else out_dtype
+    cx, cs, cy = H.code(xt), H.code(st), H.code(out_dtype)
     H.refuse_tangents(name, x, residual, weight)
     H.device_index(x, residual, weight)
     if H.needs_grad(x, residual, weight):
         return _AddNormFn.apply(x, residual, weight, eps, out_dtype)
-    x2, lx = H.rows(x if x.dim() == 2 else x.reshape(-1, d))
-    r2, lr = H.rows(residual if x.dim() == 2 else residual.reshape(-1, d))
-    desc = AddNormDesc(x2.shape[0], d, H.code(x2.dtype), H.code(r2.dtype), H.code(out_dtype), eps)
-    y, s, _ = _add_forward(x2, lx, r2, lr, H.f32(weight), desc, out_dtype, False)
-    return (y, s) if x.dim() == 2 else (y.view(x.shape), s.view(x.shape))
+    flat = x.dim() == 2
+    x2, lx = H.rows(x if flat else x.reshape(-1, d))
+    r2, lr = H.rows(residual if flat else residual.reshape(-1, d))
+    y, s, _ = _add_forward(x2, lx, r2, lr, H.f32(weight),
+                           AddNormDesc(x2.shape[0], d, cx, cs, cy, eps), out_dtype, False)
+    return (y, s) if flat else (y.view(x.shape), s.view(x.shape))
 
 
 def _grouped_rows(t, d, group):
@@ -247,27 +251,28 @@ def m3_rms_norm_8bit(x, weight, residual=None, eps=1e-5, dtype=torch.float8_e4m3
     group with a NaN has the scale NaN.  Inference only."""
     name = "m3_rms_norm_8bit"
     d, eps = _check_rows(name, x, weight, residual, eps)
-    if dtype not in (torch.float8_e4m3fn, torch.int8):
+    cx = H.code(x.dtype)
+    cs = cx if residual is None else H.code(residual.dtype)
+    e4m3 = dtype is torch.float8_e4m3fn
+    if not e4m3 and dtype is not torch.int8:
         raise TypeError(f"{name}: dtype is torch.float8_e4m3fn or torch.int8")
-    if group not in (None, 32, 64, 128) or (group and d % group):
+    if group is not None and (group not in (32, 64, 128) or d % group):
         raise ValueError(f"{name}: group is None, 32, 64 or 128 and divides d")
     if H.needs_grad(x, weight, residual):
         raise ValueError(f"{name} has no derivative: call it under torch.no_grad()")
     H.refuse_tangents(name, x, weight, residual)
     dev = H.device_index(x, weight, residual)
     x2, lx = _grouped_rows(x, d, group)
-    r2, lr = (None, 0) if residual is None else _grouped_rows(residual, d, group)
+    q = torch.empty_like(x, dtype=dtype, memory_format=_DENSE)
+    scale = x.new_empty((*x.shape[:-1], d // group if group else 1), dtype=torch.float32)
+    s, r2, lr = None, None, 0
+    if residual is not None:
+        r2, lr = _grouped_rows(residual, d, group)
+        s = torch.empty_like(residual, memory_format=_DENSE)
     rows = x2.shape[0]
-    q = torch.empty(x.shape, device=x.device, dtype=dtype)
-    scale = torch.empty((*x.shape[:-1], d // group if group else 1), device=x.device,
-                        dtype=torch.float32)
-    s = None if r2 is None else torch.empty(x.shape, device=x.device, dtype=r2.dtype)
     if rows:
         w = H.f32(weight)
-        H.launch(dev, _lib.load().m3_norm8_fwd,
-                 Norm8Desc(rows, d, group or 0, H.code(x2.dtype),
-                           H.code(x2.dtype if r2 is None else r2.dtype),
-                           dtype is torch.float8_e4m3fn, eps),
+        H.launch(dev, _lib.load().m3_norm8_fwd, Norm8Desc(rows, d, group or 0, cx, cs, e4m3, eps),
                  x2.data_ptr(), lx, H.ptr(r2), lr, w.data_ptr(), q.data_ptr(), scale.data_ptr(),
                  H.ptr(s))
     return (q, scale) if s is None else (q, scale, s)

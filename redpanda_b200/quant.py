@@ -167,12 +167,13 @@ def m3_rows_linear_q4(x, weight, bias=None, norm_weight=None, eps=0.0, residual=
     if not isinstance(weight, Q4Weight):
         raise TypeError(f"{name}: weight is a Q4Weight")
     n, k = weight.d_out, weight.d_in
-    if x.dim() != 2 or x.shape[1] != k or x.shape[0] > MAX_ROWS:
+    shape, ty = x.shape, x.dtype
+    if len(shape) != 2 or shape[1] != k or shape[0] > MAX_ROWS:
         raise ValueError(f"{name}: x is (rows, d_in) with at most {MAX_ROWS} rows and the weight's "
                          f"d_in")
     if H.needs_grad(x, bias, norm_weight, residual, out0, out1):
         raise ValueError(f"{name} has no derivative: call it under torch.no_grad()")
-    code = H.code(x.dtype)
+    code = H.code(ty)
     if (bias is not None and bias.shape != (n,)) or \
             (norm_weight is not None and norm_weight.shape != (k,)):
         raise ValueError(f"{name}: bias is (d_out,) and norm_weight (d_in,)")
@@ -184,20 +185,25 @@ def m3_rows_linear_q4(x, weight, bias=None, norm_weight=None, eps=0.0, residual=
         raise ValueError(f"{name}: split lies between 0 and d_out")
     H.refuse_tangents(name, x, bias, norm_weight, residual)
     dev = H.device_index(x, weight.codes, weight.scales, bias, norm_weight, residual, out0, out1)
-    rows = x.shape[0]
-    if out0 is None and split > 0:
-        out0 = torch.empty(rows, split, device=x.device, dtype=x.dtype)
-    if out1 is None and split < n:
-        out1 = torch.empty(rows, n - split, device=x.device, dtype=x.dtype)
-    l0 = 0 if out0 is None else _rows(out0, "out0", (rows, split), x.dtype)
-    l1 = 0 if out1 is None else _rows(out1, "out1", (rows, n - split), x.dtype)
-    lr = 0 if residual is None else _rows(residual, "residual", (rows, n), x.dtype)
+    rows, rest = shape[0], n - split
+    l0, l1, lr = split, rest, 0
+    if out0 is not None:
+        l0 = _rows(out0, "out0", (rows, split), ty)
+    elif split:
+        out0 = x.new_empty(rows, split)
+    if out1 is not None:
+        l1 = _rows(out1, "out1", (rows, rest), ty)
+    elif rest:
+        out1 = x.new_empty(rows, rest)
+    if residual is not None:
+        lr = _rows(residual, "residual", (rows, n), ty)
     if rows == 0:
         return out0, out1
     x2, lx = H.rows(x)
     b, nw = H.f32(bias), H.f32(norm_weight)
     H.launch(dev, _lib.load().m3_rows_linear_q4,
              RowsQ4Desc(rows, k, n, weight.group, weight.has_center, code, split, bool(silu), eps),
-             x2.data_ptr(), lx, H.ptr(nw), weight.codes.data_ptr(), weight.scales.data_ptr(),
-             H.ptr(b), H.ptr(residual), lr, H.ptr(out0), l0, H.ptr(out1), l1, bool(overlap))
+             x2.data_ptr(), lx, H.ptr(nw), weight.codes.data_ptr(),
+             weight.scales.data_ptr(), H.ptr(b),
+             H.ptr(residual), lr, H.ptr(out0), l0, H.ptr(out1), l1, bool(overlap))
     return out0, out1
