@@ -216,20 +216,34 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
   }
 }
 
-// One token per row: a thread owns V channels and walks rows.
+// One token per row: a thread owns V channels and walks rows, the next row's loads
+// ahead of the present one's arithmetic.
+template <typename T, int V>
+struct StepRow {
+  Pack<T, V> x, r, g;
+  Pack<float, V> h;
+  __device__ __forceinline__ void load(const GatedStepParams& p, int b, int c) {
+    x = ld_pack<T, V>(static_cast<const T*>(p.x) + (size_t)b * p.ld_x + c);
+    r = ld_pack<T, V>(static_cast<const T*>(p.rg) + (size_t)b * p.ld_r + c);
+    g = ld_pack<T, V>(static_cast<const T*>(p.ig) + (size_t)b * p.ld_i + c);
+    h = ld_pack<float, V>(p.h + (size_t)b * p.D + c);
+  }
+};
 template <typename T, int V>
 __global__ void __launch_bounds__(256) gated_step_kernel(const GatedStepParams p) {
   const int c = (blockIdx.x * 32 + threadIdx.x) * V;
-  if (c >= p.D) return;
+  int b = blockIdx.y * blockDim.y + threadIdx.y;
+  const int step = gridDim.y * blockDim.y;
+  if (c >= p.D || b >= p.B) return;
+  StepRow<T, V> now;
+  now.load(p, b, c);
   float k[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) k[j] = -p.c * softplus_f(p.decay[c + j]);
-  for (int b = blockIdx.y * blockDim.y + threadIdx.y; b < p.B; b += gridDim.y * blockDim.y) {
-    const Pack<T, V> x = ld_pack<T, V>(static_cast<const T*>(p.x) + (size_t)b * p.ld_x + c),
-                     r = ld_pack<T, V>(static_cast<const T*>(p.rg) + (size_t)b * p.ld_r + c),
-                     g = ld_pack<T, V>(static_cast<const T*>(p.ig) + (size_t)b * p.ld_i + c);
-    float* hp = p.h + (size_t)b * p.D + c;
-    Pack<float, V> h = ld_pack<float, V>(hp);
+  for (; b < p.B; b += step) {
+    StepRow<T, V> next;
+    if (b + step < p.B) next.load(p, b + step, c);
+    Pack<float, V> h;
     Pack<T, V> y;
     y.zero();
 #pragma unroll
@@ -237,11 +251,11 @@ __global__ void __launch_bounds__(256) gated_step_kernel(const GatedStepParams p
       constexpr int o = V > 1 ? 1 : 0;
       float2 a, m, inv;
       decay2<false>(mul2(make_float2(k[j], k[j + o]),
-                  sigmoid2(make_float2(r.get(j), r.get(j + o)))), a, m);
+                         sigmoid2(make_float2(now.r.get(j), now.r.get(j + o)))), a, m);
       root2(m, m, inv);
-      const float2 in = mul2(mul2(m, sigmoid2(make_float2(g.get(j), g.get(j + o)))),
-                             make_float2(x.get(j), x.get(j + o)));
-      const float2 q = fma2(a, make_float2(h.get(j), h.get(j + o)), in);
+      const float2 in = mul2(mul2(m, sigmoid2(make_float2(now.g.get(j), now.g.get(j + o)))),
+                             make_float2(now.x.get(j), now.x.get(j + o)));
+      const float2 q = fma2(a, make_float2(now.h.get(j), now.h.get(j + o)), in);
       h.put(j, q.x);
       y.put(j, q.x);
       if (V > 1) {
@@ -249,19 +263,26 @@ __global__ void __launch_bounds__(256) gated_step_kernel(const GatedStepParams p
         y.put(j + o, q.y);
       }
     }
-    st_pack<float, V>(hp, h);
+    st_pack<float, V>(p.h + (size_t)b * p.D + c, h);
     st_pack<T, V>(static_cast<T*>(p.y) + (size_t)b * p.D + c, y);
+    now = next;
   }
 }
 
 template <typename T, int V>
 cudaError_t step_impl(const GatedStepParams& p, cudaStream_t s) {
+  static OncePerDevice known;
   const int tiles = (p.D + 32 * V - 1) / (32 * V);
   const int ty = p.B < 8 ? p.B : 8;
-  long long gy = (p.B + ty - 1) / ty;
-  const long long cap = (8LL * p.sms + tiles - 1) / tiles;
-  if (gy > cap) gy = cap;
-  if (gy > 65535) gy = 65535;
+  // one wave of CTAs, of rows in equal number
+  const int per = resident_ctas<gated_step_kernel<T, V>>(known, 256, 0);
+  if (per <= 0) return cudaErrorInvalidConfiguration;
+  long long gy = (p.B + ty - 1) / ty, cap = (long long)per * p.sms / tiles;
+  cap = cap < 1 ? 1 : cap > 65535 ? 65535 : cap;
+  if (gy > cap) {
+    const long long each = (gy + cap - 1) / cap;
+    gy = (gy + each - 1) / each;
+  }
   gated_step_kernel<T, V><<<dim3(tiles, (unsigned)gy), dim3(32, ty), 0, s>>>(p);
   return cudaGetLastError();
 }
@@ -354,12 +375,17 @@ cudaError_t launch_gated_fwd(const GatedParams& p, cudaStream_t s) {
 
 cudaError_t launch_gated_step(const GatedStepParams& p, cudaStream_t s) {
   const int e = dsize(p.dtype);
-  const bool v4 = p.D % 4 == 0 && p.ld_x % 4 == 0 && p.ld_r % 4 == 0 && p.ld_i % 4 == 0 &&
-                  aligned(p.h, 16) && aligned(p.x, 4 * e) && aligned(p.rg, 4 * e) &&
-                  aligned(p.ig, 4 * e) && aligned(p.y, 4 * e);
+  auto ok = [&](int v) {
+    const int b = v * e < 16 ? v * e : 16;
+    return p.D % v == 0 && p.ld_x % v == 0 && p.ld_r % v == 0 && p.ld_i % v == 0 &&
+           aligned(p.h, 16) && aligned(p.x, b) && aligned(p.rg, b) && aligned(p.ig, b) &&
+           aligned(p.y, b);
+  };
+  // 4 channels per thread: 8 of bf16 took 4.8 us instead of 3.8 for 100 rows of 4000,
+  // 14.4 instead of 14.0 for 2048 of 2048
   if (p.dtype == M3_BF16)
-    return v4 ? step_impl<__nv_bfloat16, 4>(p, s) : step_impl<__nv_bfloat16, 1>(p, s);
-  return v4 ? step_impl<float, 4>(p, s) : step_impl<float, 1>(p, s);
+    return ok(4) ? step_impl<__nv_bfloat16, 4>(p, s) : step_impl<__nv_bfloat16, 1>(p, s);
+  return ok(4) ? step_impl<float, 4>(p, s) : step_impl<float, 1>(p, s);
 }
 
 }  // namespace m3
