@@ -310,7 +310,7 @@ typedef struct m3_rows_q4_desc {
  *           outputs, blocks of 64 columns; both numbers rounded up, the columns to
  *           whole groups of 128 where group is 128.  Word j of lane l of a block
  *           holds, in bits 4 (h + 2 v + 4 e) up, the code of output l / 4 + 8 h and
- *           column 16 j + 8 v + 2 (l % 4) + e of the tile and block (h, v, e: 0, 1).
+ *           column 32 (j / 2) + 8 (l % 4) + 4 (j % 2) + 2 v + e (h, v, e: 0, 1).
  *   scales  (tiles, groups, 8) of two outputs each, l and l + 8: bf16 pairs of
  *           scale and center (64 bits) with center, else their two scales (32
  *           bits); 8- or 4-byte aligned; groups cover the rounded-up columns

@@ -20,8 +20,7 @@
 // A warp takes MT tiles of 16 outputs; the CTA's warps split tiles (mw) and the
 // columns (kw), whose totals are added in order.  Codes are laid out once so that a
 // lane's 16 bytes are its operand of four instructions (64 columns).  Inputs are
-// staged in shared memory as the instruction's fragments, `chunk` columns at a time;
-// codes and scales come through a ring of asynchronous copies per warp.
+// staged in shared memory, `chunk` columns at a time; codes and scales come through a ring of asynchronous copies per warp.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -33,6 +32,8 @@
 
 namespace m3 {
 namespace {
+
+constexpr int kPad = 32;           // columns behind a staged row
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], unsigned b0,
                                          unsigned b1) {
@@ -58,15 +59,6 @@ __device__ __forceinline__ void unpack(unsigned w, unsigned (&a)[4]) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ float2 load2(const T* p, int left, bool vec) {
-  if (vec && left > 1) {
-    const Pack<T, 2> v = ld_pack<T, 2>(p);
-    return make_float2(v.get(0), v.get(1));
-  }
-  return make_float2(left > 0 ? Elem<T>::get(p[0]) : 0.f, left > 1 ? Elem<T>::get(p[1]) : 0.f);
-}
-
 __device__ __forceinline__ float warp_total(float v, int width) {
   for (int m = width / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
   return v;
@@ -81,63 +73,67 @@ __device__ __forceinline__ float below(float v) {   // v without its top 16 bits
   return t == v ? 0.f : v - t;
 }
 
-// The inputs' fragments of two instructions (32 columns of k): a lane's 16 bytes
-// (b0, b1 of each) at (pair of instructions, column of the operand, lane % 4).  Only
-// the `cols` columns in use are kept; lanes of others read the last one's, and their
-// results are not used.
+// The inputs in shared memory: `cols` rows of bf16 (part by part, row by row), of the
+// chunk's columns and 32 more (so that 8 lanes' 16 bytes lie in different banks).  The
+// instruction's order of the 16 columns it takes at a time is free as long as both
+// operands agree: lane l's two instructions of 32 columns take the 8 columns from
+// 8 (l % 4), so its operands are 16 consecutive bytes of a row.
 //
-// Stages the columns from k0 of every row: fragments, the groups' sums of the
-// inputs and the squares' sums of every unit of U columns.
+// Stages the columns from k0 of every row, with the groups' sums of the inputs and
+// the squares' sums of every 128 columns.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, int left, bool vec) {
+  if (vec && left >= 4) {
+    const Pack<T, 4> v = ld_pack<T, 4>(p);
+    return make_float4(v.get(0), v.get(1), v.get(2), v.get(3));
+  }
+  return make_float4(left > 0 ? Elem<T>::get(p[0]) : 0.f, left > 1 ? Elem<T>::get(p[1]) : 0.f,
+                     left > 2 ? Elem<T>::get(p[2]) : 0.f, left > 3 ? Elem<T>::get(p[3]) : 0.f);
+}
+__device__ __forceinline__ uint2 top_halves(const float4& v) {
+  return make_uint2(top_halves(make_float2(v.x, v.y)), top_halves(make_float2(v.z, v.w)));
+}
+__device__ __forceinline__ float4 below(const float4& v) {
+  return make_float4(below(v.x), below(v.y), below(v.z), below(v.w));
+}
+
 template <typename T, int NB, int G, bool CENTER>
-__device__ void stage(const RowsQ4Params& p, int k0, int units, unsigned* frag, float* xs,
-                      float* sq, int parts) {
-  constexpr int U = G > 64 ? G : 64;
+__device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* xs, float* sq,
+                      int parts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int cols = parts * p.rows;
-  const T* x = static_cast<const T*>(p.x);
-  for (int u = warp; u < units; u += warps) {
+  const int row = (p.chunk + kPad) * 2;                 // bytes
+  const T* x = static_cast<const T*>(p.x) + k0;
+  const bool vec = p.vec != 0;
+  for (int c0 = warp * 128; c0 < n; c0 += warps * 128) {
+    const int c = c0 + lane * 4, left = p.d_in - k0 - c, at = left > 0 ? c : 0;
     // every row's loads before any is used
-    float2 v[kQ4Rows][U / 64], w[U / 64];
+    float4 v[kQ4Rows], w;
 #pragma unroll
-    for (int h = 0; h < U / 64; ++h) {
-      const int k = k0 + u * U + h * 64 + 2 * lane, left = p.d_in - k, at = left > 0 ? k : 0;
-#pragma unroll
-      for (int r = 0; r < kQ4Rows; ++r)
-        if (r < p.rows) v[r][h] = load2(x + (size_t)r * p.ld_x + at, left, p.vec != 0);
-      if (p.norm_w != nullptr) w[h] = load2(p.norm_w + at, left, p.vec != 0);
-    }
+    for (int r = 0; r < kQ4Rows; ++r)
+      if (r < p.rows) v[r] = load4(x + (size_t)r * p.ld_x + at, left, vec);
+    if (p.norm_w != nullptr) w = load4(p.norm_w + k0 + at, left, vec);
 #pragma unroll
     for (int r = 0; r < kQ4Rows; ++r) {
       if (r >= p.rows) break;
-      float sum = 0.f, ss = 0.f;
-#pragma unroll
-      for (int h = 0; h < U / 64; ++h) {
-        const int in = u * U + h * 64 + 2 * lane;
-        float2 y = v[r][h];
-        if (p.norm_w != nullptr) {
-          ss = fmaf(y.x, y.x, fmaf(y.y, y.y, ss));
-          y.x *= w[h].x;
-          y.y *= w[h].y;
-        }
-        if (CENTER) sum += y.x + y.y;
-        // instruction k / 16; pairs t and (half) t + 4 of its 16 columns
-        const int ks = in >> 4, half = lane >> 2 & 1, t = lane & 3;
-        unsigned* f = frag + (((ks >> 1) * cols + r) * 4 + t) * 4 + (ks & 1) * 2 + half;
-        *f = top_halves(y);
-        if (parts == 3) {
-          y = make_float2(below(y.x), below(y.y));
-          f[p.rows * 16] = top_halves(y);
-          f[p.rows * 32] = top_halves(make_float2(below(y.x), below(y.y)));
-        }
+      float4 y = v[r];
+      if (p.norm_w != nullptr) {
+        float ss = fmaf(y.x, y.x, y.y * y.y) + fmaf(y.z, y.z, y.w * y.w);
+        ss = warp_total(ss, 32);
+        if (lane == 0) sq[(k0 + c0) / 128 * kQ4Rows + r] = ss;
+        y = make_float4(y.x * w.x, y.y * w.y, y.z * w.z, y.w * w.w);
       }
       if (CENTER) {
-        sum = warp_total(sum, G < 64 ? 16 : 32);
-        if (G < 64 ? (lane & 15) == 0 : lane == 0)
-          xs[(G < 64 ? u * 2 + (lane >> 4) : u) * (8 * NB) + r] = sum;
+        const float sum = warp_total((y.x + y.y) + (y.z + y.w), G / 4);
+        if (lane % (G / 4) == 0 && c < n) xs[c / G * (8 * NB) + r] = sum;
       }
-      if (p.norm_w != nullptr) {
-        ss = warp_total(ss, 32);
-        if (lane == 0) sq[(k0 / U + u) * kQ4Rows + r] = ss;
+      if (c < n) {
+        char* to = rows + r * row + c * 2;
+        *reinterpret_cast<uint2*>(to) = top_halves(y);
+        if (parts == 3) {
+          y = below(y);
+          *reinterpret_cast<uint2*>(to + p.rows * row) = top_halves(y);
+          *reinterpret_cast<uint2*>(to + 2 * p.rows * row) = top_halves(below(y));
+        }
       }
     }
   }
@@ -152,19 +148,19 @@ struct Ring {
   static constexpr int kSlots = MT * BU == 1 ? 8 : MT * BU == 2 ? 6 : 4;
 };
 
-// shared memory: the warps' rings, the fragments, the groups' sums, and the squares'
-// sums of all units; the totals lie over rings and fragments at the end
+// shared memory: the warps' rings, the inputs, the groups' sums, and the squares' sums
+// of all columns; the totals lie over rings and inputs at the end
 struct Layout {
-  int frag, xs, sq, total;         // bytes
+  int x, xs, sq, total;            // bytes
 };
 template <int NB, int MT, int G, bool CENTER>
 __host__ __device__ inline Layout layout(int warps, int cols, int chunk, int units, bool norm) {
   using R = Ring<MT, G, CENTER>;
   Layout l;
-  l.frag = warps * R::kSlots * R::kSlot;
-  l.xs = l.frag + chunk * 2 * cols;
+  l.x = warps * R::kSlots * R::kSlot;
+  l.xs = l.x + (chunk + kPad) * 2 * cols;
   l.sq = l.xs + (CENTER ? chunk / G * 8 * NB * 4 : 0);
-  l.total = l.sq + (norm ? units * kQ4Rows * 4 : 0);
+  l.total = l.sq + (norm ? (units * R::U + 127) / 128 * kQ4Rows * 4 : 0);
   return l;
 }
 
@@ -189,7 +185,7 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
   const Layout lay = layout<NB, MT, G, CENTER>(p.mw * p.kw, cols, p.chunk, units,
                                                p.norm_w != nullptr);
   char* ring = smem + warp * R::kSlots * R::kSlot;
-  unsigned* frag = reinterpret_cast<unsigned*>(smem + lay.frag);
+  char* rows = smem + lay.x;
   float* xs = reinterpret_cast<float*>(smem + lay.xs);
   float* sq = reinterpret_cast<float*>(smem + lay.sq);
   const int tiles = (p.d_out + 15) / 16, tile0 = (blockIdx.x * p.mw + mw) * MT;
@@ -228,15 +224,18 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
   if (CENTER)   // the columns of the inputs' lower parts have no sum of their own
     for (int i = threadIdx.x; i < p.chunk / G * 8 * NB; i += blockDim.x) xs[i] = 0.f;
 
-  int at[NB];                                        // of the lane's fragments
+  // the lane's operands of block 0; lanes of columns that are not in use read the last
+  // one's, and their results are not used
+  const char* mine[NB];
 #pragma unroll
-  for (int c = 0; c < NB; ++c) at[c] = (min(c * 8 + (lane >> 2), cols - 1) * 4 + (lane & 3)) * 4;
+  for (int c = 0; c < NB; ++c)
+    mine[c] = rows + min(c * 8 + (lane >> 2), cols - 1) * (p.chunk + kPad) * 2 + (lane & 3) * 16;
   float tot[MT][NB][4] = {};
   int slot = 0;
   for (int i0 = 0; i0 * p.kw < units; i0 += per_chunk) {   // chunks of the columns
     const int u0 = i0 * p.kw;
     __syncthreads();
-    stage<T, NB, G, CENTER>(p, u0 * U, min(chunk_units, units - u0), frag, xs, sq, parts);
+    stage<T, NB, G, CENTER>(p, u0 * U, min(chunk_units, units - u0) * U, rows, xs, sq, parts);
     __syncthreads();
     const int end = min(per, i0 + per_chunk);
     for (int i = i0; i < end; ++i) {
@@ -246,7 +245,6 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
       const char* from = ring + slot * R::kSlot;
       slot = slot + 1 == R::kSlots ? 0 : slot + 1;
       const int u = (i - i0) * p.kw + kw;            // in the chunk
-      const unsigned* fu = frag + u * (U / 32) * cols * 16;
       float acc[MT][NB][4];
 #pragma unroll
       for (int b = 0; b < BU; ++b) {
@@ -260,7 +258,7 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
           uint4 f[NB];
 #pragma unroll
           for (int c = 0; c < NB; ++c)
-            f[c] = *reinterpret_cast<const uint4*>(fu + (b * 2 + jp) * cols * 16 + at[c]);
+            f[c] = *reinterpret_cast<const uint4*>(mine[c] + (u * BU + b) * 128 + jp * 64);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             if (first)
@@ -312,11 +310,11 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
     }
   }
 
-  // the rows' 1 / sqrt(mean(x^2) + eps): units in order, strided over a warp's lanes
+  // the rows' 1 / sqrt(mean(x^2) + eps): 128 columns at a time, strided over a warp's lanes
   if (p.norm_w != nullptr)
     for (int r = warp; r < p.rows; r += blockDim.x >> 5) {
       float v = 0.f;
-      for (int u = lane; u < units; u += 32) v += sq[u * kQ4Rows + r];
+      for (int u = lane; u * 128 < p.d_in; u += 32) v += sq[u * kQ4Rows + r];
       v = warp_total(v, 32);
       if (lane == 0) s_rstd[r] = rsqrtf(v / (float)p.d_in + p.eps);
     }

@@ -112,9 +112,9 @@ class Q4Weight:
         tiles, cols = -(-d_out // 16), -(-d_in // unit) * unit
         full = q.new_full((tiles * 16, cols), 8)
         full[:d_out, :d_in] = q
-        # output 8 h + l / 4, column 64 b + 16 j + 8 v + 2 (l % 4) + e
-        q = full.view(tiles, 2, 8, cols // 64, 4, 2, 4, 2).permute(0, 3, 2, 6, 4, 7, 5, 1)
-        codes = (q[..., 0] | q[..., 1] << 4).flatten(5).view(torch.int32).view(tiles, -1, 32, 4)
+        # output 8 h + l / 4, column 64 b + 32 (j / 2) + 8 (l % 4) + 4 (j % 2) + 2 v + e
+        q = full.view(tiles, 2, 8, cols // 64, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1)
+        codes = (q[..., 0] | q[..., 1] << 4).flatten(6).view(torch.int32).view(tiles, -1, 32, 4)
         parts = []
         for t in (scale, center):
             if t is not None:
@@ -128,8 +128,8 @@ class Q4Weight:
         """The weight (d_out, d_in) that the codes stand for."""
         tiles, groups = self.scales.shape[:2]
         cols = groups * self.group
-        b = self.codes.view(torch.uint8).view(tiles, cols // 64, 8, 4, 4, 2, 2)
-        q = torch.stack([b & 15, b >> 4], 7).permute(0, 7, 2, 1, 4, 6, 3, 5)
+        b = self.codes.view(torch.uint8).view(tiles, cols // 64, 8, 4, 2, 2, 2, 2)
+        q = torch.stack([b & 15, b >> 4], 8).permute(0, 8, 2, 1, 4, 3, 5, 7, 6)
         q = q.reshape(tiles * 16, groups, self.group).float() - 8
         s = self.scales.float()
         if not self.has_center:

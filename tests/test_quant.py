@@ -38,8 +38,9 @@ def test_layout_and_back(n, k, group, center):
     blocks = q.codes.shape[1]
     for o in range(n):
         for c in range(k):
-            word = int(q.codes[o // 16, c // 64, (o % 8) * 4 + c % 8 // 2, c % 64 // 16])
-            at = 4 * (o % 16 // 8 + 2 * (c % 16 // 8) + 4 * (c % 2))
+            word = int(q.codes[o // 16, c // 64, (o % 8) * 4 + c % 32 // 8,
+                               c % 64 // 32 * 2 + c % 8 // 4])
+            at = 4 * (o % 16 // 8 + 2 * (c % 4 // 2) + 4 * (c % 2))
             assert (word >> at) & 15 == codes[o, c]
     assert blocks * 64 % max(group, 64) == 0
 
