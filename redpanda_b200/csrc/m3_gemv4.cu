@@ -104,13 +104,31 @@ __device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* x
   const int row = (p.chunk + kPad) * 2;                 // bytes
   const T* x = static_cast<const T*>(p.x) + k0;
   const bool vec = p.vec != 0;
+  const bool raw = sizeof(T) == 2 && parts == 1 && p.vec8 != 0;   // rows as they are
+  if (raw) {
+    for (int r = 0; r < p.rows; ++r)
+      for (int c = (warp * 32 + lane) * 8; c < n; c += warps * 256) {
+        const int left = (p.d_in - k0 - c) * 2, bytes = left < 0 ? 0 : left < 16 ? left : 16;
+        const T* from = x + (size_t)r * p.ld_x + (bytes > 0 ? c : 0);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         (unsigned)__cvta_generic_to_shared(rows + r * row + c * 2)),
+                     "l"(from), "r"(bytes)
+                     : "memory");
+      }
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    if (!CENTER) return;
+    __syncthreads();
+  }
   for (int c0 = warp * 128; c0 < n; c0 += warps * 128) {
     const int c = c0 + lane * 4, left = p.d_in - k0 - c, at = left > 0 ? c : 0;
     // every row's loads before any is used
     float4 v[kQ4Rows], w;
 #pragma unroll
     for (int r = 0; r < kQ4Rows; ++r)
-      if (r < p.rows) v[r] = load4(x + (size_t)r * p.ld_x + at, left, vec);
+      if (r < p.rows) {
+        if (raw) v[r] = load4(reinterpret_cast<const T*>(rows + r * row) + (c < n ? c : 0), 4, true);
+        else v[r] = load4(x + (size_t)r * p.ld_x + at, left, vec);
+      }
     if (p.norm_w != nullptr) w = load4(p.norm_w + k0 + at, left, vec);
 #pragma unroll
     for (int r = 0; r < kQ4Rows; ++r) {
@@ -126,7 +144,7 @@ __device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* x
         const float sum = warp_total((y.x + y.y) + (y.z + y.w), G / 4);
         if (lane % (G / 4) == 0 && c < n) xs[c / G * (8 * NB) + r] = sum;
       }
-      if (c < n) {
+      if (c < n && !raw) {
         char* to = rows + r * row + c * 2;
         *reinterpret_cast<uint2*>(to) = top_halves(y);
         if (parts == 3) {
