@@ -4,6 +4,8 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <initializer_list>
+
 #include "m3_api_util.h"
 #include "m3_internal.h"
 #include "m3_ops.h"
@@ -76,7 +78,8 @@ int check_gated(const m3_gated_desc* d) {
 }
 
 // Fills what the gated recurrence's forward and backward share; returns a status.
-int fill_gated(const m3_gated_desc* d, const m3_gated_args* a, bool backward, GatedParams* p) {
+int fill_gated(const m3_gated_desc* d, const m3_gated_args* a, bool backward,
+               std::initializer_list<const void*> more, GatedParams* p) {
   const int e = dsize(d->dtype);
   if (!a || !a->x || !a->rg || !a->ig || !a->decay) return M3_ERR_NULL;
   if (a->ld_x < d->d_inner || a->ld_r < d->d_inner || a->ld_i < d->d_inner) return M3_ERR_SHAPE;
@@ -89,9 +92,15 @@ int fill_gated(const m3_gated_desc* d, const m3_gated_args* a, bool backward, Ga
   p->ld_x = a->ld_x; p->ld_r = a->ld_r; p->ld_i = a->ld_i;
   p->decay = a->decay; p->c = d->c; p->h0 = a->state; p->lengths = a->lengths;
   p->B = d->batch; p->L = d->seqlen; p->D = d->d_inner; p->dtype = d->dtype;
-  const int v = 16 / e;
-  p->vec = d->d_inner % v == 0 && a->ld_x % v == 0 && a->ld_r % v == 0 && a->ld_i % v == 0 &&
-           aligned(a->x, 16) && aligned(a->rg, 16) && aligned(a->ig, 16);
+  // rows of vectors (16 bytes), of words, or of half words; `more`: the other arrays
+  auto rows_of = [&](int bytes) {
+    const int v = bytes / e;
+    bool ok = d->d_inner % v == 0 && a->ld_x % v == 0 && a->ld_r % v == 0 && a->ld_i % v == 0 &&
+              aligned(a->x, bytes) && aligned(a->rg, bytes) && aligned(a->ig, bytes);
+    for (const void* q : more) ok = ok && aligned(q, bytes);
+    return ok;
+  };
+  p->copy = rows_of(16) ? 2 : e == 4 || rows_of(4) ? 1 : 0;
   gated_plan(p->B, p->L, p->D, backward, device_sms(), p);
   if (p->splits > 1) p->err = device_err_ptr();
   return M3_OK;
@@ -548,8 +557,7 @@ int m3_gated_fwd(const m3_gated_desc* desc, const m3_gated_args* args, void* y, 
     return M3_ERR_ALIAS;
   GatedParams p;
   memset(&p, 0, sizeof(p));
-  if ((rc = fill_gated(desc, args, false, &p)) != M3_OK) return rc;
-  p.vec = p.vec && aligned(y, 16);
+  if ((rc = fill_gated(desc, args, false, {y}, &p)) != M3_OK) return rc;
   p.y = y; p.h_last = h_last; p.ckpt = ckpt;
   return status(launch_gated_fwd(p, static_cast<cudaStream_t>(stream)));
 }
@@ -576,10 +584,8 @@ int m3_gated_bwd(const m3_gated_desc* desc, const m3_gated_args* args, const voi
     if (o == args->x || o == args->rg || o == args->ig || o == g) return M3_ERR_ALIAS;
   GatedBwdParams q;
   memset(&q, 0, sizeof(q));
-  if ((rc = fill_gated(desc, args, true, &q.f)) != M3_OK) return rc;
+  if ((rc = fill_gated(desc, args, true, {g, d_x, d_rg, d_ig}, &q.f)) != M3_OK) return rc;
   if (!workspace || workspace_bytes < m3_gated_bwd_workspace_bytes(desc)) return M3_ERR_WORKSPACE;
-  q.f.vec = q.f.vec && aligned(g, 16) && aligned(d_x, 16) && aligned(d_rg, 16) &&
-            aligned(d_ig, 16);
   q.f.ckpt = const_cast<float*>(ckpt);
   q.g = g; q.dx = d_x; q.drg = d_rg; q.dig = d_ig; q.ddecay = d_decay;
   q.part = static_cast<float*>(workspace);

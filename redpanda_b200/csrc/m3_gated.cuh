@@ -109,32 +109,49 @@ template <int LC, int TS> struct Lanes {
   static constexpr int kSub = 32 / LC, kTile = 2 * LC, kSteps = TS * kSub;
 };
 
+// How rows are copied, by what their starts and lengths allow: 16 bytes at a time,
+// words (fp32, and bf16 rows of whole words), or words that bf16 rows start in the
+// middle of.  All asynchronous: without, a row that is not aligned to 16 bytes would
+// be waited for where it is asked for (2 x 16001 x 1281 fp32: XX us).
+enum Copy { kHalfWords = 0, kWords = 1, kVectors = 2 };
+
 // A warp's rows of NA arrays: kSteps steps of a tile, row (i, sub) (step i of run
 // sub) at i * kSub + sub, so that lanes read neighbouring words.  Each warp copies
 // and reads its own rows only; rows past the length and channels past D are not
 // copied, and what lies there is not used.
-template <typename T, int NA, int LC, int TS, bool VEC>
+template <typename T, int NA, int LC, int TS, int MODE>
 struct Stage {
   using La = Lanes<LC, TS>;
-  static constexpr int kRow = La::kTile * (int)sizeof(T);          // bytes
-  static constexpr int kArray = La::kSteps * kRow;
+  static_assert(MODE != kHalfWords || sizeof(T) == 2, "fp32 rows are whole words");
+  static constexpr bool kPairs = MODE == kVectors || (MODE == kWords && sizeof(T) == 2);
+  // bytes; a row that starts in the middle of a word has one word more
+  static constexpr int kRow = La::kTile * (int)sizeof(T) + (MODE == kHalfWords ? 4 : 0);
+  static constexpr int kArray = (La::kSteps * kRow + 15) / 16 * 16;
   static constexpr int kBytes = NA * kArray;                       // per warp
   static constexpr int V = 16 / (int)sizeof(T), PR = La::kTile / V, RI = 32 / PR;
   const T* p[NA];                    // of step t0 of the row: this lane's first piece
+  const T* lo[NA]; const T* hi[NA];  // kHalfWords: the array's bounds
+
+  __device__ __forceinline__ void word(unsigned s, const void* g) const {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(g) : "memory");
+  }
+  static __device__ __forceinline__ int row_at(int rr) {
+    return (rr % TS * La::kSub + rr / TS) * kRow;
+  }
 
   // rows t0 .. below n; channels c0 .. below D
   __device__ __forceinline__ void issue(char* buf, const long long (&ld)[NA], int t0, int n,
                                         int c0, int D) const {
     const int lane = threadIdx.x;
-    if constexpr (VEC) {
+    const unsigned to = (unsigned)__cvta_generic_to_shared(buf);
+    if constexpr (MODE == kVectors) {
       const int row = lane / PR, c = lane % PR * V;
       if (c0 + c < D) {
 #pragma unroll
         for (int i = 0; i < La::kSteps / RI; ++i) {
           const int rr = i * RI + row;
           if (t0 + rr < n) {
-            const int at = (rr % TS * La::kSub + rr / TS) * kRow + c * (int)sizeof(T);
-            const unsigned s = (unsigned)__cvta_generic_to_shared(buf) + at;
+            const unsigned s = to + row_at(rr) + c * (int)sizeof(T);
 #pragma unroll
             for (int k = 0; k < NA; ++k)
               asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s + k * kArray),
@@ -143,26 +160,61 @@ struct Stage {
           }
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    } else {
-      const int sub = lane / LC, c = c0 + lane % LC * 2;
+    } else if constexpr (MODE == kWords) {
+      constexpr int E = 4 / (int)sizeof(T), W = La::kTile / E;     // elements of a word, words of a row
 #pragma unroll
-      for (int k = 0; k < NA; ++k)
-        for (int i = 0; i < TS; ++i)
-          if (t0 + sub * TS + i < n) {
-            const T* g = p[k] + (long long)(sub * TS + i) * ld[k];
-            T* s = reinterpret_cast<T*>(buf + k * kArray + (i * La::kSub + sub) * kRow) +
-                   lane % LC * 2;
-            if (c < D) s[0] = g[0];
-            if (c + 1 < D) s[1] = g[1];
+      for (int i = 0; i < La::kSteps * W / 32; ++i) {
+        const int rr = (i * 32 + lane) / W, w = (i * 32 + lane) % W;
+        if (t0 + rr < n && c0 + w * E < D) {
+#pragma unroll
+          for (int k = 0; k < NA; ++k)
+            word(to + k * kArray + row_at(rr) + w * 4, p[k] + rr * ld[k] + w * E);
+        }
+      }
+    } else {
+      // word w of a row holds its channels 2 w and 2 w + 1, or 2 w - 1 and 2 w; a lane
+      // copies the word of its first channel, and a run's last lane the one behind it
+      const int sub = lane / LC, w = lane % LC, c = c0 + 2 * w;
+#pragma unroll
+      for (int k = 0; k < NA; ++k) {
+        const T* g = p[k] + sub * TS * ld[k] + 2 * w;
+        // whether a word can pass the array's ends
+        const bool inside = p[k] > lo[k] && p[k] + (La::kSteps - 1) * ld[k] + La::kTile < hi[k];
+#pragma unroll
+        for (int i = 0; i < TS; ++i, g += ld[k]) {
+          const uintptr_t at = reinterpret_cast<uintptr_t>(g);
+          const int odd = (int)(at >> 1 & 1);
+          const T* a = reinterpret_cast<const T*>(at & ~(uintptr_t)3);
+          const unsigned s = to + k * kArray + row_at(sub * TS + i) + w * 4;
+          if (t0 + sub * TS + i >= n || c - odd >= D) continue;
+          const bool next = odd && w == LC - 1 && c + 1 < D;
+          if (inside) {
+            word(s, a);
+            if (next) word(s + 4, a + 2);
+          } else {
+            T* q = reinterpret_cast<T*>(buf + (s - to));
+            if (a >= lo[k]) q[0] = a[0];
+            if (a + 1 < hi[k]) q[1] = a[1];
+            if (next) {
+              q[2] = a[2];
+              if (a + 3 < hi[k]) q[3] = a[3];
+            }
           }
+        }
+      }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // p[k] for the row that starts at `row` (b L + t0)
-  __device__ __forceinline__ void at(int k, const void* base, long long row, long long ld, int c0) {
+  // p[k] for the row that starts at `row` (b L + t0), of `rows`
+  __device__ __forceinline__ void at(int k, const void* base, long long row, long long rows,
+                                     long long ld, int c0, int D) {
     const int lane = threadIdx.x;
-    p[k] = static_cast<const T*>(base) + (row + (VEC ? lane / PR : 0)) * ld + c0 +
-           (VEC ? lane % PR * V : lane % LC * 2);
+    p[k] = static_cast<const T*>(base) + (row + (MODE == kVectors ? lane / PR : 0)) * ld + c0 +
+           (MODE == kVectors ? lane % PR * V : 0);
+    if constexpr (MODE == kHalfWords) {
+      lo[k] = static_cast<const T*>(base);
+      hi[k] = lo[k] + (rows - 1) * ld + D;
+    }
   }
   // all but the last LEFT calls of issue are complete
   template <int LEFT = 0>
@@ -170,19 +222,43 @@ struct Stage {
     asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
     __syncwarp();
   }
+  // Whether the rows of this lane's run start in the middle of a word: bit k for its
+  // first step's, bit NA + k for whether that changes from step to step
+  // (kHalfWords; row: b L + the step)
+  __device__ __forceinline__ unsigned odd_rows(const void* const (&base)[NA],
+                                               const long long (&ld)[NA], long long row,
+                                               int c0) const {
+    unsigned m = 0;
+    if constexpr (MODE == kHalfWords)
+#pragma unroll
+      for (int k = 0; k < NA; ++k) {
+        m |= (unsigned)((reinterpret_cast<uintptr_t>(base[k]) >> 1) + row * ld[k] + c0 & 1) << k;
+        m |= (unsigned)(ld[k] & 1) << (NA + k);
+      }
+    return m;
+  }
   // the lane's pair of step i of array k
-  static __device__ __forceinline__ float2 get(const char* buf, int k, int i) {
-    const Pack<T, 2> v = ld_pack<T, 2>(
-        reinterpret_cast<const T*>(buf + k * kArray + i * La::kSub * kRow) + 2 * threadIdx.x);
-    return make_float2(v.get(0), v.get(1));
+  static __device__ __forceinline__ float2 get(const char* buf, int k, int i, unsigned odd) {
+    const char* from = buf + k * kArray + i * La::kSub * kRow;
+    if constexpr (MODE == kHalfWords) {
+      const unsigned* q = reinterpret_cast<const unsigned*>(
+          from + threadIdx.x / LC * kRow) + threadIdx.x % LC;
+      const unsigned a = q[0], b = q[1];
+      const bool o = (odd >> k ^ (odd >> (NA + k) & i)) & 1;
+      return make_float2(__uint_as_float(o ? a & 0xffff0000u : a << 16),
+                         __uint_as_float(o ? b << 16 : a & 0xffff0000u));
+    } else {
+      const Pack<T, 2> v = ld_pack<T, 2>(reinterpret_cast<const T*>(from) + 2 * threadIdx.x);
+      return make_float2(v.get(0), v.get(1));
+    }
   }
 };
 
 // A lane's pair of channels in a (.., D) array, element by element where a pair
 // may be cut or is not aligned.
-template <bool VEC, typename T>
+template <bool PAIR, typename T>
 __device__ __forceinline__ void store_pair(T* p, float2 v, int left) {
-  if constexpr (VEC) {
+  if constexpr (PAIR) {
     if (left > 0) {
       if constexpr (sizeof(T) == 2) *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v);
       else *reinterpret_cast<float2*>(p) = v;

@@ -52,12 +52,12 @@ __device__ __forceinline__ Factors factors(float2 k, float2 x, float2 rg, float2
   return f;
 }
 
-template <typename T, int LC, int TS, bool VEC>
+template <typename T, int LC, int TS, int MODE>
 __global__ void __launch_bounds__(256, 2)
     gated_bwd_kernel(const GatedBwdParams q) {
   extern __shared__ __align__(16) char smem[];
   static_assert(TS == kGatedCkpt, "a run starts at a checkpoint");
-  using St = Stage<T, 4, LC, TS, VEC>;
+  using St = Stage<T, 4, LC, TS, MODE>;
   using La = Lanes<LC, TS>;
   const GatedParams& p = q.f;
   const int lane = threadIdx.x, w = __shfl_sync(0xffffffffu, threadIdx.y, 0), W = blockDim.y;
@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(256, 2)
   const int left = p.D - c, D = p.D, L = p.L, span = S * W * La::kSteps;
   const int tw0 = (rank * W + w) * La::kSteps, own = lane / LC * TS;   // of the warp; of the run
   const long long ld[4] = {p.ld_x, p.ld_r, p.ld_i, D};
+  const void* const bases[4] = {p.x, p.rg, p.ig, q.g};
   char* buf = smem + w * St::kBytes;
   const Joint<LC> joint(smem + W * St::kBytes, W, S);
   St st;
@@ -81,10 +82,10 @@ __global__ void __launch_bounds__(256, 2)
   auto start = [&](int b, int n) {
     const int tw = (n - 1) / span * span + tw0;
     const long long row = (long long)b * L + tw;
-    st.at(0, p.x, row, ld[0], c0);
-    st.at(1, p.rg, row, ld[1], c0);
-    st.at(2, p.ig, row, ld[2], c0);
-    st.at(3, q.g, row, ld[3], c0);
+    st.at(0, p.x, row, (long long)p.B * L, ld[0], c0, D);
+    st.at(1, p.rg, row, (long long)p.B * L, ld[1], c0, D);
+    st.at(2, p.ig, row, (long long)p.B * L, ld[2], c0, D);
+    st.at(3, q.g, row, (long long)p.B * L, ld[3], c0, D);
     st.issue(buf, ld, tw, n, c0, D);
   };
   int n = row_length(p.lengths, blockIdx.y, L), n2;
@@ -99,9 +100,9 @@ __global__ void __launch_bounds__(256, 2)
     for (int t0 = passes * span + tw0 + own; t0 - tw0 - own < L; t0 += span)
       for (int i = 0; i < TS && t0 + i < L; ++i) {
         const size_t at = (size_t)(base + t0 + i) * D + c;
-        store_pair<VEC>(static_cast<T*>(q.dx) + at, f2(0.f), left);
-        store_pair<VEC>(static_cast<T*>(q.drg) + at, f2(0.f), left);
-        store_pair<VEC>(static_cast<T*>(q.dig) + at, f2(0.f), left);
+        store_pair<St::kPairs>(static_cast<T*>(q.dx) + at, f2(0.f), left);
+        store_pair<St::kPairs>(static_cast<T*>(q.drg) + at, f2(0.f), left);
+        store_pair<St::kPairs>(static_cast<T*>(q.dig) + at, f2(0.f), left);
       }
     float2 carry = f2(0.f);                          // a_{t+1} q_{t+1}
     int tw = (passes - 1) * span + tw0;
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(256, 2)
     float2 h = tw + own < n ? load_pair(ck, left) : f2(0.f);
     for (int k0 = passes; k0 > 0; --k0, tw -= span) {
       const int t0 = tw + own;
+      const unsigned odd = st.odd_rows(bases, ld, base + t0, c0);
       St::wait();
       // FAST: every step of the warp is one of the sequence, and no decay is far from 1
       auto pass = [&](auto fast) {
@@ -117,9 +119,9 @@ __global__ void __launch_bounds__(256, 2)
         float2 a[TS], X[TS], I[TS], A[TS], R[TS], g[TS];
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const Factors f = factors<FAST>(k, St::get(buf, 0, i), St::get(buf, 1, i),
-                                          St::get(buf, 2, i), h);
-          g[i] = St::get(buf, 3, i);
+          const Factors f = factors<FAST>(k, St::get(buf, 0, i, odd), St::get(buf, 1, i, odd),
+                                          St::get(buf, 2, i, odd), h);
+          g[i] = St::get(buf, 3, i, odd);
           a[i] = f.a, X[i] = f.X, I[i] = f.I, A[i] = f.A, R[i] = f.R;
           if (!FAST && t0 + i >= n) {                // the state stays, nothing has a gradient
             a[i] = f2(1.f);
@@ -152,9 +154,9 @@ __global__ void __launch_bounds__(256, 2)
           part = add2(part, e);
           if (FAST || t0 + i < L) {
             const size_t o = at + (size_t)i * D;
-            store_pair<VEC>(static_cast<T*>(q.dx) + o, mul2(qt, X[i]), left);
-            store_pair<VEC>(static_cast<T*>(q.drg) + o, mul2(e, R[i]), left);
-            store_pair<VEC>(static_cast<T*>(q.dig) + o, mul2(qt, I[i]), left);
+            store_pair<St::kPairs>(static_cast<T*>(q.dx) + o, mul2(qt, X[i]), left);
+            store_pair<St::kPairs>(static_cast<T*>(q.drg) + o, mul2(e, R[i]), left);
+            store_pair<St::kPairs>(static_cast<T*>(q.dig) + o, mul2(qt, I[i]), left);
           }
         }
         sum = add2(sum, part);
@@ -214,11 +216,11 @@ cudaError_t reduce(const GatedBwdParams& q, cudaStream_t s) {
                           (const float*)q.part, p.rows * p.splits, p.D, p.decay, q.ddecay);
 }
 
-template <typename T, int LC, bool VEC>
+template <typename T, int LC, int MODE>
 cudaError_t bwd_impl(const GatedBwdParams& q, cudaStream_t s) {
-  constexpr int TS = kGatedBwdSteps, kBytes = Stage<T, 4, LC, TS, VEC>::kBytes, kTile = 2 * LC;
+  constexpr int TS = kGatedBwdSteps, kBytes = Stage<T, 4, LC, TS, MODE>::kBytes, kTile = 2 * LC;
   const GatedParams& p = q.f;
-  const cudaError_t e = allow_smem<gated_bwd_kernel<T, LC, TS, VEC>>(
+  const cudaError_t e = allow_smem<gated_bwd_kernel<T, LC, TS, MODE>>(
       kGatedWarps * kBytes + joint_bytes(LC, kGatedWarps, 8));
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -232,22 +234,26 @@ cudaError_t bwd_impl(const GatedBwdParams& q, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = p.splits > 1 ? 1 : 0;
-  const cudaError_t r = cudaLaunchKernelEx(&cfg, gated_bwd_kernel<T, LC, TS, VEC>, q);
+  const cudaError_t r = cudaLaunchKernelEx(&cfg, gated_bwd_kernel<T, LC, TS, MODE>, q);
   return r != cudaSuccess ? r : reduce(q, s);
 }
 
-template <typename T, bool VEC>
+template <typename T, int MODE>
 cudaError_t bwd_lanes(const GatedBwdParams& q, cudaStream_t s) {
-  if (q.f.lanes == 32) return bwd_impl<T, 32, VEC>(q, s);
-  return q.f.lanes == 16 ? bwd_impl<T, 16, VEC>(q, s) : bwd_impl<T, 8, VEC>(q, s);
+  if (q.f.lanes == 32) return bwd_impl<T, 32, MODE>(q, s);
+  return q.f.lanes == 16 ? bwd_impl<T, 16, MODE>(q, s) : bwd_impl<T, 8, MODE>(q, s);
 }
 
 }  // namespace
 
 cudaError_t launch_gated_bwd(const GatedBwdParams& q, cudaStream_t s) {
-  if (q.f.dtype == M3_BF16)
-    return q.f.vec ? bwd_lanes<__nv_bfloat16, true>(q, s) : bwd_lanes<__nv_bfloat16, false>(q, s);
-  return q.f.vec ? bwd_lanes<float, true>(q, s) : bwd_lanes<float, false>(q, s);
+  const int copy = q.f.copy;
+  if (q.f.dtype == M3_F32)
+    return copy == kVectors ? bwd_lanes<float, kVectors>(q, s) : bwd_lanes<float, kWords>(q, s);
+  using B = __nv_bfloat16;
+  return copy == kVectors ? bwd_lanes<B, kVectors>(q, s)
+         : copy == kWords ? bwd_lanes<B, kWords>(q, s)
+                          : bwd_lanes<B, kHalfWords>(q, s);
 }
 
 }  // namespace m3

@@ -24,10 +24,10 @@ __device__ __forceinline__ int row_length(const int* lengths, int b, int L) {
   return n < 0 ? 0 : n > L ? L : n;
 }
 
-template <typename T, int LC, int TS, bool VEC>
+template <typename T, int LC, int TS, int MODE>
 __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) {
   extern __shared__ __align__(16) char smem[];
-  using St = Stage<T, 3, LC, TS, VEC>;
+  using St = Stage<T, 3, LC, TS, MODE>;
   using La = Lanes<LC, TS>;
   const int lane = threadIdx.x, w = __shfl_sync(0xffffffffu, threadIdx.y, 0), W = blockDim.y;
   const int S = p.splits, rank = blockIdx.x % S;
@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
   const int left = p.D - c, D = p.D, L = p.L, span = S * W * La::kSteps;
   const int tw0 = (rank * W + w) * La::kSteps, own = lane / LC * TS;   // of the warp; of the run
   const long long ld[3] = {p.ld_x, p.ld_r, p.ld_i};
+  const void* const base[3] = {p.x, p.rg, p.ig};
   char* buf = smem + w * St::kBytes;
   const Joint<LC> joint(smem + W * St::kBytes, W, S);
   St st;
@@ -47,9 +48,9 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
   // the copies of a row's first pass start while the row before it is finished
   auto start = [&](int b, int n) {
     const long long row = (long long)b * L + tw0;
-    st.at(0, p.x, row, ld[0], c0);
-    st.at(1, p.rg, row, ld[1], c0);
-    st.at(2, p.ig, row, ld[2], c0);
+    st.at(0, p.x, row, (long long)p.B * L, ld[0], c0, D);
+    st.at(1, p.rg, row, (long long)p.B * L, ld[1], c0, D);
+    st.at(2, p.ig, row, (long long)p.B * L, ld[2], c0, D);
     st.issue(buf, ld, tw0, n, c0, D);
   };
   int n = row_length(p.lengths, blockIdx.y, L), n2;
@@ -70,6 +71,7 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
                                               (tw0 + own) / kGatedCkpt) * D + c;
     for (int s0 = 0; s0 < n; s0 += span, tw += span) {
       const int t0 = tw + own;
+      const unsigned odd = st.odd_rows(base, ld, (long long)b * L + t0, c0);
       St::wait();
       // FAST: every step of the warp is one of the sequence, and no decay is far from 1
       auto pass = [&](auto fast) {
@@ -78,8 +80,8 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
         Run run{f2(1.f), f2(0.f)};
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const float2 x = St::get(buf, 0, i), r = sigmoid2(St::get(buf, 1, i)),
-                       g = sigmoid2(St::get(buf, 2, i));
+          const float2 x = St::get(buf, 0, i, odd), r = sigmoid2(St::get(buf, 1, i, odd)),
+                       g = sigmoid2(St::get(buf, 2, i, odd));
           float2 m, inv;
           decay2<FAST>(mul2(k, r), a[i], m);
           root2(m, m, inv);
@@ -103,10 +105,10 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
           if (i % kGatedCkpt == 0 && ck != nullptr && (FAST || t0 + i < n))
-            store_pair<VEC>(ck + (size_t)(i / kGatedCkpt) * D, h, left);
+            store_pair<St::kPairs>(ck + (size_t)(i / kGatedCkpt) * D, h, left);
           h = fma2(a[i], h, v[i]);
-          if (FAST) store_pair<VEC>(y + (size_t)i * D, h, left);
-          else if (t0 + i < L) store_pair<VEC>(y + (size_t)i * D, t0 + i < n ? h : f2(0.f), left);
+          if (FAST) store_pair<St::kPairs>(y + (size_t)i * D, h, left);
+          else if (t0 + i < L) store_pair<St::kPairs>(y + (size_t)i * D, t0 + i < n ? h : f2(0.f), left);
         }
       };
       if (near && tw + La::kSteps <= n) pass(std::true_type());
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
       store_pair<false>(p.h_last + (size_t)b * D + c, carry, left);
     for (; tw - tw0 < L; tw += span) {               // steps past the length
       for (int i = 0; i < TS && tw + own + i < L; ++i)
-        store_pair<VEC>(y + (size_t)i * D, f2(0.f), left);
+        store_pair<St::kPairs>(y + (size_t)i * D, f2(0.f), left);
       y += (size_t)span * D;
     }
   }
@@ -129,24 +131,25 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
 
 // Many rows: a warp walks 64 channels of a row by itself, so that there is nothing
 // to join; the CTA's warps are workers of their own.  Two buffers of 4 steps.
-template <typename T, bool VEC>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParams p) {
   extern __shared__ __align__(16) char smem[];
   constexpr int TS = 4;
   static_assert(TS == kGatedCkpt, "a pass starts at a checkpoint");
-  using St = Stage<T, 3, 32, TS, VEC>;
+  using St = Stage<T, 3, 32, TS, MODE>;
   const int lane = threadIdx.x, w = threadIdx.y;
   const int c0 = blockIdx.x * 64, c = c0 + lane * 2, left = p.D - c, D = p.D, L = p.L;
   const long long ld[3] = {p.ld_x, p.ld_r, p.ld_i};
+  const void* const base[3] = {p.x, p.rg, p.ig};
   char* buf = smem + w * 2 * St::kBytes;
   St st;
   const int step = gridDim.y * blockDim.y;
   int b = blockIdx.y * blockDim.y + w, nb, n, tn = 0;   // (nb, tn): the pass that is copied next
   if (b >= p.B) return;
   auto at = [&](int row) {
-    st.at(0, p.x, (long long)row * L, ld[0], c0);
-    st.at(1, p.rg, (long long)row * L, ld[1], c0);
-    st.at(2, p.ig, (long long)row * L, ld[2], c0);
+    st.at(0, p.x, (long long)row * L, (long long)p.B * L, ld[0], c0, D);
+    st.at(1, p.rg, (long long)row * L, (long long)p.B * L, ld[1], c0, D);
+    st.at(2, p.ig, (long long)row * L, (long long)p.B * L, ld[2], c0, D);
   };
   nb = b;
   int nn = n = row_length(p.lengths, b, L);             // the length of nb
@@ -183,26 +186,27 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
     float* ck = p.ckpt == nullptr ? nullptr : p.ckpt + (size_t)b * ((L + TS - 1) / TS) * D + c;
     for (int t0 = 0; t0 < n; t0 += TS) {
       ahead();
+      const unsigned odd = st.odd_rows(base, ld, (long long)b * L + t0, c0);
       St::template wait<1>();
       const char* from = buf + get * St::kBytes;
       get ^= 1;
       if (ck != nullptr) {
-        store_pair<VEC>(ck, h, left);
+        store_pair<St::kPairs>(ck, h, left);
         ck += D;
       }
       auto pass = [&](auto fast) {
         constexpr bool FAST = decltype(fast)::value;
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const float2 x = St::get(from, 0, i), r = sigmoid2(St::get(from, 1, i)),
-                       g = sigmoid2(St::get(from, 2, i));
+          const float2 x = St::get(from, 0, i, odd), r = sigmoid2(St::get(from, 1, i, odd)),
+                       g = sigmoid2(St::get(from, 2, i, odd));
           float2 a, m, inv;
           decay2<FAST>(mul2(k, r), a, m);
           root2(m, m, inv);
           const float2 v = fma2(a, h, mul2(mul2(m, g), x));
           if (FAST || t0 + i < n) {
             h = v;
-            store_pair<VEC>(y, h, left);
+            store_pair<St::kPairs>(y, h, left);
             y += D;
           }
         }
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
       __syncwarp();
     }
     if (p.h_last != nullptr) store_pair<false>(p.h_last + (size_t)b * D + c, h, left);
-    for (int t = n; t < L; ++t, y += D) store_pair<VEC>(y, f2(0.f), left);
+    for (int t = n; t < L; ++t, y += D) store_pair<St::kPairs>(y, f2(0.f), left);
   }
 }
 
@@ -287,10 +291,10 @@ cudaError_t step_impl(const GatedStepParams& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-template <typename T, int LC, bool VEC>
+template <typename T, int LC, int MODE>
 cudaError_t fwd_impl(const GatedParams& p, cudaStream_t s) {
-  constexpr int TS = kGatedFwdSteps, kBytes = Stage<T, 3, LC, TS, VEC>::kBytes, kTile = 2 * LC;
-  const cudaError_t e = allow_smem<gated_fwd_kernel<T, LC, TS, VEC>>(
+  constexpr int TS = kGatedFwdSteps, kBytes = Stage<T, 3, LC, TS, MODE>::kBytes, kTile = 2 * LC;
+  const cudaError_t e = allow_smem<gated_fwd_kernel<T, LC, TS, MODE>>(
       kGatedWarps * kBytes + joint_bytes(LC, kGatedWarps, 8));
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -304,23 +308,23 @@ cudaError_t fwd_impl(const GatedParams& p, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = p.splits > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, gated_fwd_kernel<T, LC, TS, VEC>, p);
+  return cudaLaunchKernelEx(&cfg, gated_fwd_kernel<T, LC, TS, MODE>, p);
 }
 
-template <typename T, bool VEC>
+template <typename T, int MODE>
 cudaError_t fwd_rows(const GatedParams& p, cudaStream_t s) {
-  constexpr int kBytes = 2 * Stage<T, 3, 32, 4, VEC>::kBytes;
-  const cudaError_t e = allow_smem<gated_rows_fwd_kernel<T, VEC>>(4 * kBytes);
+  constexpr int kBytes = 2 * Stage<T, 3, 32, 4, MODE>::kBytes;
+  const cudaError_t e = allow_smem<gated_rows_fwd_kernel<T, MODE>>(4 * kBytes);
   if (e != cudaSuccess) return e;
-  gated_rows_fwd_kernel<T, VEC><<<dim3((p.D + 63) / 64, p.rows), dim3(32, p.warps), p.warps * kBytes, s>>>(p);
+  gated_rows_fwd_kernel<T, MODE><<<dim3((p.D + 63) / 64, p.rows), dim3(32, p.warps), p.warps * kBytes, s>>>(p);
   return cudaGetLastError();
 }
 
-template <typename T, bool VEC>
+template <typename T, int MODE>
 cudaError_t fwd_lanes(const GatedParams& p, cudaStream_t s) {
-  if (p.solo) return fwd_rows<T, VEC>(p, s);
-  if (p.lanes == 32) return fwd_impl<T, 32, VEC>(p, s);
-  return p.lanes == 16 ? fwd_impl<T, 16, VEC>(p, s) : fwd_impl<T, 8, VEC>(p, s);
+  if (p.solo) return fwd_rows<T, MODE>(p, s);
+  if (p.lanes == 32) return fwd_impl<T, 32, MODE>(p, s);
+  return p.lanes == 16 ? fwd_impl<T, 16, MODE>(p, s) : fwd_impl<T, 8, MODE>(p, s);
 }
 
 }  // namespace
@@ -368,9 +372,12 @@ void gated_plan(int B, int L, int D, bool backward, int sms, GatedParams* p) {
 }
 
 cudaError_t launch_gated_fwd(const GatedParams& p, cudaStream_t s) {
-  if (p.dtype == M3_BF16)
-    return p.vec ? fwd_lanes<__nv_bfloat16, true>(p, s) : fwd_lanes<__nv_bfloat16, false>(p, s);
-  return p.vec ? fwd_lanes<float, true>(p, s) : fwd_lanes<float, false>(p, s);
+  if (p.dtype == M3_F32)
+    return p.copy == kVectors ? fwd_lanes<float, kVectors>(p, s) : fwd_lanes<float, kWords>(p, s);
+  using B = __nv_bfloat16;
+  return p.copy == kVectors ? fwd_lanes<B, kVectors>(p, s)
+         : p.copy == kWords ? fwd_lanes<B, kWords>(p, s)
+                            : fwd_lanes<B, kHalfWords>(p, s);
 }
 
 cudaError_t launch_gated_step(const GatedStepParams& p, cudaStream_t s) {

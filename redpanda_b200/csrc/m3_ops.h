@@ -224,7 +224,7 @@ struct GatedParams {
   int dtype;
   int lanes, warps, splits, rows;                        // per run, per CTA, per cluster; grid
   int solo;                                              // a warp walks its rows by itself
-  int vec;                                               // 16-byte loads, vector stores
+  int copy;                                              // how rows are copied (m3_gated.cuh)
   int* err;                                              // the device's error word
 };
 struct GatedBwdParams {

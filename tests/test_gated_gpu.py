@@ -275,3 +275,34 @@ def test_state_version_moves_and_saved_states_raise():
 def test_many_rows_walked_by_one_cta(ty):
     """More rows than one wave of CTAs: each walks several, of other lengths."""
     check(*inputs(1500, 11, 64, T[ty], 4, state=True, ragged=True))
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 66, 67, 1])
+def test_more_rows_than_warps(D, ty):
+    """Rows and channel tiles for a warp each, forward (3552 and more)."""
+    check(*inputs(3600, 9, D, T[ty], D, state=True, ragged=True))
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("B,L,D", [(1, 900, 1001), (2, 515, 130), (1, 4100, 63), (3, 40, 999)])
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+def test_rows_of_every_alignment(B, L, D, offset, ty):
+    """Views that start at every offset from 16 bytes, with strides of their own, and
+    whose first and last elements are the storage's."""
+    ty = T[ty]
+    g = torch.Generator().manual_seed(D + offset)
+    decay, up = torch.randn(D, generator=g) - 3, torch.randn(B, L, D, generator=g).to(ty)
+    flat = [torch.randn(offset + B * L * (D + k) - k, generator=g).to(ty) for k in range(3)]
+
+    def views(ts):
+        return [t.as_strided((B, L, D), (L * (D + k), D + k, 1), offset) for k, t in enumerate(ts)]
+    ref = O.gated(*views(flat), decay, g=up)
+    base = [t.cuda().requires_grad_(True) for t in flat]
+    dd = decay.cuda().requires_grad_(True)
+    y = G.m3_gated_scan(*views(base), dd)
+    assert O.excess(y, ref["y"], ref["+y"], ty) <= 1
+    grads = torch.autograd.grad(y, (*base, dd), up.cuda())
+    for t, k in zip(views(grads[:3]), ("dx", "drg", "dig")):
+        assert O.excess(t, ref[k], ref["+" + k], ty) <= 1
+    assert O.excess(grads[3], ref["ddecay"], ref["+ddecay"], torch.float32) <= 1
