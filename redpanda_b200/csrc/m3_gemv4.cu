@@ -12,7 +12,7 @@
 // weights as the 16-row operand): q - 8 is exact in bf16, and an fp32 input is the
 // sum of three bf16 numbers of 8 bits each, cut off its mantissa, so every product
 // is exact; the parts of the rows take columns of their own (8 columns hold 8 rows of
-// bf16, or 2 of fp32).  A group's sum is at most 8 instructions long and is folded
+// bf16, or 2 of fp32); the inputs' sums are a product with ones.  A group's sum is at most 8 instructions long and is folded
 // into fp32 totals with its scale, so the tensor core's own accumulation, which
 // cuts bits, is never long.  The norm's factor 1 / sqrt(mean(x^2) + eps) is a row's,
 // and is applied to the total.
@@ -79,8 +79,7 @@ __device__ __forceinline__ float below(float v) {   // v without its top 16 bits
 // operands agree: lane l's two instructions of 32 columns take the 8 columns from
 // 8 (l % 4), so its operands are 16 consecutive bytes of a row.
 //
-// Stages the columns from k0 of every row, with the groups' sums of the inputs and
-// the squares' sums of every 128 columns.
+// Stages the columns from k0 of every row, with the squares' sums of every 128 columns.
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p, int left, bool vec) {
   if (vec && left >= 4) {
@@ -97,15 +96,34 @@ __device__ __forceinline__ float4 below(const float4& v) {
   return make_float4(below(v.x), below(v.y), below(v.z), below(v.w));
 }
 
-template <typename T, int NB, int G, bool CENTER>
-__device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* xs, float* sq,
-                      int parts) {
+// Sums of every row's value over the lanes of a warp: lane l has that of row
+// l / (32 / R) (R rows, a power of two; 5 + R shuffles instead of 5 R).
+template <int R>
+__device__ __forceinline__ float row_totals(const float (&v)[kQ4Rows]) {
+  const int lane = threadIdx.x & 31;
+  float a[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) a[r] = v[r];
+  int m = 16;
+#pragma unroll
+  for (int n = R / 2; n > 0; n >>= 1, m >>= 1)
+#pragma unroll
+    for (int r = 0; r < n; ++r) {
+      const bool up = lane & m;
+      const float keep = up ? a[r + n] : a[r], give = up ? a[r] : a[r + n];
+      a[r] = keep + __shfl_xor_sync(0xffffffffu, give, m);
+    }
+  float t = a[0];
+  for (; m > 0; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
+  return t;
+}
+
+template <typename T>
+__device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* sq, int parts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int row = (p.chunk + kPad) * 2;                 // bytes
+  const int row = (p.chunk + kPad) * 2;              // bytes
   const T* x = static_cast<const T*>(p.x) + k0;
-  const bool vec = p.vec != 0;
-  const bool raw = sizeof(T) == 2 && parts == 1 && p.vec8 != 0;   // rows as they are
-  if (raw) {
+  if (sizeof(T) == 2 && parts == 1 && p.vec8 != 0) {   // rows as they are
     for (int r = 0; r < p.rows; ++r)
       for (int c = (warp * 32 + lane) * 8; c < n; c += warps * 256) {
         const int left = (p.d_in - k0 - c) * 2, bytes = left < 0 ? 0 : left < 16 ? left : 16;
@@ -116,35 +134,27 @@ __device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* x
                      : "memory");
       }
     asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-    if (!CENTER) return;
-    __syncthreads();
+    return;
   }
+  const bool vec = p.vec != 0;
   for (int c0 = warp * 128; c0 < n; c0 += warps * 128) {
     const int c = c0 + lane * 4, left = p.d_in - k0 - c, at = left > 0 ? c : 0;
     // every row's loads before any is used
     float4 v[kQ4Rows], w;
+    float ss[kQ4Rows] = {};
 #pragma unroll
     for (int r = 0; r < kQ4Rows; ++r)
-      if (r < p.rows) {
-        if (raw) v[r] = load4(reinterpret_cast<const T*>(rows + r * row) + (c < n ? c : 0), 4, true);
-        else v[r] = load4(x + (size_t)r * p.ld_x + at, left, vec);
-      }
+      if (r < p.rows) v[r] = load4(x + (size_t)r * p.ld_x + at, left, vec);
     if (p.norm_w != nullptr) w = load4(p.norm_w + k0 + at, left, vec);
 #pragma unroll
     for (int r = 0; r < kQ4Rows; ++r) {
       if (r >= p.rows) break;
       float4 y = v[r];
       if (p.norm_w != nullptr) {
-        float ss = fmaf(y.x, y.x, y.y * y.y) + fmaf(y.z, y.z, y.w * y.w);
-        ss = warp_total(ss, 32);
-        if (lane == 0) sq[(k0 + c0) / 128 * kQ4Rows + r] = ss;
+        ss[r] = fmaf(y.x, y.x, y.y * y.y) + fmaf(y.z, y.z, y.w * y.w);
         y = make_float4(y.x * w.x, y.y * w.y, y.z * w.z, y.w * w.w);
       }
-      if (CENTER) {
-        const float sum = warp_total((y.x + y.y) + (y.z + y.w), G / 4);
-        if (lane % (G / 4) == 0 && c < n) xs[c / G * (8 * NB) + r] = sum;
-      }
-      if (c < n && !raw) {
+      if (c < n) {
         char* to = rows + r * row + c * 2;
         *reinterpret_cast<uint2*>(to) = top_halves(y);
         if (parts == 3) {
@@ -152,6 +162,16 @@ __device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* x
           *reinterpret_cast<uint2*>(to + p.rows * row) = top_halves(y);
           *reinterpret_cast<uint2*>(to + 2 * p.rows * row) = top_halves(below(y));
         }
+      }
+    }
+    if (p.norm_w != nullptr) {
+      float* to = sq + (k0 + c0) / 128 * kQ4Rows;
+      if (p.rows == 1) {
+        const float t = row_totals<1>(ss);
+        if (lane == 0) to[0] = t;
+      } else {
+        const float t = row_totals<8>(ss);
+        if (lane % 4 == 0) to[lane / 4] = t;
       }
     }
   }
@@ -166,18 +186,17 @@ struct Ring {
   static constexpr int kSlots = MT * BU == 1 ? 8 : MT * BU == 2 ? 6 : 4;
 };
 
-// shared memory: the warps' rings, the inputs, the groups' sums, and the squares' sums
-// of all columns; the totals lie over rings and inputs at the end
+// shared memory: the warps' rings, the inputs, and the squares' sums of all columns;
+// the totals lie over rings and inputs at the end
 struct Layout {
-  int x, xs, sq, total;            // bytes
+  int x, sq, total;                // bytes
 };
 template <int NB, int MT, int G, bool CENTER>
 __host__ __device__ inline Layout layout(int warps, int cols, int chunk, int units, bool norm) {
   using R = Ring<MT, G, CENTER>;
   Layout l;
   l.x = warps * R::kSlots * R::kSlot;
-  l.xs = l.x + (chunk + kPad) * 2 * cols;
-  l.sq = l.xs + (CENTER ? chunk / G * 8 * NB * 4 : 0);
+  l.sq = l.x + (chunk + kPad) * 2 * cols;
   l.total = l.sq + (norm ? (units * R::U + 127) / 128 * kQ4Rows * 4 : 0);
   return l;
 }
@@ -204,7 +223,6 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
                                                p.norm_w != nullptr);
   char* ring = smem + warp * R::kSlots * R::kSlot;
   char* rows = smem + lay.x;
-  float* xs = reinterpret_cast<float*>(smem + lay.xs);
   float* sq = reinterpret_cast<float*>(smem + lay.sq);
   const int tiles = (p.d_out + 15) / 16, tile0 = (blockIdx.x * p.mw + mw) * MT;
   pdl_launch_dependents();
@@ -239,9 +257,14 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
 #pragma unroll
   for (int i = 0; i < R::kSlots - 1; ++i) copy();
   pdl_wait();
-  if (CENTER)   // the columns of the inputs' lower parts have no sum of their own
-    for (int i = threadIdx.x; i < p.chunk / G * 8 * NB; i += blockDim.x) xs[i] = 0.f;
-
+  // the bias and residual of this thread's first output
+  const int outs = 16 * MT * p.mw, o_r = threadIdx.x / outs, o_at = blockIdx.x * outs + threadIdx.x % outs;
+  float add_bias = 0.f, add_res = 0.f;
+  if (o_r < p.rows && o_at < p.d_out) {
+    if (p.bias != nullptr) add_bias = p.bias[o_at];
+    if (p.residual != nullptr)
+      add_res = Elem<T>::get(static_cast<const T*>(p.residual)[(size_t)o_r * p.ld_r + o_at]);
+  }
   // the lane's operands of block 0; lanes of columns that are not in use read the last
   // one's, and their results are not used
   const char* mine[NB];
@@ -253,7 +276,7 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
   for (int i0 = 0; i0 * p.kw < units; i0 += per_chunk) {   // chunks of the columns
     const int u0 = i0 * p.kw;
     __syncthreads();
-    stage<T, NB, G, CENTER>(p, u0 * U, min(chunk_units, units - u0) * U, rows, xs, sq, parts);
+    stage<T>(p, u0 * U, min(chunk_units, units - u0) * U, rows, sq, parts);
     __syncthreads();
     const int end = min(per, i0 + per_chunk);
     for (int i = i0; i < end; ++i) {
@@ -263,7 +286,7 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
       const char* from = ring + slot * R::kSlot;
       slot = slot + 1 == R::kSlots ? 0 : slot + 1;
       const int u = (i - i0) * p.kw + kw;            // in the chunk
-      float acc[MT][NB][4];
+      float acc[MT][NB][4], sum[NB][4];              // sum: of the inputs, in every row
 #pragma unroll
       for (int b = 0; b < BU; ++b) {
         uint4 w[MT];
@@ -277,6 +300,16 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
 #pragma unroll
           for (int c = 0; c < NB; ++c)
             f[c] = *reinterpret_cast<const uint4*>(mine[c] + (u * BU + b) * 128 + jp * 64);
+          if (CENTER) {
+            constexpr unsigned kOnes = 0x3f803f80u;
+            const unsigned one[4] = {kOnes, kOnes, kOnes, kOnes};
+#pragma unroll
+            for (int c = 0; c < NB; ++c) {
+              if (first) sum[c][0] = sum[c][1] = sum[c][2] = sum[c][3] = 0.f;
+              mma16816(sum[c], one, f[c].x, f[c].y);
+              mma16816(sum[c], one, f[c].z, f[c].w);
+            }
+          }
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             if (first)
@@ -312,12 +345,10 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
                 tot[m][c][2] = fmaf(s1, acc[m][c][2], tot[m][c][2]);
                 tot[m][c][3] = fmaf(s1, acc[m][c][3], tot[m][c][3]);
                 if (CENTER) {
-                  const float2 v = *reinterpret_cast<const float2*>(
-                      xs + (u * GU + g) * (8 * NB) + c * 8 + 2 * (lane & 3));
-                  tot[m][c][0] = fmaf(c0, v.x, tot[m][c][0]);
-                  tot[m][c][1] = fmaf(c0, v.y, tot[m][c][1]);
-                  tot[m][c][2] = fmaf(c1, v.x, tot[m][c][2]);
-                  tot[m][c][3] = fmaf(c1, v.y, tot[m][c][3]);
+                  tot[m][c][0] = fmaf(c0, sum[c][0], tot[m][c][0]);
+                  tot[m][c][1] = fmaf(c0, sum[c][1], tot[m][c][1]);
+                  tot[m][c][2] = fmaf(c1, sum[c][0], tot[m][c][2]);
+                  tot[m][c][3] = fmaf(c1, sum[c][1], tot[m][c][3]);
                 }
               }
             }
@@ -339,7 +370,6 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
   __syncthreads();
   // totals of every warp: (kw, outputs of the CTA, columns)
   float* red = reinterpret_cast<float*>(smem);
-  const int outs = 16 * MT * p.mw;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -359,9 +389,13 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
       for (int k = 0; k < p.kw; ++k)
         v += red[((size_t)k * outs + o) * (8 * NB + 1) + s * p.rows + r];
     if (p.norm_w != nullptr) v *= s_rstd[r];
-    if (p.bias != nullptr) v += p.bias[out];
-    if (p.residual != nullptr)
-      v += Elem<T>::get(static_cast<const T*>(p.residual)[(size_t)r * p.ld_r + out]);
+    if (i != threadIdx.x) {
+      add_bias = p.bias != nullptr ? p.bias[out] : 0.f;
+      add_res = p.residual != nullptr
+                    ? Elem<T>::get(static_cast<const T*>(p.residual)[(size_t)r * p.ld_r + out])
+                    : 0.f;
+    }
+    v = add_res + (v + add_bias);
     if (out < p.split) {
       if (p.silu) v = __fdiv_rn(v, 1.f + expf(-v));
       static_cast<T*>(p.out0)[(size_t)r * p.ld0 + out] = Elem<T>::put(v);

@@ -73,6 +73,8 @@ class StepGraph:
         with torch.no_grad(), torch.cuda.graph(self.graph, capture_error_mode="thread_local"):
             self.outputs = run(self.cache)
         self.hidden = self.outputs[0]
+        # 4-bit weights that the graph reads, past a later quantize_step_
+        self._held = [layer["mixer"].step_q4 for layer in model.layers]
 
     def _views(self, flat):
         """(h, dBu) views of each layer's slice of a flat state buffer."""
@@ -159,11 +161,15 @@ def _main():
     ap.add_argument("--small", type=int, default=Mamba3Block.small_step_max_batch,
                     help="Mamba3Block.small_step_max_batch (0: cuBLAS projections)")
     ap.add_argument("--steps", type=int, default=20)
+    ap.add_argument("--q4", type=int, default=0,
+                    help="columns per scale of 4-bit in_proj, x_proj and out_proj (0: full weights)")
     args = ap.parse_args()
     torch.manual_seed(0)
     cfg = MambaConfig(d_model=512, n_layer=args.layers, d_state=32, n_track_state=8, mimo_p=2,
                       vocab_size=8192)
     model = Mamba(cfg).cuda().eval()
+    if args.q4:
+        model.quantize_step_(group=args.q4, names=("in_proj", "x_proj", "out_proj"))
     Mamba3Block.small_step_max_batch = args.small
     for batch in (int(b) for b in args.batch.split(",")):
         g = StepGraph(model, batch)
@@ -179,7 +185,8 @@ def _main():
         e1.record()
         torch.cuda.synchronize()
         print(f"batch {batch}: {e0.elapsed_time(e1) / args.steps * 1e3:.1f} us per step "
-              f"(small_step_max_batch {args.small})", flush=True)
+              f"(small_step_max_batch {args.small}"
+              + (f", 4-bit weights in groups of {args.q4})" if args.q4 else ")"), flush=True)
 
 
 if __name__ == "__main__":

@@ -550,8 +550,10 @@ class Mamba(nn.Module):
     ``fuse_add_norm`` (class or instance attribute): in training, run each layer's
     residual addition and the next layer's norm as one launch each way
     (``m3_add_rms_norm``) on CUDA streams of float32 or bfloat16.  Off by default,
-    where results are torch's; the kernel's norms differ by rounding.  Not used
-    with ``grad_checkpoint``, whose layers hold their norm."""
+    where results are torch's; the kernel's norms differ by rounding.  The norm
+    modules are then not called (their hooks do not run).  Not used with
+    ``grad_checkpoint``, whose layers hold their norm, nor under an autocast to
+    another type than bfloat16."""
 
     fuse_add_norm = False
 
@@ -592,6 +594,8 @@ class Mamba(nn.Module):
 
     def _add_norm_ok(self, x):
         types = (torch.float32, torch.bfloat16)
+        if torch.is_autocast_enabled("cuda") and not _bf16_layer():
+            return False
         return (self.fuse_add_norm and torch.is_grad_enabled() and x.is_cuda
                 and not (self.grad_checkpoint and self.training) and x.dtype in types
                 and self.config.d_model <= MAX_D
@@ -623,8 +627,9 @@ class Mamba(nn.Module):
         ``step_fused_`` on at most ``Mamba3Block.small_step_max_batch`` rows, and
         step graphs captured from now on.  Larger batches, priming and training keep
         the full weights.  The copies are of the present weights: a step after the
-        weights have changed raises until this is called again.  ``names=()`` goes
-        back to the full weights.  Returns the model."""
+        weights have changed, or in a copy of the model, raises until this is called
+        again, and a step graph keeps the copies it was captured with.  ``names=()``
+        goes back to the full weights.  Returns the model."""
         names = tuple(names)
         if not set(names) <= {"in_proj", "x_proj", "out_proj"}:
             raise ValueError("quantize_step_: names are of in_proj, x_proj, out_proj")

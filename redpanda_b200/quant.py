@@ -56,9 +56,11 @@ class Q4Weight:
     def quantize(cls, weight, group=64, center=True):
         """Nearest codes of ``weight`` (d_out, d_in): with ``center`` a group's
         smallest and largest weight get the codes 0 and 15, without, the largest
-        magnitude gets 1 or 15."""
+        magnitude gets 1 or 15.  The weights have to be finite."""
         cls._check(weight.shape, group)
         w = weight.detach().to(torch.float32)
+        if not bool(torch.isfinite(w).all()):
+            raise ValueError("Q4Weight: weights have to be finite")
         d_out, d_in = w.shape
         n = -(-d_in // group)
         # the last group's missing columns as copies of its last: they change no extreme
@@ -66,7 +68,7 @@ class Q4Weight:
         lo, hi = w.amin(2), w.amax(2)
         tiny = torch.finfo(torch.float32).tiny
         if center:
-            scale = ((hi - lo) / 15).to(torch.bfloat16)
+            scale = (hi / 15 - lo / 15).to(torch.bfloat16)
             mid = (lo + 8 * scale.float()).to(torch.bfloat16)
             off = mid.float()
         else:

@@ -199,6 +199,10 @@ def test_fused_addition_and_norm_is_off_where_it_does_not_apply():
     assert not m._add_norm_ok(x)
     m.eval()
     assert m._add_norm_ok(x)
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert not m._add_norm_ok(x)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert m._add_norm_ok(x)
 
 
 def test_step_on_4_bit_weights():
@@ -241,6 +245,11 @@ def test_step_on_4_bit_weights():
             m.step_fused_(ids[:, 0], mine())
         m.layers[1]["mixer"].out_proj.weight.mul_(0.5)
         m.quantize_step_(names=())
+        held = graph.hidden.clone()
+        graph.load_(cb)        # the graph has its own 4-bit weights
+        ref = stand_in.step_fused_(ids[:, 0], [tuple(t.clone() for t in e) for e in cb])[0]
+        assert (graph.step(ids[:, 0])[0] - ref).abs().max() <= 5e-5 * ref.abs().max()
+        assert not torch.equal(held, graph.hidden)
         assert torch.equal(m.step_fused_(ids[:, 0], mine())[0],
                            full.step_fused_(ids[:, 0], mine())[0])
     assert set(m.state_dict()) == set(full.state_dict())

@@ -63,6 +63,14 @@ def test_quantize_is_near(n, k, group, center):
     assert (far <= tol.repeat_interleave(group, 1)[:, :k]).all()
 
 
+def test_quantize_of_the_largest_weights():
+    """A range that overflows as a difference."""
+    w = torch.tensor([[-3e38, 3e38, 1e38, 0.0]])
+    back = Q.Q4Weight.quantize(w, 32).dequantize()
+    # a code's step is 4e37, its scale and center 2^-8 off
+    assert torch.isfinite(back).all() and ((back - w).abs() <= 2e37 + 15 * 4e37 / 256 + 3e38 / 256).all()
+
+
 def test_quantize_of_constant_groups():
     w = torch.full((3, 64), 0.75)
     w[1] = 0
@@ -76,6 +84,8 @@ def test_quantize_of_constant_groups():
     lambda: Q.Q4Weight.quantize(z(4)),
     lambda: Q.Q4Weight.quantize(z(0, 4)),
     lambda: Q.Q4Weight.quantize(z(1, 65537)),
+    lambda: Q.Q4Weight.quantize(torch.tensor([[1.0, float("nan")]])),
+    lambda: Q.Q4Weight.quantize(torch.tensor([[1.0, float("-inf")]])),
     lambda: Q.Q4Weight.from_codes(z(4, 64).int() + 16, z(4, 1)),
     lambda: Q.Q4Weight.from_codes(z(4, 64).int() - 1, z(4, 1)),
     lambda: Q.Q4Weight.from_codes(z(4, 64).int(), z(4, 2)),
