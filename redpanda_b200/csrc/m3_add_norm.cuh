@@ -21,8 +21,8 @@ cudaError_t with_types(int x, int s, int y, F&& f) {
 // Instantiation of a row length, as norm_dispatch, but with 16 elements per thread in
 // rows past 2048 (past 1024 in the 8-bit norm: `from`): these kernels hold two or three
 // arrays, and a CTA of 512 threads with 8 elements each fills an SM by itself with too
-// little in flight (16384 x 4096 bf16: forward 116 against 90 us, backward 137
-// against 104).
+// little in flight (16384 x 4096 bf16: forward 116 against 92 us, backward 137
+// against 116).
 template <int E, int MAXT, typename F>
 cudaError_t add_size(int vec, int nt, F&& f) {
   if constexpr (std::decay_t<F>::kWide)

@@ -5,7 +5,8 @@
 // The norm is that of s as stored, so that the backward, which reads s, has the
 // forward's values.  Bound by memory: x and res in, s and y out.  Layout as in
 // m3_norm.cu: a warp or a CTA per row, the row in registers between the sum and
-// the output, the next row's loads ahead of the reduction, persistent CTAs.
+// the output, the next row's loads ahead of the reduction, persistent CTAs.  131072 x
+// 768, bf16 branch into an fp32 stream, bf16 y: 212 us (5.7 TB/s).
 #include "m3_add_norm.cuh"
 
 namespace m3 {

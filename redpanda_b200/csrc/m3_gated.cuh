@@ -12,7 +12,8 @@
 // unit's ex2 instead, whose results are low by 2e-8 on average, a state would be
 // low by that times 1 / (1 - a): 2e-5 at a = 0.999.
 //
-// All pairs below are two channels in one packed register pair.
+// All pairs below are two channels in one packed register pair: with scalar
+// instructions instead the forward took 82 against 75 us (256 x 64 x 2048 bf16).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -26,7 +27,10 @@
 namespace m3 {
 
 constexpr int kGatedCkpt = 4;         // steps between the backward's checkpoints
-constexpr int kGatedFwdSteps = 8, kGatedBwdSteps = 4;   // of a thread at a time
+// Steps of a thread at a time.  Forward 4 means as many joins again (prompt of 16384 x
+// 1024 bf16: 56 against 50 us); backward 8 holds six values for each in registers and
+// spills (256 x 64 x 2048 bf16: 161 against 139 us before other changes).
+constexpr int kGatedFwdSteps = 8, kGatedBwdSteps = 4;
 constexpr int kGatedWarps = 8;                          // of a CTA, at most
 
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
@@ -111,8 +115,10 @@ template <int LC, int TS> struct Lanes {
 
 // How rows are copied, by what their starts and lengths allow: 16 bytes at a time,
 // words (fp32, and bf16 rows of whole words), or words that bf16 rows start in the
-// middle of.  All asynchronous: without, a row that is not aligned to 16 bytes would
-// be waited for where it is asked for (2 x 16001 x 1281 fp32: XX us).
+// middle of.  All asynchronous: with plain loads a row that is not aligned to 16 bytes
+// is waited for where it is asked for (2 x 16001 x 1281 fp32: 447 against 165 us
+// forward, 832 against 333 backward; 256 x 64 x 2047 bf16, half words: 224 against 163
+// and 520 against 322; 2046, words: 224 against 75 and 511 against 146).
 enum Copy { kHalfWords = 0, kWords = 1, kVectors = 2 };
 
 // A warp's rows of NA arrays: kSteps steps of a tile, row (i, sub) (step i of run
@@ -281,8 +287,8 @@ __device__ __forceinline__ float2 load_pair(const float* p, int left) {
 //
 // The cluster's CTAs write their runs into each other's shared memory, counted by
 // an mbarrier of the receiver's (two in turn, S x LC x 16 bytes each time).  A
-// cluster barrier there would wait for every store to memory before it (prompt of
-// 16384 x 1024: 51 against XX us).  A slot is written again two calls later, by a CTA
+// cluster barrier there waits for every store to memory before it (2 x 16001 x 1280
+// fp32: forward 109 against 97 us, backward 230 against 187 us).  A slot is written again two calls later, by a CTA
 // that by then has this CTA's run of the call between, which was sent after every
 // warp here had read the slot.  The wait is bounded: after kMbarMaxPolls polls the
 // thread sets `dead`, waits no more, and the kernel records M3_ERR_DEVICE.
@@ -341,11 +347,11 @@ __device__ __forceinline__ Run as_run(const float4& v) {
 }
 
 // The value in front of this run; turn: the call's number.  first: `carry` is the value
-// in front of all, else the last call's.  On return carry is the value behind all, in the last warp's last
-// run's lanes.
+// in front of all, else the last call's.  On return carry is the value behind all, in
+// the last warp's last run's lanes.
 template <int LC, int DIR>
-__device__ __forceinline__ float2 join(const Joint<LC>& j, int turn, const Run& mine, int w, int rank,
-                                       bool first, float2& carry, bool& dead) {
+__device__ __forceinline__ float2 join(const Joint<LC>& j, int turn, const Run& mine, int w,
+                                       int rank, bool first, float2& carry, bool& dead) {
   const int flip = turn & 1;
   const int warps = j.warps, S = j.S;
   constexpr int kSub = 32 / LC;

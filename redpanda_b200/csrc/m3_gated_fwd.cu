@@ -1,12 +1,24 @@
 // Gated linear recurrence, forward over whole sequences and single tokens.
 // Formulas and the precision of the decay: m3_gated.cuh.
 //
-// A CTA holds 64 channels, two per lane, and its warps hold consecutive runs of 8
-// steps; a cluster of up to 8 CTAs holds that many runs more where there are too
-// few rows and channel tiles for the GPU.  Each pass of a CTA (cluster) over its
-// runs loads every input once: a thread computes a and b = m i x of its steps,
-// the run's product and sum, joins the runs ahead (join()), and walks its steps
-// from there.  The copies of the next pass's rows are in flight meanwhile.
+// Bound by memory (x and the gates in, y out) and by the MUFU unit (two exponentials,
+// two reciprocals and a root per element: 37 us at 256 x 64 x 2048, 41 us of bf16
+// bytes).  Two kernels:
+//
+// Where rows and channel tiles give every warp of the GPU its own, a warp walks 64
+// channels of a row by itself, 4 steps at a time, the next ones' copies in flight;
+// nothing is stored but y.  256 x 64 x 2048 bf16: 56 us (4.8 TB/s; MUFU 73 % busy), 65
+// us with two warps per row that are joined.
+//
+// With fewer, a CTA holds a tile of 64, 32 or 16 channels, two per lane, and its warps
+// hold consecutive runs of 8 steps; a cluster of up to 8 CTAs holds that many runs
+// more.  Each pass of a CTA (cluster) over its runs loads every input once: a thread
+// computes a and b = m i x of its steps, the run's product and sum, joins the runs
+// ahead (join()), and walks its steps from there; the copies of the next pass's rows
+// are in flight meanwhile.  One prompt of 16384 x 1024 bf16: 50 us (2.7 TB/s), 11
+// passes of 4.5 us each, of which half is the wait for the runs ahead and for the
+// slowest warp; 101 us with tiles of 64 channels only (before
+// mbarriers).
 #include "m3_gated.cuh"
 
 #include <type_traits>
@@ -221,7 +233,8 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
 }
 
 // One token per row: a thread owns V channels and walks rows, the next row's loads
-// ahead of the present one's arithmetic.
+// ahead of the present one's arithmetic.  Bound by memory: 2048 x 2048 bf16 14 us (4.8
+// TB/s).
 template <typename T, int V>
 struct StepRow {
   Pack<T, V> x, r, g;
@@ -316,7 +329,8 @@ cudaError_t fwd_rows(const GatedParams& p, cudaStream_t s) {
   constexpr int kBytes = 2 * Stage<T, 3, 32, 4, MODE>::kBytes;
   const cudaError_t e = allow_smem<gated_rows_fwd_kernel<T, MODE>>(4 * kBytes);
   if (e != cudaSuccess) return e;
-  gated_rows_fwd_kernel<T, MODE><<<dim3((p.D + 63) / 64, p.rows), dim3(32, p.warps), p.warps * kBytes, s>>>(p);
+  gated_rows_fwd_kernel<T, MODE>
+      <<<dim3((p.D + 63) / 64, p.rows), dim3(32, p.warps), p.warps * kBytes, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -343,13 +357,17 @@ void gated_plan(int B, int L, int D, bool backward, int sms, GatedParams* p) {
     p->rows = B / 4 + (B % 4 != 0) < 65535 ? (B + 3) / 4 : 65535;
     return;
   }
+  // few warps per CTA while rows are many: 256 x 64 x 2048 bf16 backward 111 us at two,
+  // 118 at four, 127 at eight
   int warps = 2;
   while (warps < kGatedWarps && tiles64 * B * warps * 2 <= wave) warps *= 2;
   if (warps > segs) warps = segs;
   p->warps = warps;
   const long long slots = wave / warps;
   // Of the tile widths and time splits whose every CTA has a pass of its own, the one
-  // with most CTAs in one wave; wide tiles and few splits among equals.
+  // with most CTAs in one wave; wide tiles and few splits among equals.  Measured: 1 x
+  // 16384 x 1024 bf16 128 CTAs of tile 64 93 us, 256 of 32 49, 384 of 16 49; 2 x 16001 x
+  // 1280 fp32 backward 160 CTAs 336, 280 187, 320 (a second, part-filled wave) 204.
   auto tiles = [&](int l) { return (long long)(D + 2 * l - 1) / (2 * l); };
   long long most = tiles(32) * B;
   for (int l = 32; l >= 8; l /= 2)
