@@ -41,16 +41,14 @@ def _forward(prepared, decay, c, state, lengths, want_state, want_ckpt):
     x = prepared[0][0]
     B, L, D = x.shape
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    h = torch.empty((B, D), device=x.device, dtype=torch.float32) if want_state else None
+    h = decay.new_empty(B, D) if want_state else None
     if B == 0 or L == 0:
         if h is not None:
             h.copy_(state) if state is not None else h.zero_()
         return y, h, None
     lib = _lib.load()
     desc = GatedDesc(B, L, D, H.code(x.dtype), c)
-    ckpt = None
-    if want_ckpt:
-        ckpt = torch.empty(lib.m3_gated_ckpt_floats(desc), device=x.device, dtype=torch.float32)
+    ckpt = decay.new_empty(lib.m3_gated_ckpt_floats(desc)) if want_ckpt else None
     H.launch(x.get_device(), lib.m3_gated_fwd, desc, _args(prepared, decay, state, lengths),
              y.data_ptr(), H.ptr(h), H.ptr(ckpt))
     return y, h, ckpt
@@ -106,7 +104,7 @@ class _GatedScanFn(torch.autograd.Function):
             desc = GatedDesc(B, L, D, H.code(ty), c)
             with H.on_device(index):
                 nws = lib.m3_gated_bwd_workspace_bytes(desc)
-            ws = torch.empty(nws, device=x.device, dtype=torch.uint8)
+            ws = decay.new_empty(-(-nws // 4))
             # the checkpoints hold what the state before x was
             H.launch(index, lib.m3_gated_bwd, desc,
                      _args(tuple(zip((x, r, i), lds)), decay, None, lengths), g.data_ptr(),

@@ -142,14 +142,15 @@ class _AddNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, weight, eps, out_dtype):
-        d = x.shape[-1]
-        x2, lx = H.rows(x if x.dim() == 2 else x.reshape(-1, d))
-        r2, lr = H.rows(residual if x.dim() == 2 else residual.reshape(-1, d))
+        flat, d = x.dim() == 2, x.shape[-1]
+        x2, lx = H.rows(x if flat else x.reshape(-1, d))
+        r2, lr = H.rows(residual if flat else residual.reshape(-1, d))
         w = H.f32(weight)
         desc = AddNormDesc(x2.shape[0], d, H.code(x2.dtype), H.code(r2.dtype), H.code(out_dtype),
                            eps)
         y, s, st = _add_forward(x2, lx, r2, lr, w, desc, out_dtype, True)
-        y, s = y.view(x.shape), s.view(x.shape)
+        if not flat:
+            y, s = y.view(x.shape), s.view(x.shape)
         H.save(ctx, s, w, st)
         ctx.cfg = (desc, x.dtype, out_dtype, weight.dtype)
         ctx.set_materialize_grads(False)
@@ -159,29 +160,30 @@ class _AddNormFn(torch.autograd.Function):
     @H.once_differentiable
     def backward(ctx, gy, gs):
         if gy is None and gs is None:
-            return (None,) * 5
+            return None, None, None, None, None
         desc, xt, yt, wt = ctx.cfg
         s, w, st = ts = ctx.saved_tensors
+        ls = desc.d
         if ctx.hooked is not None:
             H.check_saved(ctx, ts, gs if gy is None else gy)
-        shape, d = s.shape, s.shape[-1]
-        (s2, ls), w, st = H.rows(s.reshape(-1, d)), w.contiguous(), st.contiguous()
-        if gs is not None and (gs.dtype is not s.dtype or not gs.is_contiguous()):
-            gs = gs.to(s.dtype).contiguous()
+            s, w, st = s.contiguous(), w.contiguous(), st.contiguous()
+        ty = s.dtype
+        if gs is not None and (gs.dtype is not ty or not gs.is_contiguous()):
+            gs = gs.to(ty).contiguous()
         if gy is None:      # the norm's result was not used
-            return (gs if xt is gs.dtype else gs.to(xt)), gs, None, None, None
+            return (gs if xt is ty else gs.to(xt)), gs, None, None, None
         if gy.dtype is not yt or not gy.is_contiguous():
             gy = gy.to(yt).contiguous()
-        ds = torch.empty(shape, device=s.device, dtype=s.dtype)
-        dx = None if xt is s.dtype else torch.empty(shape, device=s.device, dtype=xt)
+        ds = torch.empty_like(s)
+        dx = None if xt is ty else torch.empty_like(s, dtype=xt)
         dw = torch.empty_like(w)
         if desc.rows:
             lib = _lib.load()
             dev = s.get_device()
             with H.on_device(dev):
                 nws = lib.m3_add_norm_bwd_workspace_bytes(desc)
-            ws = torch.empty(nws, device=s.device, dtype=torch.uint8)
-            H.launch(dev, lib.m3_add_norm_bwd, desc, s2.data_ptr(), ls, w.data_ptr(),
+            ws = w.new_empty(-(-nws // 4))
+            H.launch(dev, lib.m3_add_norm_bwd, desc, s.data_ptr(), ls, w.data_ptr(),
                      st.data_ptr(), gy.data_ptr(), H.ptr(gs), ds.data_ptr(), H.ptr(dx),
                      dw.data_ptr(), ws.data_ptr(), nws)
         else:
