@@ -58,8 +58,9 @@ __device__ __forceinline__ float softplus_f(float x) {
   return x > 20.f ? x : log1pf(expf(x));
 }
 
-// a = e^l and p = e^l - 1 for l <= 0 (l below -87: as -87, where a is 2e-38).  NEAR:
-// l >= -kNear, where n is 0; the same bits with half the instructions.
+// a = e^l and p = e^l - 1 for l <= 0; a is 0 from l = -87 down, where e^l is 2e-38 (a
+// gradient holds l a, which would grow with l otherwise).  NEAR: l >= -kNear, where n
+// is 0; the same bits with half the instructions.
 constexpr float kNear = 0.34f;        // below ln(2) / 2
 template <bool NEAR>
 __device__ __forceinline__ void decay2(float2 l, float2& a, float2& p) {
@@ -84,6 +85,8 @@ __device__ __forceinline__ void decay2(float2 l, float2& a, float2& p) {
         __uint_as_float((__float_as_uint(j.x) << 23) + 0x3f800000u),
         __uint_as_float((__float_as_uint(j.y) << 23) + 0x3f800000u));
     a = fma2(s, e, s);
+    if (l.x == -87.f) a.x = 0.f;
+    if (l.y == -87.f) a.y = 0.f;
     p = fma2(s, e, add2(s, f2(-1.f)));
   }
 }

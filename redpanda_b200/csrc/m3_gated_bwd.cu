@@ -113,7 +113,8 @@ __global__ void __launch_bounds__(256, 2)
     int tw = (passes - 1) * span + tw0;
     size_t at = (size_t)(base + tw + own) * D + c;
     const float* ck = p.ckpt + ((size_t)b * ((L + TS - 1) / TS) + (tw + own) / TS) * D + c;
-    float2 h = tw + own < n ? load_pair(ck, left) : f2(0.f);
+    // (a row without steps has no pass, and tw lies before it)
+    float2 h = passes > 0 && tw + own < n ? load_pair(ck, left) : f2(0.f);
     for (int k0 = passes; k0 > 0; --k0, tw -= span) {
       const int t0 = tw + own;
       const unsigned odd = st.odd_rows(bases, ld, base + t0, c0);

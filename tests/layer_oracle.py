@@ -13,6 +13,8 @@ analysis, e = 2^-24).  With l = -c softplus(decay) r, r = sigmoid(rg):
   (e^l - 1) <= 1), p's own 2 e and the product 2 e; half of these through the
   root; the root's MUFU form and product 3 e.
 * i: (1.3 |ig| + 10) e.
+* From l = -87 down (e^l = 1.6e-38, where fp32 ends) the kernel's a is 0: an error of
+  all of a, relative 1 (l itself off by lam e: from -87 (1 - lam e)).
 """
 
 import torch
@@ -29,7 +31,8 @@ def gated(x, rg, ig, decay, c=8.0, state=None, lengths=None, g=None):
     l = -c * softplus(decay) * r
     a, m = torch.exp(l), torch.sqrt(-torch.expm1(2 * l))
     lam = 1.3 * rg.abs() + 18
-    ea = (lam * l.abs() + 5) * E                     # relative error of a
+    gone = l <= -87 * (1 - lam * E)
+    ea = torch.where(gone, 1.0, (lam * l.abs() + 5) * E)   # relative error of a
     em = (lam / 2 + 5) * E                           # of m
     ei = (1.3 * ig.abs() + 10) * E
     b = m * i * x

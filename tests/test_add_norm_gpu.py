@@ -237,3 +237,42 @@ def test_8bit_of_zero_rows_tiny_rows_and_nan():
         assert torch.isnan(scale[2]).all()
         assert scale[4, 0] == 2.0 ** -126 and not q[4, :32].any() and q[4, 32:].all()
         assert torch.isfinite(scale[3]).all() and q[3, 3] == 0
+
+
+def test_one_tensor_as_branch_and_stream():
+    """x + x, whose gradient is the sum of both places'."""
+    x, _, w, gy, gs = inputs(7, 200, *[torch.float32] * 3, 6)
+    a, wc = x.cuda().requires_grad_(True), w.cuda()
+    y, s = N.m3_add_rms_norm(a, a, wc)
+    assert torch.equal(s.detach().cpu(), x + x)
+    (da,) = torch.autograd.grad((y, s), (a,), (gy.cuda(), gs.cuda()))
+    b = x.cuda().requires_grad_(True)
+    c = x.cuda().requires_grad_(True)
+    y, s = N.m3_add_rms_norm(b, c, wc)
+    db, dc = torch.autograd.grad((y, s), (b, c), (gy.cuda(), gs.cuda()))
+    assert torch.equal(da, db + dc)
+
+
+def test_a_stream_changed_behind_the_call_raises_in_backward():
+    """The sum is read again by the backward pass."""
+    a = torch.randn(3, 64, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda")
+    y, s = N.m3_add_rms_norm(a, torch.zeros(3, 64, device="cuda"), w)
+    with torch.no_grad():
+        s.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
+def test_infinite_rows_are_nan_and_no_other():
+    x = torch.randn(5, 300, generator=torch.Generator().manual_seed(3)).cuda()
+    w = torch.ones(300, device="cuda")
+    good = N.m3_add_rms_norm(x, x, w)[0]
+    q0, s0 = N.m3_rms_norm_8bit(x, w)
+    x[2, 7] = float("inf")
+    y, _ = N.m3_add_rms_norm(x, x, w)
+    q, sc = N.m3_rms_norm_8bit(x, w)
+    keep = [0, 1, 3, 4]
+    assert torch.isnan(y[2, 7]) and torch.equal(y[keep], good[keep])
+    assert torch.isnan(sc[2]).all() and torch.equal(sc[keep], s0[keep])
+    assert torch.equal(q[keep].view(torch.uint8), q0[keep].view(torch.uint8))

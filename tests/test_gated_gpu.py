@@ -306,3 +306,80 @@ def test_rows_of_every_alignment(B, L, D, offset, ty):
     for t, k in zip(views(grads[:3]), ("dx", "drg", "dig")):
         assert O.excess(t, ref[k], ref["+" + k], ty) <= 1
     assert O.excess(grads[3], ref["ddecay"], ref["+ddecay"], torch.float32) <= 1
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("B,L,D", [(1, 1, 1), (3, 64, 96), (2, 777, 33), (1, 3000, 64),
+                                   (2, 130, 200), (3600, 9, 64)])
+def test_decays_near_one(B, L, D, ty):
+    """Decays whose exponent needs no range reduction, in every channel of a warp."""
+    x, rg, ig, _, gr, st, lens = inputs(B, L, D, T[ty], B + 3 * L + D, True, True)
+    decay = torch.rand(D, generator=torch.Generator().manual_seed(D)) * 3 - 7
+    check(x, rg, ig, decay, gr, st, lens)
+
+
+@pytest.mark.parametrize("c", [0.5, 300.0])
+def test_other_factors_of_the_decay(c):
+    x, rg, ig, decay, gr, st, lens = inputs(2, 300, 70, torch.float32, 12, True, True)
+    check(x, rg, ig, decay, gr, st, lens, c=c)
+
+
+def test_rows_without_steps_among_long_ones():
+    """Few long rows, split over clusters, of length 0 first, last, alone and all."""
+    x, rg, ig, decay, gr, st, _ = inputs(4, 2500, 64, torch.float32, 13, True)
+    for lens in ([0, 2500, 3, 0], [0, 0, 0, 0], [2500, 0, 0, 1], [0, 0, 0, 2500]):
+        check(x, rg, ig, decay, gr, st, torch.tensor(lens))
+
+
+def test_long_rows_side_by_side_on_two_streams():
+    """Two calls whose clusters run at the same time give what each gives alone."""
+    sets = [cuda(*inputs(1, 20000, 512, torch.bfloat16, s))[:5] for s in (21, 22)]
+
+    def once(x, rg, ig, decay, gr):
+        leaves = [t.detach().requires_grad_(True) for t in (x, rg, ig, decay)]
+        y = G.m3_gated_scan(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, gr)]
+    alone = [once(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(once(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for res in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(alone[i], res))
+
+
+def test_replays_read_the_buffers_as_they_are_then():
+    """A captured scan, its backward pass and a step replayed on changed inputs."""
+    first, second = (cuda(*inputs(2, 900, 48, torch.float32, s, state=True))[:6] for s in (1, 2))
+    static = [t.clone().requires_grad_(i < 4) for i, t in enumerate(first)]
+    h = torch.zeros(2, 48, device="cuda")
+
+    def run(x, rg, ig, decay, gr, st, h):
+        y, last = G.m3_gated_scan_with_state(x, rg, ig, decay, state=st)
+        grads = torch.autograd.grad(y, (x, rg, ig, decay), gr)
+        with torch.no_grad():
+            out = G.m3_gated_step_(h, x[:, 0], rg[:, 0], ig[:, 0], decay)
+        return [y.detach(), last, *grads, out]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(*static, h)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*static, h)
+    for src in (second, first):
+        with torch.no_grad():
+            for a, b in zip(static, src):
+                a.copy_(b)
+        h.zero_()
+        graph.replay()
+        leaves = [t.clone().requires_grad_(i < 4) for i, t in enumerate(src)]
+        for a, b in zip(out, run(*leaves, torch.zeros_like(h))):
+            assert torch.equal(a, b)

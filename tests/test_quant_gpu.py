@@ -173,3 +173,39 @@ def test_another_stream_and_capture():
         third = once()
     graph.replay()
     assert torch.equal(first, second) and torch.equal(first, third)
+
+
+def test_one_weight_on_two_streams_and_replays_of_changed_rows():
+    q, _ = weight(700, 600, 64, True, 15)
+    xs = torch.randn(6, 3, 600, generator=torch.Generator().manual_seed(5)).cuda()
+    alone = [Q.m3_rows_linear_q4(x, q)[0] for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = {}
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i, x in enumerate(xs):
+        with torch.cuda.stream(streams[i % 2]):
+            got[i] = Q.m3_rows_linear_q4(x, q, overlap=True)[0]
+    torch.cuda.synchronize()
+    assert all(torch.equal(got[i], alone[i]) for i in got)
+    static, graph = xs[0].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = Q.m3_rows_linear_q4(static, q)[0]
+    for x, ref in zip(xs, alone):
+        static.copy_(x)
+        graph.replay()
+        assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_quantized_weight_and_its_product(ty):
+    """From a float weight to a product: what the dequantised weight gives."""
+    g = torch.Generator().manual_seed(1)
+    w, x = torch.randn(300, 200, generator=g), torch.randn(5, 200, generator=g).to(T[ty])
+    q = Q.Q4Weight.quantize(w, 32)
+    d = q.dequantize()
+    scale = (d.abs().amax(1, keepdim=True) * 2).expand_as(d)     # >= |q - 8| scale + |center|
+    out = Q.m3_rows_linear_q4(x.cuda(), q.to("cuda"))[0]
+    ref, tol = product(x, dict(w=d, spread=scale, group=32), None, None, None, 0)
+    far = (out.cpu().double() - ref).abs()
+    assert (far <= tol * 1.01 + half_step(T[ty]) * (ref.abs() + tol)).all()
