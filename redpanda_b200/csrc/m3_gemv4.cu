@@ -459,10 +459,12 @@ cudaError_t with_type(RowsQ4Params p, cudaStream_t s) {
   // Warps along the columns while tiles are few, along the outputs where there are more
   // than one wave of CTAs: fewer copies of the inputs are staged (65536 outputs, 3 rows
   // of 8192 bf16: 256 CTAs 79 us, 512 90, 1024 101; 3000 outputs, 8 rows of 6000: 188 CTAs
-  // 35, 94 32, 47 39).
+  // 35, 94 32, 47 39).  As many as fill the wave: 40000 outputs, 8 rows of 8192 fp32 5
+  // warps 163, 8 warps in fewer CTAs 187; 50000, 8 rows of 4096 bf16 6 warps 36, 8 45.
   int mt = 1, mw = 1;
   if (tiles > 2LL * p.sms) mt = 2;
-  while (mw < 8 && tiles > 2LL * p.sms * mt * mw) mw *= 2;
+  const long long wave = 2LL * p.sms * mt;
+  if (tiles > wave) mw = tiles > 8 * wave ? 8 : (int)((tiles + wave - 1) / wave);
   p.mw = mw;
   p.kw = 8 / mw < units ? 8 / mw : units;
   switch (nb * 2 + (mt - 1)) {

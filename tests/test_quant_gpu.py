@@ -103,6 +103,13 @@ def test_large(rows, k, n, group, center, ty):
     run(rows, k, n, group, center, ty, norm=True)
 
 
+@pytest.mark.parametrize("ty,k,rows", [("f32", 130, 3), ("bf16", 300, 5)])
+@pytest.mark.parametrize("n", [11000, 27001, 34000, 45007, 50000, 64999, 75001, 80000])
+def test_every_number_of_warps_along_the_outputs(n, ty, k, rows):
+    """Tiles that fill one wave of CTAs with 2 to 8 warps' worth each, and more than one."""
+    run(rows, k, n, 64, True, ty, norm=True, split=n // 3, silu=True)
+
+
 def test_strides_split_ends_and_the_residual_in_place():
     g = torch.Generator().manual_seed(4)
     q, w = weight(48, 96, 32, True, 7)
