@@ -92,7 +92,7 @@ int fill_gated(const m3_gated_desc* d, const m3_gated_args* a, bool backward,
   p->ld_x = a->ld_x; p->ld_r = a->ld_r; p->ld_i = a->ld_i;
   p->decay = a->decay; p->c = d->c; p->h0 = a->state; p->lengths = a->lengths;
   p->B = d->batch; p->L = d->seqlen; p->D = d->d_inner; p->dtype = d->dtype;
-  // rows of vectors (16 bytes), of words, or of half words; `more`: the other arrays
+  // rows of vectors (16 bytes), of words, or any; `more`: the other arrays
   auto rows_of = [&](int bytes) {
     const int v = bytes / e;
     bool ok = d->d_inner % v == 0 && a->ld_x % v == 0 && a->ld_r % v == 0 && a->ld_i % v == 0 &&

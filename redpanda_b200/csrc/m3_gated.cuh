@@ -116,13 +116,16 @@ template <int LC, int TS> struct Lanes {
   static constexpr int kSub = 32 / LC, kTile = 2 * LC, kSteps = TS * kSub;
 };
 
-// How rows are copied, by what their starts and lengths allow: 16 bytes at a time,
-// words (fp32, and bf16 rows of whole words), or words that bf16 rows start in the
-// middle of.  All asynchronous: with plain loads a row that is not aligned to 16 bytes
-// is waited for where it is asked for (2 x 16001 x 1281 fp32: 447 against 165 us
-// forward, 832 against 333 backward; 256 x 64 x 2047 bf16, half words: 224 against 163
-// and 520 against 322; 2046, words: 224 against 75 and 511 against 146).
-enum Copy { kHalfWords = 0, kWords = 1, kVectors = 2 };
+// How rows are copied and read, by what their starts and lengths allow, always
+// asynchronously: 16 bytes at a time; words (fp32, and bf16 rows of whole words); bf16 rows
+// that start anywhere, 16 bytes at a time from the 16 that the first element lies in, and
+// 16 more, to be read behind the row's shift in there.  With plain loads a row that is
+// not aligned to 16 bytes is waited for where it is asked for (2 x 16001 x 1281 fp32: 447
+// against 165 us forward, 832 against 333 backward).  Rows that start anywhere (256 x 64 x
+// 2047 bf16): 103 forward and 190 backward; by words, of which two hold a lane's pair, and
+// with neighbours in a pair 161 and 320.  Whole words copied as those rows are: 98 and 188
+// against 76 and 146 (2046).
+enum Copy { kAny = 0, kWords = 1, kVectors = 2 };
 
 // A warp's rows of NA arrays: kSteps steps of a tile, row (i, sub) (step i of run
 // sub) at i * kSub + sub, so that lanes read neighbouring words.  Each warp copies
@@ -131,25 +134,53 @@ enum Copy { kHalfWords = 0, kWords = 1, kVectors = 2 };
 template <typename T, int NA, int LC, int TS, int MODE>
 struct Stage {
   using La = Lanes<LC, TS>;
-  static_assert(MODE != kHalfWords || sizeof(T) == 2, "fp32 rows are whole words");
+  static_assert(MODE != kAny || sizeof(T) == 2, "fp32 rows are whole words");
+  // A lane's channels are neighbours where pairs are whole and aligned in every array, else
+  // LC apart, so that accesses of one element are those of consecutive lanes.
   static constexpr bool kPairs = MODE == kVectors || (MODE == kWords && sizeof(T) == 2);
-  // bytes; a row that starts in the middle of a word has one word more
-  static constexpr int kRow = La::kTile * (int)sizeof(T) + (MODE == kHalfWords ? 4 : 0);
-  static constexpr int kArray = (La::kSteps * kRow + 15) / 16 * 16;
-  static constexpr int kBytes = NA * kArray;                       // per warp
+  static constexpr int kNext = kPairs ? 1 : LC;                    // to the second channel
+  static constexpr int kRow = La::kTile * (int)sizeof(T) + (MODE == kAny ? 16 : 0);   // bytes
+  static constexpr int kArray = La::kSteps * kRow, kBytes = NA * kArray;                  // per warp
   static constexpr int V = 16 / (int)sizeof(T), PR = La::kTile / V, RI = 32 / PR;
+  static_assert(La::kSteps % RI == 0 && La::kSteps <= 32, "copies take whole rows");
   const T* p[NA];                    // of step t0 of the row: this lane's first piece
-  const T* lo[NA]; const T* hi[NA];  // kHalfWords: the array's bounds
+  struct Shift { unsigned at[NA], step[NA]; };        // of a run's rows, in bytes
 
-  __device__ __forceinline__ void word(unsigned s, const void* g) const {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(g) : "memory");
+  // a lane's first channel in the tile
+  static __device__ __forceinline__ int channel() {
+    return threadIdx.x % LC * (kPairs ? 2 : 1);
   }
   static __device__ __forceinline__ int row_at(int rr) {
     return (rr % TS * La::kSub + rr / TS) * kRow;
   }
+  static __device__ __forceinline__ void copy16(unsigned s, uintptr_t g) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(g) : "memory");
+  }
+  // the 16 bytes at g, less what lies outside the array
+  static __device__ __forceinline__ void copy_part(unsigned s, uintptr_t g, uintptr_t lo,
+                                                   uintptr_t hi) {
+    if (g >= lo) {
+      const int n = hi - g < 16 ? (int)(hi - g) : 16;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(g), "r"(n)
+                   : "memory");
+    } else {
+      for (int i = 0; i < 16; i += (int)sizeof(T))
+        if (g + i >= lo && g + i < hi) {
+          if constexpr (sizeof(T) == 2)
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(s + i),
+                         "h"(*reinterpret_cast<const unsigned short*>(g + i))
+                         : "memory");
+          else
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(s + i),
+                         "r"(*reinterpret_cast<const unsigned*>(g + i))
+                         : "memory");
+        }
+    }
+  }
 
-  // rows t0 .. below n; channels c0 .. below D
-  __device__ __forceinline__ void issue(char* buf, const long long (&ld)[NA], int t0, int n,
+  // rows t0 .. below n; channels c0 .. below D; of the arrays at base, `rows` rows each
+  __device__ __forceinline__ void issue(char* buf, const void* const (&base)[NA],
+                                        const long long (&ld)[NA], long long rows, int t0, int n,
                                         int c0, int D) const {
     const int lane = threadIdx.x;
     const unsigned to = (unsigned)__cvta_generic_to_shared(buf);
@@ -163,9 +194,7 @@ struct Stage {
             const unsigned s = to + row_at(rr) + c * (int)sizeof(T);
 #pragma unroll
             for (int k = 0; k < NA; ++k)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s + k * kArray),
-                           "l"(p[k] + (long long)(i * RI) * ld[k])
-                           : "memory");
+              copy16(s + k * kArray, reinterpret_cast<uintptr_t>(p[k] + (long long)(i * RI) * ld[k]));
           }
         }
       }
@@ -177,53 +206,51 @@ struct Stage {
         if (t0 + rr < n && c0 + w * E < D) {
 #pragma unroll
           for (int k = 0; k < NA; ++k)
-            word(to + k * kArray + row_at(rr) + w * 4, p[k] + rr * ld[k] + w * E);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + k * kArray +
+                                                                          row_at(rr) + w * 4),
+                         "l"(p[k] + rr * ld[k] + w * E)
+                         : "memory");
         }
       }
     } else {
-      // word w of a row holds its channels 2 w and 2 w + 1, or 2 w - 1 and 2 w; a lane
-      // copies the word of its first channel, and a run's last lane the one behind it
-      const int sub = lane / LC, w = lane % LC, c = c0 + 2 * w;
+      const int row = lane / PR, width = min(D - c0, La::kTile) * (int)sizeof(T);
 #pragma unroll
       for (int k = 0; k < NA; ++k) {
-        const T* g = p[k] + sub * TS * ld[k] + 2 * w;
-        // whether a word can pass the array's ends
-        const bool inside = p[k] > lo[k] && p[k] + (La::kSteps - 1) * ld[k] + La::kTile < hi[k];
+        const uintptr_t lo = reinterpret_cast<uintptr_t>(base[k]),
+                        hi = lo + ((rows - 1) * ld[k] + D) * (long long)sizeof(T);
+        const uintptr_t mine = reinterpret_cast<uintptr_t>(p[k]);
+        const long long bytes = ld[k] * (long long)sizeof(T);      // from row to row
+        const uintptr_t first = mine - row * bytes;                // row 0
+        auto needed = [&](int rr, uintptr_t from, uintptr_t g) {
+          return t0 + rr < n && g < from + width;
+        };
+        if ((first & ~(uintptr_t)15) >= lo && first + (La::kSteps - 1) * bytes + kRow <= hi) {
+          auto copy = [&](int rr, uintptr_t from, int piece) {
+            const uintptr_t g = (from & ~(uintptr_t)15) + piece * 16;
+            if (needed(rr, from, g)) copy16(to + k * kArray + row_at(rr) + piece * 16, g);
+          };
 #pragma unroll
-        for (int i = 0; i < TS; ++i, g += ld[k]) {
-          const uintptr_t at = reinterpret_cast<uintptr_t>(g);
-          const int odd = (int)(at >> 1 & 1);
-          const T* a = reinterpret_cast<const T*>(at & ~(uintptr_t)3);
-          const unsigned s = to + k * kArray + row_at(sub * TS + i) + w * 4;
-          if (t0 + sub * TS + i >= n || c - odd >= D) continue;
-          const bool next = odd && w == LC - 1 && c + 1 < D;
-          if (inside) {
-            word(s, a);
-            if (next) word(s + 4, a + 2);
-          } else {
-            T* q = reinterpret_cast<T*>(buf + (s - to));
-            if (a >= lo[k]) q[0] = a[0];
-            if (a + 1 < hi[k]) q[1] = a[1];
-            if (next) {
-              q[2] = a[2];
-              if (a + 3 < hi[k]) q[3] = a[3];
-            }
+          for (int i = 0; i < La::kSteps / RI; ++i)
+            copy(i * RI + row, mine + (long long)(i * RI) * bytes, lane % PR);
+          if (lane < La::kSteps) copy(lane, first + lane * bytes, PR);
+        } else {                                     // pieces may pass the array's ends
+#pragma unroll 1
+          for (int i = lane; i < La::kSteps * (PR + 1); i += 32) {
+            const int rr = i / (PR + 1), piece = i % (PR + 1);
+            const uintptr_t from = first + rr * bytes,
+                            g = (from & ~(uintptr_t)15) + piece * 16;
+            if (needed(rr, from, g)) copy_part(to + k * kArray + row_at(rr) + piece * 16, g, lo, hi);
           }
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // p[k] for the row that starts at `row` (b L + t0), of `rows`
-  __device__ __forceinline__ void at(int k, const void* base, long long row, long long rows,
-                                     long long ld, int c0, int D) {
+  // p[k] for the row that starts at `row` (b L + t0)
+  __device__ __forceinline__ void at(int k, const void* base, long long row, long long ld, int c0) {
     const int lane = threadIdx.x;
-    p[k] = static_cast<const T*>(base) + (row + (MODE == kVectors ? lane / PR : 0)) * ld + c0 +
+    p[k] = static_cast<const T*>(base) + (row + (MODE == kWords ? 0 : lane / PR)) * ld + c0 +
            (MODE == kVectors ? lane % PR * V : 0);
-    if constexpr (MODE == kHalfWords) {
-      lo[k] = static_cast<const T*>(base);
-      hi[k] = lo[k] + (rows - 1) * ld + D;
-    }
   }
   // all but the last LEFT calls of issue are complete
   template <int LEFT = 0>
@@ -231,54 +258,57 @@ struct Stage {
     asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
     __syncwarp();
   }
-  // Whether the rows of this lane's run start in the middle of a word: bit k for its
-  // first step's, bit NA + k for whether that changes from step to step
-  // (kHalfWords; row: b L + the step)
-  __device__ __forceinline__ unsigned odd_rows(const void* const (&base)[NA],
-                                               const long long (&ld)[NA], long long row,
-                                               int c0) const {
-    unsigned m = 0;
-    if constexpr (MODE == kHalfWords)
+  // of this lane's run, whose first step is row b L + t
+  static __device__ __forceinline__ Shift shifts(const void* const (&base)[NA],
+                                                 const long long (&ld)[NA], long long row,
+                                                 int c0) {
+    Shift m = {};
+    if constexpr (MODE == kAny)
 #pragma unroll
       for (int k = 0; k < NA; ++k) {
-        m |= (unsigned)((reinterpret_cast<uintptr_t>(base[k]) >> 1) + row * ld[k] + c0 & 1) << k;
-        m |= (unsigned)(ld[k] & 1) << (NA + k);
+        m.step[k] = (unsigned)ld[k] * (unsigned)sizeof(T);
+        m.at[k] = (unsigned)reinterpret_cast<uintptr_t>(base[k]) + (unsigned)row * m.step[k] +
+                  c0 * (unsigned)sizeof(T);
       }
     return m;
   }
   // the lane's pair of step i of array k
-  static __device__ __forceinline__ float2 get(const char* buf, int k, int i, unsigned odd) {
+  static __device__ __forceinline__ float2 get(const char* buf, int k, int i, const Shift& m) {
     const char* from = buf + k * kArray + i * La::kSub * kRow;
-    if constexpr (MODE == kHalfWords) {
-      const unsigned* q = reinterpret_cast<const unsigned*>(
-          from + threadIdx.x / LC * kRow) + threadIdx.x % LC;
-      const unsigned a = q[0], b = q[1];
-      const bool o = (odd >> k ^ (odd >> (NA + k) & i)) & 1;
-      return make_float2(__uint_as_float(o ? a & 0xffff0000u : a << 16),
-                         __uint_as_float(o ? b << 16 : a & 0xffff0000u));
-    } else {
+    if constexpr (kPairs) {
       const Pack<T, 2> v = ld_pack<T, 2>(reinterpret_cast<const T*>(from) + 2 * threadIdx.x);
       return make_float2(v.get(0), v.get(1));
+    } else {
+      const unsigned shift = MODE == kAny ? m.at[k] + i * m.step[k] & 15u : 0u;
+      const T* q = reinterpret_cast<const T*>(from + threadIdx.x / LC * kRow + shift) + channel();
+      return make_float2(Elem<T>::get(q[0]), Elem<T>::get(q[LC]));
     }
   }
 };
 
-// A lane's pair of channels in a (.., D) array, element by element where a pair
-// may be cut or is not aligned.
-template <bool PAIR, typename T>
+// A lane's two channels in a (.., D) array, NEXT apart (St: the Stage), of which `left`
+// are there from the first one on.
+template <typename St, typename T>
 __device__ __forceinline__ void store_pair(T* p, float2 v, int left) {
-  if constexpr (PAIR) {
+  if constexpr (St::kPairs) {
     if (left > 0) {
       if constexpr (sizeof(T) == 2) *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v);
       else *reinterpret_cast<float2*>(p) = v;
     }
   } else {
     if (left > 0) p[0] = Elem<T>::put(v.x);
-    if (left > 1) p[1] = Elem<T>::put(v.y);
+    if (left > St::kNext) p[St::kNext] = Elem<T>::put(v.y);
   }
 }
-__device__ __forceinline__ float2 load_pair(const float* p, int left) {
-  return make_float2(left > 0 ? p[0] : 0.f, left > 1 ? p[1] : 0.f);
+// the same of fp32 arrays that need not be aligned to pairs
+template <typename St>
+__device__ __forceinline__ void store_each(float* p, float2 v, int left) {
+  if (left > 0) p[0] = v.x;
+  if (left > St::kNext) p[St::kNext] = v.y;
+}
+template <typename St>
+__device__ __forceinline__ float2 load_each(const float* p, int left) {
+  return make_float2(left > 0 ? p[0] : 0.f, left > St::kNext ? p[St::kNext] : 0.f);
 }
 
 // ------------------------------------------------------------------ joins

@@ -67,15 +67,16 @@ __global__ void __launch_bounds__(256, 2)
   const GatedParams& p = q.f;
   const int lane = threadIdx.x, w = __shfl_sync(0xffffffffu, threadIdx.y, 0), W = blockDim.y;
   const int S = p.splits, rank = blockIdx.x % S;
-  const int c0 = blockIdx.x / S * La::kTile, c = c0 + lane % LC * 2;
+  const int c0 = blockIdx.x / S * La::kTile, c = c0 + St::channel();
   const int left = p.D - c, D = p.D, L = p.L, span = S * W * La::kSteps;
   const int tw0 = (rank * W + w) * La::kSteps, own = lane / LC * TS;   // of the warp; of the run
   const long long ld[4] = {p.ld_x, p.ld_r, p.ld_i, D};
+  const long long rows = (long long)p.B * L;
   const void* const bases[4] = {p.x, p.rg, p.ig, q.g};
   char* buf = smem + w * St::kBytes;
   const Joint<LC> joint(smem + W * St::kBytes, W, S);
   St st;
-  const float2 dec = load_pair(p.decay + c, left);
+  const float2 dec = load_each<St>(p.decay + c, left);
   const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
   const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
   float2 sum = f2(0.f);
@@ -87,11 +88,11 @@ __global__ void __launch_bounds__(256, 2)
   auto start = [&](int b, int n) {
     const int tw = (n - 1) / span * span + tw0;
     const long long row = (long long)b * L + tw;
-    st.at(0, p.x, row, (long long)p.B * L, ld[0], c0, D);
-    st.at(1, p.rg, row, (long long)p.B * L, ld[1], c0, D);
-    st.at(2, p.ig, row, (long long)p.B * L, ld[2], c0, D);
-    st.at(3, q.g, row, (long long)p.B * L, ld[3], c0, D);
-    st.issue(buf, ld, tw, n, c0, D);
+    st.at(0, p.x, row, ld[0], c0);
+    st.at(1, p.rg, row, ld[1], c0);
+    st.at(2, p.ig, row, ld[2], c0);
+    st.at(3, q.g, row, ld[3], c0);
+    st.issue(buf, bases, ld, rows, tw, n, c0, D);
   };
   int n = row_length(p.lengths, blockIdx.y, L), n2;
   if (n > 0) start(blockIdx.y, n);
@@ -105,19 +106,19 @@ __global__ void __launch_bounds__(256, 2)
     for (int t0 = passes * span + tw0 + own; t0 - tw0 - own < L; t0 += span)
       for (int i = 0; i < TS && t0 + i < L; ++i) {
         const size_t at = (size_t)(base + t0 + i) * D + c;
-        store_pair<St::kPairs>(static_cast<T*>(q.dx) + at, f2(0.f), left);
-        store_pair<St::kPairs>(static_cast<T*>(q.drg) + at, f2(0.f), left);
-        store_pair<St::kPairs>(static_cast<T*>(q.dig) + at, f2(0.f), left);
+        store_pair<St>(static_cast<T*>(q.dx) + at, f2(0.f), left);
+        store_pair<St>(static_cast<T*>(q.drg) + at, f2(0.f), left);
+        store_pair<St>(static_cast<T*>(q.dig) + at, f2(0.f), left);
       }
     float2 carry = f2(0.f);                          // a_{t+1} q_{t+1}
     int tw = (passes - 1) * span + tw0;
     size_t at = (size_t)(base + tw + own) * D + c;
     const float* ck = p.ckpt + ((size_t)b * ((L + TS - 1) / TS) + (tw + own) / TS) * D + c;
     // (a row without steps has no pass, and tw lies before it)
-    float2 h = passes > 0 && tw + own < n ? load_pair(ck, left) : f2(0.f);
+    float2 h = passes > 0 && tw + own < n ? load_each<St>(ck, left) : f2(0.f);
     for (int k0 = passes; k0 > 0; --k0, tw -= span) {
       const int t0 = tw + own;
-      const unsigned odd = st.odd_rows(bases, ld, base + t0, c0);
+      const auto shift = St::shifts(bases, ld, base + t0, c0);
       St::wait();
       // FAST: every step of the warp is one of the sequence, and no decay is far from 1
       auto pass = [&](auto fast) {
@@ -125,9 +126,9 @@ __global__ void __launch_bounds__(256, 2)
         float2 a[TS], X[TS], I[TS], A[TS], R[TS], g[TS];
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const Factors f = factors<FAST>(k, St::get(buf, 0, i, odd), St::get(buf, 1, i, odd),
-                                          St::get(buf, 2, i, odd), h);
-          g[i] = St::get(buf, 3, i, odd);
+          const Factors f = factors<FAST>(k, St::get(buf, 0, i, shift), St::get(buf, 1, i, shift),
+                                          St::get(buf, 2, i, shift), h);
+          g[i] = St::get(buf, 3, i, shift);
           a[i] = f.a, X[i] = f.X, I[i] = f.I, A[i] = f.A, R[i] = f.R;
           if (!FAST && t0 + i >= n) {                // the state stays, nothing has a gradient
             a[i] = f2(1.f);
@@ -144,9 +145,9 @@ __global__ void __launch_bounds__(256, 2)
         if (k0 > 1) {
 #pragma unroll
           for (int z = 0; z < 4; ++z) st.p[z] -= (long long)span * ld[z];
-          st.issue(buf, ld, tw - span, n, c0, D);
+          st.issue(buf, bases, ld, rows, tw - span, n, c0, D);
           ck -= (size_t)(span / TS) * D;
-          h = load_pair(ck, left);                   // every pass but the last is full
+          h = load_each<St>(ck, left);                   // every pass but the last is full
         } else if (n2 > 0) {
           start(nb, n2);
         }
@@ -160,9 +161,9 @@ __global__ void __launch_bounds__(256, 2)
           part = add2(part, e);
           if (FAST || t0 + i < L) {
             const size_t o = at + (size_t)i * D;
-            store_pair<St::kPairs>(static_cast<T*>(q.dx) + o, mul2(qt, X[i]), left);
-            store_pair<St::kPairs>(static_cast<T*>(q.drg) + o, mul2(e, R[i]), left);
-            store_pair<St::kPairs>(static_cast<T*>(q.dig) + o, mul2(qt, I[i]), left);
+            store_pair<St>(static_cast<T*>(q.dx) + o, mul2(qt, X[i]), left);
+            store_pair<St>(static_cast<T*>(q.drg) + o, mul2(e, R[i]), left);
+            store_pair<St>(static_cast<T*>(q.dig) + o, mul2(qt, I[i]), left);
           }
         }
         sum = add2(sum, part);
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(256, 2)
   if (w == 0 && lane < LC) {
     float2 v = s[lane];
     for (int i = 1; i < W; ++i) v = add2(v, s[i * LC + lane]);
-    store_pair<false>(q.part + ((size_t)blockIdx.y * S + rank) * D + c, v, left);
+    store_each<St>(q.part + ((size_t)blockIdx.y * S + rank) * D + c, v, left);
   }
 }
 
@@ -259,7 +260,7 @@ cudaError_t launch_gated_bwd(const GatedBwdParams& q, cudaStream_t s) {
   using B = __nv_bfloat16;
   return copy == kVectors ? bwd_lanes<B, kVectors>(q, s)
          : copy == kWords ? bwd_lanes<B, kWords>(q, s)
-                          : bwd_lanes<B, kHalfWords>(q, s);
+                          : bwd_lanes<B, kAny>(q, s);
 }
 
 }  // namespace m3

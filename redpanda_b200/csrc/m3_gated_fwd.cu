@@ -43,15 +43,16 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
   using La = Lanes<LC, TS>;
   const int lane = threadIdx.x, w = __shfl_sync(0xffffffffu, threadIdx.y, 0), W = blockDim.y;
   const int S = p.splits, rank = blockIdx.x % S;
-  const int c0 = blockIdx.x / S * La::kTile, c = c0 + lane % LC * 2;
+  const int c0 = blockIdx.x / S * La::kTile, c = c0 + St::channel();
   const int left = p.D - c, D = p.D, L = p.L, span = S * W * La::kSteps;
   const int tw0 = (rank * W + w) * La::kSteps, own = lane / LC * TS;   // of the warp; of the run
   const long long ld[3] = {p.ld_x, p.ld_r, p.ld_i};
+  const long long rows = (long long)p.B * L;
   const void* const base[3] = {p.x, p.rg, p.ig};
   char* buf = smem + w * St::kBytes;
   const Joint<LC> joint(smem + W * St::kBytes, W, S);
   St st;
-  const float2 dec = load_pair(p.decay + c, left);
+  const float2 dec = load_each<St>(p.decay + c, left);
   const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
   const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
   int turn = 0;
@@ -60,21 +61,21 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
   // the copies of a row's first pass start while the row before it is finished
   auto start = [&](int b, int n) {
     const long long row = (long long)b * L + tw0;
-    st.at(0, p.x, row, (long long)p.B * L, ld[0], c0, D);
-    st.at(1, p.rg, row, (long long)p.B * L, ld[1], c0, D);
-    st.at(2, p.ig, row, (long long)p.B * L, ld[2], c0, D);
-    st.issue(buf, ld, tw0, n, c0, D);
+    st.at(0, p.x, row, ld[0], c0);
+    st.at(1, p.rg, row, ld[1], c0);
+    st.at(2, p.ig, row, ld[2], c0);
+    st.issue(buf, base, ld, rows, tw0, n, c0, D);
   };
   int n = row_length(p.lengths, blockIdx.y, L), n2;
   if (n > 0) start(blockIdx.y, n);
   for (int b = blockIdx.y; b < p.B; b += gridDim.y, n = n2) {
     const int nb = b + gridDim.y;
     n2 = nb < p.B ? row_length(p.lengths, nb, L) : 0;
-    float2 carry = p.h0 != nullptr ? load_pair(p.h0 + (size_t)b * D + c, left) : f2(0.f);
+    float2 carry = p.h0 != nullptr ? load_each<St>(p.h0 + (size_t)b * D + c, left) : f2(0.f);
     if (n == 0) {
       if (n2 > 0) start(nb, n2);
       if (p.h_last != nullptr && rank == 0 && w == 0 && lane < LC)
-        store_pair<false>(p.h_last + (size_t)b * D + c, carry, left);
+        store_each<St>(p.h_last + (size_t)b * D + c, carry, left);
     }
     int tw = tw0;
     T* y = static_cast<T*>(p.y) + ((size_t)b * L + tw0 + own) * D + c;
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
                                               (tw0 + own) / kGatedCkpt) * D + c;
     for (int s0 = 0; s0 < n; s0 += span, tw += span) {
       const int t0 = tw + own;
-      const unsigned odd = st.odd_rows(base, ld, (long long)b * L + t0, c0);
+      const auto shift = St::shifts(base, ld, (long long)b * L + t0, c0);
       St::wait();
       // FAST: every step of the warp is one of the sequence, and no decay is far from 1
       auto pass = [&](auto fast) {
@@ -92,8 +93,8 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
         Run run{f2(1.f), f2(0.f)};
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const float2 x = St::get(buf, 0, i, odd), r = sigmoid2(St::get(buf, 1, i, odd)),
-                       g = sigmoid2(St::get(buf, 2, i, odd));
+          const float2 x = St::get(buf, 0, i, shift), r = sigmoid2(St::get(buf, 1, i, shift)),
+                       g = sigmoid2(St::get(buf, 2, i, shift));
           float2 m, inv;
           decay2<FAST>(mul2(k, r), a[i], m);
           root2(m, m, inv);
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
         if (s0 + span < n) {
 #pragma unroll
           for (int q = 0; q < 3; ++q) st.p[q] += (long long)span * ld[q];
-          st.issue(buf, ld, tw + span, n, c0, D);
+          st.issue(buf, base, ld, rows, tw + span, n, c0, D);
         } else if (n2 > 0) {
           start(nb, n2);
         }
@@ -117,10 +118,10 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
           if (i % kGatedCkpt == 0 && ck != nullptr && (FAST || t0 + i < n))
-            store_pair<St::kPairs>(ck + (size_t)(i / kGatedCkpt) * D, h, left);
+            store_pair<St>(ck + (size_t)(i / kGatedCkpt) * D, h, left);
           h = fma2(a[i], h, v[i]);
-          if (FAST) store_pair<St::kPairs>(y + (size_t)i * D, h, left);
-          else if (t0 + i < L) store_pair<St::kPairs>(y + (size_t)i * D, t0 + i < n ? h : f2(0.f), left);
+          if (FAST) store_pair<St>(y + (size_t)i * D, h, left);
+          else if (t0 + i < L) store_pair<St>(y + (size_t)i * D, t0 + i < n ? h : f2(0.f), left);
         }
       };
       if (near && tw + La::kSteps <= n) pass(std::true_type());
@@ -130,10 +131,10 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
       if (ck != nullptr) ck += (size_t)(span / kGatedCkpt) * D;
     }
     if (n > 0 && p.h_last != nullptr && rank == 0 && w == W - 1 && lane >= 32 - LC)
-      store_pair<false>(p.h_last + (size_t)b * D + c, carry, left);
+      store_each<St>(p.h_last + (size_t)b * D + c, carry, left);
     for (; tw - tw0 < L; tw += span) {               // steps past the length
       for (int i = 0; i < TS && tw + own + i < L; ++i)
-        store_pair<St::kPairs>(y + (size_t)i * D, f2(0.f), left);
+        store_pair<St>(y + (size_t)i * D, f2(0.f), left);
       y += (size_t)span * D;
     }
   }
@@ -149,9 +150,10 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
   constexpr int TS = 4;
   static_assert(TS == kGatedCkpt, "a pass starts at a checkpoint");
   using St = Stage<T, 3, 32, TS, MODE>;
-  const int lane = threadIdx.x, w = threadIdx.y;
-  const int c0 = blockIdx.x * 64, c = c0 + lane * 2, left = p.D - c, D = p.D, L = p.L;
+  const int w = threadIdx.y;
+  const int c0 = blockIdx.x * 64, c = c0 + St::channel(), left = p.D - c, D = p.D, L = p.L;
   const long long ld[3] = {p.ld_x, p.ld_r, p.ld_i};
+  const long long rows = (long long)p.B * L;
   const void* const base[3] = {p.x, p.rg, p.ig};
   char* buf = smem + w * 2 * St::kBytes;
   St st;
@@ -159,9 +161,9 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
   int b = blockIdx.y * blockDim.y + w, nb, n, tn = 0;   // (nb, tn): the pass that is copied next
   if (b >= p.B) return;
   auto at = [&](int row) {
-    st.at(0, p.x, (long long)row * L, (long long)p.B * L, ld[0], c0, D);
-    st.at(1, p.rg, (long long)row * L, (long long)p.B * L, ld[1], c0, D);
-    st.at(2, p.ig, (long long)row * L, (long long)p.B * L, ld[2], c0, D);
+    st.at(0, p.x, (long long)row * L, ld[0], c0);
+    st.at(1, p.rg, (long long)row * L, ld[1], c0);
+    st.at(2, p.ig, (long long)row * L, ld[2], c0);
   };
   nb = b;
   int nn = n = row_length(p.lengths, b, L);             // the length of nb
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
       }
     }
     if (nb < p.B) {
-      st.issue(buf + put * St::kBytes, ld, tn, nn, c0, D);
+      st.issue(buf + put * St::kBytes, base, ld, rows, tn, nn, c0, D);
 #pragma unroll
       for (int q = 0; q < 3; ++q) st.p[q] += TS * ld[q];
       tn += TS;
@@ -188,37 +190,37 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
     }
   };
   ahead();
-  const float2 dec = load_pair(p.decay + c, left);
+  const float2 dec = load_each<St>(p.decay + c, left);
   const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
   const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
   for (; b < p.B; b += step) {
     n = row_length(p.lengths, b, L);
-    float2 h = p.h0 != nullptr ? load_pair(p.h0 + (size_t)b * D + c, left) : f2(0.f);
+    float2 h = p.h0 != nullptr ? load_each<St>(p.h0 + (size_t)b * D + c, left) : f2(0.f);
     T* y = static_cast<T*>(p.y) + (size_t)b * L * D + c;
     float* ck = p.ckpt == nullptr ? nullptr : p.ckpt + (size_t)b * ((L + TS - 1) / TS) * D + c;
     for (int t0 = 0; t0 < n; t0 += TS) {
       ahead();
-      const unsigned odd = st.odd_rows(base, ld, (long long)b * L + t0, c0);
+      const auto shift = St::shifts(base, ld, (long long)b * L + t0, c0);
       St::template wait<1>();
       const char* from = buf + get * St::kBytes;
       get ^= 1;
       if (ck != nullptr) {
-        store_pair<St::kPairs>(ck, h, left);
+        store_pair<St>(ck, h, left);
         ck += D;
       }
       auto pass = [&](auto fast) {
         constexpr bool FAST = decltype(fast)::value;
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-          const float2 x = St::get(from, 0, i, odd), r = sigmoid2(St::get(from, 1, i, odd)),
-                       g = sigmoid2(St::get(from, 2, i, odd));
+          const float2 x = St::get(from, 0, i, shift), r = sigmoid2(St::get(from, 1, i, shift)),
+                       g = sigmoid2(St::get(from, 2, i, shift));
           float2 a, m, inv;
           decay2<FAST>(mul2(k, r), a, m);
           root2(m, m, inv);
           const float2 v = fma2(a, h, mul2(mul2(m, g), x));
           if (FAST || t0 + i < n) {
             h = v;
-            store_pair<St::kPairs>(y, h, left);
+            store_pair<St>(y, h, left);
             y += D;
           }
         }
@@ -227,8 +229,8 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
       else pass(std::false_type());
       __syncwarp();
     }
-    if (p.h_last != nullptr) store_pair<false>(p.h_last + (size_t)b * D + c, h, left);
-    for (int t = n; t < L; ++t, y += D) store_pair<St::kPairs>(y, f2(0.f), left);
+    if (p.h_last != nullptr) store_each<St>(p.h_last + (size_t)b * D + c, h, left);
+    for (int t = n; t < L; ++t, y += D) store_pair<St>(y, f2(0.f), left);
   }
 }
 
@@ -395,7 +397,7 @@ cudaError_t launch_gated_fwd(const GatedParams& p, cudaStream_t s) {
   using B = __nv_bfloat16;
   return p.copy == kVectors ? fwd_lanes<B, kVectors>(p, s)
          : p.copy == kWords ? fwd_lanes<B, kWords>(p, s)
-                            : fwd_lanes<B, kHalfWords>(p, s);
+                            : fwd_lanes<B, kAny>(p, s);
 }
 
 cudaError_t launch_gated_step(const GatedStepParams& p, cudaStream_t s) {
