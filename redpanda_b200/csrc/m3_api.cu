@@ -740,7 +740,7 @@ int m3_rows_linear_q4(const m3_rows_q4_desc* desc, const void* x, int64_t ld_x,
   p.pdl = overlap != 0;
   p.sms = device_sms();
   p.vec = aligned(x, 4 * e) && ld_x % 4 == 0 && aligned(norm_w, 16);
-  p.vec8 = aligned(x, 16) && ld_x % 8 == 0;
+  p.vec8 = aligned(x, 16) && ld_x % 8 == 0 ? 2 : aligned(x, 4) && ld_x % 2 == 0 ? 1 : 0;
   return launch_rows_q4(p, static_cast<cudaStream_t>(stream)) == cudaSuccess ? M3_OK
                                                                              : M3_ERR_LAUNCH;
 }

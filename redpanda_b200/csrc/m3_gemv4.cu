@@ -85,15 +85,16 @@ __device__ __forceinline__ float below(float v) {   // v without its top 16 bits
 // operands agree: lane l's two instructions of 32 columns take the 8 columns from
 // 8 (l % 4), so its operands are 16 consecutive bytes of a row.
 //
-// Stages the columns from k0 of every row, with the squares' sums of every 128 columns.
+__device__ __forceinline__ float4 load4(const float* p, int left, bool vec) {
+  if (vec && left >= 4) return *reinterpret_cast<const float4*>(p);
+  return make_float4(left > 0 ? p[0] : 0.f, left > 1 ? p[1] : 0.f, left > 2 ? p[2] : 0.f,
+                     left > 3 ? p[3] : 0.f);
+}
+// Element j of a row of which `left` are there (any address but the row's start is one of
+// the row's own); the bits, so that a load's result is not used where it is asked for.
 template <typename T>
-__device__ __forceinline__ float4 load4(const T* p, int left, bool vec) {
-  if (vec && left >= 4) {
-    const Pack<T, 4> v = ld_pack<T, 4>(p);
-    return make_float4(v.get(0), v.get(1), v.get(2), v.get(3));
-  }
-  return make_float4(left > 0 ? Elem<T>::get(p[0]) : 0.f, left > 1 ? Elem<T>::get(p[1]) : 0.f,
-                     left > 2 ? Elem<T>::get(p[2]) : 0.f, left > 3 ? Elem<T>::get(p[3]) : 0.f);
+__device__ __forceinline__ T element(const T* p, int j, int left) {
+  return p[max(min(j, left - 1), 0)];
 }
 __device__ __forceinline__ uint2 top_halves(const float4& v) {
   return make_uint2(top_halves(make_float2(v.x, v.y)), top_halves(make_float2(v.z, v.w)));
@@ -124,38 +125,113 @@ __device__ __forceinline__ float row_totals(const float (&v)[kQ4Rows]) {
   return t;
 }
 
+// f(r, columns of row r) for every row of bf16, four columns from x, of which `left` are
+// there; every load before any value is widened, four rows at a time where elements are
+// loaded one by one (a value widened beside its load is waited for there: 4 rows with the
+// norm, 4985 -> 1617 23 against 14 us).
+template <typename T, typename F>
+__device__ __forceinline__ void for_rows(const T* x, long long ld, int rows, int left, bool vec,
+                                         F&& f) {
+  if (__all_sync(0xffffffffu, vec && left >= 4)) {
+    Pack<T, 4> v[kQ4Rows];
+#pragma unroll
+    for (int r = 0; r < kQ4Rows; ++r)
+      if (r < rows) v[r] = ld_pack<T, 4>(x + r * ld);
+#pragma unroll
+    for (int r = 0; r < kQ4Rows; ++r) {
+      if (r >= rows) break;
+      f(r, make_float4(v[r].get(0), v[r].get(1), v[r].get(2), v[r].get(3)));
+    }
+  } else {
+#pragma unroll
+    for (int r0 = 0; r0 < kQ4Rows; r0 += 4) {
+      T e[4][4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r0 + r < rows)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) e[r][j] = element(x + (r0 + r) * ld, j, left);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r0 + r < rows) {
+          auto get = [&](int j) { return j < left ? Elem<T>::get(e[r][j]) : 0.f; };
+          f(r0 + r, make_float4(get(0), get(1), get(2), get(3)));
+        }
+    }
+  }
+}
+
+// Stages the columns from k0 of every row, with the squares' sums of every 128 columns.
+// bf16 rows without a norm are copied as they are, 16 or 4 bytes at a time, or, where they
+// start in the middle of a word, by elements (7 rows, 7050 -> 1299: by words 10 us, split
+// as the others are 35).
 template <typename T>
 __device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* sq, int parts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int row = (p.chunk + kPad) * 2;              // bytes
   const T* x = static_cast<const T*>(p.x) + k0;
-  if (sizeof(T) == 2 && parts == 1 && p.vec8 != 0) {   // rows as they are
-    for (int r = 0; r < p.rows; ++r)
-      for (int c = (warp * 32 + lane) * 8; c < n; c += warps * 256) {
-        const int left = (p.d_in - k0 - c) * 2, bytes = left < 0 ? 0 : left < 16 ? left : 16;
-        const T* from = x + (size_t)r * p.ld_x + (bytes > 0 ? c : 0);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                         (unsigned)__cvta_generic_to_shared(rows + r * row + c * 2)),
-                     "l"(from), "r"(bytes)
-                     : "memory");
+  if constexpr (sizeof(T) == 2) {
+    if (parts == 1 && p.vec8 == 2) {
+      for (int r = 0; r < p.rows; ++r)
+        for (int c = (warp * 32 + lane) * 8; c < n; c += warps * 256) {
+          const int left = (p.d_in - k0 - c) * 2, bytes = left < 0 ? 0 : left < 16 ? left : 16;
+          const T* from = x + (size_t)r * p.ld_x + (bytes > 0 ? c : 0);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           (unsigned)__cvta_generic_to_shared(rows + r * row + c * 2)),
+                       "l"(from), "r"(bytes)
+                       : "memory");
+        }
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+      return;
+    }
+    if (parts == 1 && p.vec8 == 1) {
+      for (int r = 0; r < p.rows; ++r)
+        for (int c = (warp * 32 + lane) * 2; c < n; c += warps * 64) {
+          const int left = (p.d_in - k0 - c) * 2, bytes = left < 0 ? 0 : left < 4 ? left : 4;
+          const T* from = x + (size_t)r * p.ld_x + (bytes > 0 ? c : 0);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                           (unsigned)__cvta_generic_to_shared(rows + r * row + c * 2)),
+                       "l"(from), "r"(bytes)
+                       : "memory");
+        }
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+      return;
+    }
+    if (parts == 1) {
+      for (int c0 = warp * 128; c0 < n; c0 += warps * 128) {
+#pragma unroll
+        for (int r0 = 0; r0 < kQ4Rows; r0 += 4) {
+          unsigned short v[4][4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r0 + r < p.rows)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int c = c0 + lane + 32 * j;
+                v[r][j] = reinterpret_cast<const unsigned short*>(x)[(r0 + r) * p.ld_x +
+                                                                     (c < p.d_in - k0 ? c : 0)];
+              }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r0 + r < p.rows)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int c = c0 + lane + 32 * j;
+                if (c < n)
+                  *reinterpret_cast<unsigned short*>(rows + (r0 + r) * row + c * 2) =
+                      c < p.d_in - k0 ? v[r][j] : (unsigned short)0;
+              }
+        }
       }
-    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-    return;
+      return;
+    }
   }
   const bool vec = p.vec != 0;
   for (int c0 = warp * 128; c0 < n; c0 += warps * 128) {
     const int c = c0 + lane * 4, left = p.d_in - k0 - c, at = left > 0 ? c : 0;
-    // every row's loads before any is used
-    float4 v[kQ4Rows], w;
+    float4 w;
     float ss[kQ4Rows] = {};
-#pragma unroll
-    for (int r = 0; r < kQ4Rows; ++r)
-      if (r < p.rows) v[r] = load4(x + (size_t)r * p.ld_x + at, left, vec);
-    if (p.norm_w != nullptr) w = load4(p.norm_w + k0 + at, left, vec);
-#pragma unroll
-    for (int r = 0; r < kQ4Rows; ++r) {
-      if (r >= p.rows) break;
-      float4 y = v[r];
+    auto split = [&](int r, float4 y) {
       if (p.norm_w != nullptr) {
         ss[r] = fmaf(y.x, y.x, y.y * y.y) + fmaf(y.z, y.z, y.w * y.w);
         y = make_float4(y.x * w.x, y.y * w.y, y.z * w.z, y.w * w.w);
@@ -169,6 +245,21 @@ __device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* s
           *reinterpret_cast<uint2*>(to + 2 * p.rows * row) = top_halves(below(y));
         }
       }
+    };
+    if constexpr (sizeof(T) == 4) {                  // every row's loads before any is used
+      float4 v[kQ4Rows];
+#pragma unroll
+      for (int r = 0; r < kQ4Rows; ++r)
+        if (r < p.rows) v[r] = load4(x + (size_t)r * p.ld_x + at, left, vec);
+      if (p.norm_w != nullptr) w = load4(p.norm_w + k0 + at, left, vec);
+#pragma unroll
+      for (int r = 0; r < kQ4Rows; ++r) {
+        if (r >= p.rows) break;
+        split(r, v[r]);
+      }
+    } else {
+      if (p.norm_w != nullptr) w = load4(p.norm_w + k0 + at, left, vec);
+      for_rows(x + at, p.ld_x, p.rows, left, vec, split);
     }
     if (p.norm_w != nullptr) {
       float* to = sq + (k0 + c0) / 128 * kQ4Rows;
@@ -217,7 +308,7 @@ __device__ __forceinline__ void copy16(char* to, const char* from) {
 template <typename T, int NB, int MT, int G, bool CENTER>
 __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
   using R = Ring<MT, G, CENTER>;
-  constexpr int U = R::U, BU = R::BU, GU = R::GU;
+  constexpr int U = R::U, BU = R::BU;
   extern __shared__ __align__(16) char smem[];
   __shared__ float s_rstd[kQ4Rows];
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);

@@ -264,7 +264,7 @@ struct RowsQ4Params {
   void* out1; long long ld1;
   int rows, d_in, d_out, split, silu, group, center, dtype;
   int pdl, sms;
-  int vec, vec8;                                         // x and norm_w in vectors of 4, x of 8
+  int vec, vec8;                                         // x and norm_w in vectors of 4; bf16 x in vectors of 8 (2), words (1) or not
   int mw, kw, chunk;                                     // set by the launcher
 };
 cudaError_t launch_rows_q4(const RowsQ4Params& p, cudaStream_t s);

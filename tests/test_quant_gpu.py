@@ -110,6 +110,26 @@ def test_every_number_of_warps_along_the_outputs(n, ty, k, rows):
     run(rows, k, n, 64, True, ty, norm=True, split=n // 3, silu=True)
 
 
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("rows", [1, 4, 8])
+@pytest.mark.parametrize("k,ld,off", [(130, 130, 0), (1002, 1002, 0), (1001, 1001, 0), (3, 3, 0),
+                                      (2, 2, 0), (515, 520, 0), (515, 520, 1), (514, 518, 1),
+                                      (514, 518, 2), (1000, 1009, 9), (7050, 7050, 0),
+                                      (4985, 4987, 1)])
+def test_bf16_rows_of_every_alignment(k, ld, off, rows, norm):
+    """Rows that 16 bytes, words or elements may be copied from, that end inside them."""
+    g = torch.Generator().manual_seed(k + rows)
+    q, w = weight(40, k, 64, True, 3)
+    base = torch.randn(rows * ld + off, generator=g).to(torch.bfloat16)
+    cut = lambda t: t[off:].view(rows, ld)[:, :k]  # noqa: E731
+    nw = torch.randn(k, generator=g) * 0.3 + 1 if norm else None
+    got = Q.m3_rows_linear_q4(cut(base.cuda()), q, norm_weight=nw.cuda() if norm else None,
+                              eps=EPS)[0]
+    ref, tol = product(cut(base), w, None, nw, None, 0)
+    far = (got.cpu().double() - ref).abs()
+    assert (far <= tol * 1.01 + half_step(torch.bfloat16) * (ref.abs() + tol)).all()
+
+
 def test_strides_split_ends_and_the_residual_in_place():
     g = torch.Generator().manual_seed(4)
     q, w = weight(48, 96, 32, True, 7)
