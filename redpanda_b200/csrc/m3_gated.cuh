@@ -20,6 +20,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "m3_api_util.h"
 #include "m3_bulk.cuh"
 #include "m3_math.cuh"
 #include "m3_vec.cuh"
@@ -450,6 +451,32 @@ __device__ __forceinline__ float2 join(const Joint<LC>& j, int turn, const Run& 
   }
   c = fma2(before.P, c, before.V);
   return kSub > 1 ? fma2(ahead.P, c, ahead.V) : c;
+}
+
+// CTAs of kGatedWarps warps in clusters of k that are resident at once, 0 on an error; asked
+// for once per device.
+template <auto* kern>
+int resident_in_clusters(OncePerDevice& known, int k, int smem) {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) { cudaGetLastError(); return 0; }
+  if ((n = known.value[dev].load(std::memory_order_acquire)) > 0) return n;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = k;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(k);
+  cfg.blockDim = dim3(32, kGatedWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (allow_smem<kern>(smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  known.value[dev].store(n * k, std::memory_order_release);
+  return n * k;
 }
 
 }  // namespace m3

@@ -253,6 +253,13 @@ cudaError_t bwd_lanes(const GatedBwdParams& q, cudaStream_t s) {
 
 }  // namespace
 
+int gated_bwd_in_clusters(int k) {
+  static OncePerDevice known[9];
+  constexpr int kBytes = Stage<float, 4, 32, kGatedBwdSteps, kVectors>::kBytes;
+  return resident_in_clusters<gated_bwd_kernel<float, 32, kGatedBwdSteps, kVectors>>(
+      known[k], k, kGatedWarps * kBytes + joint_bytes(32, kGatedWarps, k));
+}
+
 cudaError_t launch_gated_bwd(const GatedBwdParams& q, cudaStream_t s) {
   const int copy = q.f.copy;
   if (q.f.dtype == M3_F32)

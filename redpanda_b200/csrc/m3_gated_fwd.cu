@@ -345,6 +345,13 @@ cudaError_t fwd_lanes(const GatedParams& p, cudaStream_t s) {
 
 }  // namespace
 
+static int fwd_in_clusters(int k) {
+  static OncePerDevice known[9];
+  constexpr int kBytes = Stage<float, 3, 32, kGatedFwdSteps, kVectors>::kBytes;
+  return resident_in_clusters<gated_fwd_kernel<float, 32, kGatedFwdSteps, kVectors>>(
+      known[k], k, kGatedWarps * kBytes + joint_bytes(32, kGatedWarps, k));
+}
+
 int gated_segments(int L) { return (L + kGatedCkpt - 1) / kGatedCkpt; }
 
 void gated_plan(int B, int L, int D, bool backward, int sms, GatedParams* p) {
@@ -367,15 +374,19 @@ void gated_plan(int B, int L, int D, bool backward, int sms, GatedParams* p) {
   p->warps = warps;
   const long long slots = wave / warps;
   // Of the tile widths and time splits whose every CTA has a pass of its own, the one
-  // with most CTAs in one wave; wide tiles and few splits among equals.  Measured: 1 x
-  // 16384 x 1024 bf16 128 CTAs of tile 64 93 us, 256 of 32 49, 384 of 16 49; 2 x 16001 x
-  // 1280 fp32 backward 160 CTAs 336, 280 187, 320 (a second, part-filled wave) 204.
+  // with most CTAs in one wave; wide tiles and few splits among equals.  A cluster lies in
+  // one group of SMs, so fewer CTAs are resident in clusters (1 x 12523 x 3592 bf16: 57
+  // clusters of 7, of which 56 are resident, 178 us, of 6 142; 2 x 16001 x 1280 fp32
+  // backward: 40 of 7, of which 37 are, 288, of 6 200).  Measured: 1 x 16384 x 1024 bf16 128
+  // CTAs of tile 64 93 us, 256 of 32 49, 384 of 16 49.
   auto tiles = [&](int l) { return (long long)(D + 2 * l - 1) / (2 * l); };
   long long most = tiles(32) * B;
   for (int l = 32; l >= 8; l /= 2)
     for (int k = 1; k <= 8; ++k) {
       const long long ctas = tiles(l) * B * k;
-      if (ctas <= slots && ctas > most && segs >= (long long)k * warps * (32 / l)) {
+      if (ctas > slots || ctas <= most || segs < (long long)k * warps * (32 / l)) continue;
+      if (k == 1 || (warps == kGatedWarps &&
+                     ctas <= (backward ? gated_bwd_in_clusters(k) : fwd_in_clusters(k)))) {
         most = ctas;
         p->lanes = l;
         p->splits = k;

@@ -237,6 +237,7 @@ struct GatedBwdParams {
 int gated_segments(int L);                               // checkpoints per row and channel
 // sets lanes, warps, splits and rows
 void gated_plan(int B, int L, int D, bool backward, int sms, GatedParams* p);
+int gated_bwd_in_clusters(int k);                        // the backward's CTAs resident in clusters of k
 cudaError_t launch_gated_fwd(const GatedParams& p, cudaStream_t s);
 cudaError_t launch_gated_bwd(const GatedBwdParams& p, cudaStream_t s);
 
