@@ -18,7 +18,7 @@
 // Seven arrays and the checkpoints (1 byte per element) move: 256 x 64 x 2048 bf16 105
 // us (4.8 TB/s), at half of the issue slots with 16 warps per SM of 128 registers (96
 // registers for more warps spill: 121 us; a warp per row without joins spills at 96 and
-// is slower at 128: 123 us).  2 x 16001 x 1280 fp32, ragged: 187 us (4.6 TB/s).
+// is slower at 128: 123 us).  2 x 16001 x 1280 fp32: 200 us (5.7 TB/s).
 #include "m3_gated.cuh"
 
 #include <type_traits>
