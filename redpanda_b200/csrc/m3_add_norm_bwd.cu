@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(MAXT, MINB) add_norm_bwd_kernel(const AddNormB
 template <typename TX, typename TS, typename TY>
 struct Launch {
   static constexpr bool kWide = sizeof(TX) == 2 || sizeof(TS) == 2 || sizeof(TY) == 2;
+  static constexpr bool kEven = true;
   static constexpr bool kWarpRows = false;
   const AddNormBwdParams& p;
   cudaStream_t s;
@@ -143,7 +144,7 @@ cudaError_t launch_add_norm_bwd(const AddNormBwdParams& p, cudaStream_t s) {
     return p.d % v == 0 && rows_ok(p.s, p.ld_s, es, v) && rows_ok(p.gy, p.d, ey, v) &&
            rows_ok(p.gs, p.d, es, v) && rows_ok(p.ds, p.d, es, v) && rows_ok(p.dx, p.d, ex, v);
   };
-  const int vec = ex + es + ey < 12 && ok(8) ? 8 : ok(4) ? 4 : 1;
+  const int vec = ex + es + ey < 12 && ok(8) ? 8 : ok(4) ? 4 : ok(2) ? 2 : 1;
   return with_types(p.dtype_x, p.dtype_s, p.dtype_y, [&](auto tx, auto ts, auto ty) {
     return add_dispatch(p.d, vec, kFrom, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
   });

@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(MAXT, MINB) add_norm_fwd_kernel(const AddNormP
 template <typename TX, typename TS, typename TY>
 struct Launch {
   static constexpr bool kWide = sizeof(TX) == 2 || sizeof(TS) == 2 || sizeof(TY) == 2;
+  static constexpr bool kEven = true;
   static constexpr bool kWarpRows = true;
   const AddNormParams& p;
   cudaStream_t s;
@@ -99,7 +100,7 @@ cudaError_t launch_add_norm_fwd(const AddNormParams& p, cudaStream_t s) {
     return p.d % v == 0 && rows_ok(p.x, p.ld_x, ex, v) && rows_ok(p.res, p.ld_r, es, v) &&
            rows_ok(p.s, p.d, es, v) && rows_ok(p.y, p.d, ey, v);
   };
-  const int vec = ex + es + ey < 12 && ok(8) ? 8 : ok(4) ? 4 : 1;
+  const int vec = ex + es + ey < 12 && ok(8) ? 8 : ok(4) ? 4 : ok(2) ? 2 : 1;
   return with_types(p.dtype_x, p.dtype_s, p.dtype_y, [&](auto tx, auto ts, auto ty) {
     return add_dispatch(p.d, vec, kFrom, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
   });

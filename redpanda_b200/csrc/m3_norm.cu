@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* part, in
 
 template <typename TX, typename TY>
 struct LaunchFwd {
-  static constexpr bool kWide = sizeof(TX) == 2 && sizeof(TY) == 2, kWarpRows = true;
+  static constexpr bool kWide = sizeof(TX) == 2 && sizeof(TY) == 2, kWarpRows = true, kEven = false;
   const NormParams& p;
   cudaStream_t s;
   template <int VEC, int NV, bool WARP, int MAXT, int MINB>
@@ -247,7 +247,7 @@ struct LaunchFwd {
 
 template <typename TX, typename TY>
 struct LaunchBwd {
-  static constexpr bool kWide = sizeof(TX) == 2 && sizeof(TY) == 2, kWarpRows = false;
+  static constexpr bool kWide = sizeof(TX) == 2 && sizeof(TY) == 2, kWarpRows = false, kEven = false;
   const NormBwdParams& p;
   cudaStream_t s;
   template <int VEC, int NV, bool WARP, int MAXT, int MINB>

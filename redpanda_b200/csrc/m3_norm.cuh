@@ -93,7 +93,8 @@ inline int norm_vec(int d, int dtype_x, int dtype_y, bool ok8, bool ok4) {
   return ok4 && d % 4 == 0 ? 4 : 1;
 }
 
-// The instantiation of a row length: f<VEC, NV, WARP, MAXT, MINB>(threads, grid).
+// The instantiation of a row length: f<VEC, NV, WARP, MAXT, MINB>(threads, grid).  Vectors
+// of 8 where F has kWide, of 2 where it has kEven.
 template <int E, typename F>
 cudaError_t norm_size(int vec, int nt, F&& f) {
   auto with = [&](auto v) -> cudaError_t {
@@ -109,6 +110,8 @@ cudaError_t norm_size(int vec, int nt, F&& f) {
   };
   if constexpr (std::decay_t<F>::kWide)
     if (vec == 8) return with(std::integral_constant<int, 8>());
+  if constexpr (std::decay_t<F>::kEven)
+    if (vec == 2) return with(std::integral_constant<int, 2>());
   return vec == 4 ? with(std::integral_constant<int, 4>())
                   : with(std::integral_constant<int, 1>());
 }
@@ -118,6 +121,8 @@ cudaError_t norm_warp(int vec, F&& f) {
   constexpr int MINB = E <= 16 ? 5 : 4;
   if constexpr (std::decay_t<F>::kWide)
     if (vec == 8) return f.template operator()<8, E / 8, true, 128, MINB>(128);
+  if constexpr (std::decay_t<F>::kEven)
+    if (vec == 2) return f.template operator()<2, E / 2, true, 128, MINB>(128);
   return vec == 4 ? f.template operator()<4, E / 4, true, 128, MINB>(128)
                   : f.template operator()<1, E, true, 128, MINB>(128);
 }

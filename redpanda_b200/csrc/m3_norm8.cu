@@ -65,6 +65,7 @@ __device__ __forceinline__ void store8(unsigned char* p, const float (&v)[VEC]) 
   }
   if constexpr (VEC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(b[0], b[1]);
   else if constexpr (VEC == 4) *reinterpret_cast<unsigned*>(p) = b[0];
+  else if constexpr (VEC == 2) *reinterpret_cast<unsigned short*>(p) = (unsigned short)b[0];
   else *p = (unsigned char)b[0];
 }
 
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm8_kernel(const Norm8Params p) 
       m = row_max<WARP>(m, red, flip);
 #pragma unroll
       for (int i = 0; i < NV; ++i) top[i] = m;
-    } else if constexpr (VEC > 1) {
+    } else if constexpr (VEC > 2) {
       // a group's columns lie in group / VEC neighbouring lanes
       const int span = p.group / VEC;
 #pragma unroll
@@ -167,6 +168,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm8_kernel(const Norm8Params p) 
 template <typename TX, typename TS>
 struct Launch {
   static constexpr bool kWide = true, kWarpRows = true;
+  static constexpr bool kEven = true;
   const Norm8Params& p;
   cudaStream_t s;
   template <int VEC, int NV, bool WARP, int MAXT, int MINB>
@@ -193,8 +195,8 @@ cudaError_t launch_norm8(const Norm8Params& p, cudaStream_t s) {
     return p.d % v == 0 && rows_ok(p.x, p.ld_x, ex, v) && rows_ok(p.res, p.ld_r, es, v) &&
            rows_ok(p.s, p.d, es, v) && aligned(p.q, v);
   };
-  const int vec = ok(8) ? 8 : ok(4) ? 4 : 1;
-  if (p.group != 0 && vec == 1) return cudaErrorInvalidValue;   // refused by the entry
+  const int vec = ok(8) ? 8 : ok(4) ? 4 : ok(2) ? 2 : 1;
+  if (p.group != 0 && vec < 4) return cudaErrorInvalidValue;   // refused by the entry
   return with_types(p.dtype_x, p.dtype_s, M3_F32, [&](auto tx, auto ts, auto) {
     return add_dispatch(p.d, vec, 1024, Launch<decltype(tx), decltype(ts)>{p, s});
   });

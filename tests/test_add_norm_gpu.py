@@ -276,3 +276,21 @@ def test_infinite_rows_are_nan_and_no_other():
     assert torch.isnan(y[2, 7]) and torch.equal(y[keep], good[keep])
     assert torch.isnan(sc[2]).all() and torch.equal(sc[keep], s0[keep])
     assert torch.equal(q[keep].view(torch.uint8), q0[keep].view(torch.uint8))
+
+
+EVEN = [(5, 2), (7, 30), (300, 130), (9, 258), (9, 514), (9, 770), (5, 1022), (4, 1026), (3, 2050),
+        (3, 5002), (2, 8194), (2, 16386), (1, 32766)]
+
+
+@pytest.mark.parametrize("tx,ts,ty", [("f32", "f32", "f32"), ("bf16", "f32", "bf16"),
+                                      ("bf16", "bf16", "bf16"), ("f32", "bf16", "f32")])
+@pytest.mark.parametrize("rows,d", EVEN)
+def test_rows_of_whole_pairs(rows, d, tx, ts, ty):
+    test_matches_definition(rows, d, tx, ts, ty)
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("tx,ts", [("f32", None), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("rows,d", EVEN)
+def test_8bit_rows_of_whole_pairs(rows, d, tx, ts, dtype):
+    test_8bit_matches_definition(rows, d, None, tx, ts, dtype)
