@@ -40,6 +40,7 @@ namespace m3 {
 namespace {
 
 constexpr int kPad = 32;           // columns behind a staged row
+constexpr int kSquares = 128;      // columns of a sum of the norm's squares: a warp's at a time
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], unsigned b0,
                                          unsigned b1) {
@@ -161,7 +162,8 @@ __device__ __forceinline__ void for_rows(const T* x, long long ld, int rows, int
   }
 }
 
-// Stages the columns from k0 of every row, with the squares' sums of every 128 columns.
+// Stages the columns from k0 of every row, with the squares' sums of every 128 columns (k0
+// is a multiple of 128 where there is a norm: each sum is written once).
 // bf16 rows without a norm are copied as they are, 16 or 4 bytes at a time, or, where they
 // start in the middle of a word, by elements (7 rows, 7050 -> 1299: by words 10 us, split
 // as the others are 35).
@@ -262,7 +264,7 @@ __device__ void stage(const RowsQ4Params& p, int k0, int n, char* rows, float* s
       for_rows(x + at, p.ld_x, p.rows, left, vec, split);
     }
     if (p.norm_w != nullptr) {
-      float* to = sq + (k0 + c0) / 128 * kQ4Rows;
+      float* to = sq + (k0 + c0) / kSquares * kQ4Rows;
       if (p.rows == 1) {
         const float t = row_totals<1>(ss);
         if (lane == 0) to[0] = t;
@@ -294,7 +296,7 @@ __host__ __device__ inline Layout layout(int warps, int cols, int chunk, int uni
   Layout l;
   l.x = warps * R::kSlots * R::kSlot;
   l.sq = l.x + (chunk + kPad) * 2 * cols;
-  l.total = l.sq + (norm ? (units * R::U + 127) / 128 * kQ4Rows * 4 : 0);
+  l.total = l.sq + (norm ? (units * R::U + kSquares - 1) / kSquares * kQ4Rows * 4 : 0);
   return l;
 }
 
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(256, 2) rows_q4_kernel(const RowsQ4Params p) {
   if (p.norm_w != nullptr)
     for (int r = warp; r < p.rows; r += blockDim.x >> 5) {
       float v = 0.f;
-      for (int u = lane; u * 128 < p.d_in; u += 32) v += sq[u * kQ4Rows + r];
+      for (int u = lane; u * kSquares < p.d_in; u += 32) v += sq[u * kQ4Rows + r];
       v = warp_total(v, 32);
       if (lane == 0) s_rstd[r] = rsqrtf(v / (float)p.d_in + p.eps);
     }
@@ -511,12 +513,18 @@ cudaError_t launch(RowsQ4Params p, cudaStream_t s) {
   const int cols = p.rows * (sizeof(T) == 4 || norm ? 3 : 1);
   // As many columns at a time as fit, a whole number of units of every warp, of fewer
   // warps where one unit of each does not fit (at one warp along the columns it does:
-  // the rings' 68 KB, 128 columns' 7 KB and 32 KB of squares' sums at d_in = kQ4MaxIn).
+  // the rings' 68 KB, 128 columns' 7 KB and 16 KB of squares' sums at d_in = kQ4MaxIn).
+  // The norm's squares are summed by 128 columns, so every chunk but the last is whole
+  // ones of these.
   auto bytes = [&](int chunk) {
     return layout<NB, MT, G, CENTER>(p.mw * p.kw, cols, chunk, units, norm).total;
   };
-  while (p.kw > 1 && bytes(p.kw * U) > kSmem) --p.kw;
-  const int step = p.kw * U;
+  auto step_of = [&](int kw) {
+    const int one = kw * U;
+    return norm && one % kSquares != 0 && units > kw ? 2 * one : one;
+  };
+  while (p.kw > 1 && bytes(step_of(p.kw)) > kSmem) --p.kw;
+  const int step = step_of(p.kw);
   int chunk = (units * U + step - 1) / step * step;
   while (chunk > step && bytes(chunk) > kSmem) chunk -= step;
   p.chunk = chunk;

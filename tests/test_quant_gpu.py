@@ -236,3 +236,44 @@ def test_quantized_weight_and_its_product(ty):
     ref, tol = product(x, dict(w=d, spread=scale, group=32), None, None, None, 0)
     far = (out.cpu().double() - ref).abs()
     assert (far <= tol * 1.01 + half_step(T[ty]) * (ref.abs() + tol)).all()
+
+
+def norm_in_chunks(rows, k, n, group, center, ty):
+    """The product with the norm ahead, on the GPU; every 13th output against the
+    definition (13 and a tile's 16 have no common divisor), whose columns all count in
+    the row's mean square."""
+    g = torch.Generator("cuda").manual_seed(rows + k + n + group)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    codes = torch.randint(0, 16, (n, k), generator=g, device="cuda", dtype=torch.uint8)
+    scale = torch.rand(n, -(-k // group), generator=g, device="cuda").add_(0.1).mul_(0.1).bfloat16()
+    mid = rnd(*scale.shape).mul_(0.1).bfloat16() if center else None
+    x, b, nw = rnd(rows, k).to(T[ty]), rnd(n), rnd(k) * 0.3 + 1
+    q = Q.Q4Weight.from_codes(codes, scale, mid, group)
+    out = Q.m3_rows_linear_q4(x, q, b, norm_weight=nw, eps=EPS)[0]
+    at = torch.arange(0, n, 13, device="cuda")
+    wide = lambda t: t[at].double().repeat_interleave(group, 1)[:, :k]  # noqa: E731
+    w = (codes[at].double() - 8) * wide(scale)
+    spread = w.abs()
+    if center:
+        w, spread = w + wide(mid), spread + wide(mid).abs()
+    ref, tol = product(x, dict(w=w, spread=spread, group=group), b[at], nw, None, 0)
+    far = (out[:, at].double() - ref).abs()
+    assert (far <= tol * 1.01 + half_step(T[ty]) * (ref.abs() + tol)).all(), float((far / tol).max())
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n,group", [(8, 2048, 50304, 64), (2, 8192, 40000, 64),
+                                            (8, 3000, 65536, 32), (8, 8192, 40000, 32),
+                                            (4, 4096, 50304, 32)])
+def test_norm_over_inputs_staged_in_parts(rows, k, n, group, ty):
+    """One warp along the columns, and inputs that are staged in two to six parts."""
+    norm_in_chunks(rows, k, n, group, True, ty)
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n", [9000, 16000, 27001, 34000, 45007, 50000, 64999, 75001])
+def test_norm_for_every_number_of_warps_and_parts(n, group, ty):
+    """1 to 8 warps' worth of tiles; inputs in one part and in two to five."""
+    for rows, k in ((8, 2048), (8, 3001), (5, 4100), (8, 4992)):
+        norm_in_chunks(rows, k, n, group, (n + k) % 2 == 0, ty)
