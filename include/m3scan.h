@@ -313,7 +313,7 @@ typedef struct m3_rows_q4_desc {
  *           column 32 (j / 2) + 8 (l % 4) + 4 (j % 2) + 2 v + e (h, v, e: 0, 1).
  *   scales  (tiles, groups, 8) of two outputs each, l and l + 8: bf16 pairs of
  *           scale and center (64 bits) with center, else their two scales (32
- *           bits); 8- or 4-byte aligned; groups cover the rounded-up columns
+ *           bits); 16-byte aligned; groups cover the rounded-up columns
  *   x (rows, ld_x); norm_w (d_in,) float32 or NULL; bias (d_out,) float32 or NULL;
  *   residual (rows, ld_r) or NULL: it may be out0 itself (same stride, split ==
  *   d_out), no other overlap of an output with an input. */

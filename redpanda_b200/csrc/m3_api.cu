@@ -713,7 +713,7 @@ int m3_rows_linear_q4(const m3_rows_q4_desc* desc, const void* x, int64_t ld_x,
       (split < d_out && ld1 < d_out - split))
     return M3_ERR_SHAPE;
   const int e = dsize(desc->dtype);
-  if (!aligned(codes, 16) || !aligned(scales, desc->center ? 8 : 4) || !aligned(x, e) ||
+  if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(x, e) ||
       !aligned(norm_w, 4) || !aligned(bias, 4) || !aligned(residual, e) ||
       (split > 0 && !aligned(out0, e)) || (split < d_out && !aligned(out1, e)))
     return M3_ERR_ALIGN;

@@ -270,3 +270,15 @@ def test_checkpoint_floats():
     f = lambda B, L, D: _lib.load().m3_gated_ckpt_floats(  # noqa: E731
         _lib.GatedDesc(B, L, D, 0, 8.0))
     assert f(2, 1, 8) == 16 and f(2, 4, 8) == 16 and f(2, 9, 8) == 48 and f(1, 0, 8) == 0
+
+
+@pytest.mark.parametrize("center", [0, 1])
+def test_scales_of_4_bit_weights_start_at_16_bytes(center):
+    """They are copied 16 bytes at a time."""
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(8192)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256     # host memory: never dereferenced
+    for off in (2, 4, 8, 12):
+        desc = _lib.RowsQ4Desc(2, 40, 6, 64, center, 0, 6, 0, 0.0)
+        assert lib.m3_rows_linear_q4(desc, p, 40, None, p + 512, p + 1024 + off, None, None, 0,
+                                     p + 2048, 6, None, 0, 0, None) == 5
