@@ -617,8 +617,11 @@ class Mamba(nn.Module):
             return self.norm_f(x)
         h = m3_rms_norm(x, norms[0].weight, norms[0].eps, out_dtype=out_type(norms[0]))
         for layer, norm in zip(self.layers, norms[1:]):
-            h, x = m3_add_rms_norm(layer["mixer"](h), x, norm.weight, norm.eps,
-                                   out_dtype=out_type(norm))
+            branch = layer["mixer"](h)
+            # the sum has the residual's type: a stream narrower than the branch
+            # (bf16 embeddings, fp32 weights) widens, as in torch's addition
+            x = x.to(torch.promote_types(x.dtype, branch.dtype))
+            h, x = m3_add_rms_norm(branch, x, norm.weight, norm.eps, out_dtype=out_type(norm))
         return h
 
     def quantize_step_(self, group=64, names=("in_proj", "out_proj"), center=True):

@@ -255,3 +255,36 @@ def test_step_on_4_bit_weights():
     assert set(m.state_dict()) == set(full.state_dict())
     with pytest.raises(ValueError):
         m.quantize_step_(names=("dt_proj",))
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+def test_fused_addition_and_norm_of_a_narrow_stream(autocast):
+    """bf16 embeddings: the stream gets the type of torch's sums, float32 behind the
+    first layer of fp32 weights.  Against the same model unfused on the same norm
+    kernels: fp32 within a few hundred roundings of 2^-24 (a stream held in bf16 is
+    2^-9 = 2e-3 off); with a bf16 stream on both sides, or where a gradient is rounded
+    to bf16 up to three times, as in the test above.  The loss is linear: the sum of an
+    RMS norm's squares hardly depends on its row, and its gradients are differences."""
+    m = model()
+    for norm in m._norms():
+        norm.use_kernel = True
+    g = torch.Generator().manual_seed(6)
+    emb = torch.randn(4, 17, 64, generator=g).bfloat16().cuda().requires_grad_(True)
+    up = torch.randn(4, 17, 64, generator=g).cuda()
+    res = []
+    for fused in (False, True):
+        m.fuse_add_norm = fused
+        m.zero_grad(set_to_none=True)
+        emb.grad = None
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            assert m._add_norm_ok(emb) == fused
+            h = m(None, input_embeds=emb)
+        assert h.dtype == torch.float32
+        (h * up).sum().backward()
+        assert emb.grad.dtype == torch.bfloat16
+        res.append([emb.grad.float(), h.detach()] + [p.grad.clone() for p in m.parameters()
+                                                     if p.grad is not None])
+    assert len(res[0]) == len(res[1])
+    for i, (a, b) in enumerate(zip(*res)):
+        bar = 2e-2 if autocast or i == 0 else 5e-5
+        assert (a - b).abs().max() <= bar * a.abs().max().clamp(min=1e-12)
