@@ -11,6 +11,7 @@ on CPU tensors (a ``Q4Weight`` may be made on the CPU and moved).
 """
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from . import _launch as H
@@ -189,6 +190,7 @@ def m3_rows_linear_q4(x, weight, bias=None, norm_weight=None, eps=0.0, residual=
     dev = H.device_index(x, weight.codes, weight.scales, bias, norm_weight, residual, out0, out1)
     rows, rest = shape[0], n - split
     l0, l1, lr = split, rest, 0
+    given = [t for t in (out0, out1) if t is not None]
     if out0 is not None:
         l0 = _rows(out0, "out0", (rows, split), ty)
     elif split:
@@ -208,4 +210,6 @@ def m3_rows_linear_q4(x, weight, bias=None, norm_weight=None, eps=0.0, residual=
              x2.data_ptr(), lx, H.ptr(nw), weight.codes.data_ptr(),
              weight.scales.data_ptr(), H.ptr(b),
              H.ptr(residual), lr, H.ptr(out0), l0, H.ptr(out1), l1, bool(overlap))
+    if given:
+        increment_version(given)    # a backward pass that has saved one raises
     return out0, out1

@@ -282,3 +282,28 @@ def test_scales_of_4_bit_weights_start_at_16_bytes(center):
         desc = _lib.RowsQ4Desc(2, 40, 6, 64, center, 0, 6, 0, 0.0)
         assert lib.m3_rows_linear_q4(desc, p, 40, None, p + 512, p + 1024 + off, None, None, 0,
                                      p + 2048, 6, None, 0, 0, None) == 5
+
+
+@pytest.mark.parametrize("rows", [0, 2])
+def test_outputs_given_to_the_4_bit_product_count_as_changed(rows, launches):
+    """A backward pass that has saved one raises."""
+    w = Q.Q4Weight.quantize(torch.ones(6, 40), 32)
+    for given in ("out0", "out1", "residual"):
+        leaf = torch.ones(rows, {"out0": 2, "out1": 4, "residual": 6}[given], requires_grad=True)
+        buf = leaf * 1
+        y = buf.square()
+        args = {given: buf, "split": 2}
+        if given == "residual":
+            args = {"residual": buf, "out0": buf}
+        with torch.no_grad():
+            Q.m3_rows_linear_q4(z(rows, 40), w, **args)
+        if rows:
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                y.sum().backward()
+        else:
+            y.sum().backward()
+    r = torch.ones(2, 6, requires_grad=True)      # one that is only read does not
+    y = (r * 1).square()
+    with torch.no_grad():
+        Q.m3_rows_linear_q4(z(2, 40), w, residual=r)
+    y.sum().backward()
