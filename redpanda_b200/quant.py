@@ -186,7 +186,7 @@ def m3_rows_linear_q4(x, weight, bias=None, norm_weight=None, eps=0.0, residual=
     split = n if split is None else int(split)
     if not 0 <= split <= n:
         raise ValueError(f"{name}: split lies between 0 and d_out")
-    H.refuse_tangents(name, x, bias, norm_weight, residual)
+    H.refuse_tangents(name, x, bias, norm_weight, residual, out0, out1)
     dev = H.device_index(x, weight.codes, weight.scales, bias, norm_weight, residual, out0, out1)
     rows, rest = shape[0], n - split
     l0, l1, lr = split, rest, 0

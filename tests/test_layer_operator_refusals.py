@@ -307,3 +307,13 @@ def test_outputs_given_to_the_4_bit_product_count_as_changed(rows, launches):
     with torch.no_grad():
         Q.m3_rows_linear_q4(z(2, 40), w, residual=r)
     y.sum().backward()
+
+
+@pytest.mark.parametrize("given", ["out0", "out1"])
+def test_outputs_with_forward_mode_tangents_are_refused(given):
+    """They would keep the tangent of what they held."""
+    w = Q.Q4Weight.quantize(torch.ones(6, 40), 32)
+    with forward_ad.dual_level():
+        out = forward_ad.make_dual(z(2, 3), torch.ones(2, 3))
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            Q.m3_rows_linear_q4(z(2, 40), w, split=3, **{given: out})
