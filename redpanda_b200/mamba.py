@@ -631,8 +631,11 @@ class Mamba(nn.Module):
         step graphs captured from now on.  Larger batches, priming and training keep
         the full weights.  The copies are of the present weights: a step after the
         weights have changed, or in a copy of the model, raises until this is called
-        again, and a step graph keeps the copies it was captured with.  ``names=()``
-        goes back to the full weights.  Returns the model."""
+        again, and a step graph keeps the copies it was captured with.  Changes are
+        seen by the weight's address and version counter; one that autograd does not
+        count (through ``.data``, or by another library that shares the memory) is not
+        seen, and has to be followed by this call.  ``names=()`` goes back to the full
+        weights.  Returns the model."""
         names = tuple(names)
         if not set(names) <= {"in_proj", "x_proj", "out_proj"}:
             raise ValueError("quantize_step_: names are of in_proj, x_proj, out_proj")
