@@ -528,7 +528,8 @@ typedef struct m3_add_norm_desc {
  *   s = x + res, rounded to dtype_s;  y = s * rstd * w, rstd = 1 / sqrt(mean(s^2) + eps)
  *   x (rows, ld_x), res (rows, ld_r), w (d,) float32, y and s (rows, d), rstd
  *   (rows,) float32 for the backward, or NULL.  s may be res when ld_r == d, or x
- *   when ld_x == d and both have one element type. */
+ *   when ld_x == d and both have one element type; no other output shares bytes
+ *   with an input or another output (M3_ERR_ALIAS). */
 M3_API int m3_add_norm_fwd(const m3_add_norm_desc* desc, const void* x, int64_t ld_x,
             const void* res, int64_t ld_r, const float* w, void* y, void* s, float* rstd,
             void* stream);
@@ -536,7 +537,8 @@ M3_API int m3_add_norm_fwd(const m3_add_norm_desc* desc, const void* x, int64_t 
 /* Backward: s (rows, ld_s) and rstd of the forward, gy (rows, d) the gradient of
  * y, gs (rows, d) that of s or NULL (zero).  ds (rows, d) is the gradient of res;
  * dx (rows, d) that of x where dtype_x is not dtype_s, else NULL (ds serves).  dw
- * (d,) float32, summed over the rows in a fixed order. */
+ * (d,) float32, summed over the rows in a fixed order.  ds may be gs; no other
+ * output shares bytes with an input or another output (M3_ERR_ALIAS). */
 M3_API size_t m3_add_norm_bwd_workspace_bytes(const m3_add_norm_desc* desc);
 M3_API int m3_add_norm_bwd(const m3_add_norm_desc* desc, const void* s, int64_t ld_s,
             const float* w, const float* rstd, const void* gy, const void* gs, void* ds, void* dx,
@@ -558,7 +560,8 @@ typedef struct m3_norm8_desc {
  *   x (rows, ld_x), res (rows, ld_r) or NULL, w (d,) float32, q (rows, d) bytes,
  *   scale (rows,) or (rows, d / group) float32, s (rows, d), not used without res.
  * A group with a NaN has the scale NaN.  With groups, rows and pointers aligned to
- * 4 elements (q to 4 bytes). */
+ * 4 elements (q to 4 bytes).  s may be res or x, as in m3_add_norm_fwd; no other
+ * output shares bytes with an input or another output (M3_ERR_ALIAS). */
 M3_API int m3_norm8_fwd(const m3_norm8_desc* desc, const void* x, int64_t ld_x, const void* res,
             int64_t ld_r, const float* w, void* q, float* scale, void* s, void* stream);
 
@@ -682,7 +685,9 @@ typedef struct m3_gated_args {
  *           not read
  *   h_last  (B, D) float32 or NULL: the state at each row's length (not state)
  *   ckpt    m3_gated_ckpt_floats() floats for the backward (the state in front of
- *           every 4 steps), 8-byte aligned, or NULL */
+ *           every 4 steps), 8-byte aligned, or NULL
+ * Here and below an output that shares bytes with an input or another output is
+ * refused (M3_ERR_ALIAS). */
 M3_API size_t m3_gated_ckpt_floats(const m3_gated_desc* desc);
 M3_API int m3_gated_fwd(const m3_gated_desc* desc, const m3_gated_args* args, void* y,
             float* h_last, float* ckpt, void* stream);

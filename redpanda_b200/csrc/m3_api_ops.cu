@@ -68,6 +68,30 @@ int check_sel(const m3_sel_desc* d) {
   return M3_OK;
 }
 
+// Bytes of an array: `rows` of them, ld apart, of width elements of size e.
+struct Span {
+  const void* p;
+  size_t n;
+};
+Span span(const void* p, int64_t rows, int64_t ld, int64_t width, int e) {
+  const unsigned __int128 n = ((unsigned __int128)(rows - 1) * ld + width) * e;
+  return {p, n > SIZE_MAX ? SIZE_MAX : (size_t)n};
+}
+bool meet(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.p && b.p && (x < y ? y - x < a.n : x - y < b.n);
+}
+// an output that shares bytes with an input or with another output
+bool shared(std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+  for (const Span* o = outs.begin(); o != outs.end(); ++o) {
+    for (const Span& i : ins)
+      if (meet(*o, i)) return true;
+    for (const Span* q = outs.begin(); q != o; ++q)
+      if (meet(*o, *q)) return true;
+  }
+  return false;
+}
+
 int check_gated(const m3_gated_desc* d) {
   if (!d) return M3_ERR_NULL;
   if (d->batch < 1 || d->seqlen < 1 || d->d_inner < 1 || !(d->c > 0.f) || d->c > 3e38f)
@@ -77,15 +101,28 @@ int check_gated(const m3_gated_desc* d) {
   return M3_OK;
 }
 
-// Fills what the gated recurrence's forward and backward share; returns a status.
-int fill_gated(const m3_gated_desc* d, const m3_gated_args* a, bool backward,
-               std::initializer_list<const void*> more, GatedParams* p) {
+// Arguments that the gated recurrence's entries share, and outputs that share bytes with
+// them, with one another or with other inputs (`ins`); returns a status.
+int check_gated_args(const m3_gated_desc* d, const m3_gated_args* a,
+                     std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
   const int e = dsize(d->dtype);
   if (!a || !a->x || !a->rg || !a->ig || !a->decay) return M3_ERR_NULL;
   if (a->ld_x < d->d_inner || a->ld_r < d->d_inner || a->ld_i < d->d_inner) return M3_ERR_SHAPE;
   if (!aligned(a->x, e) || !aligned(a->rg, e) || !aligned(a->ig, e) || !aligned(a->decay, 4) ||
       !aligned(a->state, 4) || !aligned(a->lengths, 4))
     return M3_ERR_ALIGN;
+  const int64_t B = d->batch, D = d->d_inner, rows = B * d->seqlen;
+  if (shared(outs, {span(a->x, rows, a->ld_x, D, e), span(a->rg, rows, a->ld_r, D, e),
+                    span(a->ig, rows, a->ld_i, D, e), span(a->decay, 1, D, D, 4),
+                    span(a->state, B, D, D, 4), span(a->lengths, 1, B, B, 4)}))
+    return M3_ERR_ALIAS;
+  return shared(outs, ins) ? M3_ERR_ALIAS : M3_OK;
+}
+
+// Fills what the forward and backward share; returns a status.
+int fill_gated(const m3_gated_desc* d, const m3_gated_args* a, bool backward,
+               std::initializer_list<const void*> more, GatedParams* p) {
+  const int e = dsize(d->dtype);
   const int rc = check_device();
   if (rc != M3_OK) return rc;
   p->x = a->x; p->rg = a->rg; p->ig = a->ig;
@@ -267,8 +304,15 @@ int m3_add_norm_fwd(const m3_add_norm_desc* desc, const void* x, int64_t ld_x, c
       !aligned(sum, dsize(desc->dtype_s)) || !aligned(y, dsize(desc->dtype_y)) ||
       !aligned(w, 4) || !aligned(rstd, 4))
     return M3_ERR_ALIGN;
-  if (y == x || y == res || y == sum || (sum == res && ld_r != desc->d) ||
-      (sum == x && (ld_x != desc->d || desc->dtype_x != desc->dtype_s)))
+  const int64_t n = desc->rows, d = desc->d;
+  const Span xs = span(x, n, ld_x, d, dsize(desc->dtype_x));
+  const Span rs = span(res, n, ld_r, d, dsize(desc->dtype_s));
+  const Span ss = span(sum, n, d, d, dsize(desc->dtype_s)), ws = span(w, 1, d, d, 4);
+  // the sum may be one of its own terms, element by element
+  const bool in_res = sum == res && ld_r == d;
+  const bool in_x = sum == x && ld_x == d && desc->dtype_x == desc->dtype_s;
+  if (shared({span(y, n, d, d, dsize(desc->dtype_y)), span(rstd, 1, n, n, 4)}, {xs, rs, ss, ws}) ||
+      meet(ss, ws) || (!in_res && meet(ss, rs)) || (!in_x && meet(ss, xs)))
     return M3_ERR_ALIAS;
   if ((rc = check_device()) != M3_OK) return rc;
   AddNormParams p;
@@ -301,7 +345,14 @@ int m3_add_norm_bwd(const m3_add_norm_desc* desc, const void* sum, int64_t ld_s,
       !aligned(dx, dsize(desc->dtype_x)) || !aligned(gy, dsize(desc->dtype_y)) ||
       !aligned(w, 4) || !aligned(rstd, 4) || !aligned(dw, 4) || !aligned(workspace, 4))
     return M3_ERR_ALIGN;
-  if (ds == sum || ds == gy || (dx && (dx == sum || dx == gy || dx == gs || dx == ds)))
+  const int64_t n = desc->rows, d = desc->d;
+  const Span dss = span(ds, n, d, d, es), gss = span(gs, n, d, d, es);
+  // ds may be gs, element by element
+  if (shared({dss, span(dx, n, d, d, dsize(desc->dtype_x)), span(dw, 1, d, d, 4)},
+             {span(sum, n, ld_s, d, es), span(gy, n, d, d, dsize(desc->dtype_y)),
+              span(w, 1, d, d, 4), span(rstd, 1, n, n, 4)}) ||
+      (ds != gs && meet(dss, gss)) || meet(span(dx, n, d, d, dsize(desc->dtype_x)), gss) ||
+      meet(span(dw, 1, d, d, 4), gss))
     return M3_ERR_ALIAS;
   if ((rc = check_device()) != M3_OK) return rc;
   if (!workspace || workspace_bytes < m3_add_norm_bwd_workspace_bytes(desc))
@@ -331,8 +382,12 @@ int m3_norm8_fwd(const m3_norm8_desc* desc, const void* x, int64_t ld_x, const v
       !aligned(q, v) || !aligned(w, 4) || !aligned(scale, 4) || ld_x % v != 0 ||
       (res && ld_r % v != 0))
     return M3_ERR_ALIGN;
-  if (q == x || q == res || (res && (q == sum || (sum == res && ld_r != desc->d) ||
-                                     (sum == x && (ld_x != desc->d || ex != es)))))
+  const int64_t n = desc->rows, d = desc->d, per = g ? d / g : 1;
+  const Span xs = span(x, n, ld_x, d, ex), rs = span(res, n, ld_r, d, es);
+  const Span ss = span(res ? sum : nullptr, n, d, d, es), ws = span(w, 1, d, d, 4);
+  const bool in_res = sum == res && ld_r == d, in_x = sum == x && ld_x == d && ex == es;
+  if (shared({span(q, n, d, d, 1), span(scale, n, per, per, 4)}, {xs, rs, ss, ws}) ||
+      meet(ss, ws) || (!in_res && meet(ss, rs)) || (!in_x && meet(ss, xs)))
     return M3_ERR_ALIAS;
   const int rc = check_device();
   if (rc != M3_OK) return rc;
@@ -553,8 +608,13 @@ int m3_gated_fwd(const m3_gated_desc* desc, const m3_gated_args* args, void* y, 
   if (!args || !y) return M3_ERR_NULL;
   if (!aligned(y, dsize(desc->dtype)) || !aligned(h_last, 4) || !aligned(ckpt, 8))
     return M3_ERR_ALIGN;
-  if ((h_last && h_last == args->state) || y == args->x || y == args->rg || y == args->ig)
-    return M3_ERR_ALIAS;
+  const int64_t B = desc->batch, L = desc->seqlen, D = desc->d_inner;
+  const int64_t cks = B * gated_segments(desc->seqlen);
+  if ((rc = check_gated_args(desc, args,
+                             {span(y, B * L, D, D, dsize(desc->dtype)), span(h_last, B, D, D, 4),
+                              span(ckpt, cks, D, D, 4)},
+                             {})) != M3_OK)
+    return rc;
   GatedParams p;
   memset(&p, 0, sizeof(p));
   if ((rc = fill_gated(desc, args, false, {y}, &p)) != M3_OK) return rc;
@@ -580,8 +640,12 @@ int m3_gated_bwd(const m3_gated_desc* desc, const m3_gated_args* args, const voi
   if (!aligned(g, e) || !aligned(d_x, e) || !aligned(d_rg, e) || !aligned(d_ig, e) ||
       !aligned(ckpt, 8) || !aligned(d_decay, 4) || !aligned(workspace, 4))
     return M3_ERR_ALIGN;
-  for (void* o : {d_x, d_rg, d_ig})
-    if (o == args->x || o == args->rg || o == args->ig || o == g) return M3_ERR_ALIAS;
+  const int64_t rows = (int64_t)desc->batch * desc->seqlen, D = desc->d_inner;
+  const int64_t cks = (int64_t)desc->batch * gated_segments(desc->seqlen);
+  auto all = [&](const void* p) { return span(p, rows, D, D, e); };
+  if ((rc = check_gated_args(desc, args, {all(d_x), all(d_rg), all(d_ig), span(d_decay, 1, D, D, 4)},
+                             {all(g), span(ckpt, cks, D, D, 4)})) != M3_OK)
+    return rc;
   GatedBwdParams q;
   memset(&q, 0, sizeof(q));
   if ((rc = fill_gated(desc, args, true, {g, d_x, d_rg, d_ig}, &q.f)) != M3_OK) return rc;
@@ -596,18 +660,14 @@ int m3_gated_step(const m3_gated_desc* desc, const m3_gated_args* args, float* h
                   void* stream) {
   int rc = check_gated(desc);
   if (rc != M3_OK) return rc;
-  if (!args || !h || !y || !args->x || !args->rg || !args->ig || !args->decay) return M3_ERR_NULL;
-  if (desc->seqlen != 1 || args->ld_x < desc->d_inner || args->ld_r < desc->d_inner ||
-      args->ld_i < desc->d_inner)
-    return M3_ERR_SHAPE;
+  if (!args || !h || !y) return M3_ERR_NULL;
+  if (desc->seqlen != 1) return M3_ERR_SHAPE;
   if (args->state || args->lengths) return M3_ERR_UNSUPPORTED;
   const int e = dsize(desc->dtype);
-  if (!aligned(args->x, e) || !aligned(args->rg, e) || !aligned(args->ig, e) || !aligned(y, e) ||
-      !aligned(args->decay, 4) || !aligned(h, 4))
-    return M3_ERR_ALIGN;
-  if (y == h || y == args->x || y == args->rg || y == args->ig || h == args->x || h == args->rg ||
-      h == args->ig)
-    return M3_ERR_ALIAS;
+  if (!aligned(y, e) || !aligned(h, 4)) return M3_ERR_ALIGN;
+  const int64_t B = desc->batch, D = desc->d_inner;
+  if ((rc = check_gated_args(desc, args, {span(y, B, D, D, e), span(h, B, D, D, 4)}, {})) != M3_OK)
+    return rc;
   if ((rc = check_device()) != M3_OK) return rc;
   GatedStepParams p;
   memset(&p, 0, sizeof(p));

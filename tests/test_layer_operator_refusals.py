@@ -317,3 +317,71 @@ def test_outputs_with_forward_mode_tangents_are_refused(given):
         out = forward_ad.make_dual(z(2, 3), torch.ones(2, 3))
         with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
             Q.m3_rows_linear_q4(z(2, 40), w, split=3, **{given: out})
+
+
+def test_c_entries_refuse_ranges_that_overlap():
+    """An output that shares some of its bytes with an input or another output; only
+    the places that the header names may be the same (no device is touched: a call
+    that passes ends at the device, or there without one)."""
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(1 << 16)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256     # host memory: never dereferenced
+    at = [p + 2048 * i for i in range(16)]             # arrays below hold up to 1024 bytes
+    n = None
+
+    def add(x=at[0], lx=64, r=at[1], lr=64, w=at[2], y=at[3], s=at[4], st=at[5], tx=0):
+        return lib.m3_add_norm_fwd(_lib.AddNormDesc(4, 64, tx, 0, 0, 1e-5), x, lx, r, lr, w, y, s,
+                                   st, n)
+    assert [add(y=at[0] + 1020), add(y=at[1] - 1020), add(y=at[4] + 16), add(s=at[0] + 512),
+            add(s=at[1] + 4), add(r=at[4] - 4), add(x=at[0] + 1020, s=at[0] + 2040),
+            add(y=at[2] + 252), add(s=at[2]), add(st=at[3] + 1020), add(st=at[1]), add(st=at[2] + 8),
+            # strided rows reach further, and in place needs whole rows of one type
+            add(x=at[6], lx=1024, y=at[8]), add(s=at[1], lr=65), add(s=at[0], tx=1)] == [11] * 15
+
+    def addb(s=at[0], w=at[1], st=at[2], gy=at[3], gs=at[4], ds=at[5], dx=n, dw=at[7], tx=0):
+        return lib.m3_add_norm_bwd(_lib.AddNormDesc(4, 64, tx, 0, 0, 1e-5), s, 64, w, st, gy, gs, ds,
+                                   dx, dw, n, 0, n)
+    assert [addb(ds=at[0] + 4), addb(ds=at[3] - 8), addb(ds=at[4] + 8), addb(ds=at[1]),
+            addb(dw=at[0] + 512), addb(dw=at[1]), addb(dw=at[5] + 1020), addb(ds=at[2]),
+            addb(tx=1, dx=at[4] + 2), addb(tx=1, dx=at[5] + 512), addb(tx=1, dx=at[7] + 4)] == [11] * 11
+
+    def n8(x=at[0], lx=64, r=n, lr=0, w=at[2], q=at[3], sc=at[4], s=n, g=32):
+        return lib.m3_norm8_fwd(_lib.Norm8Desc(4, 64, g, 0, 0, 1, 1e-5), x, lx, r, lr, w, q, sc, s,
+                                n)
+    assert [n8(q=at[0] + 1020), n8(q=at[2] + 128), n8(sc=at[0] + 4), n8(sc=at[3] + 252),
+            n8(r=at[1], lr=64, s=at[1] + 16), n8(r=at[1], lr=64, s=at[0] + 16),
+            n8(r=at[1], lr=64, s=at[2] + 16), n8(r=at[1], lr=64, s=at[3] - 16),
+            n8(r=at[1], lr=64, s=at[5], sc=at[5] + 1020)] == [11] * 9
+
+    # 2 rows of 4 steps of 16 channels: 512 bytes, 128 of a state or of checkpoints
+    def args(**kw):
+        v = dict(x=at[0], ld_x=16, rg=at[1], ld_r=16, ig=at[2], ld_i=16, decay=at[3], state=at[4],
+                 lengths=at[5])
+        return _lib.GatedArgs(**{**v, **kw})
+
+    def gated(y=at[6], h=at[7], ck=at[8], **kw):
+        return lib.m3_gated_fwd(_lib.GatedDesc(2, 4, 16, 0, 8.0), args(**kw), y, h, ck, n)
+    assert [gated(y=at[0] + 508), gated(y=at[1] + 4), gated(y=at[2] - 508), gated(y=at[3]),
+            gated(y=at[4] + 64), gated(y=at[5]), gated(h=at[4] + 64), gated(h=at[0]),
+            gated(h=at[6] + 508), gated(ck=at[6]), gated(ck=at[7] + 64), gated(ck=at[4] + 8),
+            gated(ck=at[3]), gated(x=at[9], ld_x=160, y=at[11])] == [11] * 14
+
+    def gatedb(g=at[6], ck=at[7], dx=at[8], dr=at[9], di=at[10], dd=at[11], **kw):
+        return lib.m3_gated_bwd(_lib.GatedDesc(2, 4, 16, 0, 8.0), args(state=n, **kw), g, ck, dx, dr,
+                                di, dd, n, 0, n)
+    assert [gatedb(dx=at[0] + 4), gatedb(dr=at[1] - 4), gatedb(di=at[2] + 508), gatedb(dx=at[6] + 4),
+            gatedb(dr=at[7]), gatedb(dr=at[8]), gatedb(di=at[8] + 508), gatedb(di=at[9]),
+            gatedb(dd=at[3]), gatedb(dd=at[10] + 4), gatedb(dd=at[7] + 64), gatedb(di=at[5]),
+            gatedb(dx=at[3] + 4)] == [11] * 13
+
+    def step(h=at[4], y=at[6], **kw):
+        return lib.m3_gated_step(_lib.GatedDesc(2, 1, 16, 0, 8.0), args(state=n, lengths=n, **kw), h,
+                                 y, n)
+    assert [step(h=at[0] + 64), step(h=at[2] - 64), step(y=at[4] + 64), step(y=at[1] + 124),
+            step(h=at[3] + 4), step(y=at[3])] == [11] * 6
+
+    if not torch.cuda.is_available():                  # what may be the same
+        assert {add(), add(s=at[1]), add(s=at[0]), add(s=at[1], x=at[1]), addb(), addb(gs=at[5]),
+                addb(gs=n), n8(), n8(r=at[1], lr=64, s=at[1]), n8(r=at[1], lr=64, s=at[0]),
+                gated(), gated(x=at[1], ig=at[1]), gated(state=n, h=n, ck=n), gatedb(),
+                step()} == {9}
