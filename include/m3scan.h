@@ -316,7 +316,8 @@ typedef struct m3_rows_q4_desc {
  *           bits); 16-byte aligned; groups cover the rounded-up columns
  *   x (rows, ld_x); norm_w (d_in,) float32 or NULL; bias (d_out,) float32 or NULL;
  *   residual (rows, ld_r) or NULL: it may be out0 itself (same stride, split ==
- *   d_out), no other overlap of an output with an input. */
+ *   d_out), no other overlap of an output with an input; out0 and out1 may be
+ *   columns of one buffer, but share no element (M3_ERR_ALIAS). */
 M3_API int m3_rows_linear_q4(const m3_rows_q4_desc* desc, const void* x, int64_t ld_x,
             const float* norm_w, const void* codes, const void* scales, const float* bias,
             const void* residual, int64_t ld_r, void* out0, int64_t ld0, void* out1, int64_t ld1,

@@ -728,6 +728,13 @@ int m3_rows_linear_q4(const m3_rows_q4_desc* desc, const void* x, int64_t ld_x,
       (s1 && (spans_overlap(x, xs, out1, s1) ||
               (residual && spans_overlap(residual, rs, out1, s1)))))
     return M3_ERR_ALIAS;
+  // the two outputs may be columns of one buffer, each their own
+  if (s0 && s1 && spans_overlap(out0, s0, out1, s1)) {
+    const int64_t apart =
+        (int64_t)(reinterpret_cast<uintptr_t>(out1) - reinterpret_cast<uintptr_t>(out0)) / e;
+    const int64_t at = (apart % ld0 + ld0) % ld0;    // out1's first column in a row of out0
+    if (ld0 != ld1 || at < split || at + d_out - split > ld0) return M3_ERR_ALIAS;
+  }
   const int rc = check_device();
   if (rc != M3_OK) return rc;
   RowsQ4Params p;

@@ -385,3 +385,24 @@ def test_c_entries_refuse_ranges_that_overlap():
                 addb(gs=n), n8(), n8(r=at[1], lr=64, s=at[1]), n8(r=at[1], lr=64, s=at[0]),
                 gated(), gated(x=at[1], ig=at[1]), gated(state=n, h=n, ck=n), gatedb(),
                 step()} == {9}
+
+
+def test_outputs_of_the_4_bit_product_do_not_share_elements():
+    """Halves of one buffer are two outputs; columns that both would write are refused
+    (no device is touched: a call that passes ends there)."""
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(1 << 14)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256     # host memory: never dereferenced
+    o = p + 4096
+
+    def q4(o0, l0, o1, l1, split=4, rows=3, m=10):
+        return lib.m3_rows_linear_q4(_lib.RowsQ4Desc(rows, 40, m, 64, 0, 0, split, 0, 0.0), p, 40,
+                                     None, p + 1024, p + 2048, None, None, 0, o0, l0, o1, l1, 0, None)
+    bad = [q4(o, 10, o, 10), q4(o, 10, o + 12, 10), q4(o + 8, 10, o, 10), q4(o, 10, o + 20, 10),
+           q4(o, 10, o + 40, 10), q4(o, 10, o + 16, 11), q4(o, 4, o + 44, 6), q4(o, 9, o + 16, 9),
+           q4(o, 10, o + 16, 10, rows=1, split=5)]
+    assert bad == [11] * 9
+    if not torch.cuda.is_available():
+        good = {q4(o, 10, o + 16, 10), q4(o + 24, 10, o, 10), q4(o, 12, o + 16, 12),
+                q4(o, 12, o + 24, 12), q4(o, 4, o + 48, 6), q4(o, 10, o + 16, 10, rows=1)}
+        assert good == {9}
