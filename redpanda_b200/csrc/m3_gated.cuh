@@ -312,6 +312,17 @@ __device__ __forceinline__ float2 load_each(const float* p, int left) {
   return make_float2(left > 0 ? p[0] : 0.f, left > St::kNext ? p[St::kNext] : 0.f);
 }
 
+// -c softplus(decay) of a lane's two channels; 0, a decay of 1, where there is none, which
+// has no say in the form of the decay that a warp takes (with another value there the last
+// tile's warps never took the short one: 256 x 64 x 2040 bf16 forward 60 against 58 us, 2 x
+// 16001 x 1272 fp32 backward 211 against 206; 1 x 16384 x 1000 bf16 55 either way).
+template <typename St>
+__device__ __forceinline__ float2 rates(const float* decay, float c, int left) {
+  const float2 d = load_each<St>(decay, left);
+  return make_float2(left > 0 ? -c * softplus_f(d.x) : 0.f,
+                     left > St::kNext ? -c * softplus_f(d.y) : 0.f);
+}
+
 // ------------------------------------------------------------------ joins
 // A warp's runs, the CTA's warps and, for S > 1, the cluster's CTAs hold
 // consecutive steps, forwards (DIR 1) or backwards (-1): w and rank are this warp's

@@ -76,8 +76,7 @@ __global__ void __launch_bounds__(256, 2)
   char* buf = smem + w * St::kBytes;
   const Joint<LC> joint(smem + W * St::kBytes, W, S);
   St st;
-  const float2 dec = load_each<St>(p.decay + c, left);
-  const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
+  const float2 k = rates<St>(p.decay + c, p.c, left);
   const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
   float2 sum = f2(0.f);
   int turn = 0;

@@ -52,8 +52,7 @@ __global__ void __launch_bounds__(256, 3) gated_fwd_kernel(const GatedParams p) 
   char* buf = smem + w * St::kBytes;
   const Joint<LC> joint(smem + W * St::kBytes, W, S);
   St st;
-  const float2 dec = load_each<St>(p.decay + c, left);
-  const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
+  const float2 k = rates<St>(p.decay + c, p.c, left);
   const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
   int turn = 0;
   bool dead = false;
@@ -190,8 +189,7 @@ __global__ void __launch_bounds__(128, 8) gated_rows_fwd_kernel(const GatedParam
     }
   };
   ahead();
-  const float2 dec = load_each<St>(p.decay + c, left);
-  const float2 k = make_float2(-p.c * softplus_f(dec.x), -p.c * softplus_f(dec.y));
+  const float2 k = rates<St>(p.decay + c, p.c, left);
   const bool near = __all_sync(0xffffffffu, k.x >= -kNear && k.y >= -kNear);
   for (; b < p.B; b += step) {
     n = row_length(p.lengths, b, L);

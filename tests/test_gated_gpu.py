@@ -383,3 +383,21 @@ def test_replays_read_the_buffers_as_they_are_then():
         leaves = [t.clone().requires_grad_(i < 4) for i, t in enumerate(src)]
         for a, b in zip(out, run(*leaves, torch.zeros_like(h))):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [70, 72, 65, 127])
+@pytest.mark.parametrize("far", [False, True])
+def test_channels_do_not_depend_on_their_neighbours(D, far, ty):
+    """A tile's last channels alone, or beside channels whose decays are near one or far
+    from it: the same bits, whichever form of the decay the warp takes (rows enough for a
+    warp each, so that nothing is joined)."""
+    x, rg, ig, decay, _, st, lens = inputs(2000, 5, 128, T[ty], 3, state=True, ragged=True)
+    decay = decay - 4                                  # 8 softplus(decay) below 0.34
+    decay[D:] = 2.0 if far else -6.0
+    args = cuda(x, rg, ig, decay)
+    st, lens = cuda(st, lens)
+    y, h = G.m3_gated_scan_with_state(*args, state=st, lengths=lens)
+    cut = [t[..., :D].contiguous() for t in (*args, st)]
+    y1, h1 = G.m3_gated_scan_with_state(*cut[:4], state=cut[4], lengths=lens)
+    assert torch.equal(y1, y[..., :D]) and torch.equal(h1, h[:, :D])
