@@ -556,8 +556,9 @@ typedef struct m3_norm8_desc {
 } m3_norm8_desc;
 
 /* y = the RMS norm of x, or of s = x + res rounded to dtype_s, in 8 bits:
- *   scale = max(max |y| / top, 2^-126) over a row or a group of columns,
- *   q = y / scale rounded to nearest even and held to [-top, top]
+ *   scale = max(max |y| / top, 2^-126) over a row or a group of columns, to 2^-23 of it,
+ *   q = y / scale, formed to 2^-22 of itself, then rounded to nearest even and held to
+ *   [-top, top] (a quotient that near to the border of two codes may get either)
  *   x (rows, ld_x), res (rows, ld_r) or NULL, w (d,) float32, q (rows, d) bytes,
  *   scale (rows,) or (rows, d / group) float32, s (rows, d), not used without res.
  * A group with a NaN has the scale NaN.  With groups, rows and pointers aligned to

@@ -249,8 +249,10 @@ def m3_rms_norm_8bit(x, weight, residual=None, eps=1e-5, dtype=torch.float8_e4m3
     torch.int8; ``group``: 32, 64 or 128 columns per scale (they have to divide d),
     or None, one scale per row.  q (..., d) and scale (..., 1) or (..., d / group)
     float32 stand for y = q * scale, with scale = max(max|y| / 448, 2^-126) (int8:
-    127) over the group, y in float32, q = y / scale rounded to nearest even.  A
-    group with a NaN has the scale NaN.  Inference only."""
+    127) over the group, y in float32, q = y / scale rounded to nearest even.  The
+    scale is within 2^-23 of that and the quotient within 2^-22 before its rounding:
+    next to the border of two codes either may come out.  A group with a NaN has the
+    scale NaN.  Inference only."""
     name = "m3_rms_norm_8bit"
     d, eps = _check_rows(name, x, weight, residual, eps)
     cx = H.code(x.dtype)
