@@ -19,7 +19,7 @@ cudaError_t with_types(int x, int s, int y, F&& f) {
 }
 
 // Instantiation of a row length, as norm_dispatch, but with 16 elements per thread in
-// rows past 2048 (past 1024 in the 8-bit norm: `from`): these kernels hold two or three
+// rows past F's kFrom, 2048 (1024 in the 8-bit norm): these kernels hold two or three
 // arrays, and a CTA of 512 threads with 8 elements each fills an SM by itself with too
 // little in flight (16384 x 4096 bf16: forward 116 against 92 us, backward 137
 // against 116).
@@ -37,15 +37,18 @@ inline int add_threads(int d, int from) {
   return (d + 32 * e - 1) / (32 * e) * 32;
 }
 template <typename F>
-cudaError_t add_dispatch(int d, int vec, int from, F&& f) {
-  if (d <= 256) return norm_size<8>(vec, 0, f);
-  if constexpr (std::decay_t<F>::kWarpRows) {
+cudaError_t add_dispatch(int d, int vec, F&& f) {
+  constexpr int from = std::decay_t<F>::kFrom;
+  constexpr bool kWarpRows = std::decay_t<F>::kWarpRows;
+  if (d <= 256) return norm_warp<8>(vec, f);
+  if constexpr (kWarpRows) {
     if (d <= 512) return norm_warp<16>(vec, f);
     if (d <= 768) return norm_warp<24>(vec, f);
     if (d <= 1024) return norm_warp<32>(vec, f);
   }
   const int nt = add_threads(d, from);
-  if (d <= from) return add_size<8, 768>(vec, nt, f);   // 80 registers
+  if constexpr (!kWarpRows || from > 1024)
+    if (d <= from) return add_size<8, 768>(vec, nt, f);   // 80 registers
   if (d <= 8192) return add_size<16, 512>(vec, nt, f);
   return d <= 16384 ? add_size<16, 1024>(vec, nt, f) : add_size<32, 1024>(vec, nt, f);
 }

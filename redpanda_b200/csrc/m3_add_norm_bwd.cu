@@ -14,7 +14,7 @@
 namespace m3 {
 namespace {
 
-constexpr int kFrom = 2048;
+constexpr int kRowsFrom = 2048;
 
 template <typename TX, typename TS, typename TY, int VEC, int NV, bool WARP, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) add_norm_bwd_kernel(const AddNormBwdParams p) {
@@ -115,6 +115,7 @@ template <typename TX, typename TS, typename TY>
 struct Launch {
   static constexpr bool kWide = sizeof(TX) == 2 || sizeof(TS) == 2 || sizeof(TY) == 2;
   static constexpr bool kEven = true;
+  static constexpr int kFrom = kRowsFrom;
   static constexpr bool kWarpRows = false;
   const AddNormBwdParams& p;
   cudaStream_t s;
@@ -132,8 +133,8 @@ struct Launch {
 
 // 768 threads per SM at 80 registers, 512 at 128 where a thread holds 16 elements
 int add_norm_bwd_ctas(long long rows, int d, int sms) {
-  const int rpc = d <= 256 ? 4 : 1, nt = d <= 256 ? 128 : add_threads(d, kFrom);
-  const int per = d <= kFrom ? 768 / nt : nt <= 512 ? 512 / nt : 1;
+  const int rpc = d <= 256 ? 4 : 1, nt = d <= 256 ? 128 : add_threads(d, kRowsFrom);
+  const int per = d <= kRowsFrom ? 768 / nt : nt <= 512 ? 512 / nt : 1;
   const long long want = (rows + rpc - 1) / rpc, cap = (long long)sms * per;
   return (int)(want < cap ? want : cap);
 }
@@ -146,7 +147,7 @@ cudaError_t launch_add_norm_bwd(const AddNormBwdParams& p, cudaStream_t s) {
   };
   const int vec = ex + es + ey < 12 && ok(8) ? 8 : ok(4) ? 4 : ok(2) ? 2 : 1;
   return with_types(p.dtype_x, p.dtype_s, p.dtype_y, [&](auto tx, auto ts, auto ty) {
-    return add_dispatch(p.d, vec, kFrom, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
+    return add_dispatch(p.d, vec, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
   });
 }
 

@@ -12,8 +12,6 @@
 namespace m3 {
 namespace {
 
-constexpr int kFrom = 2048;
-
 template <typename TX, typename TS, typename TY, int VEC, int NV, bool WARP, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) add_norm_fwd_kernel(const AddNormParams p) {
   constexpr int E = VEC * NV;
@@ -76,6 +74,7 @@ template <typename TX, typename TS, typename TY>
 struct Launch {
   static constexpr bool kWide = sizeof(TX) == 2 || sizeof(TS) == 2 || sizeof(TY) == 2;
   static constexpr bool kEven = true;
+  static constexpr int kFrom = 2048;
   static constexpr bool kWarpRows = true;
   const AddNormParams& p;
   cudaStream_t s;
@@ -102,7 +101,7 @@ cudaError_t launch_add_norm_fwd(const AddNormParams& p, cudaStream_t s) {
   };
   const int vec = ex + es + ey < 12 && ok(8) ? 8 : ok(4) ? 4 : ok(2) ? 2 : 1;
   return with_types(p.dtype_x, p.dtype_s, p.dtype_y, [&](auto tx, auto ts, auto ty) {
-    return add_dispatch(p.d, vec, kFrom, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
+    return add_dispatch(p.d, vec, Launch<decltype(tx), decltype(ts), decltype(ty)>{p, s});
   });
 }
 

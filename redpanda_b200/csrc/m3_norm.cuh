@@ -93,14 +93,12 @@ inline int norm_vec(int d, int dtype_x, int dtype_y, bool ok8, bool ok4) {
   return ok4 && d % 4 == 0 ? 4 : 1;
 }
 
-// The instantiation of a row length: f<VEC, NV, WARP, MAXT, MINB>(threads, grid).  Vectors
-// of 8 where F has kWide, of 2 where it has kEven.
+// The instantiation of a row length: f<VEC, NV, WARP, MAXT, MINB>(threads).  Vectors of 8
+// where F has kWide, in warps of 2 where it has kEven.  Here a CTA's rows:
 template <int E, typename F>
 cudaError_t norm_size(int vec, int nt, F&& f) {
   auto with = [&](auto v) -> cudaError_t {
     constexpr int VEC = decltype(v)::value, NV = E / VEC;
-    if constexpr (E == 8)
-      if (nt == 0) return f.template operator()<VEC, NV, true, 128, 6>(128);
     if constexpr (E == 8) {
       if (nt <= 768) return f.template operator()<VEC, NV, false, 768, 1>(nt);
     } else {
@@ -110,15 +108,13 @@ cudaError_t norm_size(int vec, int nt, F&& f) {
   };
   if constexpr (std::decay_t<F>::kWide)
     if (vec == 8) return with(std::integral_constant<int, 8>());
-  if constexpr (std::decay_t<F>::kEven)
-    if (vec == 2) return with(std::integral_constant<int, 2>());
   return vec == 4 ? with(std::integral_constant<int, 4>())
                   : with(std::integral_constant<int, 1>());
 }
-// Forward rows a warp holds at E elements per lane.
+// Rows a warp holds at E elements per lane.
 template <int E, typename F>
 cudaError_t norm_warp(int vec, F&& f) {
-  constexpr int MINB = E <= 16 ? 5 : 4;
+  constexpr int MINB = E <= 8 ? 6 : E <= 16 ? 5 : 4;
   if constexpr (std::decay_t<F>::kWide)
     if (vec == 8) return f.template operator()<8, E / 8, true, 128, MINB>(128);
   if constexpr (std::decay_t<F>::kEven)
@@ -129,6 +125,7 @@ cudaError_t norm_warp(int vec, F&& f) {
 template <typename F>
 cudaError_t norm_dispatch(int d, int vec, F&& f) {
   const int nt = norm_threads(d);
+  if (nt == 0) return norm_warp<8>(vec, f);
   if constexpr (std::decay_t<F>::kWarpRows) {
     if (d > 256 && d <= 512) return norm_warp<16>(vec, f);
     if (d > 512 && d <= 768) return norm_warp<24>(vec, f);

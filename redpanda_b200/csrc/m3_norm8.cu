@@ -171,6 +171,7 @@ template <typename TX, typename TS>
 struct Launch {
   static constexpr bool kWide = true, kWarpRows = true;
   static constexpr bool kEven = true;
+  static constexpr int kFrom = 1024;
   const Norm8Params& p;
   cudaStream_t s;
   template <int VEC, int NV, bool WARP, int MAXT, int MINB>
@@ -200,7 +201,7 @@ cudaError_t launch_norm8(const Norm8Params& p, cudaStream_t s) {
   const int vec = ok(8) ? 8 : ok(4) ? 4 : ok(2) ? 2 : 1;
   if (p.group != 0 && vec < 4) return cudaErrorInvalidValue;   // refused by the entry
   return with_types(p.dtype_x, p.dtype_s, M3_F32, [&](auto tx, auto ts, auto) {
-    return add_dispatch(p.d, vec, 1024, Launch<decltype(tx), decltype(ts)>{p, s});
+    return add_dispatch(p.d, vec, Launch<decltype(tx), decltype(ts)>{p, s});
   });
 }
 
