@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(MAXT, MINB) add_norm_bwd_kernel(const AddNormB
     ca = na;
   }
   pdl_launch_dependents();
-  float* part = p.part + (size_t)blockIdx.x * 2 * d;
+  float* part = p.part + (size_t)blockIdx.x * d;
   if constexpr (WARP) {
     const int row = threadIdx.x >> 5;
     for (int k = 0; k < rpc; ++k) {   // warps add in order
@@ -125,7 +125,7 @@ struct Launch {
     add_norm_bwd_kernel<TX, TS, TY, VEC, NV, WARP, MAXT, MINB><<<ctas, nt, 0, s>>>(p);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_norm_reduce(p.part, ctas, p.d, p.dw, nullptr, s);
+    return launch_norm_reduce(p.part, ctas, p.d, 1, p.dw, nullptr, s);
   }
 };
 

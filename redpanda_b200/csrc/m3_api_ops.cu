@@ -328,7 +328,7 @@ int m3_add_norm_fwd(const m3_add_norm_desc* desc, const void* x, int64_t ld_x, c
 size_t m3_add_norm_bwd_workspace_bytes(const m3_add_norm_desc* desc) {
   const int sms = device_sms();
   if (check_add_norm(desc) != M3_OK || sms <= 0) return 0;
-  return (size_t)add_norm_bwd_ctas(desc->rows, desc->d, sms) * 2 * desc->d * 4;
+  return (size_t)add_norm_bwd_ctas(desc->rows, desc->d, sms) * desc->d * 4;
 }
 
 int m3_add_norm_bwd(const m3_add_norm_desc* desc, const void* sum, int64_t ld_s, const float* w,

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_bwd_kernel(const NormBwdParam
 // out[c] = sum over the CTAs' partials: 32 columns per CTA, 32 strided sums
 // each, joined in order.
 __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* part, int n, int d,
-                                                           float* dw, float* db) {
+                                                           int arrays, float* dw, float* db) {
   __shared__ float s[32][33];
   const int cx = threadIdx.x & 31, k = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + cx;
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* part, in
   if (c < d) {
     const float* q = part + (size_t)which * d + c;
 #pragma unroll 4
-    for (int i = k; i < n; i += 32) a += q[(size_t)i * 2 * d];
+    for (int i = k; i < n; i += 32) a += q[(size_t)i * arrays * d];
   }
   s[k][cx] = a;
   __syncthreads();
@@ -257,7 +257,7 @@ struct LaunchBwd {
     else norm_bwd_kernel<TX, TY, VEC, NV, WARP, MAXT, MINB, false><<<ctas, nt, 0, s>>>(p);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_norm_reduce(p.part, ctas, p.d, p.dw, p.db, s);
+    return launch_norm_reduce(p.part, ctas, p.d, 2, p.dw, p.db, s);
   }
 };
 
@@ -269,10 +269,10 @@ int norm_bwd_ctas(long long rows, int d, int sms) {
   return (int)(want < cap ? want : cap);
 }
 
-cudaError_t launch_norm_reduce(const float* part, int n, int d, float* dw, float* db,
+cudaError_t launch_norm_reduce(const float* part, int n, int d, int arrays, float* dw, float* db,
                                cudaStream_t s) {
   return launch_maybe_pdl(true, norm_reduce_kernel, dim3((d + 31) / 32, db != nullptr ? 2 : 1),
-                          dim3(1024), 0, s, part, n, d, dw, db);
+                          dim3(1024), 0, s, part, n, d, arrays, dw, db);
 }
 
 cudaError_t launch_norm_fwd(const NormParams& p, cudaStream_t s) {

@@ -61,15 +61,16 @@ struct AddNormBwdParams {
   void* ds;                           // (rows, d) of dtype_s
   void* dx;                           // (rows, d) of dtype_x, or nullptr: ds serves
   float* dw;                          // (d,)
-  float* part;                        // (add_norm_bwd_ctas, 2, d), the first of each pair used
+  float* part;                        // (add_norm_bwd_ctas, d)
   long long rows; int d;
   int dtype_x, dtype_s, dtype_y;
   int sms;
 };
 int add_norm_bwd_ctas(long long rows, int d, int sms);   // partials
 cudaError_t launch_add_norm_bwd(const AddNormBwdParams& p, cudaStream_t s);
-// out[c] = sum over n partials part[(i * 2 + which) * d + c], in a fixed order (db may be nullptr)
-cudaError_t launch_norm_reduce(const float* part, int n, int d, float* dw, float* db,
+// out[c] = sum over n partials part[(i * arrays + which) * d + c], which: 0 for dw, 1 for db,
+// in a fixed order (db may be nullptr)
+cudaError_t launch_norm_reduce(const float* part, int n, int d, int arrays, float* dw, float* db,
                                cudaStream_t s);
 
 // The RMS norm (of x, or of s = x + res) in 8 bits with scales.

@@ -294,3 +294,29 @@ def test_rows_of_whole_pairs(rows, d, tx, ts, ty):
 @pytest.mark.parametrize("rows,d", EVEN)
 def test_8bit_rows_of_whole_pairs(rows, d, tx, ts, dtype):
     test_8bit_matches_definition(rows, d, None, tx, ts, dtype)
+
+
+@pytest.mark.parametrize("rows,d", [(1, 8), (3, 257), (700, 64), (5000, 1000)])
+def test_workspace_of_the_backward_is_what_it_uses(rows, d):
+    """One partial of the weight gradient for each CTA (of four rows up to 256 columns,
+    6 CTAs per SM there and 768 threads' worth further on); what lies behind stays as it
+    was."""
+    lib = N._lib.load()
+    desc = N.AddNormDesc(rows, d, 0, 0, 0, EPS)
+    n = lib.m3_add_norm_bwd_workspace_bytes(desc)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    ctas = min(-(-rows // 4) if d <= 256 else rows, 6 * sms if d <= 256 else
+               sms * (768 // (-(-d // 256) * 32)))
+    assert n == ctas * d * 4
+    x, res, w, gy, gs = inputs(rows, d, *[torch.float32] * 3, rows)
+    s, w, gy, gs = (x + res).cuda(), w.cuda(), gy.cuda(), gs.cuda()
+    rstd = (s.square().mean(1) + EPS).rsqrt()
+    ds, dw = torch.empty_like(s), torch.empty_like(w)
+    ws = torch.full((n // 4 + 64,), 7.0, device="cuda")
+    assert lib.m3_add_norm_bwd(desc, s.data_ptr(), d, w.data_ptr(), rstd.data_ptr(), gy.data_ptr(),
+                               gs.data_ptr(), ds.data_ptr(), None, dw.data_ptr(), ws.data_ptr(), n,
+                               torch.cuda.current_stream().cuda_stream) == 0
+    _, _, rds, tol, _, rdw, tolw = bounds(s.cpu(), w.cpu(), gy.cpu(), gs.cpu(), *[torch.float32] * 3)
+    near(ds, rds, tol)
+    near(dw, rdw, tolw)
+    assert (ws[n // 4:] == 7).all()
