@@ -649,7 +649,9 @@ int m3_gated_bwd(const m3_gated_desc* desc, const m3_gated_args* args, const voi
   GatedBwdParams q;
   memset(&q, 0, sizeof(q));
   if ((rc = fill_gated(desc, args, true, {g, d_x, d_rg, d_ig}, &q.f)) != M3_OK) return rc;
-  if (!workspace || workspace_bytes < m3_gated_bwd_workspace_bytes(desc)) return M3_ERR_WORKSPACE;
+  // of the plan that is launched
+  if (!workspace || workspace_bytes < (size_t)q.f.rows * q.f.splits * desc->d_inner * 4)
+    return M3_ERR_WORKSPACE;
   q.f.ckpt = const_cast<float*>(ckpt);
   q.g = g; q.dx = d_x; q.drg = d_rg; q.dig = d_ig; q.ddecay = d_decay;
   q.part = static_cast<float*>(workspace);
