@@ -263,7 +263,7 @@ M3_API int m3_silu(int64_t rows, int32_t d, const float* x, int64_t ld_x, float*
  * projection is a matrix-vector product.  One warp per output column; sums in
  * a fixed order (deterministic); weights (nn.Linear layout, (d_out, d_in)
  * row-major) 16-byte aligned with d_in % 4 == 0.  rows > 8, or inputs past 48 KB
- * of staged floats (8 rows x 1536, 4 x 3072, ...), return M3_ERR_UNSUPPORTED.
+ * of staged floats (8 rows x 1536, 2 x 6144, ...), return M3_ERR_UNSUPPORTED.
  *
  * m3_rows_linear: out = act(residual + (bias + xn W^T)) with
  *   xn = x * rsqrt(mean(x^2) + eps) * norm_w    (RMSNorm, mamba.py:82-89) when

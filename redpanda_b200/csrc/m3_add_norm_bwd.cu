@@ -7,7 +7,11 @@
 // another.  Layout as the norm's backward (m3_norm.cu): every row is read once, the
 // weight gradient of a thread's columns stays in registers over its rows, each CTA
 // writes one partial row of dw and a second launch adds them in a fixed order.  131072
-// x 768, gradients of bf16 y and of an fp32 stream: 242 us (6.7 TB/s).
+// x 768, gradients of bf16 y and of an fp32 stream: 242 us (6.7 TB/s).  Past 2048 columns
+// three rows, their next ones, the weight and its gradient fill a thread's 128 registers
+// (fp32: 92 bytes spilled), so that 16 warps are all an SM holds: 16384 x 4096 bf16 116 us,
+// fp32 212 (4.6 and 5.1 TB/s).  Past 8192 a thread of up to 1024 has 64 registers, and 250
+// to 1700 bytes are spilled: 4096 x 16384 bf16 174 us, fp32 418; 2048 x 32768 490 and 1000.
 #include "m3_add_norm.cuh"
 #include "m3_pdl.cuh"
 

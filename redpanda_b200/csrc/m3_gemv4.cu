@@ -23,10 +23,12 @@
 // staged in shared memory, `chunk` columns at a time; codes and scales come through a
 // ring of asynchronous copies per warp.
 //
-// 3 rows of bf16, 8192 x 65536, groups of 128: 68 us (4.1 TB/s; reading the codes alone
-// this way takes 55-62).  8 rows of fp32, 768 x 8192: 8.3 us.  1 row, 384 x 1536 with
-// the norm and silu: 4.3 us.  Many rows of fp32 over long inputs are bound by staging,
-// which every CTA repeats: 8 rows, 8192 x 8192: 42 us for 38 MB.
+// 3 rows of bf16, 8192 x 65536, groups of 128: 67 us (4.1 TB/s; the bytes take 42).  One
+// wave of CTAs with these rings reads the codes alone in 55-62 us, whatever the rings'
+// depth; many small CTAs read them in 43-45, but each would stage the inputs again.  8
+// rows of fp32, 768 x 8192: 8.3 us.  1 row, 384 x 1536 with the norm and silu: 4.3 us.
+// Many rows of fp32 over long inputs are bound by staging, which every CTA repeats: 8 rows,
+// 8192 x 8192: 42 us for 38 MB; 2048 x 50304 with the norm: 49 us for 60 MB.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
