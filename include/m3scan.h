@@ -305,7 +305,8 @@ typedef struct m3_rows_q4_desc {
  *   W[o,k] = scale[o,k/group] (q[o,k] - 8) + center[o,k/group],  q in 0..15,
  * in fp32 (inputs are not rounded), each output rounded once; the norm, split,
  * residual and overlap as above (the codes and scales are the weights that overlap
- * is about).  Sums in a fixed order.
+ * is about).  Sums in a fixed order; scale and center come in behind a group's sums,
+ * so a row with an infinity, or past 1e35, may give NaN.
  *   codes   (tiles, blocks, 32, 4) 32-bit words, 16-byte aligned: tiles of 16
  *           outputs, blocks of 64 columns; both numbers rounded up, the columns to
  *           whole groups of 128 where group is 128.  Word j of lane l of a block

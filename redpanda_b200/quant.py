@@ -164,8 +164,10 @@ def m3_rows_linear_q4(x, weight, bias=None, norm_weight=None, eps=0.0, residual=
     ``out0`` to update it in place.  Returns (out0, out1), of x's element type; one
     without columns is None.  ``overlap``: launch as a programmatic dependent
     launch, which reads the first codes and scales before the kernel ahead of it on
-    the stream completes (only when no queued kernel writes them).  Inference
-    only."""
+    the stream completes (only when no queued kernel writes them).  A group's codes
+    and inputs are summed before its scale and center come in: a row with an infinity,
+    or past 1e35, may give NaN where its weights as floats give an infinity or a
+    number; other rows do not change.  Inference only."""
     name = "m3_rows_linear_q4"
     if not isinstance(weight, Q4Weight):
         raise TypeError(f"{name}: weight is a Q4Weight")

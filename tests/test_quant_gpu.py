@@ -277,3 +277,21 @@ def test_norm_for_every_number_of_warps_and_parts(n, group, ty):
     """1 to 8 warps' worth of tiles; inputs in one part and in two to five."""
     for rows, k in ((8, 2048), (8, 3001), (5, 4100), (8, 4992)):
         norm_in_chunks(rows, k, n, group, (n + k) % 2 == 0, ty)
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rows_that_are_not_finite_change_no_other(norm, ty):
+    """With centers an infinity's outputs are infinite or NaN; the other rows keep their
+    bits."""
+    q, w = weight(200, 300, 64, True, 5)
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(6, 300, generator=g).to(T[ty]).cuda()
+    nw = torch.randn(300, generator=g).cuda() if norm else None
+    good = Q.m3_rows_linear_q4(x, q, norm_weight=nw, eps=EPS)[0]
+    x[1, 17], x[4, 299], x[2, 64] = float("inf"), float("-inf"), float("nan")
+    out = Q.m3_rows_linear_q4(x, q, norm_weight=nw, eps=EPS)[0]
+    keep = [0, 3, 5]
+    assert torch.equal(out[keep], good[keep])
+    for row, col in ((1, 17), (4, 299), (2, 64)):
+        assert not torch.isfinite(out[row][w["w"][:, col].cuda() != 0]).any()
